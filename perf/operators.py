@@ -219,7 +219,8 @@ def prepare(case, seed):
         if own:
             b2 = _b2()
             st["kv"] = b2.PagedKV(k, v, tables, seq_lens)
-            st["ws"] = b2.Workspace(b2.paged_decode_workspace_bytes(B, nq, nkv, D, case["L"], case["scores"]))
+            st["ws"] = b2.Workspace(b2.paged_decode_workspace_bytes(B, nq, nkv, D, tables.shape[1] * case["bs"],
+                                                                    scored=case["scores"]))
         return st
     bs, budget = case["bs"], case["budget"]
     db = -(-budget // bs)
