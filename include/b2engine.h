@@ -169,9 +169,10 @@ int b2_flash_prefill_gqa_ex(const void* q, const void* k, const void* v, void* o
 /* Device scratch owned by the caller and lent to the entry points that take
  * one, so that those never allocate (no counterpart in the reference, whose
  * only internal workspaces are the sampler's).  b2_workspace_create
- * allocates `bytes` of device memory on the current device; the handle may
- * be reused by any number of calls on that device that do not overlap in
- * time. */
+ * allocates `bytes` of device memory on the current device (and a small
+ * cleared area for arrival counters that every call leaves cleared); it
+ * synchronises the legacy default stream.  The handle may be reused by any
+ * number of calls on that device that do not overlap in time. */
 typedef struct b2_workspace b2_workspace;
 int b2_workspace_create(size_t bytes, b2_workspace** out);
 int b2_workspace_destroy(b2_workspace* ws);
@@ -255,6 +256,107 @@ int b2_gemv_int4(const void* Wq, const float* scales, const void* x, void* y, in
 int b2_append_kv_cache(const void* src_k, const void* src_v, void* dst_k, void* dst_v,
                        int num_tokens, int start_pos, int num_kv_heads, int max_seq, int head_dim,
                        void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Bounded-cache attention: long contexts served on a paged K/V cache that is
+ * kept small.  New API (no counterpart in the reference: its attention sees
+ * the whole context, and its paged runner's blocks only grow,
+ * docs/runner_interface.md:16-84).
+ *
+ * A query at position i sees position j <= i when window == 0, or when
+ * i - j < window, or when j < sinks.  The softmax scale is 1/sqrt(head_dim);
+ * q and k arrive with whatever position encoding they have.
+ * ------------------------------------------------------------------------- */
+
+/* Causal GQA attention of q_len query tokens per sequence at positions
+ * q_start .. q_start + q_len - 1 over K/V rows of positions 0 .. q_start +
+ * q_len - 1, with window and sinks as above (window 0: all earlier
+ * positions).  q, k and v through strided views (stride_d 1; element (b, h,
+ * s, d) of q is head h of query token s, at position q_start + s), out dense
+ * [batch, q_len, num_q_heads, head_dim].  seq_lens: device int32 [batch],
+ * the tokens of each sequence counted from position 0, or NULL for q_start +
+ * q_len everywhere; query rows at positions >= seq_lens[b] give zeros, and
+ * K/V rows there may hold anything, NaN included.  K and V rows of positions
+ * below seq_lens[b] must be finite.  fp16, or bf16 when bf16 != 0.
+ * head_dim up to 128 (a multiple of 8, 16-byte-aligned rows) runs on the
+ * tcgen05 tensor cores; other head_dim up to 256 and other alignments on a
+ * CUDA-core kernel.  Allocates nothing. */
+int b2_window_prefill_gqa(b2_kv_view q, b2_kv_view k, b2_kv_view v, void* out, const int* seq_lens, int64_t q_len,
+                          int64_t q_start, int num_q_heads, int num_kv_heads, int head_dim, int batch,
+                          int64_t window, int64_t sinks, int bf16, void* stream);
+
+/* One layer's paged K/V cache.  Row (slot t of block n, kv head h) of K lives
+ * at k + n*stride_block + t*stride_slot + h*stride_head (elements), V alike;
+ * a row is head_dim contiguous elements.  Strides are multiples of 8 and k, v
+ * 16-byte aligned.  The pool of the reference's runner contract,
+ * [num_blocks][block_size][kv_heads][head_dim], has stride_block =
+ * block_size*kv_heads*head_dim, stride_slot = kv_heads*head_dim, stride_head
+ * = head_dim; head-major blocks swap the last two.  block_tables is device
+ * int32 [batch][max_blocks], seq_lens device int32 [batch] (a length above
+ * max_blocks*block_size is cut to it). */
+typedef struct b2_paged_kv {
+    void* k;
+    void* v;
+    const int* block_tables;
+    const int* seq_lens;
+    int64_t stride_block;
+    int64_t stride_slot;
+    int64_t stride_head;
+    int num_blocks;
+    int block_size;
+    int max_blocks;
+    int bf16; /* 0: half rows, else bf16 */
+} b2_paged_kv;
+
+/* GQA attention of the newest token of each sequence (position seq_lens[b] -
+ * 1, whose K/V row is already in the cache) over its paged rows, with window
+ * and sinks as above.  q is [batch] rows of num_q_heads*head_dim elements
+ * (the cache's type), ldq elements apart; out dense [batch, num_q_heads,
+ * head_dim].  Only rows of visible positions are read, and table entries
+ * only of blocks that hold one (so blocks the window has left behind can be
+ * freed); visible positions whose entry is outside [0, num_blocks) are left
+ * out of the softmax.  A sequence that sees nothing gives zeros.
+ *
+ * scores != NULL (fp32 [num_blocks][num_kv_heads][block_size], following the
+ * blocks): the weight that the group's query heads together give to each
+ * visible position is added to its score; the newest position's score starts
+ * from nothing (its slot may hold anything).  Sequences of one call must not
+ * share blocks then.  One writer per score: the same bits every run.
+ *
+ * The positions of all (sequence, kv head) pairs are cut into equal shares,
+ * one per resident CTA; a pair cut between CTAs is joined from partial
+ * results in `ws` by the last of them.  ws == NULL is allowed without scores:
+ * each pair then stays on one CTA.  ws needs
+ * b2_paged_decode_workspace_bytes(..., max_positions, ...) bytes
+ * (B2_ERR_WORKSPACE otherwise), max_positions being max_blocks*block_size,
+ * or window + sinks when that is smaller and window > 0.  head_dim a multiple
+ * of 8 up to 256.  Allocates nothing; graph-capturable (lengths and tables
+ * are read on the device). */
+int b2_paged_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv* kv, void* out, float* scores, int batch,
+                        int num_q_heads, int num_kv_heads, int head_dim, int window, int sinks, b2_workspace* ws,
+                        void* stream);
+size_t b2_paged_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                                       int64_t max_positions, int scored);
+
+/* Shrinks every sequence longer than `budget` to `budget` positions, chosen
+ * per kv head: the first `sinks`, the last `recent` and, of those between,
+ * the ones with the largest scores (equal scores: the lowest position; NaN
+ * counts as the largest).  sinks + recent <= budget.  The kept positions' K
+ * and V rows and scores move, order kept, to positions 0 .. n-1 with n =
+ * min(seq_lens[b], budget): of the same blocks when dst_tables is NULL, else
+ * of the blocks of dst_tables (device int32 [batch][max_dst_blocks],
+ * max_dst_blocks*block_size >= budget, disjoint from the source blocks), which
+ * leaves the source as it was (blocks shared with other sequences, say).
+ * Sequences within the budget keep everything (copied when dst_tables is
+ * given).  kept (int32 [batch][num_kv_heads][budget]) receives the kept
+ * positions in order, -1 past n; new_lens (int32 [batch], may be
+ * kv->seq_lens) receives n.  K rows keep the position encoding they were
+ * written with.  Entries of either table outside [0, num_blocks) are neither
+ * read nor written through.  In place, sequences must not share blocks.
+ * Allocates nothing. */
+int b2_paged_kv_evict(const b2_paged_kv* kv, float* scores, const int* dst_tables, int max_dst_blocks, int batch,
+                      int num_kv_heads, int head_dim, int budget, int sinks, int recent, int* kept, int* new_lens,
+                      void* stream);
 
 /* ---------------------------------------------------------------------------
  * Sampler  (replaces engine::SamplerGPU, src/runtime/sampler.h:10-65)

@@ -31,6 +31,12 @@ class KVView(C.Structure):
     _fields_ = [("data", vp), ("stride_b", i64), ("stride_h", i64), ("stride_s", i64), ("stride_d", i64)]
 
 
+class PagedKVStruct(C.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("block_tables", vp), ("seq_lens", vp), ("stride_block", i64),
+                ("stride_slot", i64), ("stride_head", i64), ("num_blocks", i32), ("block_size", i32),
+                ("max_blocks", i32), ("bf16", i32)]
+
+
 class TokenizerInfo(C.Structure):
     _fields_ = [("vocab_size", i64), ("n_ids", i64), ("n_merges", i64), ("pre_tokenizer", i32), ("nfc", i32),
                 ("ignore_merges", i32), ("chat_format", i32), ("bos_id", i32), ("eos_id", i32), ("n_stop", i32),
@@ -71,6 +77,10 @@ _SIGS = {
     "b2_workspace_bytes": (C.c_size_t, [vp]),
     "b2_flash_prefill_workspace_bytes": (C.c_size_t, [i64, i32, i32, i32, i32]),
     "b2_flash_prefill_gqa_ws": (i32, [vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, f32, i64, vp, vp]),
+    "b2_window_prefill_gqa": (i32, [KVView, KVView, KVView, vp, vp, i64, i64, i32, i32, i32, i32, i64, i64, i32, vp]),
+    "b2_paged_decode_gqa": (i32, [vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
+    "b2_paged_decode_workspace_bytes": (C.c_size_t, [i32, i32, i32, i32, i64, i32]),
+    "b2_paged_kv_evict": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
     "b2_swiglu": (i32, [vp, vp, vp, i64, vp]),
     "b2_matmul_transB": (i32, [vp, vp, vp, i32, i32, i32, vp]),
     "b2_matmul_transB_f32": (i32, [vp, vp, vp, i32, i32, i32, vp]),
@@ -220,6 +230,137 @@ def decode_gqa_split(q, kview: KVView, vview: KVView, seq_lens, out, B, nq, nkv,
     cap = 0 if split_buffer is None else split_buffer.numel()
     call("b2_decode_gqa_split", ptr(q), kview, vview, ptr(seq_lens), ptr(out), B, nq, nkv, D, max_seq_len,
          ptr(split_buffer), cap, stream_ptr(stream))
+
+
+class Workspace:
+    """Device scratch lent to the entry points that take one (b2_workspace_*)."""
+
+    def __init__(self, nbytes: int):
+        h = vp()
+        call("b2_workspace_create", max(1, int(nbytes)), C.byref(h))
+        self.h = h
+
+    @property
+    def nbytes(self) -> int:
+        return int(lib().b2_workspace_bytes(self.h))
+
+    def close(self):
+        if getattr(self, "h", None):
+            lib().b2_workspace_destroy(self.h)
+            self.h = None
+
+    __del__ = close
+
+
+# ---------------------------------------------------------------------------
+# bounded-cache attention (b2_window_prefill_gqa, b2_paged_decode_gqa,
+# b2_paged_kv_evict)
+# ---------------------------------------------------------------------------
+
+def _is_bf16(t) -> int:
+    import torch
+    if t.dtype == torch.bfloat16:
+        return 1
+    if t.dtype == torch.float16:
+        return 0
+    raise ValueError(f"expected a float16 or bfloat16 tensor, got {t.dtype}")
+
+
+def _need(t, name, dtype, shape):
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+
+
+def window_prefill_gqa(q, k, v, out, window=0, sinks=0, seq_lens=None, stream=None):
+    """Causal GQA attention of a chunk of query tokens in which a query sees
+    the last `window` positions (0: all) and the first `sinks` ones.  q
+    [B, S, nq, D], k and v [B, T, nkv, D] with T >= S: the queries are the last
+    S of the T positions; any strides with contiguous rows.  out [B, S, nq, D]
+    contiguous.  seq_lens (int32 [B], optional): tokens of each sequence;
+    rows past it come out zero."""
+    import torch
+    B, S, nq, D = q.shape
+    T, nkv = k.shape[1], k.shape[2]
+    bf = _is_bf16(q)
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or T < S or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+    _need(out, "out", q.dtype, (B, S, nq, D))
+    if seq_lens is not None:
+        _need(seq_lens, "seq_lens", torch.int32, (B,))
+    views = [KVView(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1), t.stride(3)) for t in (q, k, v)]
+    call("b2_window_prefill_gqa", *views, out.data_ptr(), ptr(seq_lens), S, T - S, nq, nkv, D, B, window, sinks, bf,
+         stream_ptr(stream))
+    return out
+
+
+class PagedKV:
+    """One layer's paged K/V cache as the operators take it: k and v pools
+    [num_blocks, block_size, nkv, D] (any strides with contiguous rows, the
+    same for both: a pool kept [num_blocks, nkv, block_size, D] is passed
+    through .transpose(1, 2)), block_tables int32 [B, max_blocks] and
+    seq_lens int32 [B].  Holds references to the tensors, copies nothing."""
+
+    def __init__(self, k, v, block_tables, seq_lens):
+        import torch
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
+            raise ValueError("k and v must be [num_blocks, block_size, nkv, D] of one type with the same strides and "
+                             "contiguous rows")
+        if block_tables.dim() != 2:
+            raise ValueError("block_tables must be [batch, max_blocks]")
+        B, mb = block_tables.shape
+        _need(block_tables, "block_tables", torch.int32, (B, mb))
+        _need(seq_lens, "seq_lens", torch.int32, (B,))
+        self.k, self.v, self.block_tables, self.seq_lens = k, v, block_tables, seq_lens
+        self.batch, self.nkv, self.head_dim = B, k.shape[2], k.shape[3]
+        self.num_blocks, self.block_size = k.shape[0], k.shape[1]
+        self.c = PagedKVStruct(k.data_ptr(), v.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), k.stride(0),
+                               k.stride(1), k.stride(2), k.shape[0], k.shape[1], mb, _is_bf16(k))
+        self.ref = C.addressof(self.c)
+
+    def check_scores(self, scores):
+        import torch
+        _need(scores, "scores", torch.float32, (self.num_blocks, self.nkv, self.block_size))
+
+
+def paged_decode_workspace_bytes(batch, nq, nkv, head_dim, max_positions, scored=False) -> int:
+    return int(lib().b2_paged_decode_workspace_bytes(batch, nq, nkv, head_dim, max_positions, int(scored)))
+
+
+def paged_decode_gqa(q, kv: PagedKV, out, window=0, sinks=0, scores=None, ws: Workspace | None = None, stream=None):
+    """Attention of the newest token of each sequence over its paged rows.  q
+    [B, nq, D] (rows of heads contiguous), out [B, nq, D] contiguous; scores
+    (float32 [num_blocks, nkv, block_size], optional) accumulates every
+    visible position's weight and needs a workspace."""
+    B, nq, D = q.shape
+    if B != kv.batch or D != kv.head_dim or q.dtype != kv.k.dtype or q.stride(2) != 1 or q.stride(1) != D:
+        raise ValueError(f"q {q.dtype} {tuple(q.shape)} does not fit the cache ({kv.batch} sequences, "
+                         f"head_dim {kv.head_dim}, {kv.k.dtype})")
+    _need(out, "out", q.dtype, (B, nq, D))
+    if scores is not None:
+        kv.check_scores(scores)
+    call("b2_paged_decode_gqa", q.data_ptr(), q.stride(0), kv.ref, out.data_ptr(), ptr(scores), B, nq, kv.nkv, D,
+         window, sinks, ws.h if ws is not None else None, stream_ptr(stream))
+    return out
+
+
+def paged_kv_evict(kv: PagedKV, scores, budget, kept, new_lens, sinks=0, recent=0, dst_tables=None, stream=None):
+    """Keep `budget` positions of every longer sequence, per kv head: the
+    first `sinks`, the last `recent`, and the best scores between them (ties
+    to the lowest position).  Rows and scores move, in order, to positions
+    0.. of the same blocks, or of the blocks of dst_tables (int32 [B,
+    max_dst_blocks]).  kept int32 [B, nkv, budget] (-1 past a sequence's new
+    length), new_lens int32 [B] (may be kv.seq_lens)."""
+    import torch
+    kv.check_scores(scores)
+    _need(kept, "kept", torch.int32, (kv.batch, kv.nkv, budget))
+    _need(new_lens, "new_lens", torch.int32, (kv.batch,))
+    mdb = 0
+    if dst_tables is not None:
+        mdb = dst_tables.shape[1]
+        _need(dst_tables, "dst_tables", torch.int32, (kv.batch, mdb))
+    call("b2_paged_kv_evict", kv.ref, scores.data_ptr(), ptr(dst_tables), mdb, kv.batch, kv.nkv, kv.head_dim, budget,
+         sinks, recent, kept.data_ptr(), new_lens.data_ptr(), stream_ptr(stream))
 
 
 class Sampler:

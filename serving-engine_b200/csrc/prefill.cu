@@ -38,6 +38,7 @@
 
 #include "prefill.cuh"
 #include "tc.cuh"
+#include "workspace.cuh"
 
 namespace b2 {
 int causal_attention_rows(const __half* q, const __half* k, const __half* v, __half* out, int64_t S, int nq,
@@ -827,21 +828,23 @@ extern "C" int b2_flash_prefill_gqa_ex(const void* q, const void* k, const void*
     return b2_flash_prefill_gqa_ws(q, k, v, out, S, nq, nkv, D, batch, bf16, rope_theta, start_pos, nullptr, stream);
 }
 
-struct b2_workspace {
-    void* ptr = nullptr;
-    size_t bytes = 0;
-};
-
 extern "C" int b2_workspace_create(size_t bytes, b2_workspace** out) {
     B2_REQUIRE(out && bytes > 0);
     *out = nullptr;
     b2_workspace* w = new (std::nothrow) b2_workspace();
     if (!w) return B2_ERR_INVALID;
-    const cudaError_t e = cudaMalloc(&w->ptr, bytes);
+    void* c = nullptr;
+    cudaError_t e = cudaMalloc(&w->ptr, bytes);
+    if (e == cudaSuccess) e = cudaMalloc(&c, kWsCounters * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(c, 0, kWsCounters * sizeof(int));
+    if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
     if (e != cudaSuccess) {
+        cudaFree(c);
+        cudaFree(w->ptr);
         delete w;
         return (int)e;
     }
+    w->counters = static_cast<int*>(c);
     w->bytes = bytes;
     *out = w;
     return B2_OK;
@@ -849,6 +852,7 @@ extern "C" int b2_workspace_create(size_t bytes, b2_workspace** out) {
 
 extern "C" int b2_workspace_destroy(b2_workspace* ws) {
     if (!ws) return B2_OK;
+    cudaFree(ws->counters);
     cudaFree(ws->ptr);
     delete ws;
     return B2_OK;
