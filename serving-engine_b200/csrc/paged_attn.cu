@@ -4,6 +4,34 @@
 //
 //   out = sum_i p_i v_i,  p = softmax over the visible positions of
 //   q . k_i / sqrt(D);  score_i += sum over the group's heads of p_i
+//
+// The work is one read of the visible K and V rows: 4 D bytes per (position,
+// kv head) for up to 4 D G flops (G heads of the group), so HBM bounds it.
+//
+// Split.  A (sequence, kv head, group of up to 16 heads) is a segment of
+// units of U positions; all segments' units, end to end, are cut into equal
+// ranges, one per CTA of a grid that is resident at once (stream-K).  Every SM
+// so streams the same bytes whatever the batch, the heads and the lengths.  A
+// CTA whose range covers a segment writes its outputs; a segment cut between
+// CTAs leaves a partial (max, sum, unnormalised output) per piece in the
+// workspace, and the CTA that arrives last at the segment's counter adds the
+// pieces in order (same bits whoever is last).
+//
+// Inside a CTA each of 4 warps streams its own quarter of every unit through
+// its own ring of shared-memory stages (cp.async, no barrier between warps),
+// with its own running max and sum; the warps meet once per segment.  Rows
+// come through the block table 16 bytes per lane, rows that are not visible
+// are filled with zeros and never read.  Products on mma.sync m16n8k16 (heads
+// as M, fp32 accumulation): the 2 x 16 x D MACs per position are far below its
+// rate at this memory speed, and it takes any row addresses, where tensor-map
+// copies would need one map per layout and whole swizzle atoms per block.  P
+// is split into a 16-bit value and a 16-bit remainder, so that rounding the
+// weights costs no accuracy next to the output's own rounding.
+//
+// Weights (scores): the logits go to the workspace as they are computed (G
+// floats beside 4 D bytes of row), and a second kernel turns them into
+// weights with the joined max and sum: G/(2 D) more traffic than the rows,
+// instead of reading K again.
 #include <cmath>
 
 #include "paged.cuh"
@@ -11,106 +39,598 @@
 
 namespace b2 {
 
+constexpr int kPgWarps = 4;
+constexpr int kPgThreads = kPgWarps * 32;
+constexpr int kPgStages = 3;
+constexpr int kPgMinUnits = 4;  // a range is at least this many units
+
 struct PagedArgs {
     const void* q;
     int64_t ldq;
     b2_paged_kv kv;
     void* out;
     float* scores;
-    int nq, nkv, D, window, sinks;
+    int batch, nq, nkv, D, group, hg, gs, window, sinks;
     float scale_log2;
-    float2* stats;  // [batch][nq]: (max, sum) of the softmax in the log2 domain
+    float* parts;   // [2 * grid][gs][D], unnormalised partial outputs
+    float2* pml;    // [2 * grid][gs], their (max, sum)
+    int* counters;  // [grid], null: segments are not cut
+    float2* stats;  // [batch][nq], the joined (max, sum); scores only
+    float* logits;  // [batch][nq][cap]; scores only
+    int cap;
 };
 
+// DP: head dim rounded up to 64, 128 or 256.  GH: more than 8 heads a segment.
+template <int DP, bool GH>
+struct PagedCfg {
+    static constexpr int TP = DP == 64 ? 32 : 16;     // positions per warp and unit
+    static constexpr int U = kPgWarps * TP;           // positions per unit
+    static constexpr int ROW = DP * 2;                // bytes of a row
+    static constexpr int CH = DP / 8;                 // 16-byte chunks of a row
+    static constexpr int STAGE = 2 * TP * ROW;        // K and V rows of a warp's tile
+    static constexpr int G = GH ? 16 : 8;             // rows kept of the 16 of an MMA
+    static constexpr int NB = GH ? 1 : 2;             // buffers of the warps' meeting
+    static constexpr int LDO = DP + 4;
+    static constexpr int OFF_O = kPgWarps * kPgStages * STAGE;
+    static constexpr int BYTES = OFF_O + NB * G * LDO * 4;
+    static constexpr int CTAS = DP == 256 ? 1 : 2;    // per SM
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+// 16 bytes, or 16 zero bytes without reading src
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
 template <bool BF16>
-__device__ __forceinline__ float ld16f(const void* p, int64_t i) {
-    if constexpr (BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-    return __half2float(static_cast<const __half*>(p)[i]);
+__device__ __forceinline__ void mma16816(float& c0, float& c1, float& c2, float& c3, uint32_t a0, uint32_t a1,
+                                         uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c0), "+f"(c1), "+f"(c2), "+f"(c3)
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c0), "+f"(c1), "+f"(c2), "+f"(c3)
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The positions that the newest token of a sequence of L sees, numbered 0 ..
-// n-1: the first s0, then those from lo on.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    if constexpr (BF16) {
+        __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&h);
+    } else {
+        return f2_to_h2(a, b);
+    }
+}
+// (a, b) as 16-bit values and what the rounding left, again in 16 bits
+template <bool BF16>
+__device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack16<BF16>(a, b);
+    float2 f;
+    if constexpr (BF16) {
+        f.x = __uint_as_float(hi << 16);
+        f.y = __uint_as_float(hi & 0xffff0000u);
+    } else {
+        f = h2_to_f2(hi);
+    }
+    lo = pack16<BF16>(a - f.x, b - f.y);
+}
+template <bool BF16>
+__device__ __forceinline__ void store16(void* p, int64_t i, float v) {
+    if constexpr (BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// What the newest token of a sequence of L tokens sees, in units of U
+// positions: ns units over the first s0 positions, then units from w0 (lo
+// rounded down to 16) on, of which positions lo .. L-1 count.  A sequence
+// that sees nothing still has one unit, which writes its zeros.
+template <int U>
 struct Seen {
-    int L, lo, s0, n;
-    __device__ Seen(const PagedArgs& a, int b) {
+    int L, lo, s0, ns, w0, n;
+    __device__ __forceinline__ void of(const PagedArgs& a, int b) {
         L = paged_len(a.kv, b);
         lo = a.window > 0 ? max(0, L - a.window) : 0;
         s0 = min(a.sinks, lo);
-        n = s0 + L - lo;
+        ns = (s0 + U - 1) / U;
+        w0 = lo & ~15;
+        n = max(1, ns + (L - w0 + U - 1) / U);
     }
-    __device__ int pos(int i) const { return i < s0 ? i : i - s0 + lo; }
+    __device__ __forceinline__ int base(int u) const { return u < ns ? u * U : w0 + (u - ns) * U; }
+    __device__ __forceinline__ bool sees(int u, int pos) const { return u < ns ? pos < s0 : pos >= lo && pos < L; }
 };
 
-__device__ __forceinline__ int64_t paged_row(const b2_paged_kv& kv, int b, int kvh, int pos) {
-    const int blk = kv.block_tables[(int64_t)b * kv.max_blocks + pos / kv.block_size];
-    if (blk < 0 || blk >= kv.num_blocks) return -1;
-    return blk * kv.stride_block + (pos % kv.block_size) * kv.stride_slot + kvh * kv.stride_head;
+// A place in the list of all units: segment hh (kv head x head group) of
+// sequence b, unit u of it.
+template <int U>
+struct Place {
+    int b, hh, u;
+    Seen<U> s;
+    __device__ __forceinline__ void next(const PagedArgs& a) {
+        if (++u < s.n) return;
+        u = 0;
+        if (++hh < a.nkv * a.hg) return;
+        hh = 0;
+        if (++b < a.batch) s.of(a, b);
+    }
+};
+
+template <int DP, bool GH, bool BF16>
+__global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn_kernel(const PagedArgs a) {
+    using C = PagedCfg<DP, GH>;
+    constexpr int U = C::U, TP = C::TP, G = C::G;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int s_scan[kPgWarps];
+    __shared__ int s_b, s_before, s_last;
+    __shared__ uint32_t s_there[kPgWarps][kPgStages];
+    __shared__ float s_m[kPgWarps][16], s_l[kPgWarps][16];
+    __shared__ float2 s_ml[16];
+    float* s_o = reinterpret_cast<float*>(smem + C::OFF_O);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int c = blockIdx.x;
+    const int heads = a.nkv * a.hg;
+
+    // chunks of a row past D are never copied: they stay zero
+    if (a.D < DP)
+        for (int i = tid; i < C::OFF_O / 16; i += kPgThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    griddep_wait();
+
+    // ---- this CTA's range of units, and the place where it starts
+    const int per = (a.batch + kPgThreads - 1) / kPgThreads;
+    const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) {
+        Seen<U> s;
+        s.of(a, b);
+        mine += s.n * heads;
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(~0u, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < kPgWarps; ++w) {
+        if (w < warp) incl += s_scan[w];
+        total += s_scan[w];
+    }
+    const int upc = max(kPgMinUnits, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    int r0 = c * upc, r1 = min(total, r0 + upc);
+    if (c >= (total + upc - 1) / upc) return;
+    {
+        int before = incl - mine;
+        if (r0 >= before && r0 < incl) {  // one thread
+            int b = b0;
+            for (;; ++b) {
+                Seen<U> s;
+                s.of(a, b);
+                if (r0 < before + s.n * heads) break;
+                before += s.n * heads;
+            }
+            s_b = b;
+            s_before = before;
+        }
+    }
+    __syncthreads();
+    Place<U> at;
+    at.b = s_b;
+    at.s.of(a, at.b);
+    at.hh = (r0 - s_before) / at.s.n;
+    at.u = (r0 - s_before) - at.hh * at.s.n;
+    if (!a.counters) {  // whole segments only: those that begin in the range
+        if (at.u > 0) {
+            r0 += at.s.n - at.u;
+            at.u = at.s.n - 1;
+            at.next(a);
+        }
+        if (r0 >= r1) return;
+        // the end moves to the end of the segment that holds unit r1 - 1
+        Place<U> e = at;
+        int r = r0;
+        while (r < r1) {
+            r += e.s.n;
+            e.u = e.s.n - 1;
+            e.next(a);
+        }
+        r1 = r;
+    }
+
+    // ---- producer: rows of the unit at `pp` into a stage
+    Place<U> pp = at;
+    int pr = r0, pid = -1;
+    auto fetch_id = [&]() {  // block of row (lane % TP) of the unit, -1 where it is not visible
+        pid = -1;
+        if (pr < r1) {
+            const int pos = pp.s.base(pp.u) + warp * TP + (lane & (TP - 1));
+            if (pp.s.sees(pp.u, pos)) pid = a.kv.block_tables[(int64_t)pp.b * a.kv.max_blocks + (unsigned)pos / (unsigned)a.kv.block_size];
+        }
+    };
+    const uint32_t ring = smem_addr(smem) + warp * kPgStages * C::STAGE;
+    const int chunk = lane % C::CH;
+    auto issue = [&](int stage) {
+        if (pr < r1) {
+            const int pos = pp.s.base(pp.u) + warp * TP + (lane & (TP - 1));
+            const bool there = (unsigned)pid < (unsigned)a.kv.num_blocks;
+            const int64_t off = (int64_t)pid * a.kv.stride_block + (int64_t)((unsigned)pos % (unsigned)a.kv.block_size) * a.kv.stride_slot +
+                                (pp.hh / a.hg) * a.kv.stride_head;
+            const uint32_t mask = __ballot_sync(~0u, there);
+            if (lane == 0) s_there[warp][stage] = mask;
+            const uint32_t st = ring + stage * C::STAGE;
+            const uint16_t *K = static_cast<const uint16_t*>(a.kv.k), *V = static_cast<const uint16_t*>(a.kv.v);
+#pragma unroll
+            for (int i = 0; i < TP * C::CH / 32; ++i) {
+                const int r = lane / C::CH + i * (32 / C::CH);
+                const int64_t ro = __shfl_sync(~0u, off, r);
+                const bool ok = (mask >> r) & 1;
+                if (chunk * 8 < a.D) {
+                    const uint32_t d = st + r * C::ROW + ((chunk ^ (r & 7)) << 4);
+                    const int64_t so = ok ? ro + chunk * 8 : 0;
+                    cp16(d, K + so, ok);
+                    cp16(d + TP * C::ROW, V + so, ok);
+                }
+            }
+            ++pr;
+            pp.next(a);
+            fetch_id();
+        }
+        cp_commit();
+    };
+    fetch_id();
+#pragma unroll
+    for (int s = 0; s < kPgStages - 1; ++s) issue(s);
+
+    // ---- consumer
+    uint32_t qa[DP / 16][GH ? 4 : 2];
+    float o[DP / 8][GH ? 4 : 2], m0, m1, l0, l1;
+    auto start = [&]() {  // a new segment (or the rest of one): its queries, nothing summed yet
+        const int kvh = at.hh / a.hg, h0 = kvh * a.group + (at.hh - kvh * a.hg) * a.gs;
+        const int nh = min(a.gs, (kvh + 1) * a.group - h0);
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + at.b * a.ldq + (int64_t)h0 * a.D;
+        const int r = lane >> 2, k = (lane & 3) * 2;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+            for (int e = 0; e < (GH ? 4 : 2); ++e) {
+                const int row = GH ? r + (e & 1) * 8 : r, col = kk * 16 + k + (GH ? e >> 1 : e) * 8;
+                qa[kk][e] = row < nh && col < a.D ? *reinterpret_cast<const uint32_t*>(q + (int64_t)row * a.D + col) : 0u;
+            }
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < (GH ? 4 : 2); ++e) o[n][e] = 0.f;
+        m0 = m1 = -INFINITY;
+        l0 = l1 = 0.f;
+    };
+
+    start();
+    int piece0 = r0;  // where the current piece of a segment began
+    for (int r = r0; r < r1; ++r) {
+        const int stage = (r - r0) % kPgStages;
+        cp_wait<kPgStages - 2>();
+        __syncwarp();
+        const uint32_t there = s_there[warp][stage];
+        const uint32_t st = ring + stage * C::STAGE;
+        if (there) {
+#pragma unroll
+            for (int t = 0; t < TP / 16; ++t) {
+                // S = Q K^T: 16 heads x 16 positions
+                float s[2][4] = {};
+                const uint32_t kb = st + t * 16 * C::ROW, vb = kb + TP * C::ROW;
+                const int mi = lane >> 3, mr = lane & 7;
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    uint32_t kf[4];
+                    ldsm4(kf, kb + ((mi >> 1) * 8 + mr) * C::ROW + (((kk * 2 + (mi & 1)) ^ mr) << 4));
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        if constexpr (GH)
+                            mma16816<BF16>(s[n][0], s[n][1], s[n][2], s[n][3], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3],
+                                           kf[2 * n], kf[2 * n + 1]);
+                        else
+                            mma16816<BF16>(s[n][0], s[n][1], s[n][2], s[n][3], qa[kk][0], 0u, qa[kk][1], 0u, kf[2 * n],
+                                           kf[2 * n + 1]);
+                    }
+                }
+                const int col = (lane & 3) * 2;
+                const uint32_t tm = there >> (t * 16);
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[n][e] = (tm >> (n * 8 + col + (e & 1))) & 1 ? s[n][e] * a.scale_log2 : -INFINITY;
+                if (a.logits) {
+                    const int kvh = at.hh / a.hg, h0 = kvh * a.group + (at.hh - kvh * a.hg) * a.gs;
+                    const int nh = min(a.gs, (kvh + 1) * a.group - h0);
+                    float* lg = a.logits + ((int64_t)at.b * a.nq + h0 + (lane >> 2)) * a.cap + at.u * U + warp * TP +
+                                t * 16 + col;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        if ((lane >> 2) < nh) *reinterpret_cast<float2*>(lg + n * 8) = make_float2(s[n][0], s[n][1]);
+                        if (GH && (lane >> 2) + 8 < nh)
+                            *reinterpret_cast<float2*>(lg + 8 * (int64_t)a.cap + n * 8) = make_float2(s[n][2], s[n][3]);
+                    }
+                }
+                // running max of the rows; finite, so that exp2(-inf - m) is 0
+                float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+                t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, 1));
+                t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, 2));
+                const float n0 = fmaxf(fmaxf(m0, t0), -1e30f);
+                float t1 = 0.f, n1 = 0.f;
+                bool moved = n0 > m0;
+                if constexpr (GH) {
+                    t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+                    t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, 1));
+                    t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, 2));
+                    n1 = fmaxf(fmaxf(m1, t1), -1e30f);
+                    moved |= n1 > m1;
+                }
+                if (__any_sync(~0u, moved)) {
+                    const float a0 = ex2(m0 - n0), a1 = GH ? ex2(m1 - n1) : 0.f;
+                    l0 *= a0;
+                    l1 *= a1;
+#pragma unroll
+                    for (int n = 0; n < DP / 8; ++n) {
+                        o[n][0] *= a0;
+                        o[n][1] *= a0;
+                        if constexpr (GH) {
+                            o[n][2] *= a1;
+                            o[n][3] *= a1;
+                        }
+                    }
+                    m0 = n0;
+                    m1 = n1;
+                }
+                uint32_t ph[4] = {}, pl[4] = {};
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const float p0 = ex2(s[n][0] - m0), p1 = ex2(s[n][1] - m0);
+                    l0 += p0 + p1;
+                    split16<BF16>(p0, p1, ph[2 * n], pl[2 * n]);
+                    if constexpr (GH) {
+                        const float p2 = ex2(s[n][2] - m1), p3 = ex2(s[n][3] - m1);
+                        l1 += p2 + p3;
+                        split16<BF16>(p2, p3, ph[2 * n + 1], pl[2 * n + 1]);
+                    }
+                }
+                // O += P V, the weights as value + remainder
+#pragma unroll
+                for (int n = 0; n < DP / 16; ++n) {
+                    uint32_t vf[4];
+                    ldsm4t(vf, vb + ((mi & 1) * 8 + mr) * C::ROW + (((n * 2 + (mi >> 1)) ^ mr) << 4));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float* d = o[2 * n + h];
+                        if constexpr (GH) {
+                            mma16816<BF16>(d[0], d[1], d[2], d[3], ph[0], ph[1], ph[2], ph[3], vf[2 * h], vf[2 * h + 1]);
+                            mma16816<BF16>(d[0], d[1], d[2], d[3], pl[0], pl[1], pl[2], pl[3], vf[2 * h], vf[2 * h + 1]);
+                        } else {
+                            float z2 = 0.f, z3 = 0.f;
+                            mma16816<BF16>(d[0], d[1], z2, z3, ph[0], 0u, ph[2], 0u, vf[2 * h], vf[2 * h + 1]);
+                            mma16816<BF16>(d[0], d[1], z2, z3, pl[0], 0u, pl[2], 0u, vf[2 * h], vf[2 * h + 1]);
+                        }
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        issue((r - r0 + kPgStages - 1) % kPgStages);
+
+        const bool done = at.u == at.s.n - 1;
+        if (done || r == r1 - 1) {
+            // ---- the warps meet: max and sum of each row, then the outputs, in warp order
+            l0 += __shfl_xor_sync(~0u, l0, 1);
+            l0 += __shfl_xor_sync(~0u, l0, 2);
+            l1 += __shfl_xor_sync(~0u, l1, 1);
+            l1 += __shfl_xor_sync(~0u, l1, 2);
+            if ((lane & 3) == 0) {
+                s_m[warp][lane >> 2] = m0;
+                s_l[warp][lane >> 2] = l0;
+                if (GH) {
+                    s_m[warp][(lane >> 2) + 8] = m1;
+                    s_l[warp][(lane >> 2) + 8] = l1;
+                }
+            }
+            __syncthreads();
+            float w[GH ? 2 : 1];
+#pragma unroll
+            for (int e = 0; e < (GH ? 2 : 1); ++e) {
+                const int row = (lane >> 2) + 8 * e;
+                float M = -1e30f;
+#pragma unroll
+                for (int v = 0; v < kPgWarps; ++v) M = fmaxf(M, s_m[v][row]);
+                w[e] = ex2(s_m[warp][row] - M);
+                if (warp == 0 && (lane & 3) == 0) {
+                    float Ls = 0.f;
+#pragma unroll
+                    for (int v = 0; v < kPgWarps; ++v) Ls = fmaf(s_l[v][row], ex2(s_m[v][row] - M), Ls);
+                    s_ml[row] = make_float2(M, Ls);
+                }
+            }
+#pragma unroll 1
+            for (int turn = 0; turn < kPgWarps / C::NB; ++turn) {
+                if (warp / C::NB == turn) {
+                    float* buf = s_o + (warp % C::NB) * G * C::LDO;
+#pragma unroll
+                    for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+                        for (int e = 0; e < (GH ? 2 : 1); ++e) {
+                            float2* d = reinterpret_cast<float2*>(buf + ((lane >> 2) + 8 * e) * C::LDO + n * 8 + (lane & 3) * 2);
+                            float2 v = turn ? *d : make_float2(0.f, 0.f);
+                            v.x = fmaf(o[n][2 * e], w[e], v.x);
+                            v.y = fmaf(o[n][2 * e + 1], w[e], v.y);
+                            *d = v;
+                        }
+                }
+                __syncthreads();
+            }
+            const int kvh = at.hh / a.hg, h0 = kvh * a.group + (at.hh - kvh * a.hg) * a.gs;
+            const int nh = min(a.gs, (kvh + 1) * a.group - h0);
+            auto sum = [&](int row, int d) {
+                float v = s_o[row * C::LDO + d];
+                if (C::NB == 2) v += s_o[(G + row) * C::LDO + d];
+                return v;
+            };
+            const int64_t oat = ((int64_t)at.b * a.nq + h0) * a.D;
+            const int seg0 = r - at.u;  // first unit of the segment
+            if (done && piece0 == seg0) {
+                for (int i = tid; i < nh * a.D; i += kPgThreads) {
+                    const int row = i / a.D, d = i - row * a.D;
+                    const float Ls = s_ml[row].y;
+                    store16<BF16>(a.out, oat + i, Ls > 0.f ? sum(row, d) / Ls : 0.f);
+                }
+                if (a.stats && tid < nh) a.stats[(int64_t)at.b * a.nq + h0 + tid] = s_ml[tid];
+            } else {
+                const int slot = 2 * c + (piece0 == seg0 ? 1 : 0);
+                float* part = a.parts + (int64_t)slot * a.gs * a.D;
+                for (int i = tid; i < nh * a.D; i += kPgThreads) part[i] = sum(i / a.D, i % a.D);
+                if (tid < nh) a.pml[(int64_t)slot * a.gs + tid] = s_ml[tid];
+                __threadfence();
+                __syncthreads();
+                const int cf = seg0 / upc, pieces = (seg0 + at.s.n - 1) / upc - cf + 1;
+                if (tid == 0) s_last = atomicAdd(a.counters + cf, 1) == pieces - 1;
+                __syncthreads();
+                if (s_last) {
+                    // ---- last of the segment's CTAs: its pieces in order
+                    __threadfence();
+                    if (tid == 0) a.counters[cf] = 0;
+                    for (int row = warp; row < nh; row += kPgWarps) {
+                        float M = -1e30f, Ls = 0.f;
+                        for (int p = lane; p < pieces; p += 32)
+                            M = fmaxf(M, __ldcg(&a.pml[(int64_t)(2 * (cf + p) + (p == 0)) * a.gs + row].x));
+                        M = warp_max(M);
+                        for (int p = lane; p < pieces; p += 32) {
+                            const float2 ml = __ldcg(&a.pml[(int64_t)(2 * (cf + p) + (p == 0)) * a.gs + row]);
+                            Ls = fmaf(ml.y, ex2(ml.x - M), Ls);
+                        }
+                        Ls = warp_sum(Ls);
+                        if (lane == 0) s_ml[row] = make_float2(M, Ls);
+                    }
+                    __syncthreads();
+                    for (int i = tid; i < nh * a.D; i += kPgThreads) {
+                        const int row = i / a.D;
+                        const float2 ml = s_ml[row];
+                        float v = 0.f;
+#pragma unroll 4
+                        for (int p = 0; p < pieces; ++p) {
+                            const int64_t sl = (int64_t)(2 * (cf + p) + (p == 0)) * a.gs;
+                            v = fmaf(__ldcg(&a.parts[sl * a.D + i]), ex2(__ldcg(&a.pml[sl + row].x) - ml.x), v);
+                        }
+                        store16<BF16>(a.out, oat + i, ml.y > 0.f ? v / ml.y : 0.f);
+                    }
+                    if (a.stats && tid < nh) a.stats[(int64_t)at.b * a.nq + h0 + tid] = s_ml[tid];
+                }
+            }
+            __syncthreads();
+            at.next(a);
+            piece0 = r + 1;
+            if (r + 1 < r1) start();
+        } else {
+            at.next(a);
+        }
+    }
 }
 
-// One warp per (sequence, query head), lane l holding elements l, l + 32, ..
-template <bool BF16>
-__global__ void __launch_bounds__(32) paged_rows_kernel(const PagedArgs a) {
+// One thread per stored logit column: the weights its position gets from the
+// group's heads, in head order, onto its score.
+template <int U>
+__global__ void __launch_bounds__(256) paged_scores_kernel(const PagedArgs a) {
+    extern __shared__ float2 s_st[];  // [group] (max, 1 / sum)
     griddep_wait();
-    const int h = blockIdx.x, b = blockIdx.y, kvh = h / (a.nq / a.nkv), lane = threadIdx.x;
-    const Seen seen(a, b);
-    float q[8], o[8], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        q[e] = lane + 32 * e < a.D ? ld16f<BF16>(a.q, b * a.ldq + (int64_t)h * a.D + lane + 32 * e) : 0.f;
-        o[e] = 0.f;
+    const int kvh = blockIdx.y, b = blockIdx.z;
+    Seen<U> s;
+    s.of(a, b);
+    if ((int)(blockIdx.x * blockDim.x) >= s.n * U) return;
+    for (int h = threadIdx.x; h < a.group; h += blockDim.x) {
+        const float2 st = a.stats[(int64_t)b * a.nq + kvh * a.group + h];
+        s_st[h] = make_float2(st.x, st.y > 0.f ? 1.f / st.y : 0.f);
     }
-    for (int i = 0; i < seen.n; ++i) {
-        const int64_t r = paged_row(a.kv, b, kvh, seen.pos(i));
-        if (r < 0) continue;
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (lane + 32 * e < a.D) s = fmaf(q[e], ld16f<BF16>(a.kv.k, r + lane + 32 * e), s);
-        s = warp_sum(s) * a.scale_log2;
-        const float m_new = fmaxf(m, s);
-        const float al = exp2f(m - m_new), p = exp2f(s - m_new);
-        m = m_new;
-        l = fmaf(l, al, p);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (lane + 32 * e < a.D) o[e] = fmaf(o[e], al, p * ld16f<BF16>(a.kv.v, r + lane + 32 * e));
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int64_t at = ((int64_t)b * a.nq + h) * a.D + lane;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        if (lane + 32 * e >= a.D) continue;
-        if constexpr (BF16) static_cast<__nv_bfloat16*>(a.out)[at + 32 * e] = __float2bfloat16_rn(o[e] * inv);
-        else static_cast<__half*>(a.out)[at + 32 * e] = __float2half_rn(o[e] * inv);
-    }
-    if (a.scores && lane == 0) a.stats[(int64_t)b * a.nq + h] = make_float2(m, l);
+    __syncthreads();
+    const int i = blockIdx.x * blockDim.x + threadIdx.x, u = i / U;
+    if (u >= s.n) return;
+    const int pos = s.base(u) + i - u * U;
+    if (!s.sees(u, pos)) return;
+    const int bs = a.kv.block_size, blk = a.kv.block_tables[(int64_t)b * a.kv.max_blocks + pos / bs];
+    if ((unsigned)blk >= (unsigned)a.kv.num_blocks) return;
+    const float* lg = a.logits + ((int64_t)b * a.nq + kvh * a.group) * a.cap + i;
+    float w = 0.f;
+    for (int h = 0; h < a.group; ++h) w = fmaf(ex2(__ldcs(lg + (int64_t)h * a.cap) - s_st[h].x), s_st[h].y, w);
+    float* sc = a.scores + ((int64_t)blk * a.nkv + kvh) * bs + pos % bs;
+    *sc = pos == s.L - 1 ? w : *sc + w;
 }
 
-// One warp per (sequence, kv head, 32nd of the positions): the group's weights
-// of each position, in head order.
-template <bool BF16>
-__global__ void __launch_bounds__(32) paged_rows_scores_kernel(const PagedArgs a) {
-    griddep_wait();
-    const int kvh = blockIdx.x, b = blockIdx.y, g = a.nq / a.nkv, lane = threadIdx.x;
-    const Seen seen(a, b);
-    for (int i = blockIdx.z; i < seen.n; i += gridDim.z) {
-        const int pos = seen.pos(i);
-        const int64_t r = paged_row(a.kv, b, kvh, pos);
-        if (r < 0) continue;
-        float w = 0.f;
-        for (int h = kvh * g; h < (kvh + 1) * g; ++h) {
-            float s = 0.f;
-            for (int d = lane; d < a.D; d += 32)
-                s = fmaf(ld16f<BF16>(a.q, b * a.ldq + (int64_t)h * a.D + d), ld16f<BF16>(a.kv.k, r + d), s);
-            const float2 st = a.stats[(int64_t)b * a.nq + h];
-            w += exp2f(warp_sum(s) * a.scale_log2 - st.x) / st.y;
-        }
-        if (lane == 0) {
-            const int bs = a.kv.block_size, blk = a.kv.block_tables[(int64_t)b * a.kv.max_blocks + pos / bs];
-            float* sc = a.scores + ((int64_t)blk * a.nkv + kvh) * bs + pos % bs;
-            *sc = pos == seen.L - 1 ? w : *sc + w;
-        }
-    }
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+struct PagedSizes {
+    int gs, hg, grid;
+    int64_t cap;
+    size_t parts, pml, stats, logits;  // bytes
+};
+
+// Segments take up to 16 heads; a larger group is cut evenly.
+static PagedSizes paged_sizes(int batch, int nq, int nkv, int D, int64_t max_positions, bool scored) {
+    PagedSizes z = {};
+    const int group = nq / nkv;
+    z.hg = (group + 15) / 16;
+    z.gs = (group + z.hg - 1) / z.hg;
+    z.grid = sm_count() * (D > 128 ? 1 : 2);
+    // whole units of up to 128 positions over the sinks and over the window, whose first may begin 15 early
+    z.cap = (max_positions + 2 * 127 + 15 + 3) & ~int64_t(3);
+    z.parts = (size_t)2 * z.grid * z.gs * D * sizeof(float);
+    z.pml = (size_t)2 * z.grid * z.gs * sizeof(float2);
+    z.stats = scored ? ((size_t)batch * nq * sizeof(float2) + 15) & ~size_t(15) : 0;
+    z.logits = scored ? (size_t)batch * nq * z.cap * sizeof(float) : 0;
+    return z;
+}
+
+template <int DP, bool GH, bool BF16>
+static int paged_launch(const PagedArgs& a, const PagedSizes& z, cudaStream_t s) {
+    using C = PagedCfg<DP, GH>;
+    auto kern = paged_attn_kernel<DP, GH, BF16>;
+    B2_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
+    B2_TRY(launch(kern, dim3(z.grid), dim3(kPgThreads), C::BYTES, s, true, a));
+    if (a.scores)
+        B2_TRY(launch(paged_scores_kernel<C::U>, dim3((unsigned)((a.cap + 255) / 256), a.nkv, a.batch), dim3(256),
+                      a.group * sizeof(float2), s, true, a));
+    return B2_OK;
+}
+
+template <int DP>
+static int paged_dispatch(const PagedArgs& a, const PagedSizes& z, cudaStream_t s) {
+    if (a.kv.bf16) return a.gs > 8 ? paged_launch<DP, true, true>(a, z, s) : paged_launch<DP, false, true>(a, z, s);
+    return a.gs > 8 ? paged_launch<DP, true, false>(a, z, s) : paged_launch<DP, false, false>(a, z, s);
 }
 
 }  // namespace b2
@@ -118,7 +638,8 @@ __global__ void __launch_bounds__(32) paged_rows_scores_kernel(const PagedArgs a
 extern "C" size_t b2_paged_decode_workspace_bytes(int batch, int nq, int nkv, int D, int64_t max_positions,
                                                   int scored) {
     if (batch <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || D <= 0 || max_positions < 0) return 0;
-    return scored ? (size_t)batch * nq * sizeof(float2) : 0;
+    const b2::PagedSizes z = b2::paged_sizes(batch, nq, nkv, D, max_positions, scored != 0);
+    return z.parts + z.pml + z.stats + z.logits;
 }
 
 extern "C" int b2_paged_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv* kv, void* out, float* scores,
@@ -129,28 +650,43 @@ extern "C" int b2_paged_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv
     B2_REQUIRE(q && out && nq > 0 && nkv > 0 && nq % nkv == 0 && window >= 0 && sinks >= 0);
     const int rc = check_paged(kv, nkv, D);
     if (rc != B2_OK) return rc;
-    if (!aligned16(q) || !aligned16(out) || (ldq & 7) || batch > 65535 || nkv > 65535) return B2_ERR_UNSUPPORTED;
+    if (!aligned16(q) || !aligned16(out) || (ldq & 7)) return B2_ERR_UNSUPPORTED;
+    if (scores && !ws) return B2_ERR_WORKSPACE;
+    const int64_t span = (int64_t)kv->max_blocks * kv->block_size;
+    const int64_t most = window > 0 && (int64_t)window + sinks < span ? (int64_t)window + sinks : span;
+    const PagedSizes z = paged_sizes(batch, nq, nkv, D, most, scores != nullptr);
+    // units are counted in 32 bits; the scores' grid has (nkv, batch) as (y, z)
+    if ((int64_t)batch * nkv * z.hg * ((most >> 6) + 4) > (1ll << 31) - 1 ||
+        (scores && (batch > 65535 || nkv > 65535 || nq / nkv > 4096)))
+        return B2_ERR_UNSUPPORTED;
     PagedArgs a = {};
     a.q = q;
     a.ldq = ldq;
     a.kv = *kv;
     a.out = out;
     a.scores = scores;
+    a.batch = batch;
     a.nq = nq;
     a.nkv = nkv;
     a.D = D;
+    a.group = nq / nkv;
+    a.hg = z.hg;
+    a.gs = z.gs;
     a.window = window;
     a.sinks = sinks;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)D);
-    if (scores) {
-        if (!ws || ws->bytes < b2_paged_decode_workspace_bytes(batch, nq, nkv, D, 0, 1)) return B2_ERR_WORKSPACE;
-        a.stats = static_cast<float2*>(ws->ptr);
+    a.cap = (int)z.cap;
+    if (ws) {
+        if (ws->bytes < z.parts + z.pml + z.stats + z.logits || z.grid > kWsCounters) return B2_ERR_WORKSPACE;
+        uint8_t* w = static_cast<uint8_t*>(ws->ptr);
+        a.logits = scores ? reinterpret_cast<float*>(w) : nullptr;
+        a.stats = scores ? reinterpret_cast<float2*>(w + z.logits) : nullptr;
+        a.parts = reinterpret_cast<float*>(w + z.logits + z.stats);
+        a.pml = reinterpret_cast<float2*>(w + z.logits + z.stats + z.parts);
+        a.counters = ws->counters;
     }
     cudaStream_t s = as_stream(stream);
-    B2_TRY(launch(kv->bf16 ? paged_rows_kernel<true> : paged_rows_kernel<false>, dim3(nq, batch), dim3(32), 0, s, true,
-                  a));
-    if (scores)
-        B2_TRY(launch(kv->bf16 ? paged_rows_scores_kernel<true> : paged_rows_scores_kernel<false>, dim3(nkv, batch, 32),
-                      dim3(32), 0, s, true, a));
-    return B2_OK;
+    if (D <= 64) return paged_dispatch<64>(a, z, s);
+    if (D <= 128) return paged_dispatch<128>(a, z, s);
+    return paged_dispatch<256>(a, z, s);
 }
