@@ -14,17 +14,19 @@
 // an order in which the tiles of A, and those of B, are each consecutive.
 //   S_t = Q_t K^T   M = 128 queries, N = keys of the tile, in TMEM
 //   O_t += P_t V    P_t, 16-bit, over S_t's columns in TMEM (A operand)
-// with the order PV_A, S_A', PV_B, S_B' per key tile, so that one tile's
-// products run while the other's softmax does.  Across pairs nothing drains:
-// the next pair's Q, K and V are requested as soon as their buffers are read,
-// and its first S is issued behind the last PV, while the softmax warps still
-// write the outputs.
+// with one MMA issuer per tile, taking turns: PV_A, S_A', PV_B, S_B' per key
+// tile.  The turns keep the two softmaxes half a step apart (without them both
+// run, then both wait: 3.6 k cycles a step with, 4.6 k without), and an issuer
+// does its waiting and addressing while the other's products are queued (one
+// issuer for both tiles: 4.4 k).  Across pairs nothing drains: the next pair's
+// Q, K and V are requested as soon as their buffers are read.
 // Online softmax in the log2 domain, one query row per thread; the reference
 // max moves only when a row's max exceeds it by more than 8, so O is rescaled
-// rarely and P stays below 2^8.  Masks only in tiles that a row of the warp
-// does not see whole; 32-key stretches that no row of the warp sees cost a
-// zero store.  P is rounded to 16 bits for the product (its row sum is not):
-// one more rounding the size of the output's own.
+// rarely and P stays below 2^8.  P is handed over in two halves of 64 keys, so
+// that P V starts while the second half's exponentials run.  Masks only in
+// tiles that a row of the warp does not see whole.  P is rounded to 16 bits
+// for the product (its row sum is not): one more rounding the size of the
+// output's own.  Outputs leave through shared memory as whole 128-byte lines.
 #include <cmath>
 
 #include "tc.cuh"
@@ -113,18 +115,13 @@ struct WinCfg {
     static constexpr int ST = D == 64 ? 4 : 2;        // K and V stages
     static constexpr uint32_t OFF_K = 2 * TILE;
     static constexpr uint32_t OFF_V = OFF_K + ST * TILE;
-    static constexpr uint32_t OFF_BAR = OFF_V + ST * TILE;
+    static constexpr uint32_t OFF_OUT = OFF_V + ST * TILE;  // 32 rows x 64 outputs per softmax warp
+    static constexpr uint32_t OFF_BAR = OFF_OUT + 8 * 4096;
     // above half an SM's shared memory: one CTA, with all 512 TMEM columns, per SM
     static constexpr size_t NEED = OFF_BAR + 256 + 1024;
     static constexpr size_t SMEM = NEED > 122880 ? NEED : 122880;
-    // warps 0-7 softmax, 8 TMA, 9 MMA, 10 and 11 idle (a warpgroup gives up its registers as a whole)
-    static constexpr int THREADS = 384;
+    static constexpr int THREADS = 352;  // warps 0-7 softmax, 8 TMA, 9 and 10 MMA of tile A and of tile B
 };
-
-// The launch gives each of the three warpgroups 168 registers a thread; the
-// last one hands most of its share to the two that hold a row of S.
-constexpr int kWinRegsFew = 104, kWinRegsMany = 200;
-static_assert(kWinRegsFew + 2 * kWinRegsMany <= 3 * 168, "more registers than the block is launched with");
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t win_pack(float a, float b) {
@@ -141,6 +138,33 @@ __device__ __forceinline__ float win_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Bits below position n (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t below(int n) {
+    return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
+}
+
+// Two floats in a 64-bit register: one instruction for both.
+__device__ __forceinline__ uint64_t two(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 one_each(uint64_t a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 // One pair of query tiles of one head, and the key tiles it visits.
@@ -239,24 +263,28 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
     uint64_t* v_full = k_empty + ST;    // [ST]
     uint64_t* v_empty = v_full + ST;    // [ST]
     uint64_t* s_full = v_empty + ST;    // [tile]
-    uint64_t* p_full = s_full + 2;      // [tile]
-    uint64_t* o_done = p_full + 2;      // [tile]: the pair's last P V of the tile is done
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+    uint64_t* p_lo = s_full + 2;        // [tile]: P of the tile's first 64 keys is in TMEM
+    uint64_t* p_hi = p_lo + 2;          // [tile]: and of the others
+    uint64_t* o_done = p_hi + 2;        // [tile]: the pair's last P V of the tile is done
+    uint64_t* turn = o_done + 2;        // [tile]: its products of the next step may be issued
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         tc::mbar_init(q_full, 1);
-        tc::mbar_init(q_empty, 1);
+        tc::mbar_init(q_empty, 2);
         for (int s = 0; s < ST; ++s) {
             tc::mbar_init(&k_full[s], 1);
-            tc::mbar_init(&k_empty[s], 1);
+            tc::mbar_init(&k_empty[s], 2);
             tc::mbar_init(&v_full[s], 1);
-            tc::mbar_init(&v_empty[s], 1);
+            tc::mbar_init(&v_empty[s], 2);
         }
         for (int t = 0; t < 2; ++t) {
             tc::mbar_init(&s_full[t], 1);
-            tc::mbar_init(&p_full[t], 128);
+            tc::mbar_init(&p_lo[t], 128);
+            tc::mbar_init(&p_hi[t], 128);
             tc::mbar_init(&o_done[t], 1);
+            tc::mbar_init(&turn[t], 1);
         }
         tc::fence_barrier_init();
     }
@@ -273,201 +301,130 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
     WinItem it;
     uint32_t g = 0;  // key tiles of the pairs before this one
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWinRegsFew));
-        if (warp == 8) {
-            // ---------------- TMA producer ----------------
-            if (lane == 0) {
-                bool ok = true;
-                uint32_t k = 0;
-                for (int64_t i = blockIdx.x; ok && list.get(a, i, it); i += gridDim.x, ++k) {
-                    const int kvh = it.h / (a.nq / a.nkv);
-                    if (k > 0 && !tc::mbar_wait(q_empty, (k - 1) & 1u, err, 91)) break;
-                    tc::mbar_arrive_expect_tx(q_full, 2 * TILE);
+    if (warp == 8) {
+        // ---------------- TMA producer ----------------
+        if (lane == 0) {
+            bool ok = true;
+            uint32_t k = 0;
+            for (int64_t i = blockIdx.x; ok && list.get(a, i, it); i += gridDim.x, ++k) {
+                const int kvh = it.h / (a.nq / a.nkv);
+                if (k > 0 && !tc::mbar_wait(q_empty, (k - 1) & 1u, err, 91)) break;
+                tc::mbar_arrive_expect_tx(q_full, 2 * TILE);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-                        for (int c = 0; c < C::ATOMS; ++c)
-                            tc::tma_load_4d(sQ + t * TILE + c * ATOM, &tmQ, q_full, c * 64, it.h, it.row0 + t * 128, it.b);
-                    for (int j = 0; j < it.n; ++j, ++g) {
-                        const uint32_t s = g % ST, u = g / ST;
-                        const int row = it.tile(j) * 128;
-                        if (g >= ST && !(ok = tc::mbar_wait(&k_empty[s], (u - 1) & 1u, err, 92))) break;
-                        tc::mbar_arrive_expect_tx(&k_full[s], TILE);
+                    for (int c = 0; c < C::ATOMS; ++c)
+                        tc::tma_load_4d(sQ + t * TILE + c * ATOM, &tmQ, q_full, c * 64, it.h, it.row0 + t * 128, it.b);
+                for (int j = 0; j < it.n; ++j, ++g) {
+                    const uint32_t s = g % ST, u = g / ST;
+                    const int row = it.tile(j) * 128;
+                    if (g >= ST && !(ok = tc::mbar_wait(&k_empty[s], (u - 1) & 1u, err, 92))) break;
+                    tc::mbar_arrive_expect_tx(&k_full[s], TILE);
 #pragma unroll
-                        for (int c = 0; c < C::ATOMS; ++c)
-                            tc::tma_load_4d(sK + s * TILE + c * ATOM, &tmK, &k_full[s], c * 64, kvh, row, it.b);
-                        if (g >= ST && !(ok = tc::mbar_wait(&v_empty[s], (u - 1) & 1u, err, 93))) break;
-                        tc::mbar_arrive_expect_tx(&v_full[s], TILE);
+                    for (int c = 0; c < C::ATOMS; ++c)
+                        tc::tma_load_4d(sK + s * TILE + c * ATOM, &tmK, &k_full[s], c * 64, kvh, row, it.b);
+                    if (g >= ST && !(ok = tc::mbar_wait(&v_empty[s], (u - 1) & 1u, err, 93))) break;
+                    tc::mbar_arrive_expect_tx(&v_full[s], TILE);
 #pragma unroll
-                        for (int c = 0; c < C::ATOMS; ++c)
-                            tc::tma_load_4d(sV + s * TILE + c * ATOM, &tmV, &v_full[s], c * 64, kvh, row, it.b);
-                    }
-                }
-            }
-        } else if (warp == 9) {
-            // ---------------- MMA issuer ----------------
-            if (lane == 0) {
-                constexpr uint32_t idO = tc::idesc_f16(128, D, BF16, true);
-                const uint32_t aQ = tc::smem_u32(sQ), aK = tc::smem_u32(sK), aV = tc::smem_u32(sV);
-                bool ok = true;
-                uint32_t k = 0, np = 0;  // pairs; bit t: parity of the P tiles consumed of query tile t
-                // a descriptor's address field counts 16 bytes: steps are added to it
-                auto issue_s = [&](int t, int j) {
-                    const uint32_t idS = tc::idesc_f16(128, 0, BF16, false) | ((uint32_t)(it.width(a, t, j) >> 3) << 17);
-                    const uint64_t dq = tc::desc_k_sw128(aQ + (uint32_t)t * TILE),
-                                   dk = tc::desc_k_sw128(aK + ((g + j) % ST) * TILE);
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t off = ((uint32_t)(kk >> 2) * ATOM + (uint32_t)(kk & 3) * 32) >> 4;
-                        tc::mma_f16(tmem + (uint32_t)t * 256, dq + off, dk + off, idS, kk > 0 ? 1u : 0u);
-                    }
-                    tc::mma_commit(&s_full[t]);
-                };
-                auto issue_pv = [&](int t, int j, bool first, bool last) {
-                    const uint64_t dv = tc::desc_mn_sw128(aV + ((g + j) % ST) * TILE, ATOM);
-                    const int steps = it.width(a, t, j) >> 4;
-                    const uint32_t tP = tmem + (uint32_t)t * 256;
-                    tc::mma_f16_ts(tP + 128, tP, dv, idO, first ? 0u : 1u);
-#pragma unroll
-                    for (int kk = 1; kk < 8; ++kk)
-                        if (kk < steps) tc::mma_f16_ts(tP + 128, tP + (uint32_t)kk * 8, dv + (uint32_t)kk * 128u, idO, 1u);
-                    if (last) tc::mma_commit(&o_done[t]);
-                };
-                auto wait_k = [&](int j) { return tc::mbar_wait(&k_full[(g + j) % ST], ((g + j) / ST) & 1u, err, 94); };
-                auto wait_v = [&](int j) { return tc::mbar_wait(&v_full[(g + j) % ST], ((g + j) / ST) & 1u, err, 95); };
-                for (int64_t i = blockIdx.x; ok && list.get(a, i, it); i += gridDim.x, ++k) {
-                    ok = tc::mbar_wait(q_full, k & 1u, err, 96) && wait_k(0);
-                    if (!ok) break;
-                    tc::fence_after_sync();
-                    issue_s(0, 0);
-                    if (it.hasB && it.dB == 0) issue_s(1, 0);
-                    tc::mma_commit(&k_empty[g % ST]);
-                    if (it.n == 1) tc::mma_commit(q_empty);
-                    for (int j = 0; j < it.n; ++j) {
-                        const bool more = j + 1 < it.n;
-                        bool v_ok = false, k_ok = false;
-#pragma unroll 1
-                        for (int t = 0; t < 2; ++t) {
-                            const int from = t == 0 ? 0 : it.dB, to = t == 0 ? it.nA : it.hasB ? it.n : 0;
-                            if (j >= from && j < to) {
-                                ok = ok && tc::mbar_wait(&p_full[t], (np >> t) & 1u, err, 97) && (v_ok || wait_v(j));
-                                if (!ok) break;
-                                v_ok = true;
-                                np ^= 1u << t;
-                                tc::fence_after_sync();
-                                issue_pv(t, j, j == from, j + 1 == to);
-                            }
-                            if (j + 1 >= from && j + 1 < to) {
-                                ok = ok && (k_ok || wait_k(j + 1));
-                                if (!ok) break;
-                                k_ok = true;
-                                tc::fence_after_sync();
-                                issue_s(t, j + 1);
-                            }
-                        }
-                        if (!ok) break;
-                        tc::mma_commit(&v_empty[(g + j) % ST]);
-                        if (more) tc::mma_commit(&k_empty[(g + j + 1) % ST]);
-                        if (j + 2 == it.n) tc::mma_commit(q_empty);
-                    }
-                    g += it.n;
+                    for (int c = 0; c < C::ATOMS; ++c)
+                        tc::tma_load_4d(sV + s * TILE + c * ATOM, &tmV, &v_full[s], c * 64, kvh, row, it.b);
                 }
             }
         }
+    } else if (warp >= 9) {
+        // ---------------- MMA issuers: one per tile, so that the tensor core always has the other's
+        // products queued while one waits or computes descriptors ----------------
+        if (lane == 0) {
+            constexpr uint32_t idO = tc::idesc_f16(128, D, BF16, true);
+            constexpr uint32_t idS = tc::idesc_f16(128, 0, BF16, false);
+            const int t = warp - 9;
+            const uint32_t tP = tmem + (uint32_t)t * 256, tO = tP + 128;
+            // a descriptor's address field counts 16 bytes: steps are added to it
+            const uint64_t dq = tc::desc_k_sw128(tc::smem_u32(sQ) + (uint32_t)t * TILE);
+            const uint64_t dk0 = tc::desc_k_sw128(tc::smem_u32(sK)), dv0 = tc::desc_mn_sw128(tc::smem_u32(sV), ATOM);
+            bool ok = true;
+            uint32_t k = 0, np = 0;  // pairs; P tiles consumed
+            auto wait_k = [&](uint32_t gj) { return tc::mbar_wait(&k_full[gj % ST], (gj / ST) & 1u, err, 94); };
+            auto wait_v = [&](uint32_t gj) { return tc::mbar_wait(&v_full[gj % ST], (gj / ST) & 1u, err, 95); };
+            // Turns: A's products of a step, then B's, and so on.  The other tile's products are in the
+            // queue while this thread waits for its own operands, and the two softmaxes stay half a step apart.
+            uint32_t turns = 0;
+            auto my_turn = [&]() {
+                const bool mine = (t == 0 && turns == 0) || tc::mbar_wait(&turn[t], (turns - (t == 0)) & 1u, err, 102);
+                ++turns;
+                return mine;
+            };
+            for (int64_t i = blockIdx.x; ok && list.get(a, i, it); i += gridDim.x, ++k) {
+                const int from = t == 0 ? 0 : it.dB, to = t == 0 ? it.nA : it.hasB ? it.n : 0;
+                int w = 0;
+                for (int j = -1; j < it.n; ++j) {
+                    const uint32_t gj = g + (uint32_t)j, s = gj % ST, s1 = (gj + 1) % ST;
+                    const bool pv = j >= from && j < to, qk = j + 1 >= from && j + 1 < to;
+                    const int steps = w >> 4;
+                    if (qk) w = it.width(a, t, j + 1);
+                    if (j + 1 < it.n) ok = (j >= 0 || tc::mbar_wait(q_full, k & 1u, err, 96)) && wait_k(gj + 1);
+                    if (j >= 0) ok = ok && wait_v(gj);
+                    if (pv) ok = ok && tc::mbar_wait(&p_lo[t], np & 1u, err, 97);
+                    ok = ok && my_turn();
+                    if (!ok) break;
+                    tc::fence_after_sync();
+                    if (pv) {
+                        const uint64_t dv = dv0 + s * (TILE >> 4);
+                        tc::mma_f16_ts(tO, tP, dv, idO, j > from ? 1u : 0u);
+#pragma unroll
+                        for (int kk = 1; kk < 4; ++kk)
+                            if (kk < steps) tc::mma_f16_ts(tO, tP + (uint32_t)kk * 8, dv + (uint32_t)kk * 128u, idO, 1u);
+                        if (!(ok = tc::mbar_wait(&p_hi[t], np & 1u, err, 101))) break;
+                        ++np;
+                        tc::fence_after_sync();
+#pragma unroll
+                        for (int kk = 4; kk < 8; ++kk)
+                            if (kk < steps) tc::mma_f16_ts(tO, tP + (uint32_t)kk * 8, dv + (uint32_t)kk * 128u, idO, 1u);
+                        if (j + 1 == to) tc::mma_commit(&o_done[t]);
+                    }
+                    if (qk) {
+                        const uint64_t dk = dk0 + s1 * (TILE >> 4);
+                        const uint32_t id = idS | ((uint32_t)(w >> 3) << 17);
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t off = ((uint32_t)(kk >> 2) * ATOM + (uint32_t)(kk & 3) * 32) >> 4;
+                            tc::mma_f16(tP, dq + off, dk + off, id, kk > 0 ? 1u : 0u);
+                        }
+                        tc::mma_commit(&s_full[t]);
+                    }
+                    tc::mbar_arrive(&turn[t ^ 1]);
+                    // whatever this tile read of the step's K and V has been read once these arrive
+                    if (j >= 0) tc::mma_commit(&v_empty[s]);
+                    if (j + 1 < it.n) tc::mma_commit(&k_empty[s1]);
+                    if (j + 2 == it.n) tc::mma_commit(q_empty);
+                }
+                g += it.n;
+            }
+        }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWinRegsMany));
         // ---------------- softmax and output: tile t, one query row per thread ----------------
         const int t = warp >> 2, rq = warp & 3;
-        const int r = rq * 32 + lane;
         const uint32_t lane_base = (uint32_t)(rq * 32) << 16;
         const uint32_t tS = tmem + (uint32_t)t * 256 + lane_base, tO = tS + 128;
-        const int T = a.q_start + a.S;
+        const uint64_t scale2 = two(a.scale_log2, a.scale_log2);
         bool ok = true;
         uint32_t cs = 0, co = 0;  // S tiles and outputs of this tile so far
         for (int64_t i = blockIdx.x; ok && list.get(a, i, it); i += gridDim.x) {
             const int from = t == 0 ? 0 : it.dB, to = t == 0 ? it.nA : it.hasB ? it.n : 0;
-            const int wp = it.p0 + t * 128 + rq * 32;        // position of the warp's first row
-            const int pos = it.p0 + t * 128 + r < it.len ? it.p0 + t * 128 + r : -1;
+            const int wp = it.p0 + t * 128 + rq * 32;  // position of the warp's first row
+            const int pos = wp + lane < it.len ? wp + lane : -1;
             float m = -1e30f, l = 0.f;  // finite: a row that has seen nothing keeps P = 0 and l = 0
             for (int j = from; j < to; ++j, ++cs) {
-                ok = __all_sync(0xffffffffu, tc::mbar_wait(&s_full[t], cs & 1u, err, 98));
-                if (!ok) break;
-                tc::fence_after_sync();
                 const int kb = it.tile(j) << 7, w = it.width(a, t, j);
-                uint32_t v[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (32 * c < w) tc::tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
-                tc::tmem_wait_ld();
                 // the tile whole, for every row of the warp?
                 const bool whole = w == 128 && kb + 127 <= wp && wp + 31 < it.len &&
                                    (a.window == 0 || kb > wp + 31 - a.window || kb + 128 <= a.sinks);
-                uint32_t some = 0xf;  // 32-key stretches that some row of the warp sees
-                if (!whole) {
-                    const int hi = pos - kb, lo = a.window > 0 ? pos - a.window + 1 - kb : 0, sk = a.window > 0 ? a.sinks - kb : 0;
-                    const int whi = wp + 31 - kb, wlo = a.window > 0 ? wp - a.window + 1 - kb : 0;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        if (32 * c >= w || 32 * c > whi || (32 * c + 31 < wlo && 32 * c >= sk)) some &= ~(1u << c);
-                        if (some >> c & 1) {
-#pragma unroll
-                            for (int e = 32 * c; e < 32 * c + 32; ++e)
-                                if (e > hi || (e < lo && e >= sk)) v[e] = 0xff800000u;  // -inf
-                        }
-                    }
-                }
-                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (some >> c & 1) {
-#pragma unroll
-                        for (int e = 32 * c; e < 32 * c + 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(v[e]));
-                    }
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
-                const float m_new = fmaxf(m, mx);
-                const bool resc = m_new > m + 8.f;
-                const float m_use = resc ? m_new : m;
-                const float alpha = win_ex2(m - m_use);
-                if (j > from && __any_sync(0xffffffffu, resc)) {
-                    // the P V before has completed (S, issued behind it, has)
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t o[32];
-                        tc::tmem_ld32(tO + c, o);
-                        tc::tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tc::tmem_st32(tO + c, o);
-                    }
-                }
-                m = m_use;
-                float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (32 * c >= w) break;
-                    uint32_t pk[16];
-                    if (some >> c & 1) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            const float p0 = win_ex2(fmaf(__uint_as_float(v[32 * c + e]), a.scale_log2, -m));
-                            const float p1 = win_ex2(fmaf(__uint_as_float(v[32 * c + e + 1]), a.scale_log2, -m));
-                            l4[(e >> 1) & 3] += p0 + p1;
-                            pk[e >> 1] = win_pack<BF16>(p0, p1);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) pk[e] = 0u;
-                    }
-                    tc::tmem_st16(tS + (uint32_t)(16 * c), pk);
-                }
-                l = l * alpha + ((l4[0] + l4[1]) + (l4[2] + l4[3]));
-                tc::tmem_wait_st();
-                if (kb + w > it.len && it.len < T) {
+                if (kb + w > it.len && it.len < a.q_start + a.S) {
                     // rows past the sequence may hold anything: P is 0 there, and V has to be finite
                     const uint32_t gj = g + j, s = gj % ST;
                     ok = __all_sync(0xffffffffu, tc::mbar_wait(&v_full[s], (gj / ST) & 1u, err, 99));
                     if (!ok) break;
+                    const int r = rq * 32 + lane;
                     if (kb + r >= it.len) {
 #pragma unroll
                         for (int c = 0; c < C::ATOMS; ++c)
@@ -477,32 +434,104 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                     }
                     tc::fence_proxy_async_smem();
                 }
-                tc::fence_before_sync();
-                tc::mbar_arrive(&p_full[t]);
+                ok = __all_sync(0xffffffffu, tc::mbar_wait(&s_full[t], cs & 1u, err, 98));
+                if (!ok) break;
+                tc::fence_after_sync();
+                uint32_t v[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc::tmem_ld32(tS + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
+                tc::tmem_wait_ld();
+                if (!whole) {
+                    // visible columns of the row as bits: lo .. hi and those below sk
+                    const int hi = pos - kb, lo = a.window > 0 ? hi + 1 - a.window : 0, sk = a.window > 0 ? a.sinks - kb : 0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t see = below(hi + 1 - 32 * c) & (~below(lo - 32 * c) | below(sk - 32 * c));
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(see >> e & 1)) v[32 * c + e] = 0xff800000u;  // -inf
+                    }
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 128; e += 2)
+                    mx4[(e >> 1) & 3] = fmaxf(fmaxf(mx4[(e >> 1) & 3], __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
+                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
+                const float m_new = fmaxf(m, mx);
+                const bool resc = m_new > m + 8.f;
+                const float m_use = resc ? m_new : m;
+                const float alpha = win_ex2(m - m_use);
+                if (j > from && __any_sync(0xffffffffu, resc)) {
+                    // the P V before has completed (S, issued behind it, has)
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t o[16];
+                        tc::tmem_ld16(tO + c, o);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tc::tmem_st16(tO + c, o);
+                    }
+                }
+                m = m_use;
+                const uint64_t nm2 = two(-m, -m);
+                uint64_t l2[2] = {0, 0};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 x = one_each(fma2(two(__uint_as_float(v[32 * c + e]), __uint_as_float(v[32 * c + e + 1])), scale2, nm2));
+                        const float p0 = win_ex2(x.x), p1 = win_ex2(x.y);
+                        l2[(e >> 1) & 1] = add2(l2[(e >> 1) & 1], two(p0, p1));
+                        pk[e >> 1] = win_pack<BF16>(p0, p1);
+                    }
+                    tc::tmem_st16(tS + (uint32_t)(16 * c), pk);
+                    if (c & 1) {
+                        tc::tmem_wait_st();
+                        tc::fence_before_sync();
+                        tc::mbar_arrive(c == 1 ? &p_lo[t] : &p_hi[t]);
+                    }
+                }
+                const float2 ls = one_each(add2(l2[0], l2[1]));
+                l = l * alpha + (ls.x + ls.y);
             }
             if (ok && to > from) {
                 ok = __all_sync(0xffffffffu, tc::mbar_wait(&o_done[t], co & 1u, err, 100));
                 ++co;
                 tc::fence_after_sync();
                 const float inv_l = l > 0.f ? 1.f / l : 0.f;
-                const int row = it.row0 + t * 128 + r;
-                uint16_t* orow = static_cast<uint16_t*>(a.out) + (((int64_t)it.b * a.S + row) * a.nq + it.h) * a.D;
+                // 64 outputs of 32 rows at a time through shared memory: whole 128-byte lines leave
+                uint8_t* stage = sm + C::OFF_OUT + warp * 4096;
+                const int row = it.row0 + t * 128 + rq * 32;
+                uint16_t* obase = static_cast<uint16_t*>(a.out) + (((int64_t)it.b * a.S + row) * a.nq + it.h) * a.D;
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    uint32_t o[32];
-                    tc::tmem_ld32(tO + c, o);
-                    tc::tmem_wait_ld();
-                    if (!ok || row >= a.S) continue;
+                for (int c = 0; c < D; c += 64) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        if (c + 8 * q >= a.D) break;
-                        uint4 x;
-                        x.x = win_pack<BF16>(__uint_as_float(o[8 * q + 0]) * inv_l, __uint_as_float(o[8 * q + 1]) * inv_l);
-                        x.y = win_pack<BF16>(__uint_as_float(o[8 * q + 2]) * inv_l, __uint_as_float(o[8 * q + 3]) * inv_l);
-                        x.z = win_pack<BF16>(__uint_as_float(o[8 * q + 4]) * inv_l, __uint_as_float(o[8 * q + 5]) * inv_l);
-                        x.w = win_pack<BF16>(__uint_as_float(o[8 * q + 6]) * inv_l, __uint_as_float(o[8 * q + 7]) * inv_l);
-                        *reinterpret_cast<uint4*>(orow + c + 8 * q) = x;
+                    for (int hh = 0; hh < 2; ++hh) {
+                        uint32_t o[32];
+                        tc::tmem_ld32(tO + c + 32 * hh, o);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            uint4 x;
+                            x.x = win_pack<BF16>(__uint_as_float(o[8 * q + 0]) * inv_l, __uint_as_float(o[8 * q + 1]) * inv_l);
+                            x.y = win_pack<BF16>(__uint_as_float(o[8 * q + 2]) * inv_l, __uint_as_float(o[8 * q + 3]) * inv_l);
+                            x.z = win_pack<BF16>(__uint_as_float(o[8 * q + 4]) * inv_l, __uint_as_float(o[8 * q + 5]) * inv_l);
+                            x.w = win_pack<BF16>(__uint_as_float(o[8 * q + 6]) * inv_l, __uint_as_float(o[8 * q + 7]) * inv_l);
+                            *reinterpret_cast<uint4*>(stage + lane * 128 + (((hh * 4 + q) ^ (lane & 7)) << 4)) = x;
+                        }
                     }
+                    __syncwarp();
+                    const int ch = lane & 7;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int r = k * 4 + (lane >> 3);
+                        if (ok && row + r < a.S && c + ch * 8 < a.D)
+                            *reinterpret_cast<uint4*>(obase + (int64_t)r * a.nq * a.D + c + ch * 8) =
+                                *reinterpret_cast<const uint4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+                    }
+                    __syncwarp();
                 }
             }
             g += it.n;
