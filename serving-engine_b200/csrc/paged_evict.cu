@@ -6,12 +6,13 @@
 // order, to positions 0 .. n-1.  The bytes are the scores once, and the kept
 // rows read and written (8 D bytes each): HBM bounds it, the choice is latency.
 //
-// Two launches.  The choice is one CTA per (sequence, kv head): its scores in
-// shared memory, the n-th best found 8 bits of its ordered key at a time from
-// a histogram, then every kept position's place from ballots and one scan, ties
-// going to the lowest positions.  (A cluster of 8 CTAs per choice, histograms
-// added through distributed shared memory, took 20 us a cluster for 4096
-// scores: each of its exchanges costs more than the reading it saves.)
+// Two launches.  The choice is one CTA per (sequence, kv head): the positions'
+// ordered keys in shared memory, the n-th best found 11 bits at a time from a
+// histogram, then every kept position's place by one scan, ties going to the
+// lowest positions.  Latency bounds it: the scores are a small part of the
+// bytes.  (A cluster of 8 CTAs per choice, histograms added through
+// distributed shared memory, took 20 us a cluster for 4096 scores: each of its
+// exchanges costs more than the reading it saves.)
 // The move is spread over the GPU.
 //
 // Moving in place is safe without a second copy because kept position j comes
@@ -26,7 +27,7 @@
 namespace b2 {
 
 constexpr int kEvThreads = 1024;   // of a choice
-constexpr int kEvCached = 49152;   // scores of a choice kept in shared memory; the rest are read again
+constexpr int kEvCached = 49152;   // keys of a choice kept in shared memory; the rest are read again
 constexpr int kMvThreads = 256;    // of a move
 constexpr int kMvBatch = 4;        // 16-byte pieces in flight per thread
 constexpr int kMvRows = 128;       // rows of a CTA that moves into other blocks
@@ -40,20 +41,19 @@ struct EvictArgs {
     int nkv, D, budget, sinks, recent;
     int* kept;
     int* new_lens;
-    int cached;  // floats of shared memory for scores
+    int cached;  // keys that the choice's shared memory holds
 };
 
-// The order scores are ranked in, as unsigned keys: NaN above everything,
-// -0 equal to +0.
-__device__ __forceinline__ uint32_t rank_key(float f) {
-    if (f != f) return 0xffffffffu;
-    return float_key(f + 0.f);
-}
+// What positions are ranked by: positions that stay in any case above
+// everything, then NaN, then the scores, -0 equal to +0.
+constexpr uint32_t kEvStays = 0xffffffffu, kEvNan = 0xfffffffeu;
+__device__ __forceinline__ uint32_t rank_key(float f) { return f != f ? kEvNan : float_key(f + 0.f); }
 
 __global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const EvictArgs a) {
-    extern __shared__ float s_sc[];
-    __shared__ int s_hist[2][256];
+    extern __shared__ __align__(16) uint32_t s_key[];
+    __shared__ int s_hist[2][2048];
     __shared__ int s_pick[2];  // the bin that holds the n-th best, positions above it
+    __shared__ int s_sum[kEvThreads / 32];
     __shared__ int2 s_warp[kEvThreads / 32];
     const int kvh = blockIdx.x, b = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int bs = a.kv.block_size;
@@ -66,98 +66,139 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const Evict
         for (int j = t; j < a.budget; j += kEvThreads) kept[j] = j < n ? j : -1;
         return;
     }
-    const int m0 = a.sinks, m1 = L - a.recent;  // the positions that compete
-    auto load = [&](int i) -> float {
+    auto load = [&](int i) -> uint32_t {
+        if (i < a.sinks || i >= L - a.recent) return kEvStays;
         const int blk = bt[(unsigned)i / (unsigned)bs];
-        if ((unsigned)blk >= (unsigned)a.kv.num_blocks) return -INFINITY;
-        return a.scores[((int64_t)blk * a.nkv + kvh) * bs + (unsigned)i % (unsigned)bs];
+        if ((unsigned)blk >= (unsigned)a.kv.num_blocks) return rank_key(-INFINITY);
+        return rank_key(a.scores[((int64_t)blk * a.nkv + kvh) * bs + (unsigned)i % (unsigned)bs]);
     };
-    const int cached = min(L, a.cached);
-    if (t < 256) s_hist[0][t] = 0;
-#pragma unroll 8
-    for (int i = t; i < cached; i += kEvThreads) s_sc[i] = load(i);
-    auto key = [&](int i) { return rank_key(i < cached ? s_sc[i] : load(i)); };
-    int need = n - a.sinks - a.recent;  // of the competing ones that stay
-    uint32_t thr = need > 0 ? 0u : 0xffffffffu;
-    if (need > 0) {
-        for (int pass = 0; pass < 4; ++pass) {
-            const int shift = 24 - 8 * pass;
-            int* hist = s_hist[pass & 1];
-            __syncthreads();
-            for (int i = m0 + t; i < m1; i += kEvThreads) {
-                const uint32_t k = key(i);
-                if (pass == 0 || (k ^ thr) >> (shift + 8) == 0) atomicAdd(&hist[(k >> shift) & 255], 1);
-            }
-            __syncthreads();
-            if (warp == 0) {  // lane l: bins 8 l .. 8 l + 7, counted from the top
-                int h[8], mine = 0;
+    const int cached = min(L, a.cached) & ~3;
+    s_hist[0][t] = 0;
+    s_hist[0][t + kEvThreads] = 0;
+    // 8 positions a thread at a time: their table entries in one round trip, their scores in the next
+    for (int i0 = t; i0 < cached; i0 += 8 * kEvThreads) {
+        int blk[8];
+        float f[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    h[e] = hist[lane * 8 + e];
-                    mine += h[e];
-                }
-                int above = mine;
+        for (int e = 0; e < 8; ++e) {
+            const int i = i0 + e * kEvThreads;
+            blk[e] = i < cached ? bt[(unsigned)i / (unsigned)bs] : -1;
+        }
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int v = __shfl_down_sync(~0u, above, o);
-                    if (lane + o < 32) above += v;
-                }
-                above -= mine;
+        for (int e = 0; e < 8; ++e) {
+            const int i = i0 + e * kEvThreads;
+            f[e] = -INFINITY;
+            if ((unsigned)blk[e] < (unsigned)a.kv.num_blocks)
+                f[e] = a.scores[((int64_t)blk[e] * a.nkv + kvh) * bs + (unsigned)i % (unsigned)bs];
+        }
 #pragma unroll
-                for (int e = 7; e >= 0; --e) {
-                    if (above < need && need <= above + h[e]) {
-                        s_pick[0] = lane * 8 + e;
-                        s_pick[1] = above;
-                    }
-                    above += h[e];
-                }
-            } else if (warp <= 8) {
-                s_hist[(pass + 1) & 1][t - 32] = 0;
-            }
-            __syncthreads();
-            thr |= (uint32_t)s_pick[0] << shift;
-            need -= s_pick[1];
+        for (int e = 0; e < 8; ++e) {
+            const int i = i0 + e * kEvThreads;
+            if (i < cached) s_key[i] = i < a.sinks || i >= L - a.recent ? kEvStays : rank_key(f[e]);
         }
     }
-    __syncthreads();
-    // need is now how many positions with key == thr stay.  A position's place: the forced and better ones before
-    // it, and the equal ones before it as far as they stay.  A warp takes a stretch of positions, 32 at a time.
-    const int q = ((L + kEvThreads - 1) / kEvThreads) * 32, q0 = min(L, warp * q), q1 = min(L, q0 + q);
-    auto kind = [&](int i) -> int {  // 1: stays, 2: equal, 0: goes
-        if (i >= q1) return 0;
-        if (i < m0 || i >= m1) return 1;
-        const uint32_t k = key(i);
-        return k > thr ? 1 : k == thr ? 2 : 0;
+    // keys of positions i .. i + 3 (i a multiple of 4); past the end a key no position of this choice has
+    auto keys = [&](int i) -> uint4 {
+        if (i < cached) return *reinterpret_cast<const uint4*>(s_key + i);
+        return make_uint4(load(i), i + 1 < L ? load(i + 1) : 0u, i + 2 < L ? load(i + 2) : 0u, i + 3 < L ? load(i + 3) : 0u);
     };
-    int2 before = make_int2(0, 0);
-    for (int i = q0; i < q1; i += 32) {
-        const int k = kind(i + lane);
-        before.x += __popc(__ballot_sync(~0u, k == 1));
-        before.y += __popc(__ballot_sync(~0u, k == 2));
+    int need = n;
+    uint32_t thr = 0;
+    for (int pass = 0; pass < 3; ++pass) {  // bits 31 .. 21, 20 .. 10, 9 .. 0
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
+        int* hist = s_hist[pass & 1];
+        __syncthreads();
+#pragma unroll 2
+        for (int i = 4 * t; i < L; i += 4 * kEvThreads) {
+            const uint4 v = keys(i);
+            const uint32_t k[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e < L && (pass == 0 || (k[e] ^ thr) >> (shift + width) == 0))
+                    atomicAdd(&hist[(k[e] >> shift) & ((1 << width) - 1)], 1);
+        }
+        __syncthreads();
+        // thread t: bins 2 t and 2 t + 1, counted from the top
+        const int2 h = reinterpret_cast<const int2*>(hist)[t];
+        int above = h.x + h.y;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_down_sync(~0u, above, o);
+            if (lane + o < 32) above += v;
+        }
+        if (lane == 0) s_sum[warp] = above;
+        s_hist[(pass + 1) & 1][t] = 0;
+        s_hist[(pass + 1) & 1][t + kEvThreads] = 0;
+        __syncthreads();
+        int v = s_sum[lane];
+        if (lane <= warp) v = 0;
+        above += __reduce_add_sync(~0u, v) - h.x - h.y;
+        if (above < need && need <= above + h.x + h.y) {
+            const bool top = need <= above + h.y;
+            s_pick[0] = 2 * t + (top ? 1 : 0);
+            s_pick[1] = top ? above : above + h.y;
+        }
+        __syncthreads();
+        thr |= (uint32_t)s_pick[0] << shift;
+        need -= s_pick[1];
     }
+    // need is now how many positions with key == thr stay.  A position's place: the better ones before it, and the
+    // equal ones before it as far as they stay.  A warp takes a stretch of positions, 4 of them a lane at a time.
+    const int q = (L + 128 * 32 - 1) / (128 * 32) * 128, q0 = min(L, warp * q), q1 = min(L, q0 + q);
+    auto kinds = [&](int i) -> int {  // better ones of the 4 in the low half, equal ones in the high half; bits 4.. each
+        if (i >= q1) return 0;
+        const uint4 v = keys(i);
+        const uint32_t k[4] = {v.x, v.y, v.z, v.w};
+        int r = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < q1) r |= k[e] > thr ? 1 << e : k[e] == thr ? 0x10000 << e : 0;
+        return r;
+    };
+    auto count = [](int r) { return __popc(r & 0xf) | __popc(r & 0xf0000) << 16; };
+    int2 before = make_int2(0, 0);
+#pragma unroll 4
+    for (int i = q0; i < q1; i += 128) {
+        const int c = count(kinds(i + 4 * lane));
+        before.x += c & 0xffff;
+        before.y += c >> 16;
+    }
+    before.x = __reduce_add_sync(~0u, before.x);
+    before.y = __reduce_add_sync(~0u, before.y);
     if (lane == 0) s_warp[warp] = before;
     __syncthreads();
     before = s_warp[lane];
     if (lane >= warp) before = make_int2(0, 0);
+    before.x = __reduce_add_sync(~0u, before.x);
+    before.y = __reduce_add_sync(~0u, before.y);
+#pragma unroll 4
+    for (int i = q0; i < q1; i += 128) {
+        const int r = kinds(i + 4 * lane), c = count(r);
+        int incl = c;  // at most 128 of each: the halves do not meet
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        before.x += __shfl_xor_sync(~0u, before.x, o);
-        before.y += __shfl_xor_sync(~0u, before.y, o);
-    }
-    const unsigned under = (1u << lane) - 1;
-    for (int i = q0; i < q1; i += 32) {
-        const int k = kind(i + lane);
-        const unsigned in = __ballot_sync(~0u, k == 1), eq = __ballot_sync(~0u, k == 2);
-        const int e = before.y + __popc(eq & under);
-        if (k == 1 || (k == 2 && e < need)) kept[before.x + __popc(in & under) + min(e, need)] = i + lane;
-        before.x += __popc(in);
-        before.y += __popc(eq);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(~0u, incl, o);
+            if (lane >= o) incl += v;
+        }
+        int in = before.x + ((incl - c) & 0xffff), eq = before.y + ((incl - c) >> 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (r >> e & 1) kept[in++ + min(eq, need)] = i + 4 * lane + e;
+            if (r >> (16 + e) & 1) {
+                if (eq < need) kept[in + eq] = i + 4 * lane + e;
+                ++eq;
+            }
+        }
+        incl = __shfl_sync(~0u, incl, 31);
+        before.x += incl & 0xffff;
+        before.y += incl >> 16;
     }
 }
 
-// grid (row ranges, or column slices in place; kv heads; sequences)
+// grid (kv heads; row ranges, or column slices in place; sequences): the heads
+// of one range run together, so that their rows' DRAM pages do
 __global__ void __launch_bounds__(kMvThreads, 4) evict_move_kernel(const EvictArgs a) {
-    const int kvh = blockIdx.y, b = blockIdx.z, rank = blockIdx.x, cs = gridDim.x, t = threadIdx.x;
+    const int kvh = blockIdx.x, b = blockIdx.z, rank = blockIdx.y, cs = gridDim.y, t = threadIdx.x;
     const int bs = a.kv.block_size;
     griddep_wait();
     griddep_launch_dependents();
@@ -207,11 +248,11 @@ __global__ void __launch_bounds__(kMvThreads, 4) evict_move_kernel(const EvictAr
             }
 #pragma unroll
             for (int e = 0; e < kMvBatch; ++e)
-                if (from[e] >= 0) v[e] = base[from[e] >> 3];
+                if (from[e] >= 0) v[e] = __ldcs(base + (from[e] >> 3));
             if (!a.dst) __syncthreads();
 #pragma unroll
             for (int e = 0; e < kMvBatch; ++e)
-                if (from[e] >= 0) base[to[e] >> 3] = v[e];
+                if (from[e] >= 0) __stcs(base + (to[e] >> 3), v[e]);
         }
     }
     if (a.dst || rank == 0) {
@@ -261,11 +302,11 @@ extern "C" int b2_paged_kv_evict(const b2_paged_kv* kv, float* scores, const int
     a.kept = kept;
     a.new_lens = new_lens;
     const int64_t span = (int64_t)kv->max_blocks * kv->block_size;
-    a.cached = (int)(span < kEvCached ? span : kEvCached);
+    a.cached = (int)(span < kEvCached ? (span + 3) & ~int64_t(3) : kEvCached);
     cudaStream_t s = as_stream(stream);
     B2_TRY(cudaFuncSetAttribute(evict_choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvCached * 4));
     B2_TRY(launch(evict_choose_kernel, dim3(nkv, batch), dim3(kEvThreads), (size_t)a.cached * sizeof(float), s, true, a));
     const int64_t parts = dst_tables ? ((int64_t)budget + kMvRows - 1) / kMvRows : kMvSlices;
-    B2_TRY(launch(evict_move_kernel, dim3((unsigned)parts, nkv, batch), dim3(kMvThreads), 0, s, true, a));
+    B2_TRY(launch(evict_move_kernel, dim3(nkv, (unsigned)parts, batch), dim3(kMvThreads), 0, s, true, a));
     return B2_OK;
 }
