@@ -17,6 +17,22 @@ inline int check_paged(const b2_paged_kv* kv, int nkv, int D) {
     return B2_OK;
 }
 
+// Division of positions (below 2^30) by the block size: one wide multiply
+// instead of a divide.  m = floor(2^(30 + s) / d) + 1 with 2^s >= d gives
+// floor(x / d) for every x < 2^30: the excess x (m d - 2^(30+s)) / (d 2^(30+s))
+// is below 2^30 d / (d 2^(30+s)) <= 1 / d.
+struct BlockDiv {
+    uint32_t m;
+    int shift, d;
+    __device__ __forceinline__ int block(int pos) const { return (int)(((uint64_t)(uint32_t)pos * m) >> shift); }
+    __device__ __forceinline__ int slot(int pos, int block) const { return pos - block * d; }
+};
+inline BlockDiv block_div(int d) {
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    return BlockDiv{(uint32_t)((1ull << (30 + s)) / (unsigned)d + 1), 30 + s, d};
+}
+
 // Length of sequence b, cut to what its table row can hold.
 __device__ __forceinline__ int paged_len(const b2_paged_kv& kv, int b) {
     return max(0, min(kv.seq_lens[b], kv.max_blocks * kv.block_size));

@@ -48,6 +48,7 @@ struct PagedArgs {
     const void* q;
     int64_t ldq;
     b2_paged_kv kv;
+    BlockDiv div;
     void* out;
     float* scores;
     int batch, nq, nkv, D, group, hg, gs, window, sinks;
@@ -167,19 +168,24 @@ struct Seen {
     __device__ __forceinline__ bool sees(int u, int pos) const { return u < ns ? pos < s0 : pos >= lo && pos < L; }
 };
 
-// A place in the list of all units: segment hh (kv head x head group) of
-// sequence b, unit u of it.
+// A place in the list of all units: head group g of kv head kvh of sequence b,
+// unit u of that segment.
 template <int U>
 struct Place {
-    int b, hh, u;
+    int b, kvh, g, u;
     Seen<U> s;
     __device__ __forceinline__ void next(const PagedArgs& a) {
         if (++u < s.n) return;
         u = 0;
-        if (++hh < a.nkv * a.hg) return;
-        hh = 0;
+        if (++g < a.hg) return;
+        g = 0;
+        if (++kvh < a.nkv) return;
+        kvh = 0;
         if (++b < a.batch) s.of(a, b);
     }
+    // First query head of the segment, and how many it has.
+    __device__ __forceinline__ int head0(const PagedArgs& a) const { return kvh * a.group + g * a.gs; }
+    __device__ __forceinline__ int heads(const PagedArgs& a) const { return min(a.gs, a.group - g * a.gs); }
 };
 
 template <int DP, bool GH, bool BF16>
@@ -246,8 +252,12 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
     Place<U> at;
     at.b = s_b;
     at.s.of(a, at.b);
-    at.hh = (r0 - s_before) / at.s.n;
-    at.u = (r0 - s_before) - at.hh * at.s.n;
+    {
+        const int hh = (r0 - s_before) / at.s.n;
+        at.u = (r0 - s_before) - hh * at.s.n;
+        at.kvh = hh / a.hg;
+        at.g = hh - at.kvh * a.hg;
+    }
     if (!a.counters) {  // whole segments only: those that begin in the range
         if (at.u > 0) {
             r0 += at.s.n - at.u;
@@ -273,7 +283,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
         pid = -1;
         if (pr < r1) {
             const int pos = pp.s.base(pp.u) + warp * TP + (lane & (TP - 1));
-            if (pp.s.sees(pp.u, pos)) pid = a.kv.block_tables[(int64_t)pp.b * a.kv.max_blocks + (unsigned)pos / (unsigned)a.kv.block_size];
+            if (pp.s.sees(pp.u, pos)) pid = a.kv.block_tables[(int64_t)pp.b * a.kv.max_blocks + a.div.block(pos)];
         }
     };
     const uint32_t ring = smem_addr(smem) + warp * kPgStages * C::STAGE;
@@ -282,8 +292,8 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
         if (pr < r1) {
             const int pos = pp.s.base(pp.u) + warp * TP + (lane & (TP - 1));
             const bool there = (unsigned)pid < (unsigned)a.kv.num_blocks;
-            const int64_t off = (int64_t)pid * a.kv.stride_block + (int64_t)((unsigned)pos % (unsigned)a.kv.block_size) * a.kv.stride_slot +
-                                (pp.hh / a.hg) * a.kv.stride_head;
+            const int64_t off = (int64_t)pid * a.kv.stride_block + (int64_t)a.div.slot(pos, a.div.block(pos)) * a.kv.stride_slot +
+                                (int64_t)pp.kvh * a.kv.stride_head;
             const uint32_t mask = __ballot_sync(~0u, there);
             if (lane == 0) s_there[warp][stage] = mask;
             const uint32_t st = ring + stage * C::STAGE;
@@ -314,8 +324,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
     uint32_t qa[DP / 16][GH ? 4 : 2];
     float o[DP / 8][GH ? 4 : 2], m0, m1, l0, l1;
     auto start = [&]() {  // a new segment (or the rest of one): its queries, nothing summed yet
-        const int kvh = at.hh / a.hg, h0 = kvh * a.group + (at.hh - kvh * a.hg) * a.gs;
-        const int nh = min(a.gs, (kvh + 1) * a.group - h0);
+        const int h0 = at.head0(a), nh = at.heads(a);
         const uint16_t* q = static_cast<const uint16_t*>(a.q) + at.b * a.ldq + (int64_t)h0 * a.D;
         const int r = lane >> 2, k = (lane & 3) * 2;
 #pragma unroll
@@ -370,8 +379,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
                     for (int e = 0; e < 4; ++e)
                         s[n][e] = (tm >> (n * 8 + col + (e & 1))) & 1 ? s[n][e] * a.scale_log2 : -INFINITY;
                 if (a.logits) {
-                    const int kvh = at.hh / a.hg, h0 = kvh * a.group + (at.hh - kvh * a.hg) * a.gs;
-                    const int nh = min(a.gs, (kvh + 1) * a.group - h0);
+                    const int h0 = at.head0(a), nh = at.heads(a);
                     float* lg = a.logits + ((int64_t)at.b * a.nq + h0 + (lane >> 2)) * a.cap + at.u * U + warp * TP +
                                 t * 16 + col;
 #pragma unroll
@@ -494,8 +502,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
                 }
                 __syncthreads();
             }
-            const int kvh = at.hh / a.hg, h0 = kvh * a.group + (at.hh - kvh * a.hg) * a.gs;
-            const int nh = min(a.gs, (kvh + 1) * a.group - h0);
+            const int h0 = at.head0(a), nh = at.heads(a);
             auto sum = [&](int row, int d) {
                 float v = s_o[row * C::LDO + d];
                 if (C::NB == 2) v += s_o[(G + row) * C::LDO + d];
@@ -580,12 +587,12 @@ __global__ void __launch_bounds__(256) paged_scores_kernel(const PagedArgs a) {
     if (u >= s.n) return;
     const int pos = s.base(u) + i - u * U;
     if (!s.sees(u, pos)) return;
-    const int bs = a.kv.block_size, blk = a.kv.block_tables[(int64_t)b * a.kv.max_blocks + pos / bs];
+    const int bs = a.kv.block_size, at = a.div.block(pos), blk = a.kv.block_tables[(int64_t)b * a.kv.max_blocks + at];
     if ((unsigned)blk >= (unsigned)a.kv.num_blocks) return;
     const float* lg = a.logits + ((int64_t)b * a.nq + kvh * a.group) * a.cap + i;
     float w = 0.f;
     for (int h = 0; h < a.group; ++h) w = fmaf(ex2(__ldcs(lg + (int64_t)h * a.cap) - s_st[h].x), s_st[h].y, w);
-    float* sc = a.scores + ((int64_t)blk * a.nkv + kvh) * bs + pos % bs;
+    float* sc = a.scores + ((int64_t)blk * a.nkv + kvh) * bs + a.div.slot(pos, at);
     *sc = pos == s.L - 1 ? w : *sc + w;
 }
 
@@ -663,6 +670,7 @@ extern "C" int b2_paged_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv
     a.q = q;
     a.ldq = ldq;
     a.kv = *kv;
+    a.div = block_div(kv->block_size);
     a.out = out;
     a.scores = scores;
     a.batch = batch;
