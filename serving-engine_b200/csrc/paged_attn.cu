@@ -53,6 +53,7 @@ struct PagedArgs {
     float* scores;
     int batch, nq, nkv, D, group, hg, gs, window, sinks;
     float scale_log2;
+    int whole;      // blocks are whole groups of 16 positions
     float* parts;   // [2 * grid][gs][D], unnormalised partial outputs
     float2* pml;    // [2 * grid][gs], their (max, sum)
     int* counters;  // [grid], null: segments are not cut
@@ -298,16 +299,35 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
             if (lane == 0) s_there[warp][stage] = mask;
             const uint32_t st = ring + stage * C::STAGE;
             const uint16_t *K = static_cast<const uint16_t*>(a.kv.k), *V = static_cast<const uint16_t*>(a.kv.v);
+            if (mask == ~0u && a.whole && a.D == DP) {
+                // every 16 rows are consecutive slots of one block: one address and a stride
+                constexpr int STEP = 32 / C::CH;  // rows per instruction
 #pragma unroll
-            for (int i = 0; i < TP * C::CH / 32; ++i) {
-                const int r = lane / C::CH + i * (32 / C::CH);
-                const int64_t ro = __shfl_sync(~0u, off, r);
-                const bool ok = (mask >> r) & 1;
-                if (chunk * 8 < a.D) {
-                    const uint32_t d = st + r * C::ROW + ((chunk ^ (r & 7)) << 4);
-                    const int64_t so = ok ? ro + chunk * 8 : 0;
-                    cp16(d, K + so, ok);
-                    cp16(d + TP * C::ROW, V + so, ok);
+                for (int t = 0; t < TP / 16; ++t) {
+                    const int64_t o0 = __shfl_sync(~0u, off, 16 * t) + (lane / C::CH) * a.kv.stride_slot + chunk * 8;
+                    const uint16_t *kp = K + o0, *vp = V + o0;
+                    uint32_t d = st + (16 * t + lane / C::CH) * C::ROW;
+#pragma unroll
+                    for (int i = 0; i < 16 / STEP; ++i) {
+                        const uint32_t x = d + i * STEP * C::ROW + ((chunk ^ ((lane / C::CH + i * STEP) & 7)) << 4);
+                        cp16(x, kp, true);
+                        cp16(x + TP * C::ROW, vp, true);
+                        kp += STEP * a.kv.stride_slot;
+                        vp += STEP * a.kv.stride_slot;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < TP * C::CH / 32; ++i) {
+                    const int r = lane / C::CH + i * (32 / C::CH);
+                    const int64_t ro = __shfl_sync(~0u, off, r);
+                    const bool ok = (mask >> r) & 1;
+                    if (chunk * 8 < a.D) {
+                        const uint32_t d = st + r * C::ROW + ((chunk ^ (r & 7)) << 4);
+                        const int64_t so = ok ? ro + chunk * 8 : 0;
+                        cp16(d, K + so, ok);
+                        cp16(d + TP * C::ROW, V + so, ok);
+                    }
                 }
             }
             ++pr;
@@ -683,6 +703,7 @@ extern "C" int b2_paged_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv
     a.window = window;
     a.sinks = sinks;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)D);
+    a.whole = kv->block_size % 16 == 0;
     a.cap = (int)z.cap;
     if (ws) {
         if (ws->bytes < z.parts + z.pml + z.stats + z.logits || z.grid > kWsCounters) return B2_ERR_WORKSPACE;
