@@ -9,10 +9,13 @@
 // kv head) for up to 4 D G flops (G heads of the group), so HBM bounds it.
 //
 // Split.  A (sequence, kv head, group of up to 16 heads) is a segment of
-// units of U positions; all segments' units, end to end, are cut into equal
-// ranges, one per CTA of a grid that is resident at once (stream-K).  Every SM
-// so streams the same bytes whatever the batch, the heads and the lengths.  A
-// CTA whose range covers a segment writes its outputs; a segment cut between
+// units of U positions.  Every CTA of a grid that is resident at once takes an
+// equal share of the units, in one of two ways.  Pieces: every segment is cut
+// into pieces of the same size, one per CTA, when a size within an eighth (or
+// two units) of the even share gives no more pieces than CTAs -- one segment
+// end per CTA.  Stream-K otherwise: all units end to end, cut evenly, whatever
+// the lengths -- up to three segment ends per CTA but no idle ones.
+// A CTA that covers a segment writes its outputs; a segment cut between
 // CTAs leaves a partial (max, sum, unnormalised output) per piece in the
 // workspace, and the CTA that arrives last at the segment's counter adds the
 // pieces in order (same bits whoever is last).
@@ -140,9 +143,9 @@ __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t
     lo = pack16<BF16>(a - f.x, b - f.y);
 }
 template <bool BF16>
-__device__ __forceinline__ void store16(void* p, int64_t i, float v) {
-    if constexpr (BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(p)[i] = __float2half_rn(v);
+__device__ __forceinline__ void store4(void* p, int64_t i, float4 v, float scale) {
+    const uint2 x = make_uint2(pack16<BF16>(v.x * scale, v.y * scale), pack16<BF16>(v.z * scale, v.w * scale));
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = x;
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
     using C = PagedCfg<DP, GH>;
     constexpr int U = C::U, TP = C::TP, G = C::G;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int s_scan[kPgWarps];
+    __shared__ int s_scan[kPgWarps], s_count[kPgWarps][8];
     __shared__ int s_b, s_before, s_last;
     __shared__ uint32_t s_there[kPgWarps][kPgStages];
     __shared__ float s_m[kPgWarps][16], s_l[kPgWarps][16];
@@ -208,56 +211,98 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
     if (a.D < DP)
         for (int i = tid; i < C::OFF_O / 16; i += kPgThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     griddep_wait();
+    griddep_launch_dependents();
 
     // ---- this CTA's range of units, and the place where it starts
     const int per = (a.batch + kPgThreads - 1) / kPgThreads;
     const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-    int mine = 0;
-    for (int b = b0; b < b1; ++b) {
-        Seen<U> s;
-        s.of(a, b);
-        mine += s.n * heads;
-    }
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(~0u, incl, o);
-        if (lane >= o) incl += v;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int w = 0; w < kPgWarps; ++w) {
-        if (w < warp) incl += s_scan[w];
-        total += s_scan[w];
-    }
-    const int upc = max(kPgMinUnits, (total + (int)gridDim.x - 1) / (int)gridDim.x);
-    int r0 = c * upc, r1 = min(total, r0 + upc);
-    if (c >= (total + upc - 1) / upc) return;
-    {
-        int before = incl - mine;
-        if (r0 >= before && r0 < incl) {  // one thread
-            int b = b0;
-            for (;; ++b) {
-                Seen<U> s;
-                s.of(a, b);
-                if (r0 < before + s.n * heads) break;
-                before += s.n * heads;
-            }
-            s_b = b;
-            s_before = before;
+    // Sum of count(units) over the sequences before this thread's own, and over all of them; every thread calls it.
+    auto scan = [&](auto count, int& total) -> int2 {
+        int mine = 0;
+        for (int b = b0; b < b1; ++b) {
+            Seen<U> s;
+            s.of(a, b);
+            mine += count(s.n);
         }
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(~0u, incl, o);
+            if (lane >= o) incl += v;
+        }
+        __syncthreads();
+        if (lane == 31) s_scan[warp] = incl;
+        __syncthreads();
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < kPgWarps; ++w) {
+            if (w < warp) incl += s_scan[w];
+            total += s_scan[w];
+        }
+        return make_int2(incl - mine, incl);
+    };
+    int total = 0;
+    int2 span = scan([&](int n) { return n * heads; }, total);
+    const int grid = (int)gridDim.x;
+    int upc = max(kPgMinUnits, (total + grid - 1) / grid);
+    // size of equal pieces: the smallest of 8 candidates that gives at most a piece per CTA
+    bool pieced = false;
+    if (a.counters && (int64_t)a.batch * heads <= grid) {
+        const int step = (upc + 63) / 64, size = upc + (tid & 7) * step;
+        int n = 0;
+        for (int b = tid >> 3; b < a.batch; b += kPgThreads / 8) {
+            Seen<U> s;
+            s.of(a, b);
+            n += (s.n + size - 1) / size * heads;
+        }
+        n += __shfl_xor_sync(~0u, n, 8);
+        n += __shfl_xor_sync(~0u, n, 16);
+        if (lane < 8) s_count[warp][lane] = n;
+        __syncthreads();
+        for (int k = 7; k >= 0; --k) {
+            int all = 0;
+#pragma unroll
+            for (int w = 0; w < kPgWarps; ++w) all += s_count[w][k];
+            if (all <= grid && k * step <= max(2, upc / 8)) {
+                pieced = true;
+                n = k;
+            }
+        }
+        if (pieced) {
+            upc += n * step;
+            span = scan([&](int n) { return (n + upc - 1) / upc * heads; }, total);
+        }
+    }
+    // what this CTA starts with, counted in pieces or in units
+    const int first = pieced ? c : c * upc;
+    if (first >= total) return;
+    if (first >= span.x && first < span.y) {  // one thread
+        int b = b0, before = span.x;
+        for (;; ++b) {
+            Seen<U> s;
+            s.of(a, b);
+            const int here = (pieced ? (s.n + upc - 1) / upc : s.n) * heads;
+            if (first < before + here) break;
+            before += here;
+        }
+        s_b = b;
+        s_before = before;
     }
     __syncthreads();
     Place<U> at;
     at.b = s_b;
     at.s.of(a, at.b);
+    int r0, r1;         // units, counted from the first one of the segment or of all
+    int cf, pieces;     // first CTA of the segment and how many share it (pieces only)
     {
-        const int hh = (r0 - s_before) / at.s.n;
-        at.u = (r0 - s_before) - hh * at.s.n;
+        pieces = pieced ? (at.s.n + upc - 1) / upc : at.s.n;
+        const int hh = (first - s_before) / pieces, rest = first - s_before - hh * pieces;
+        cf = c - rest;
+        at.u = pieced ? rest * upc : rest;
         at.kvh = hh / a.hg;
         at.g = hh - at.kvh * a.hg;
+        r0 = pieced ? at.u : first;
+        r1 = min(pieced ? at.s.n : total, r0 + upc);
     }
     if (!a.counters) {  // whole segments only: those that begin in the range
         if (at.u > 0) {
@@ -343,6 +388,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
     // ---- consumer
     uint32_t qa[DP / 16][GH ? 4 : 2];
     float o[DP / 8][GH ? 4 : 2], m0, m1, l0, l1;
+    float* logits = nullptr;  // where this lane's of the segment go
     auto start = [&]() {  // a new segment (or the rest of one): its queries, nothing summed yet
         const int h0 = at.head0(a), nh = at.heads(a);
         const uint16_t* q = static_cast<const uint16_t*>(a.q) + at.b * a.ldq + (int64_t)h0 * a.D;
@@ -360,6 +406,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
             for (int e = 0; e < (GH ? 4 : 2); ++e) o[n][e] = 0.f;
         m0 = m1 = -INFINITY;
         l0 = l1 = 0.f;
+        if (a.logits) logits = a.logits + ((int64_t)at.b * a.nq + h0 + (lane >> 2)) * a.cap + warp * TP + (lane & 3) * 2;
     };
 
     start();
@@ -399,9 +446,8 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
                     for (int e = 0; e < 4; ++e)
                         s[n][e] = (tm >> (n * 8 + col + (e & 1))) & 1 ? s[n][e] * a.scale_log2 : -INFINITY;
                 if (a.logits) {
-                    const int h0 = at.head0(a), nh = at.heads(a);
-                    float* lg = a.logits + ((int64_t)at.b * a.nq + h0 + (lane >> 2)) * a.cap + at.u * U + warp * TP +
-                                t * 16 + col;
+                    const int nh = at.heads(a);
+                    float* lg = logits + at.u * U + t * 16;
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
                         if ((lane >> 2) < nh) *reinterpret_cast<float2*>(lg + n * 8) = make_float2(s[n][0], s[n][1]);
@@ -523,57 +569,71 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
                 __syncthreads();
             }
             const int h0 = at.head0(a), nh = at.heads(a);
-            auto sum = [&](int row, int d) {
-                float v = s_o[row * C::LDO + d];
-                if (C::NB == 2) v += s_o[(G + row) * C::LDO + d];
+            auto sum = [&](int row, int d) -> float4 {
+                float4 v = *reinterpret_cast<const float4*>(s_o + row * C::LDO + d);
+                if (C::NB == 2) {
+                    const float4 x = *reinterpret_cast<const float4*>(s_o + (G + row) * C::LDO + d);
+                    v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+                }
                 return v;
             };
             const int64_t oat = ((int64_t)at.b * a.nq + h0) * a.D;
             const int seg0 = r - at.u;  // first unit of the segment
+            const int quads = a.D / 4;
             if (done && piece0 == seg0) {
-                for (int i = tid; i < nh * a.D; i += kPgThreads) {
-                    const int row = i / a.D, d = i - row * a.D;
+                for (int i = tid; i < nh * quads; i += kPgThreads) {
+                    const int row = i / quads, d = (i - row * quads) * 4;
                     const float Ls = s_ml[row].y;
-                    store16<BF16>(a.out, oat + i, Ls > 0.f ? sum(row, d) / Ls : 0.f);
+                    store4<BF16>(a.out, oat + row * a.D + d, sum(row, d), Ls > 0.f ? 1.f / Ls : 0.f);
                 }
                 if (a.stats && tid < nh) a.stats[(int64_t)at.b * a.nq + h0 + tid] = s_ml[tid];
             } else {
                 const int slot = 2 * c + (piece0 == seg0 ? 1 : 0);
                 float* part = a.parts + (int64_t)slot * a.gs * a.D;
-                for (int i = tid; i < nh * a.D; i += kPgThreads) part[i] = sum(i / a.D, i % a.D);
+                for (int i = tid; i < nh * quads; i += kPgThreads) {
+                    const int row = i / quads, d = (i - row * quads) * 4;
+                    *reinterpret_cast<float4*>(part + row * a.D + d) = sum(row, d);
+                }
                 if (tid < nh) a.pml[(int64_t)slot * a.gs + tid] = s_ml[tid];
                 __threadfence();
                 __syncthreads();
-                const int cf = seg0 / upc, pieces = (seg0 + at.s.n - 1) / upc - cf + 1;
+                if (!pieced) {
+                    cf = seg0 / upc;
+                    pieces = (seg0 + at.s.n - 1) / upc - cf + 1;
+                }
                 if (tid == 0) s_last = atomicAdd(a.counters + cf, 1) == pieces - 1;
                 __syncthreads();
                 if (s_last) {
-                    // ---- last of the segment's CTAs: its pieces in order
+                    // ---- last of the segment's CTAs: its pieces in order.  Piece p is in slot 2 (cf + p), the first
+                    // one in the slot after
                     __threadfence();
                     if (tid == 0) a.counters[cf] = 0;
+                    const float2* ml0 = a.pml + (int64_t)2 * cf * a.gs;
+                    const float* part0 = a.parts + (int64_t)2 * cf * a.gs * a.D;
                     for (int row = warp; row < nh; row += kPgWarps) {
                         float M = -1e30f, Ls = 0.f;
-                        for (int p = lane; p < pieces; p += 32)
-                            M = fmaxf(M, __ldcg(&a.pml[(int64_t)(2 * (cf + p) + (p == 0)) * a.gs + row].x));
+                        for (int p = lane; p < pieces; p += 32) M = fmaxf(M, __ldcg(&ml0[(2 * p + (p == 0)) * a.gs + row].x));
                         M = warp_max(M);
                         for (int p = lane; p < pieces; p += 32) {
-                            const float2 ml = __ldcg(&a.pml[(int64_t)(2 * (cf + p) + (p == 0)) * a.gs + row]);
+                            const float2 ml = __ldcg(&ml0[(2 * p + (p == 0)) * a.gs + row]);
                             Ls = fmaf(ml.y, ex2(ml.x - M), Ls);
                         }
                         Ls = warp_sum(Ls);
                         if (lane == 0) s_ml[row] = make_float2(M, Ls);
                     }
                     __syncthreads();
-                    for (int i = tid; i < nh * a.D; i += kPgThreads) {
-                        const int row = i / a.D;
+                    for (int i = tid; i < nh * quads; i += kPgThreads) {
+                        const int row = i / quads, d = (i - row * quads) * 4;
                         const float2 ml = s_ml[row];
-                        float v = 0.f;
-#pragma unroll 4
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
                         for (int p = 0; p < pieces; ++p) {
-                            const int64_t sl = (int64_t)(2 * (cf + p) + (p == 0)) * a.gs;
-                            v = fmaf(__ldcg(&a.parts[sl * a.D + i]), ex2(__ldcg(&a.pml[sl + row].x) - ml.x), v);
+                            const int64_t sl = (int64_t)(2 * p + (p == 0)) * a.gs + row;
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(part0 + sl * a.D + d));
+                            const float w = ex2(__ldcg(&ml0[sl].x) - ml.x);
+                            v = make_float4(fmaf(x.x, w, v.x), fmaf(x.y, w, v.y), fmaf(x.z, w, v.z), fmaf(x.w, w, v.w));
                         }
-                        store16<BF16>(a.out, oat + i, ml.y > 0.f ? v / ml.y : 0.f);
+                        store4<BF16>(a.out, oat + row * a.D + d, v, ml.y > 0.f ? 1.f / ml.y : 0.f);
                     }
                     if (a.stats && tid < nh) a.stats[(int64_t)at.b * a.nq + h0 + tid] = s_ml[tid];
                 }
@@ -588,32 +648,47 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
     }
 }
 
-// One thread per stored logit column: the weights its position gets from the
-// group's heads, in head order, onto its score.
+// One thread per 4 stored logit columns: the weights their positions get from
+// the group's heads, in head order, onto their scores.
 template <int U>
 __global__ void __launch_bounds__(256) paged_scores_kernel(const PagedArgs a) {
-    extern __shared__ float2 s_st[];  // [group] (max, 1 / sum)
     griddep_wait();
+    griddep_launch_dependents();
     const int kvh = blockIdx.y, b = blockIdx.z;
     Seen<U> s;
     s.of(a, b);
-    if ((int)(blockIdx.x * blockDim.x) >= s.n * U) return;
-    for (int h = threadIdx.x; h < a.group; h += blockDim.x) {
-        const float2 st = a.stats[(int64_t)b * a.nq + kvh * a.group + h];
-        s_st[h] = make_float2(st.x, st.y > 0.f ? 1.f / st.y : 0.f);
-    }
-    __syncthreads();
-    const int i = blockIdx.x * blockDim.x + threadIdx.x, u = i / U;
+    const int i = (blockIdx.x * blockDim.x + threadIdx.x) * 4, u = i / U;
     if (u >= s.n) return;
-    const int pos = s.base(u) + i - u * U;
-    if (!s.sees(u, pos)) return;
-    const int bs = a.kv.block_size, at = a.div.block(pos), blk = a.kv.block_tables[(int64_t)b * a.kv.max_blocks + at];
-    if ((unsigned)blk >= (unsigned)a.kv.num_blocks) return;
-    const float* lg = a.logits + ((int64_t)b * a.nq + kvh * a.group) * a.cap + i;
-    float w = 0.f;
-    for (int h = 0; h < a.group; ++h) w = fmaf(ex2(__ldcs(lg + (int64_t)h * a.cap) - s_st[h].x), s_st[h].y, w);
-    float* sc = a.scores + ((int64_t)blk * a.nkv + kvh) * bs + a.div.slot(pos, at);
-    *sc = pos == s.L - 1 ? w : *sc + w;
+    const int pos0 = s.base(u) + i - u * U, bs = a.kv.block_size;
+    float* sc[4];
+    float old[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        sc[e] = nullptr;
+        if (!s.sees(u, pos0 + e)) continue;
+        const int at = a.div.block(pos0 + e), blk = a.kv.block_tables[(int64_t)b * a.kv.max_blocks + at];
+        if ((unsigned)blk < (unsigned)a.kv.num_blocks)
+            sc[e] = a.scores + ((int64_t)blk * a.nkv + kvh) * bs + a.div.slot(pos0 + e, at);
+    }
+    if (!sc[0] && !sc[1] && !sc[2] && !sc[3]) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (sc[e] && pos0 + e != s.L - 1) old[e] = *sc[e];
+    const int h0 = b * a.nq + kvh * a.group;
+    const float* lg = a.logits + (int64_t)h0 * a.cap + i;
+#pragma unroll 8
+    for (int h = 0; h < a.group; ++h) {
+        const float4 x = __ldcs(reinterpret_cast<const float4*>(lg + (int64_t)h * a.cap));
+        const float2 st = a.stats[h0 + h];
+        const float inv = st.y > 0.f ? 1.f / st.y : 0.f;
+        w[0] = fmaf(ex2(x.x - st.x), inv, w[0]);
+        w[1] = fmaf(ex2(x.y - st.x), inv, w[1]);
+        w[2] = fmaf(ex2(x.z - st.x), inv, w[2]);
+        w[3] = fmaf(ex2(x.w - st.x), inv, w[3]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (sc[e]) *sc[e] = old[e] + w[e];
 }
 
 // ---------------------------------------------------------------------------
@@ -649,8 +724,8 @@ static int paged_launch(const PagedArgs& a, const PagedSizes& z, cudaStream_t s)
     B2_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
     B2_TRY(launch(kern, dim3(z.grid), dim3(kPgThreads), C::BYTES, s, true, a));
     if (a.scores)
-        B2_TRY(launch(paged_scores_kernel<C::U>, dim3((unsigned)((a.cap + 255) / 256), a.nkv, a.batch), dim3(256),
-                      a.group * sizeof(float2), s, true, a));
+        B2_TRY(launch(paged_scores_kernel<C::U>, dim3((unsigned)((a.cap + 1023) / 1024), a.nkv, a.batch), dim3(256), 0, s,
+                      true, a));
     return B2_OK;
 }
 
@@ -684,7 +759,7 @@ extern "C" int b2_paged_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv
     const PagedSizes z = paged_sizes(batch, nq, nkv, D, most, scores != nullptr);
     // units are counted in 32 bits; the scores' grid has (nkv, batch) as (y, z)
     if ((int64_t)batch * nkv * z.hg * ((most >> 6) + 4) > (1ll << 31) - 1 ||
-        (scores && (batch > 65535 || nkv > 65535 || nq / nkv > 4096)))
+        (scores && (batch > 65535 || nkv > 65535)))
         return B2_ERR_UNSUPPORTED;
     PagedArgs a = {};
     a.q = q;
