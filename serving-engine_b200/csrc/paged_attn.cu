@@ -214,89 +214,125 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
     griddep_launch_dependents();
 
     // ---- this CTA's range of units, and the place where it starts
-    const int per = (a.batch + kPgThreads - 1) / kPgThreads;
-    const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-    // Sum of count(units) over the sequences before this thread's own, and over all of them; every thread calls it.
-    auto scan = [&](auto count, int& total) -> int2 {
-        int mine = 0;
-        for (int b = b0; b < b1; ++b) {
-            Seen<U> s;
-            s.of(a, b);
-            mine += count(s.n);
+    const int grid = (int)gridDim.x;
+    int total, upc, first;   // units of all segments (or pieces); units per CTA; what this CTA starts with
+    bool pieced = false;     // equal pieces: first counts pieces, else units
+    int fb, fbefore;         // the sequence it lies in, what lies before that
+    const bool can_piece = a.counters && (int64_t)a.batch * heads <= grid;
+    // the k-th candidate for the size of equal pieces; those up to an eighth or two units above the even share are taken
+    auto size_of = [&](int k) { return upc + k * ((upc + 63) / 64); };
+    auto near = [&](int k) { return k * ((upc + 63) / 64) <= max(2, upc / 8); };
+    if (a.batch <= 32) {
+        // every warp by itself, lane b for sequence b
+        Seen<U> s;
+        s.n = 0;
+        if (lane < a.batch) s.of(a, lane);
+        total = __reduce_add_sync(~0u, s.n) * heads;
+        upc = max(kPgMinUnits, (total + grid - 1) / grid);
+        int here = s.n * heads;
+        if (can_piece) {
+            int pick = -1;
+#pragma unroll
+            for (int k = 7; k >= 0; --k)
+                if (near(k) && (int)__reduce_add_sync(~0u, (unsigned)(s.n + size_of(k) - 1) / (unsigned)size_of(k)) * heads <= grid)
+                    pick = k;
+            if (pick >= 0) {
+                pieced = true;
+                upc = size_of(pick);
+                here = (int)((unsigned)(s.n + upc - 1) / (unsigned)upc) * heads;
+            }
         }
-        int incl = mine;
+        int incl = here;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(~0u, incl, o);
             if (lane >= o) incl += v;
         }
-        __syncthreads();
-        if (lane == 31) s_scan[warp] = incl;
-        __syncthreads();
-        total = 0;
+        total = __shfl_sync(~0u, incl, 31);
+        first = pieced ? c : c * upc;
+        if (first >= total) return;
+        fb = __ffs(__ballot_sync(~0u, incl > first)) - 1;
+        fbefore = __shfl_sync(~0u, incl - here, fb);
+    } else {
+        const int per = (a.batch + kPgThreads - 1) / kPgThreads;
+        const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
+        // Sum of count(units) over the sequences before this thread's own and with them, and over all.
+        auto scan = [&](auto count) -> int2 {
+            int mine = 0;
+            for (int b = b0; b < b1; ++b) {
+                Seen<U> s;
+                s.of(a, b);
+                mine += count(s.n);
+            }
+            int incl = mine;
 #pragma unroll
-        for (int w = 0; w < kPgWarps; ++w) {
-            if (w < warp) incl += s_scan[w];
-            total += s_scan[w];
-        }
-        return make_int2(incl - mine, incl);
-    };
-    int total = 0;
-    int2 span = scan([&](int n) { return n * heads; }, total);
-    const int grid = (int)gridDim.x;
-    int upc = max(kPgMinUnits, (total + grid - 1) / grid);
-    // size of equal pieces: the smallest of 8 candidates that gives at most a piece per CTA
-    bool pieced = false;
-    if (a.counters && (int64_t)a.batch * heads <= grid) {
-        const int step = (upc + 63) / 64, size = upc + (tid & 7) * step;
-        int n = 0;
-        for (int b = tid >> 3; b < a.batch; b += kPgThreads / 8) {
-            Seen<U> s;
-            s.of(a, b);
-            n += (s.n + size - 1) / size * heads;
-        }
-        n += __shfl_xor_sync(~0u, n, 8);
-        n += __shfl_xor_sync(~0u, n, 16);
-        if (lane < 8) s_count[warp][lane] = n;
-        __syncthreads();
-        for (int k = 7; k >= 0; --k) {
-            int all = 0;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(~0u, incl, o);
+                if (lane >= o) incl += v;
+            }
+            __syncthreads();
+            if (lane == 31) s_scan[warp] = incl;
+            __syncthreads();
+            total = 0;
 #pragma unroll
-            for (int w = 0; w < kPgWarps; ++w) all += s_count[w][k];
-            if (all <= grid && k * step <= max(2, upc / 8)) {
+            for (int w = 0; w < kPgWarps; ++w) {
+                if (w < warp) incl += s_scan[w];
+                total += s_scan[w];
+            }
+            return make_int2(incl - mine, incl);
+        };
+        int2 span = scan([&](int n) { return n * heads; });
+        upc = max(kPgMinUnits, (total + grid - 1) / grid);
+        if (can_piece) {
+            const int size = size_of(tid & 7);
+            int n = 0, pick = -1;
+            for (int b = tid >> 3; b < a.batch; b += kPgThreads / 8) {
+                Seen<U> s;
+                s.of(a, b);
+                n += (s.n + size - 1) / size * heads;
+            }
+            n += __shfl_xor_sync(~0u, n, 8);
+            n += __shfl_xor_sync(~0u, n, 16);
+            if (lane < 8) s_count[warp][lane] = n;
+            __syncthreads();
+            for (int k = 7; k >= 0; --k) {
+                int all = 0;
+#pragma unroll
+                for (int w = 0; w < kPgWarps; ++w) all += s_count[w][k];
+                if (all <= grid && near(k)) pick = k;
+            }
+            if (pick >= 0) {
                 pieced = true;
-                n = k;
+                upc = size_of(pick);
+                span = scan([&](int n) { return (n + upc - 1) / upc * heads; });
             }
         }
-        if (pieced) {
-            upc += n * step;
-            span = scan([&](int n) { return (n + upc - 1) / upc * heads; }, total);
+        first = pieced ? c : c * upc;
+        if (first >= total) return;
+        if (first >= span.x && first < span.y) {  // one thread
+            int b = b0, before = span.x;
+            for (;; ++b) {
+                Seen<U> s;
+                s.of(a, b);
+                const int here = (pieced ? (s.n + upc - 1) / upc : s.n) * heads;
+                if (first < before + here) break;
+                before += here;
+            }
+            s_b = b;
+            s_before = before;
         }
+        __syncthreads();
+        fb = s_b;
+        fbefore = s_before;
     }
-    // what this CTA starts with, counted in pieces or in units
-    const int first = pieced ? c : c * upc;
-    if (first >= total) return;
-    if (first >= span.x && first < span.y) {  // one thread
-        int b = b0, before = span.x;
-        for (;; ++b) {
-            Seen<U> s;
-            s.of(a, b);
-            const int here = (pieced ? (s.n + upc - 1) / upc : s.n) * heads;
-            if (first < before + here) break;
-            before += here;
-        }
-        s_b = b;
-        s_before = before;
-    }
-    __syncthreads();
     Place<U> at;
-    at.b = s_b;
+    at.b = fb;
     at.s.of(a, at.b);
     int r0, r1;         // units, counted from the first one of the segment or of all
     int cf, pieces;     // first CTA of the segment and how many share it (pieces only)
     {
         pieces = pieced ? (at.s.n + upc - 1) / upc : at.s.n;
-        const int hh = (first - s_before) / pieces, rest = first - s_before - hh * pieces;
+        const int hh = (first - fbefore) / pieces, rest = first - fbefore - hh * pieces;
         cf = c - rest;
         at.u = pieced ? rest * upc : rest;
         at.kvh = hh / a.hg;
@@ -322,24 +358,27 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
         r1 = r;
     }
 
-    // ---- producer: rows of the unit at `pp` into a stage
+    // ---- producer: rows of the next unit into a stage.  The table entries of the two next units are on their way:
+    // lane l's is that of row l % TP of the unit (-1: not visible), with the rest of the row's offset
     Place<U> pp = at;
-    int pr = r0, pid = -1;
-    auto fetch_id = [&]() {  // block of row (lane % TP) of the unit, -1 where it is not visible
-        pid = -1;
-        if (pr < r1) {
-            const int pos = pp.s.base(pp.u) + warp * TP + (lane & (TP - 1));
-            if (pp.s.sees(pp.u, pos)) pid = a.kv.block_tables[(int64_t)pp.b * a.kv.max_blocks + a.div.block(pos)];
+    int pr = r0, pf = r0, pid[2];  // units requested, units looked up
+    int64_t add[2];
+    auto lookup = [&](int k) {
+        pid[k] = -1;
+        if (pf < r1) {
+            const int pos = pp.s.base(pp.u) + warp * TP + (lane & (TP - 1)), blk = a.div.block(pos);
+            if (pp.s.sees(pp.u, pos)) pid[k] = a.kv.block_tables[(int64_t)pp.b * a.kv.max_blocks + blk];
+            add[k] = (int64_t)a.div.slot(pos, blk) * a.kv.stride_slot + (int64_t)pp.kvh * a.kv.stride_head;
+            ++pf;
+            pp.next(a);
         }
     };
     const uint32_t ring = smem_addr(smem) + warp * kPgStages * C::STAGE;
     const int chunk = lane % C::CH;
     auto issue = [&](int stage) {
         if (pr < r1) {
-            const int pos = pp.s.base(pp.u) + warp * TP + (lane & (TP - 1));
-            const bool there = (unsigned)pid < (unsigned)a.kv.num_blocks;
-            const int64_t off = (int64_t)pid * a.kv.stride_block + (int64_t)a.div.slot(pos, a.div.block(pos)) * a.kv.stride_slot +
-                                (int64_t)pp.kvh * a.kv.stride_head;
+            const bool there = (unsigned)pid[0] < (unsigned)a.kv.num_blocks;
+            const int64_t off = (int64_t)pid[0] * a.kv.stride_block + add[0];
             const uint32_t mask = __ballot_sync(~0u, there);
             if (lane == 0) s_there[warp][stage] = mask;
             const uint32_t st = ring + stage * C::STAGE;
@@ -376,12 +415,15 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
                 }
             }
             ++pr;
-            pp.next(a);
-            fetch_id();
+            pid[0] = pid[1];
+            add[0] = add[1];
+            lookup(1);
         }
         cp_commit();
     };
-    fetch_id();
+    add[0] = add[1] = 0;
+    lookup(0);
+    lookup(1);
 #pragma unroll
     for (int s = 0; s < kPgStages - 1; ++s) issue(s);
 
@@ -595,47 +637,41 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
                     *reinterpret_cast<float4*>(part + row * a.D + d) = sum(row, d);
                 }
                 if (tid < nh) a.pml[(int64_t)slot * a.gs + tid] = s_ml[tid];
-                __threadfence();
-                __syncthreads();
                 if (!pieced) {
                     cf = seg0 / upc;
                     pieces = (seg0 + at.s.n - 1) / upc - cf + 1;
                 }
-                if (tid == 0) s_last = atomicAdd(a.counters + cf, 1) == pieces - 1;
+                __syncthreads();
+                if (tid == 0) {  // (the barrier orders the CTA's writes before this thread's fence)
+                    __threadfence();
+                    s_last = atomicAdd(a.counters + cf, 1) == pieces - 1;
+                    __threadfence();
+                }
                 __syncthreads();
                 if (s_last) {
                     // ---- last of the segment's CTAs: its pieces in order.  Piece p is in slot 2 (cf + p), the first
                     // one in the slot after
-                    __threadfence();
                     if (tid == 0) a.counters[cf] = 0;
                     const float2* ml0 = a.pml + (int64_t)2 * cf * a.gs;
                     const float* part0 = a.parts + (int64_t)2 * cf * a.gs * a.D;
-                    for (int row = warp; row < nh; row += kPgWarps) {
-                        float M = -1e30f, Ls = 0.f;
-                        for (int p = lane; p < pieces; p += 32) M = fmaxf(M, __ldcg(&ml0[(2 * p + (p == 0)) * a.gs + row].x));
-                        M = warp_max(M);
-                        for (int p = lane; p < pieces; p += 32) {
-                            const float2 ml = __ldcg(&ml0[(2 * p + (p == 0)) * a.gs + row]);
-                            Ls = fmaf(ml.y, ex2(ml.x - M), Ls);
-                        }
-                        Ls = warp_sum(Ls);
-                        if (lane == 0) s_ml[row] = make_float2(M, Ls);
-                    }
-                    __syncthreads();
                     for (int i = tid; i < nh * quads; i += kPgThreads) {
                         const int row = i / quads, d = (i - row * quads) * 4;
-                        const float2 ml = s_ml[row];
+                        float M = -1e30f, Ls = 0.f;
                         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
                         for (int p = 0; p < pieces; ++p) {
                             const int64_t sl = (int64_t)(2 * p + (p == 0)) * a.gs + row;
                             const float4 x = __ldcg(reinterpret_cast<const float4*>(part0 + sl * a.D + d));
-                            const float w = ex2(__ldcg(&ml0[sl].x) - ml.x);
-                            v = make_float4(fmaf(x.x, w, v.x), fmaf(x.y, w, v.y), fmaf(x.z, w, v.z), fmaf(x.w, w, v.w));
+                            const float2 ml = __ldcg(&ml0[sl]);
+                            const float m = fmaxf(M, ml.x), f = ex2(M - m), w = ex2(ml.x - m);
+                            M = m;
+                            Ls = fmaf(Ls, f, ml.y * w);
+                            v = make_float4(fmaf(v.x, f, x.x * w), fmaf(v.y, f, x.y * w), fmaf(v.z, f, x.z * w),
+                                            fmaf(v.w, f, x.w * w));
                         }
-                        store4<BF16>(a.out, oat + row * a.D + d, v, ml.y > 0.f ? 1.f / ml.y : 0.f);
+                        store4<BF16>(a.out, oat + row * a.D + d, v, Ls > 0.f ? 1.f / Ls : 0.f);
+                        if (a.stats && d == 0) a.stats[(int64_t)at.b * a.nq + h0 + row] = make_float2(M, Ls);
                     }
-                    if (a.stats && tid < nh) a.stats[(int64_t)at.b * a.nq + h0 + tid] = s_ml[tid];
                 }
             }
             __syncthreads();
