@@ -203,6 +203,29 @@ def stream_ptr(stream=None) -> int | None:
     return stream
 
 
+_TORCH = None
+
+
+def _torch():
+    """torch, imported on first use (an import statement costs more than a launch's other checks)."""
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = torch
+    return _TORCH
+
+
+def _stream_of(stream) -> int | None:
+    """stream_ptr without building a torch.cuda.Stream object (3.3 us a call)."""
+    if stream is not None:
+        return stream
+    c = _torch()._C
+    try:
+        return c._cuda_getCurrentRawStream(c._cuda_getDevice())
+    except AttributeError:
+        return stream_ptr()
+
+
 # ---------------------------------------------------------------------------
 # operator API (torch tensors in, torch tensors out; all compute in the library)
 # ---------------------------------------------------------------------------
@@ -249,7 +272,9 @@ class Workspace:
             lib().b2_workspace_destroy(self.h)
             self.h = None
 
-    __del__ = close
+    def __del__(self):
+        if _LIB is not None and C is not None:  # not while the interpreter shuts down
+            self.close()
 
 
 # ---------------------------------------------------------------------------
@@ -258,7 +283,7 @@ class Workspace:
 # ---------------------------------------------------------------------------
 
 def _is_bf16(t) -> int:
-    import torch
+    torch = _torch()
     if t.dtype == torch.bfloat16:
         return 1
     if t.dtype == torch.float16:
@@ -267,9 +292,14 @@ def _is_bf16(t) -> int:
 
 
 def _need(t, name, dtype, shape):
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}, "
                          f"got {t.dtype} {tuple(t.shape)}")
+
+
+def _view(t) -> KVView:
+    b, s, h, d = t.stride()
+    return KVView(t.data_ptr(), b, h, s, d)
 
 
 def window_prefill_gqa(q, k, v, out, window=0, sinks=0, seq_lens=None, stream=None):
@@ -279,18 +309,18 @@ def window_prefill_gqa(q, k, v, out, window=0, sinks=0, seq_lens=None, stream=No
     S of the T positions; any strides with contiguous rows.  out [B, S, nq, D]
     contiguous.  seq_lens (int32 [B], optional): tokens of each sequence;
     rows past it come out zero."""
-    import torch
-    B, S, nq, D = q.shape
-    T, nkv = k.shape[1], k.shape[2]
-    bf = _is_bf16(q)
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or T < S or k.dtype != q.dtype or v.dtype != q.dtype:
+    shape, dtype = q.shape, q.dtype
+    B, S, nq, D = shape
+    kb, T, nkv, kd = k.shape
+    if k.shape != v.shape or kb != B or kd != D or T < S or k.dtype != dtype or v.dtype != dtype:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
-    _need(out, "out", q.dtype, (B, S, nq, D))
+    _need(out, "out", dtype, shape)
+    lens = None
     if seq_lens is not None:
-        _need(seq_lens, "seq_lens", torch.int32, (B,))
-    views = [KVView(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1), t.stride(3)) for t in (q, k, v)]
-    call("b2_window_prefill_gqa", *views, out.data_ptr(), ptr(seq_lens), S, T - S, nq, nkv, D, B, window, sinks, bf,
-         stream_ptr(stream))
+        _need(seq_lens, "seq_lens", _torch().int32, (B,))
+        lens = seq_lens.data_ptr()
+    call("b2_window_prefill_gqa", _view(q), _view(k), _view(v), out.data_ptr(), lens, S, T - S, nq, nkv, D, B, window,
+         sinks, _is_bf16(q), _stream_of(stream))
     return out
 
 
@@ -302,7 +332,7 @@ class PagedKV:
     seq_lens int32 [B].  Holds references to the tensors, copies nothing."""
 
     def __init__(self, k, v, block_tables, seq_lens):
-        import torch
+        torch = _torch()
         if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
             raise ValueError("k and v must be [num_blocks, block_size, nkv, D] of one type with the same strides and "
                              "contiguous rows")
@@ -312,15 +342,12 @@ class PagedKV:
         _need(block_tables, "block_tables", torch.int32, (B, mb))
         _need(seq_lens, "seq_lens", torch.int32, (B,))
         self.k, self.v, self.block_tables, self.seq_lens = k, v, block_tables, seq_lens
-        self.batch, self.nkv, self.head_dim = B, k.shape[2], k.shape[3]
+        self.batch, self.nkv, self.head_dim, self.dtype = B, k.shape[2], k.shape[3], k.dtype
         self.num_blocks, self.block_size = k.shape[0], k.shape[1]
+        self.scores_shape = (self.num_blocks, self.nkv, self.block_size)
         self.c = PagedKVStruct(k.data_ptr(), v.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), k.stride(0),
                                k.stride(1), k.stride(2), k.shape[0], k.shape[1], mb, _is_bf16(k))
         self.ref = C.addressof(self.c)
-
-    def check_scores(self, scores):
-        import torch
-        _need(scores, "scores", torch.float32, (self.num_blocks, self.nkv, self.block_size))
 
 
 def paged_decode_workspace_bytes(batch, nq, nkv, head_dim, max_positions, scored=False) -> int:
@@ -332,15 +359,19 @@ def paged_decode_gqa(q, kv: PagedKV, out, window=0, sinks=0, scores=None, ws: Wo
     [B, nq, D] (rows of heads contiguous), out [B, nq, D] contiguous; scores
     (float32 [num_blocks, nkv, block_size], optional) accumulates every
     visible position's weight and needs a workspace."""
-    B, nq, D = q.shape
-    if B != kv.batch or D != kv.head_dim or q.dtype != kv.k.dtype or q.stride(2) != 1 or q.stride(1) != D:
+    shape = q.shape
+    B, nq, D = shape
+    ldq, sh, sd = q.stride()
+    if B != kv.batch or D != kv.head_dim or q.dtype != kv.dtype or sd != 1 or sh != D:
         raise ValueError(f"q {q.dtype} {tuple(q.shape)} does not fit the cache ({kv.batch} sequences, "
-                         f"head_dim {kv.head_dim}, {kv.k.dtype})")
-    _need(out, "out", q.dtype, (B, nq, D))
+                         f"head_dim {kv.head_dim}, {kv.dtype})")
+    _need(out, "out", kv.dtype, shape)
+    sc = None
     if scores is not None:
-        kv.check_scores(scores)
-    call("b2_paged_decode_gqa", q.data_ptr(), q.stride(0), kv.ref, out.data_ptr(), ptr(scores), B, nq, kv.nkv, D,
-         window, sinks, ws.h if ws is not None else None, stream_ptr(stream))
+        _need(scores, "scores", _torch().float32, kv.scores_shape)
+        sc = scores.data_ptr()
+    call("b2_paged_decode_gqa", q.data_ptr(), ldq, kv.ref, out.data_ptr(), sc, B, nq, kv.nkv, D, window, sinks,
+         ws.h if ws is not None else None, _stream_of(stream))
     return out
 
 
@@ -351,16 +382,17 @@ def paged_kv_evict(kv: PagedKV, scores, budget, kept, new_lens, sinks=0, recent=
     0.. of the same blocks, or of the blocks of dst_tables (int32 [B,
     max_dst_blocks]).  kept int32 [B, nkv, budget] (-1 past a sequence's new
     length), new_lens int32 [B] (may be kv.seq_lens)."""
-    import torch
-    kv.check_scores(scores)
+    torch = _torch()
+    _need(scores, "scores", torch.float32, kv.scores_shape)
     _need(kept, "kept", torch.int32, (kv.batch, kv.nkv, budget))
     _need(new_lens, "new_lens", torch.int32, (kv.batch,))
-    mdb = 0
+    mdb, dst = 0, None
     if dst_tables is not None:
         mdb = dst_tables.shape[1]
         _need(dst_tables, "dst_tables", torch.int32, (kv.batch, mdb))
-    call("b2_paged_kv_evict", kv.ref, scores.data_ptr(), ptr(dst_tables), mdb, kv.batch, kv.nkv, kv.head_dim, budget,
-         sinks, recent, kept.data_ptr(), new_lens.data_ptr(), stream_ptr(stream))
+        dst = dst_tables.data_ptr()
+    call("b2_paged_kv_evict", kv.ref, scores.data_ptr(), dst, mdb, kv.batch, kv.nkv, kv.head_dim, budget, sinks, recent,
+         kept.data_ptr(), new_lens.data_ptr(), _stream_of(stream))
 
 
 class Sampler:

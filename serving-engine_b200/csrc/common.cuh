@@ -91,6 +91,18 @@ inline cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// Dynamic shared memory above 48 KB has to be allowed per kernel and device:
+// asked for once on each (`done` is the kernel's own, one entry per device).
+template <typename... KArgs>
+inline cudaError_t allow_smem(void (*kernel)(KArgs...), int bytes, bool (&done)[64]) {
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev])) return e;
+    const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (r == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    return r;
+}
+
 // ---------------------------------------------------------------------------
 // device helpers
 // ---------------------------------------------------------------------------

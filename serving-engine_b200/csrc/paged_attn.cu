@@ -757,7 +757,8 @@ template <int DP, bool GH, bool BF16>
 static int paged_launch(const PagedArgs& a, const PagedSizes& z, cudaStream_t s) {
     using C = PagedCfg<DP, GH>;
     auto kern = paged_attn_kernel<DP, GH, BF16>;
-    B2_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES));
+    static bool done[64];
+    B2_TRY(allow_smem(kern, C::BYTES, done));
     B2_TRY(launch(kern, dim3(z.grid), dim3(kPgThreads), C::BYTES, s, true, a));
     if (a.scores)
         B2_TRY(launch(paged_scores_kernel<C::U>, dim3((unsigned)((a.cap + 1023) / 1024), a.nkv, a.batch), dim3(256), 0, s,

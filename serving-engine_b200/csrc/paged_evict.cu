@@ -30,7 +30,7 @@ constexpr int kEvThreads = 1024;   // of a choice
 constexpr int kEvCached = 49152;   // keys of a choice kept in shared memory; the rest are read again
 constexpr int kMvThreads = 256;    // of a move
 constexpr int kMvBatch = 4;        // 16-byte pieces in flight per thread
-constexpr int kMvRows = 128;       // rows of a CTA that moves into other blocks
+constexpr int kMvRows = 128;       // rows looked up together; those of a CTA that moves into other blocks
 constexpr int kMvSlices = 8;       // column slices in place
 
 struct EvictArgs {
@@ -41,6 +41,7 @@ struct EvictArgs {
     int nkv, D, budget, sinks, recent;
     int* kept;
     int* new_lens;
+    BlockDiv div;
     int cached;  // keys that the choice's shared memory holds
 };
 
@@ -68,9 +69,9 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const Evict
     }
     auto load = [&](int i) -> uint32_t {
         if (i < a.sinks || i >= L - a.recent) return kEvStays;
-        const int blk = bt[(unsigned)i / (unsigned)bs];
+        const int blk = bt[a.div.block(i)];
         if ((unsigned)blk >= (unsigned)a.kv.num_blocks) return rank_key(-INFINITY);
-        return rank_key(a.scores[((int64_t)blk * a.nkv + kvh) * bs + (unsigned)i % (unsigned)bs]);
+        return rank_key(a.scores[((int64_t)blk * a.nkv + kvh) * bs + a.div.slot(i, a.div.block(i))]);
     };
     const int cached = min(L, a.cached) & ~3;
     s_hist[0][t] = 0;
@@ -82,14 +83,14 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const Evict
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int i = i0 + e * kEvThreads;
-            blk[e] = i < cached ? bt[(unsigned)i / (unsigned)bs] : -1;
+            blk[e] = i < cached ? bt[a.div.block(i)] : -1;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int i = i0 + e * kEvThreads;
             f[e] = -INFINITY;
             if ((unsigned)blk[e] < (unsigned)a.kv.num_blocks)
-                f[e] = a.scores[((int64_t)blk[e] * a.nkv + kvh) * bs + (unsigned)i % (unsigned)bs];
+                f[e] = a.scores[((int64_t)blk[e] * a.nkv + kvh) * bs + a.div.slot(i, a.div.block(i))];
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -196,83 +197,72 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const Evict
 }
 
 // grid (kv heads; row ranges, or column slices in place; sequences): the heads
-// of one range run together, so that their rows' DRAM pages do
+// of one range run together, so that their rows' DRAM pages do.  One thread
+// per row looks up where it comes from and goes; the copies then take a few
+// instructions per 16 bytes (looking up per copy bounded the kernel by its
+// arithmetic: 5.0 TB/s).
 __global__ void __launch_bounds__(kMvThreads, 4) evict_move_kernel(const EvictArgs a) {
-    const int kvh = blockIdx.x, b = blockIdx.z, rank = blockIdx.y, cs = gridDim.y, t = threadIdx.x;
-    const int bs = a.kv.block_size;
+    __shared__ int64_t s_from[kMvRows], s_to[kMvRows];  // elements; from -1: nothing to move
+    const int kvh = blockIdx.x, b = blockIdx.z, rank = blockIdx.y, parts = gridDim.y, t = threadIdx.x;
     griddep_wait();
     griddep_launch_dependents();
     // (new_lens may be the lengths themselves: the minimum below is the same before and after)
     const int L = paged_len(a.kv, b), n = min(L, a.budget);
     if (kvh == 0 && rank == 0 && t == 0) a.new_lens[b] = n;
     const int* bt = a.kv.block_tables + (int64_t)b * a.kv.max_blocks;
-    const int* kept = a.kept + ((int64_t)b * a.nkv + kvh) * a.budget;
     const int* dt = a.dst ? a.dst + (int64_t)b * a.dst_blocks : bt;
+    const int* kept = a.kept + ((int64_t)b * a.nkv + kvh) * a.budget;
     const int chunks = a.D / 8;  // 16-byte pieces of a row, K's then V's
     int j0 = 0, j1 = n, first = 0, width = 2 * chunks;
+    bool scores = true;
     if (a.dst) {
         j0 = min(n, rank * kMvRows);
         j1 = min(n, j0 + kMvRows);
     } else {
-        width = (2 * chunks + cs - 1) / cs;
-        first = rank * width;
+        width = (2 * chunks + parts - 1) / parts;
+        first = min(2 * chunks, rank * width);
         width = min(width, 2 * chunks - first);
+        scores = rank == 0;
     }
-    
-    if (width > 0) {
-        const int rows = kMvThreads / width, r = t / width, piece = first + t - r * width;
-        uint4* base = static_cast<uint4*>(piece < chunks ? a.kv.k : a.kv.v);
-        const int64_t col = (int64_t)kvh * a.kv.stride_head + (piece < chunks ? piece : piece - chunks) * 8;
-        auto at = [&](const int* tab, int pos) -> int64_t {
-            const int blk = tab[(unsigned)pos / (unsigned)bs];
-            if ((unsigned)blk >= (unsigned)a.kv.num_blocks) return -1;
-            return (int64_t)blk * a.kv.stride_block + (int64_t)((unsigned)pos % (unsigned)bs) * a.kv.stride_slot + col;
-        };
-        for (int jb = j0; jb < j1; jb += rows * kMvBatch) {
-            int src[kMvBatch];
-            int64_t from[kMvBatch], to[kMvBatch];
+    // thread t: piece first + t % width of rows t / width, t / width + rows, ..
+    const int rows = width > 0 ? kMvThreads / width : 0, r = width > 0 ? t / width : 0, piece = first + t - r * width;
+    uint4* base = static_cast<uint4*>(piece < chunks ? a.kv.k : a.kv.v) + (piece < chunks ? piece : piece - chunks);
+    for (int jb = j0; jb < j1; jb += kMvRows) {
+        const int m = min(kMvRows, j1 - jb);
+        int64_t sf = -1, st = -1;
+        float sv = 0.f;
+        if (t < m) {
+            const int j = jb + t, i = __ldcg(kept + j), ib = a.div.block(i), jb2 = a.div.block(j);
+            const int sb = bt[ib], db = dt[jb2];
+            const bool go = (unsigned)sb < (unsigned)a.kv.num_blocks && (unsigned)db < (unsigned)a.kv.num_blocks &&
+                            (a.dst || i != j);
+            const int ss = a.div.slot(i, ib), ds = a.div.slot(j, jb2);
+            s_from[t] = go ? sb * a.kv.stride_block + ss * a.kv.stride_slot + kvh * a.kv.stride_head : -1;
+            s_to[t] = db * a.kv.stride_block + ds * a.kv.stride_slot + kvh * a.kv.stride_head;
+            if (go && scores) {
+                sf = ((int64_t)sb * a.nkv + kvh) * a.kv.block_size + ss;
+                st = ((int64_t)db * a.nkv + kvh) * a.kv.block_size + ds;
+                sv = a.scores[sf];
+            }
+        }
+        __syncthreads();  // (in place it also parts the batch's score reads from its writes)
+        if (sf >= 0) a.scores[st] = sv;
+        for (int k0 = 0; k0 < m; k0 += rows * kMvBatch) {
+            if (rows == 0) break;
+            int64_t from[kMvBatch];
             uint4 v[kMvBatch];
 #pragma unroll
             for (int e = 0; e < kMvBatch; ++e) {
-                const int j = jb + e * rows + r;
-                src[e] = r < rows && j < j1 ? __ldcg(kept + j) : -1;
-            }
-#pragma unroll
-            for (int e = 0; e < kMvBatch; ++e) {
-                const int j = jb + e * rows + r;
-                from[e] = -1;
-                if (src[e] < 0 || (!a.dst && src[e] == j)) continue;
-                from[e] = at(bt, src[e]);
-                to[e] = at(dt, j);
-                if (to[e] < 0) from[e] = -1;
-            }
-#pragma unroll
-            for (int e = 0; e < kMvBatch; ++e)
+                const int k = k0 + e * rows + r;
+                from[e] = r < rows && k < m ? s_from[k] : -1;
                 if (from[e] >= 0) v[e] = __ldcs(base + (from[e] >> 3));
+            }
             if (!a.dst) __syncthreads();
 #pragma unroll
             for (int e = 0; e < kMvBatch; ++e)
-                if (from[e] >= 0) __stcs(base + (to[e] >> 3), v[e]);
+                if (from[e] >= 0) __stcs(base + (s_to[k0 + e * rows + r] >> 3), v[e]);
         }
-    }
-    if (a.dst || rank == 0) {
-        auto at = [&](const int* tab, int pos) -> int64_t {
-            const int blk = tab[(unsigned)pos / (unsigned)bs];
-            if ((unsigned)blk >= (unsigned)a.kv.num_blocks) return -1;
-            return ((int64_t)blk * a.nkv + kvh) * bs + (unsigned)pos % (unsigned)bs;
-        };
-        for (int jb = j0; jb < j1; jb += kMvThreads) {
-            const int j = jb + t;
-            int64_t from = -1, to = -1;
-            float v = 0.f;
-            if (j < j1) {
-                from = at(bt, __ldcg(kept + j));
-                to = at(dt, j);
-                if (from >= 0) v = a.scores[from];
-            }
-            if (!a.dst) __syncthreads();
-            if (from >= 0 && to >= 0) a.scores[to] = v;
-        }
+        __syncthreads();
     }
 }
 
@@ -291,6 +281,7 @@ extern "C" int b2_paged_kv_evict(const b2_paged_kv* kv, float* scores, const int
     if (batch > 65535 || nkv > 65535) return B2_ERR_UNSUPPORTED;
     EvictArgs a = {};
     a.kv = *kv;
+    a.div = block_div(kv->block_size);
     a.scores = scores;
     a.dst = dst_tables;
     a.dst_blocks = max_dst_blocks;
@@ -304,7 +295,8 @@ extern "C" int b2_paged_kv_evict(const b2_paged_kv* kv, float* scores, const int
     const int64_t span = (int64_t)kv->max_blocks * kv->block_size;
     a.cached = (int)(span < kEvCached ? (span + 3) & ~int64_t(3) : kEvCached);
     cudaStream_t s = as_stream(stream);
-    B2_TRY(cudaFuncSetAttribute(evict_choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvCached * 4));
+    static bool done[64];
+    B2_TRY(allow_smem(evict_choose_kernel, kEvCached * 4, done));
     B2_TRY(launch(evict_choose_kernel, dim3(nkv, batch), dim3(kEvThreads), (size_t)a.cached * sizeof(float), s, true, a));
     const int64_t parts = dst_tables ? ((int64_t)budget + kMvRows - 1) / kMvRows : kMvSlices;
     B2_TRY(launch(evict_move_kernel, dim3(nkv, (unsigned)parts, batch), dim3(kMvThreads), 0, s, true, a));

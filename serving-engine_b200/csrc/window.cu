@@ -595,7 +595,8 @@ static int launch_window_tc(const WinArgs& a_in, cudaStream_t s) {
     if (rc == B2_OK) rc = window_map(&tv, a.v, a.nkv, T, a, BF16);
     if (rc != B2_OK) return rc;
     auto kern = window_tc_kernel<D, BF16>;
-    B2_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+    static bool done[64];
+    B2_TRY(allow_smem(kern, (int)C::SMEM, done));
     const int64_t items = (int64_t)a.batch * a.nq * ((a.S + 255) / 256);
     const unsigned grid = (unsigned)(items < sm_count() ? items : sm_count());
     B2_TRY(launch(kern, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, tq, tk, tv, a, err));
