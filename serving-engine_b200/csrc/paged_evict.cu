@@ -42,6 +42,7 @@ struct EvictArgs {
     int* kept;
     int* new_lens;
     BlockDiv div;
+    int quads;   // 4 consecutive positions (from a multiple of 4) lie in one block, their scores 16-byte aligned
     int cached;  // keys that the choice's shared memory holds
 };
 
@@ -76,27 +77,43 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const Evict
     const int cached = min(L, a.cached) & ~3;
     s_hist[0][t] = 0;
     s_hist[0][t + kEvThreads] = 0;
-    // 8 positions a thread at a time: their table entries in one round trip, their scores in the next
-    for (int i0 = t; i0 < cached; i0 += 8 * kEvThreads) {
-        int blk[8];
-        float f[8];
+    if (a.quads) {
+        // 4 consecutive positions of a block at a time, four such per thread on their way
+        constexpr int kOn = 4;
+        for (int i0 = 4 * t; i0 < cached; i0 += kOn * 4 * kEvThreads) {
+            int blk[kOn];
+            float4 f[kOn];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int i = i0 + e * kEvThreads;
-            blk[e] = i < cached ? bt[a.div.block(i)] : -1;
-        }
+            for (int e = 0; e < kOn; ++e) {
+                const int i = i0 + e * 4 * kEvThreads;
+                blk[e] = i < cached ? bt[a.div.block(i)] : -1;
+            }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int i = i0 + e * kEvThreads;
-            f[e] = -INFINITY;
-            if ((unsigned)blk[e] < (unsigned)a.kv.num_blocks)
-                f[e] = a.scores[((int64_t)blk[e] * a.nkv + kvh) * bs + a.div.slot(i, a.div.block(i))];
-        }
+            for (int e = 0; e < kOn; ++e) {
+                const int i = i0 + e * 4 * kEvThreads;
+                f[e] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if ((unsigned)blk[e] < (unsigned)a.kv.num_blocks)
+                    f[e] = *reinterpret_cast<const float4*>(a.scores + ((int64_t)blk[e] * a.nkv + kvh) * bs +
+                                                            a.div.slot(i, a.div.block(i)));
+            }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int i = i0 + e * kEvThreads;
-            if (i < cached) s_key[i] = i < a.sinks || i >= L - a.recent ? kEvStays : rank_key(f[e]);
+            for (int e = 0; e < kOn; ++e) {
+                const int i = i0 + e * 4 * kEvThreads;
+                if (i >= cached) continue;
+                uint4 k = make_uint4(rank_key(f[e].x), rank_key(f[e].y), rank_key(f[e].z), rank_key(f[e].w));
+                if (i < a.sinks || i + 4 > L - a.recent) {
+                    auto stays = [&](int x) { return x < a.sinks || x >= L - a.recent; };
+                    if (stays(i)) k.x = kEvStays;
+                    if (stays(i + 1)) k.y = kEvStays;
+                    if (stays(i + 2)) k.z = kEvStays;
+                    if (stays(i + 3)) k.w = kEvStays;
+                }
+                *reinterpret_cast<uint4*>(s_key + i) = k;
+            }
         }
+    } else {
+#pragma unroll 2
+        for (int i = t; i < cached; i += kEvThreads) s_key[i] = load(i);
     }
     // keys of positions i .. i + 3 (i a multiple of 4); past the end a key no position of this choice has
     auto keys = [&](int i) -> uint4 {
@@ -109,15 +126,19 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const Evict
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
         int* hist = s_hist[pass & 1];
         __syncthreads();
+        const int up = shift + width;
+        auto add = [&](uint32_t k) {
+            if (pass == 0 || (k ^ thr) >> up == 0) atomicAdd(&hist[(k >> shift) & ((1 << width) - 1)], 1);
+        };
 #pragma unroll 2
-        for (int i = 4 * t; i < L; i += 4 * kEvThreads) {
-            const uint4 v = keys(i);
-            const uint32_t k[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (i + e < L && (pass == 0 || (k[e] ^ thr) >> (shift + width) == 0))
-                    atomicAdd(&hist[(k[e] >> shift) & ((1 << width) - 1)], 1);
+        for (int i = 4 * t; i < cached; i += 4 * kEvThreads) {
+            const uint4 v = *reinterpret_cast<const uint4*>(s_key + i);
+            add(v.x);
+            add(v.y);
+            add(v.z);
+            add(v.w);
         }
+        for (int i = cached + t; i < L; i += kEvThreads) add(load(i));
         __syncthreads();
         // thread t: bins 2 t and 2 t + 1, counted from the top
         const int2 h = reinterpret_cast<const int2*>(hist)[t];
@@ -146,19 +167,17 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const Evict
     // need is now how many positions with key == thr stay.  A position's place: the better ones before it, and the
     // equal ones before it as far as they stay.  A warp takes a stretch of positions, 4 of them a lane at a time.
     const int q = (L + 128 * 32 - 1) / (128 * 32) * 128, q0 = min(L, warp * q), q1 = min(L, q0 + q);
-    auto kinds = [&](int i) -> int {  // better ones of the 4 in the low half, equal ones in the high half; bits 4.. each
+    auto kinds = [&](int i) -> int {  // better ones of the 4 in bits 0 .. 3, equal ones in bits 16 .. 19
         if (i >= q1) return 0;
         const uint4 v = keys(i);
-        const uint32_t k[4] = {v.x, v.y, v.z, v.w};
-        int r = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (i + e < q1) r |= k[e] > thr ? 1 << e : k[e] == thr ? 0x10000 << e : 0;
+        int r = (v.x > thr) | (v.y > thr) << 1 | (v.z > thr) << 2 | (v.w > thr) << 3 | (v.x == thr) << 16 |
+                (v.y == thr) << 17 | (v.z == thr) << 18 | (v.w == thr) << 19;
+        if (q1 - i < 4) r &= ((1 << (q1 - i)) - 1) * 0x10001;
         return r;
     };
     auto count = [](int r) { return __popc(r & 0xf) | __popc(r & 0xf0000) << 16; };
     int2 before = make_int2(0, 0);
-#pragma unroll 4
+#pragma unroll 2
     for (int i = q0; i < q1; i += 128) {
         const int c = count(kinds(i + 4 * lane));
         before.x += c & 0xffff;
@@ -172,7 +191,7 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const Evict
     if (lane >= warp) before = make_int2(0, 0);
     before.x = __reduce_add_sync(~0u, before.x);
     before.y = __reduce_add_sync(~0u, before.y);
-#pragma unroll 4
+#pragma unroll 2
     for (int i = q0; i < q1; i += 128) {
         const int r = kinds(i + 4 * lane), c = count(r);
         int incl = c;  // at most 128 of each: the halves do not meet
@@ -294,6 +313,7 @@ extern "C" int b2_paged_kv_evict(const b2_paged_kv* kv, float* scores, const int
     a.new_lens = new_lens;
     const int64_t span = (int64_t)kv->max_blocks * kv->block_size;
     a.cached = (int)(span < kEvCached ? (span + 3) & ~int64_t(3) : kEvCached);
+    a.quads = kv->block_size % 4 == 0 && aligned16(scores);
     cudaStream_t s = as_stream(stream);
     static bool done[64];
     B2_TRY(allow_smem(evict_choose_kernel, kEvCached * 4, done));

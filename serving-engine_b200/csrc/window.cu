@@ -7,8 +7,10 @@
 // Tensor-core form (window_tc_kernel, head_dim <= 128).  4 D flops per
 // visible (query, key) pair against 2 D bytes per key of each 256-query pair
 // of tiles: bound by the tensor cores and, beside them, by the exponentials.
-// One persistent CTA per SM takes pairs of 128-query tiles (A, B) of one head;
-// a pair visits only the 128-key tiles that one of its rows sees:
+// One persistent CTA per SM takes pairs of 128-query tiles (A, B), two heads of
+// a kv head's group at the same rows where it can, so that they visit the same
+// key tiles: K and V come once for both.  A pair visits only the 128-key tiles
+// that one of its rows sees:
 //   the window's tiles of A, the sinks' tiles (as wide as the sinks, in steps
 //   of 16 keys), then the tiles only B reaches --
 // an order in which the tiles of A, and those of B, are each consecutive.
@@ -167,43 +169,51 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// One pair of query tiles of one head, and the key tiles it visits.
+// One pair of query tiles and the key tiles it visits.  The tiles of a kv head
+// -- (128 rows, query head of the group), heads fastest -- are paired in order,
+// so A and B are two heads at the same rows, or B is at the next 128 rows.
 struct WinItem {
-    int b, h, row0;        // first query row of tile A
-    int len;               // tokens of the sequence
-    int p0;                // position of row0
+    int b, kvh, len;       // sequence, kv head, tokens of the sequence
+    int h[2], row[2];      // head and first query row of A and B
+    int p[2];              // the positions of those rows
     bool hasB;
-    int loA, nw, ns, hiA;  // window tiles loA .. loA + nw - 1 = hiA of A, sinks' tiles 0 .. ns - 1
+    int loA, nw, ns;       // window tiles loA .. loA + nw - 1 of A, sinks' tiles 0 .. ns - 1
     int nA, n, dB;         // A visits steps 0 .. nA - 1, B steps dB .. n - 1
 
-    // Number of valid pairs of sequence b.
     static __device__ __forceinline__ int length(const WinArgs& a, int b) {
         const int T = a.q_start + a.S;
         return a.seq_lens ? max(0, min(a.seq_lens[b], T)) : T;
     }
-    static __device__ __forceinline__ int pairs(const WinArgs& a, int len) {
-        return (max(0, len - a.q_start) + 255) >> 8;
+    // Row tiles of a sequence of len tokens that hold a token.
+    static __device__ __forceinline__ int tiles(const WinArgs& a, int len) {
+        return (max(0, len - a.q_start) + 127) >> 7;
     }
 
-    __device__ __forceinline__ void of(const WinArgs& a, int b_, int len_, int pair, int h_) {
+    // Pair i of the kv head's list, of `count` tiles.
+    __device__ __forceinline__ void of(const WinArgs& a, int b_, int len_, int kvh_, int i, int count) {
+        const int group = a.nq / a.nkv;
         b = b_;
-        h = h_;
         len = len_;
-        row0 = pair * 256;
-        p0 = a.q_start + row0;
-        hasB = row0 + 128 < a.S && p0 + 128 < len;
-        loA = a.window > 0 ? max(0, p0 - a.window + 1) >> 7 : 0;
-        hiA = min(p0 + 127, len - 1) >> 7;
+        kvh = kvh_;
+        hasB = 2 * i + 1 < count;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int e = 2 * i + (hasB ? t : 0), rt = e / group;
+            h[t] = kvh * group + e - rt * group;
+            row[t] = rt * 128;
+            p[t] = a.q_start + row[t];
+        }
+        loA = a.window > 0 ? max(0, p[0] - a.window + 1) >> 7 : 0;
+        const int hiA = min(p[0] + 127, len - 1) >> 7, st = a.window > 0 ? (a.sinks + 127) >> 7 : 0;
         nw = hiA - loA + 1;
-        const int st = a.window > 0 ? (a.sinks + 127) >> 7 : 0;
         ns = min(st, loA);
         nA = nw + ns;
         n = nA;
         dB = 0;
-        if (hasB) {
-            n += (min(p0 + 255, len - 1) >> 7) - hiA;
+        if (row[1] > row[0]) {
+            n += (min(p[1] + 127, len - 1) >> 7) - hiA;
             // B skips A's first tiles, unless they hold sinks
-            if (a.window > 0 && loA >= st) dB = (max(0, p0 + 128 - a.window + 1) >> 7) - loA;
+            if (a.window > 0 && loA >= st) dB = (max(0, p[1] - a.window + 1) >> 7) - loA;
         }
     }
     // Key tile of step j.
@@ -213,33 +223,34 @@ struct WinItem {
     // Keys of step j's tile that query tile t may see, in steps of 16.
     __device__ __forceinline__ int width(const WinArgs& a, int t, int j) const {
         const int kb = tile(j) << 7;
-        int end = min(p0 + 128 * t + 127, len - 1) + 1;
+        int end = min(p[t] + 127, len - 1) + 1;
         if (j >= nw && j < nA) end = min(end, a.sinks);
         return min(128, (end - kb + 15) & ~15);
     }
 };
 
-// The valid pairs of all sequences, each with all its heads, dealt round robin
-// to the CTAs; a sequence's later (longer) pairs first.
+// The pairs of all sequences and kv heads, dealt round robin to the CTAs; a
+// sequence's later (longer) rows first.
 struct WinList {
-    int b = 0, len = 0, np = 0;
-    int64_t before = 0;  // items of sequences before b
+    int b = 0, len = 0, count = 0, np = 0;  // of the sequence: tiles and pairs per kv head
+    int64_t before = 0;                     // items of sequences before b
     __device__ __forceinline__ bool get(const WinArgs& a, int64_t i, WinItem& it) {
         if (b == 0 && before == 0 && np == 0) enter(a);
-        while (b < a.batch && i - before >= (int64_t)np * a.nq) {
-            before += (int64_t)np * a.nq;
+        while (b < a.batch && i - before >= (int64_t)np * a.nkv) {
+            before += (int64_t)np * a.nkv;
             ++b;
             enter(a);
         }
         if (b >= a.batch) return false;
-        const int k = (int)(i - before);
-        it.of(a, b, len, np - 1 - k / a.nq, k % a.nq);
+        const int k = (int)(i - before), pair = k / a.nkv;
+        it.of(a, b, len, k - pair * a.nkv, np - 1 - pair, count);
         return true;
     }
     __device__ __forceinline__ void enter(const WinArgs& a) {
         if (b >= a.batch) return;
         len = WinItem::length(a, b);
-        np = WinItem::pairs(a, len);
+        count = WinItem::tiles(a, len) * (a.nq / a.nkv);
+        np = (count + 1) >> 1;
     }
 };
 
@@ -307,14 +318,13 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
             bool ok = true;
             uint32_t k = 0;
             for (int64_t i = blockIdx.x; ok && list.get(a, i, it); i += gridDim.x, ++k) {
-                const int kvh = it.h / (a.nq / a.nkv);
                 if (k > 0 && !tc::mbar_wait(q_empty, (k - 1) & 1u, err, 91)) break;
                 tc::mbar_arrive_expect_tx(q_full, 2 * TILE);
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int c = 0; c < C::ATOMS; ++c)
-                        tc::tma_load_4d(sQ + t * TILE + c * ATOM, &tmQ, q_full, c * 64, it.h, it.row0 + t * 128, it.b);
+                        tc::tma_load_4d(sQ + t * TILE + c * ATOM, &tmQ, q_full, c * 64, it.h[t], it.row[t], it.b);
                 for (int j = 0; j < it.n; ++j, ++g) {
                     const uint32_t s = g % ST, u = g / ST;
                     const int row = it.tile(j) * 128;
@@ -322,12 +332,12 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                     tc::mbar_arrive_expect_tx(&k_full[s], TILE);
 #pragma unroll
                     for (int c = 0; c < C::ATOMS; ++c)
-                        tc::tma_load_4d(sK + s * TILE + c * ATOM, &tmK, &k_full[s], c * 64, kvh, row, it.b);
+                        tc::tma_load_4d(sK + s * TILE + c * ATOM, &tmK, &k_full[s], c * 64, it.kvh, row, it.b);
                     if (g >= ST && !(ok = tc::mbar_wait(&v_empty[s], (u - 1) & 1u, err, 93))) break;
                     tc::mbar_arrive_expect_tx(&v_full[s], TILE);
 #pragma unroll
                     for (int c = 0; c < C::ATOMS; ++c)
-                        tc::tma_load_4d(sV + s * TILE + c * ATOM, &tmV, &v_full[s], c * 64, kvh, row, it.b);
+                        tc::tma_load_4d(sV + s * TILE + c * ATOM, &tmV, &v_full[s], c * 64, it.kvh, row, it.b);
                 }
             }
         }
@@ -411,7 +421,7 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
         uint32_t cs = 0, co = 0;  // S tiles and outputs of this tile so far
         for (int64_t i = blockIdx.x; ok && list.get(a, i, it); i += gridDim.x) {
             const int from = t == 0 ? 0 : it.dB, to = t == 0 ? it.nA : it.hasB ? it.n : 0;
-            const int wp = it.p0 + t * 128 + rq * 32;  // position of the warp's first row
+            const int wp = it.p[t] + rq * 32;  // position of the warp's first row
             const int pos = wp + lane < it.len ? wp + lane : -1;
             float m = -1e30f, l = 0.f;  // finite: a row that has seen nothing keeps P = 0 and l = 0
             for (int j = from; j < to; ++j, ++cs) {
@@ -503,8 +513,8 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                 const float inv_l = l > 0.f ? 1.f / l : 0.f;
                 // 64 outputs of 32 rows at a time through shared memory: whole 128-byte lines leave
                 uint8_t* stage = sm + C::OFF_OUT + warp * 4096;
-                const int row = it.row0 + t * 128 + rq * 32;
-                uint16_t* obase = static_cast<uint16_t*>(a.out) + (((int64_t)it.b * a.S + row) * a.nq + it.h) * a.D;
+                const int row = it.row[t] + rq * 32;
+                uint16_t* obase = static_cast<uint16_t*>(a.out) + (((int64_t)it.b * a.S + row) * a.nq + it.h[t]) * a.D;
 #pragma unroll 1
                 for (int c = 0; c < D; c += 64) {
 #pragma unroll
@@ -541,8 +551,7 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
             const int64_t row16 = (int64_t)a.nq * a.D / 8;
             for (int b = 0; b < a.batch; ++b) {
                 const int len = WinItem::length(a, b);
-                int done = WinItem::pairs(a, len) * 256;
-                if (done > 0 && a.q_start + done - 128 >= len) done -= 128;  // the last pair had no tile B
+                const int done = WinItem::tiles(a, len) * 128;
                 if (done >= a.S) continue;
                 uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + ((int64_t)b * a.S + done) * a.nq * a.D);
                 for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (a.S - done) * row16;
@@ -597,7 +606,7 @@ static int launch_window_tc(const WinArgs& a_in, cudaStream_t s) {
     auto kern = window_tc_kernel<D, BF16>;
     static bool done[64];
     B2_TRY(allow_smem(kern, (int)C::SMEM, done));
-    const int64_t items = (int64_t)a.batch * a.nq * ((a.S + 255) / 256);
+    const int64_t items = (int64_t)a.batch * a.nkv * ((((int64_t)a.S + 127) / 128 * (a.nq / a.nkv) + 1) / 2);
     const unsigned grid = (unsigned)(items < sm_count() ? items : sm_count());
     B2_TRY(launch(kern, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, tq, tk, tv, a, err));
     return B2_OK;
