@@ -42,6 +42,7 @@ struct WinArgs {
     int S, q_start, nq, nkv, D, batch;
     int window, sinks;
     float scale_log2;
+    int single;  // tiles are not paired
 };
 
 template <bool BF16>
@@ -120,7 +121,7 @@ struct WinCfg {
     static constexpr uint32_t OFF_OUT = OFF_V + ST * TILE;  // 32 rows x 64 outputs per softmax warp
     static constexpr uint32_t OFF_BAR = OFF_OUT + 8 * 4096;
     // above half an SM's shared memory: one CTA, with all 512 TMEM columns, per SM
-    static constexpr size_t NEED = OFF_BAR + 256 + 1024;
+    static constexpr size_t NEED = OFF_BAR + 512 + 1024;
     static constexpr size_t SMEM = NEED > 122880 ? NEED : 122880;
     static constexpr int THREADS = 352;  // warps 0-7 softmax, 8 TMA, 9 and 10 MMA of tile A and of tile B
 };
@@ -195,10 +196,10 @@ struct WinItem {
         b = b_;
         len = len_;
         kvh = kvh_;
-        hasB = 2 * i + 1 < count;
+        hasB = !a.single && 2 * i + 1 < count;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int e = 2 * i + (hasB ? t : 0), rt = e / group;
+            const int e = a.single ? i : 2 * i + (hasB ? t : 0), rt = e / group;
             h[t] = kvh * group + e - rt * group;
             row[t] = rt * 128;
             p[t] = a.q_start + row[t];
@@ -250,14 +251,15 @@ struct WinList {
         if (b >= a.batch) return;
         len = WinItem::length(a, b);
         count = WinItem::tiles(a, len) * (a.nq / a.nkv);
-        np = (count + 1) >> 1;
+        np = a.single ? count : (count + 1) >> 1;
     }
 };
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
     window_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                     const __grid_constant__ CUtensorMap tmV, const WinArgs a, int* err) {
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const WinArgs a,
+                     int* err) {
     using C = WinCfg<D>;
     constexpr uint32_t TILE = C::TILE, ATOM = C::ATOM;
     constexpr int ST = C::ST;
@@ -278,7 +280,10 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
     uint64_t* p_hi = p_lo + 2;          // [tile]: and of the others
     uint64_t* o_done = p_hi + 2;        // [tile]: the pair's last P V of the tile is done
     uint64_t* turn = o_done + 2;        // [tile]: its products of the next step may be issued
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
+    uint64_t* i_full = turn + 2;        // [2]: the pair in s_item is the next one
+    uint64_t* i_empty = i_full + 2;     // [2]: every warp has read it
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + 2);
+    __shared__ WinItem s_item[2];       // n 0: no more
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -296,6 +301,8 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
             tc::mbar_init(&p_hi[t], 128);
             tc::mbar_init(&o_done[t], 1);
             tc::mbar_init(&turn[t], 1);
+            tc::mbar_init(&i_full[t], 1);
+            tc::mbar_init(&i_empty[t], 10);  // 2 issuers, 8 softmax warps
         }
         tc::fence_barrier_init();
     }
@@ -308,16 +315,35 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
     griddep_wait();
     griddep_launch_dependents();
 
-    WinList list;
-    WinItem it;
     uint32_t g = 0;  // key tiles of the pairs before this one
+    // Pair k as the producer found it: into `it`, false after the last one.  lanes: the whole warp calls it.
+    auto next_item = [&](uint32_t k, bool lanes, WinItem& it, bool& ok) -> bool {
+        ok = tc::mbar_wait(&i_full[k & 1], (k >> 1) & 1u, err, 103);
+        if (lanes) ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return false;
+        it = s_item[k & 1];
+        if (lanes) __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&i_empty[k & 1]);
+        return it.n > 0;
+    };
 
     if (warp == 8) {
         // ---------------- TMA producer ----------------
         if (lane == 0) {
-            bool ok = true;
-            uint32_t k = 0;
-            for (int64_t i = blockIdx.x; ok && list.get(a, i, it); i += gridDim.x, ++k) {
+            // Pair k + 1 is worked out and published while pair k is under way: divisions and a length's load that
+            // no other warp has to wait for.
+            WinList list;
+            WinItem it, ahead;
+            auto publish = [&](uint32_t k) -> bool {
+                if (k >= 2 && !tc::mbar_wait(&i_empty[k & 1], ((k >> 1) - 1) & 1u, err, 104)) return false;
+                if (!list.get(a, blockIdx.x + (int64_t)k * gridDim.x, ahead)) ahead.n = 0;
+                s_item[k & 1] = ahead;
+                tc::mbar_arrive(&i_full[k & 1]);
+                return true;
+            };
+            bool ok = publish(0);
+            for (uint32_t k = 0; ok && ahead.n > 0; ++k) {
+                it = ahead;
                 if (k > 0 && !tc::mbar_wait(q_empty, (k - 1) & 1u, err, 91)) break;
                 tc::mbar_arrive_expect_tx(q_full, 2 * TILE);
 #pragma unroll
@@ -325,7 +351,7 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
 #pragma unroll
                     for (int c = 0; c < C::ATOMS; ++c)
                         tc::tma_load_4d(sQ + t * TILE + c * ATOM, &tmQ, q_full, c * 64, it.h[t], it.row[t], it.b);
-                for (int j = 0; j < it.n; ++j, ++g) {
+                for (int j = 0; ok && j < it.n; ++j, ++g) {
                     const uint32_t s = g % ST, u = g / ST;
                     const int row = it.tile(j) * 128;
                     if (g >= ST && !(ok = tc::mbar_wait(&k_empty[s], (u - 1) & 1u, err, 92))) break;
@@ -338,6 +364,7 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
 #pragma unroll
                     for (int c = 0; c < C::ATOMS; ++c)
                         tc::tma_load_4d(sV + s * TILE + c * ATOM, &tmV, &v_full[s], c * 64, it.kvh, row, it.b);
+                    if (j == 0) ok = publish(k + 1);
                 }
             }
         }
@@ -353,7 +380,8 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
             const uint64_t dq = tc::desc_k_sw128(tc::smem_u32(sQ) + (uint32_t)t * TILE);
             const uint64_t dk0 = tc::desc_k_sw128(tc::smem_u32(sK)), dv0 = tc::desc_mn_sw128(tc::smem_u32(sV), ATOM);
             bool ok = true;
-            uint32_t k = 0, np = 0;  // pairs; P tiles consumed
+            uint32_t np = 0;  // P tiles consumed
+            WinItem it;
             auto wait_k = [&](uint32_t gj) { return tc::mbar_wait(&k_full[gj % ST], (gj / ST) & 1u, err, 94); };
             auto wait_v = [&](uint32_t gj) { return tc::mbar_wait(&v_full[gj % ST], (gj / ST) & 1u, err, 95); };
             // Turns: A's products of a step, then B's, and so on.  The other tile's products are in the
@@ -364,7 +392,7 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                 ++turns;
                 return mine;
             };
-            for (int64_t i = blockIdx.x; ok && list.get(a, i, it); i += gridDim.x, ++k) {
+            for (uint32_t k = 0; ok && next_item(k, false, it, ok); ++k) {
                 const int from = t == 0 ? 0 : it.dB, to = t == 0 ? it.nA : it.hasB ? it.n : 0;
                 int w = 0;
                 for (int j = -1; j < it.n; ++j) {
@@ -419,7 +447,8 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
         const uint64_t scale2 = two(a.scale_log2, a.scale_log2);
         bool ok = true;
         uint32_t cs = 0, co = 0;  // S tiles and outputs of this tile so far
-        for (int64_t i = blockIdx.x; ok && list.get(a, i, it); i += gridDim.x) {
+        WinItem it;
+        for (uint32_t k = 0; ok && next_item(k, true, it, ok); ++k) {
             const int from = t == 0 ? 0 : it.dB, to = t == 0 ? it.nA : it.hasB ? it.n : 0;
             const int wp = it.p[t] + rq * 32;  // position of the warp's first row
             const int pos = wp + lane < it.len ? wp + lane : -1;
@@ -454,8 +483,11 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                 if (!whole) {
                     // visible columns of the row as bits: lo .. hi and those below sk
                     const int hi = pos - kb, lo = a.window > 0 ? hi + 1 - a.window : 0, sk = a.window > 0 ? a.sinks - kb : 0;
+                    const int whi = wp - kb, wlo = a.window > 0 ? wp + 32 - a.window - kb : 0;  // what every row sees
+                    const bool in = wp + 31 < it.len;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
+                        if (in && 32 * c + 31 <= whi && (32 * c >= wlo || 32 * c + 32 <= sk)) continue;
                         const uint32_t see = below(hi + 1 - 32 * c) & (~below(lo - 32 * c) | below(sk - 32 * c));
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
@@ -511,41 +543,33 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                 ++co;
                 tc::fence_after_sync();
                 const float inv_l = l > 0.f ? 1.f / l : 0.f;
-                // 64 outputs of 32 rows at a time through shared memory: whole 128-byte lines leave
+                // 64 outputs of 32 rows at a time leave through shared memory by TMA
                 uint8_t* stage = sm + C::OFF_OUT + warp * 4096;
-                const int row = it.row[t] + rq * 32;
-                uint16_t* obase = static_cast<uint16_t*>(a.out) + (((int64_t)it.b * a.S + row) * a.nq + it.h[t]) * a.D;
 #pragma unroll 1
                 for (int c = 0; c < D; c += 64) {
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {
-                        uint32_t o[32];
-                        tc::tmem_ld32(tO + c + 32 * hh, o);
-                        tc::tmem_wait_ld();
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            uint4 x;
-                            x.x = win_pack<BF16>(__uint_as_float(o[8 * q + 0]) * inv_l, __uint_as_float(o[8 * q + 1]) * inv_l);
-                            x.y = win_pack<BF16>(__uint_as_float(o[8 * q + 2]) * inv_l, __uint_as_float(o[8 * q + 3]) * inv_l);
-                            x.z = win_pack<BF16>(__uint_as_float(o[8 * q + 4]) * inv_l, __uint_as_float(o[8 * q + 5]) * inv_l);
-                            x.w = win_pack<BF16>(__uint_as_float(o[8 * q + 6]) * inv_l, __uint_as_float(o[8 * q + 7]) * inv_l);
-                            *reinterpret_cast<uint4*>(stage + lane * 128 + (((hh * 4 + q) ^ (lane & 7)) << 4)) = x;
-                        }
-                    }
+                    uint32_t o[64];
+                    tc::tmem_ld32(tO + c, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+                    tc::tmem_ld32(tO + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
+                    tc::tmem_wait_ld();
+                    if (lane == 0) tc::tma_store_wait_read();  // the stage's last store
                     __syncwarp();
-                    const int ch = lane & 7;
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int r = k * 4 + (lane >> 3);
-                        if (ok && row + r < a.S && c + ch * 8 < a.D)
-                            *reinterpret_cast<uint4*>(obase + (int64_t)r * a.nq * a.D + c + ch * 8) =
-                                *reinterpret_cast<const uint4*>(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+                    for (int q = 0; q < 8; ++q) {
+                        uint4 x;
+                        x.x = win_pack<BF16>(__uint_as_float(o[8 * q + 0]) * inv_l, __uint_as_float(o[8 * q + 1]) * inv_l);
+                        x.y = win_pack<BF16>(__uint_as_float(o[8 * q + 2]) * inv_l, __uint_as_float(o[8 * q + 3]) * inv_l);
+                        x.z = win_pack<BF16>(__uint_as_float(o[8 * q + 4]) * inv_l, __uint_as_float(o[8 * q + 5]) * inv_l);
+                        x.w = win_pack<BF16>(__uint_as_float(o[8 * q + 6]) * inv_l, __uint_as_float(o[8 * q + 7]) * inv_l);
+                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((q ^ (lane & 7)) << 4)) = x;
                     }
+                    tc::fence_proxy_async_smem();
                     __syncwarp();
+                    if (ok && lane == 0 && c < a.D) tc::tma_store_4d(&tmO, stage, c, it.h[t], it.row[t] + rq * 32, it.b);
                 }
             }
             g += it.n;
         }
+        if (lane == 0) tc::tma_store_wait();
         // rows of tiles past a sequence's end: zeros
         if (a.seq_lens) {
             const int64_t row16 = (int64_t)a.nq * a.D / 8;
@@ -568,10 +592,11 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
     }
 }
 
-static int window_map(CUtensorMap* m, const b2_kv_view& v, int heads, int64_t rows, const WinArgs& a, bool bf16) {
+static int window_map(CUtensorMap* m, const b2_kv_view& v, int heads, int64_t rows, uint32_t box_rows, const WinArgs& a,
+                      bool bf16) {
     const uint64_t dims[4] = {(uint64_t)a.D, (uint64_t)heads, (uint64_t)rows, (uint64_t)a.batch};
     const uint64_t st[3] = {(uint64_t)v.stride_h * 2, (uint64_t)v.stride_s * 2, (uint64_t)v.stride_b * 2};
-    const uint32_t box[4] = {64, 1, 128, 1};
+    const uint32_t box[4] = {64, 1, box_rows, 1};
     return make_tensor_map(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, v.data,
                            dims, st, box);
 }
@@ -598,17 +623,22 @@ static int launch_window_tc(const WinArgs& a_in, cudaStream_t s) {
     tidy(a.q, a.nq, a.S);
     tidy(a.k, a.nkv, T);
     tidy(a.v, a.nkv, T);
-    CUtensorMap tq, tk, tv;
-    int rc = window_map(&tq, a.q, a.nq, a.S, a, BF16);
-    if (rc == B2_OK) rc = window_map(&tk, a.k, a.nkv, T, a, BF16);
-    if (rc == B2_OK) rc = window_map(&tv, a.v, a.nkv, T, a, BF16);
+    CUtensorMap tq, tk, tv, to;
+    int rc = window_map(&tq, a.q, a.nq, a.S, 128, a, BF16);
+    if (rc == B2_OK) rc = window_map(&tk, a.k, a.nkv, T, 128, a, BF16);
+    if (rc == B2_OK) rc = window_map(&tv, a.v, a.nkv, T, 128, a, BF16);
+    const b2_kv_view out = {a.out, (int64_t)a.S * a.nq * a.D, a.D, (int64_t)a.nq * a.D, 1};
+    if (rc == B2_OK) rc = window_map(&to, out, a.nq, a.S, 32, a, BF16);
     if (rc != B2_OK) return rc;
     auto kern = window_tc_kernel<D, BF16>;
     static bool done[64];
     B2_TRY(allow_smem(kern, (int)C::SMEM, done));
-    const int64_t items = (int64_t)a.batch * a.nkv * ((((int64_t)a.S + 127) / 128 * (a.nq / a.nkv) + 1) / 2);
+    // with no more tiles than SMs a tile to each is quicker than two to half of them (77 rows of 14 heads: 5.8 us, 7.2 paired)
+    const int64_t tiles = ((int64_t)a.S + 127) / 128 * (a.nq / a.nkv);
+    a.single = tiles * a.nkv * a.batch <= sm_count();
+    const int64_t items = (int64_t)a.batch * a.nkv * (a.single ? tiles : (tiles + 1) / 2);
     const unsigned grid = (unsigned)(items < sm_count() ? items : sm_count());
-    B2_TRY(launch(kern, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, tq, tk, tv, a, err));
+    B2_TRY(launch(kern, dim3(grid), dim3(C::THREADS), C::SMEM, s, true, tq, tk, tv, to, a, err));
     return B2_OK;
 }
 
