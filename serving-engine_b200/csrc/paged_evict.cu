@@ -313,12 +313,14 @@ extern "C" int b2_paged_kv_evict(const b2_paged_kv* kv, float* scores, const int
     a.new_lens = new_lens;
     const int64_t span = (int64_t)kv->max_blocks * kv->block_size;
     a.cached = (int)(span < kEvCached ? (span + 3) & ~int64_t(3) : kEvCached);
+    const int64_t rows = budget < span ? budget : span;
+    const int64_t parts = dst_tables ? (rows + kMvRows - 1) / kMvRows : kMvSlices;
+    if (parts > 65535) return B2_ERR_UNSUPPORTED;
     a.quads = kv->block_size % 4 == 0 && aligned16(scores);
     cudaStream_t s = as_stream(stream);
     static bool done[64];
     B2_TRY(allow_smem(evict_choose_kernel, kEvCached * 4, done));
     B2_TRY(launch(evict_choose_kernel, dim3(nkv, batch), dim3(kEvThreads), (size_t)a.cached * sizeof(float), s, true, a));
-    const int64_t parts = dst_tables ? ((int64_t)budget + kMvRows - 1) / kMvRows : kMvSlices;
     B2_TRY(launch(evict_move_kernel, dim3(nkv, (unsigned)parts, batch), dim3(kMvThreads), 0, s, true, a));
     return B2_OK;
 }

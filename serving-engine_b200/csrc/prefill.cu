@@ -833,18 +833,19 @@ extern "C" int b2_workspace_create(size_t bytes, b2_workspace** out) {
     *out = nullptr;
     b2_workspace* w = new (std::nothrow) b2_workspace();
     if (!w) return B2_ERR_INVALID;
-    void* c = nullptr;
-    cudaError_t e = cudaMalloc(&w->ptr, bytes);
-    if (e == cudaSuccess) e = cudaMalloc(&c, kWsCounters * sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(c, 0, kWsCounters * sizeof(int));
-    if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
+    // one allocation: the lent bytes, then the counters
+    const size_t lent = (bytes + 255) & ~size_t(255);
+    cudaError_t e = cudaMalloc(&w->ptr, lent + kWsCounters * sizeof(int));
+    if (e == cudaSuccess) {
+        w->counters = reinterpret_cast<int*>(static_cast<char*>(w->ptr) + lent);
+        e = cudaMemset(w->counters, 0, kWsCounters * sizeof(int));
+        if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
+    }
     if (e != cudaSuccess) {
-        cudaFree(c);
         cudaFree(w->ptr);
         delete w;
         return (int)e;
     }
-    w->counters = static_cast<int*>(c);
     w->bytes = bytes;
     *out = w;
     return B2_OK;
@@ -852,7 +853,6 @@ extern "C" int b2_workspace_create(size_t bytes, b2_workspace** out) {
 
 extern "C" int b2_workspace_destroy(b2_workspace* ws) {
     if (!ws) return B2_OK;
-    cudaFree(ws->counters);
     cudaFree(ws->ptr);
     delete ws;
     return B2_OK;

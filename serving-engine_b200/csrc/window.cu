@@ -30,6 +30,7 @@
 // for the product (its row sum is not): one more rounding the size of the
 // output's own.  Outputs leave through shared memory as whole 128-byte lines.
 #include <cmath>
+#include <type_traits>
 
 #include "tc.cuh"
 
@@ -123,8 +124,14 @@ struct WinCfg {
     // above half an SM's shared memory: one CTA, with all 512 TMEM columns, per SM
     static constexpr size_t NEED = OFF_BAR + 512 + 1024;
     static constexpr size_t SMEM = NEED > 122880 ? NEED : 122880;
-    static constexpr int THREADS = 352;  // warps 0-7 softmax, 8 TMA, 9 and 10 MMA of tile A and of tile B
+    // warps 0-7 softmax, 8 TMA, 9 and 10 MMA of tile A and of tile B, 11 idle (a warpgroup gives up registers as a whole)
+    static constexpr int THREADS = 384;
 };
+
+// The launch gives each of the three warpgroups 168 registers a thread; the
+// last one hands part of its share to the two whose threads hold a row of S.
+constexpr int kWinRegsFew = 104, kWinRegsMany = 200;
+static_assert(kWinRegsFew + 2 * kWinRegsMany <= 3 * 168, "more registers than the block is launched with");
 
 template <bool BF16>
 __device__ __forceinline__ uint32_t win_pack(float a, float b) {
@@ -327,119 +334,123 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
         return it.n > 0;
     };
 
-    if (warp == 8) {
-        // ---------------- TMA producer ----------------
-        if (lane == 0) {
-            // Pair k + 1 is worked out and published while pair k is under way: divisions and a length's load that
-            // no other warp has to wait for.
-            WinList list;
-            WinItem it, ahead;
-            auto publish = [&](uint32_t k) -> bool {
-                if (k >= 2 && !tc::mbar_wait(&i_empty[k & 1], ((k >> 1) - 1) & 1u, err, 104)) return false;
-                if (!list.get(a, blockIdx.x + (int64_t)k * gridDim.x, ahead)) ahead.n = 0;
-                s_item[k & 1] = ahead;
-                tc::mbar_arrive(&i_full[k & 1]);
-                return true;
-            };
-            bool ok = publish(0);
-            for (uint32_t k = 0; ok && ahead.n > 0; ++k) {
-                it = ahead;
-                if (k > 0 && !tc::mbar_wait(q_empty, (k - 1) & 1u, err, 91)) break;
-                tc::mbar_arrive_expect_tx(q_full, 2 * TILE);
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWinRegsFew));
+        if (warp == 8) {
+            // ---------------- TMA producer ----------------
+            if (lane == 0) {
+                // Pair k + 1 is worked out and published while pair k is under way: divisions and a length's load that
+                // no other warp has to wait for.
+                WinList list;
+                WinItem it, ahead;
+                auto publish = [&](uint32_t k) -> bool {
+                    if (k >= 2 && !tc::mbar_wait(&i_empty[k & 1], ((k >> 1) - 1) & 1u, err, 104)) return false;
+                    if (!list.get(a, blockIdx.x + (int64_t)k * gridDim.x, ahead)) ahead.n = 0;
+                    s_item[k & 1] = ahead;
+                    tc::mbar_arrive(&i_full[k & 1]);
+                    return true;
+                };
+                bool ok = publish(0);
+                for (uint32_t k = 0; ok && ahead.n > 0; ++k) {
+                    it = ahead;
+                    if (k > 0 && !tc::mbar_wait(q_empty, (k - 1) & 1u, err, 91)) break;
+                    tc::mbar_arrive_expect_tx(q_full, 2 * TILE);
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                    for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int c = 0; c < C::ATOMS; ++c)
-                        tc::tma_load_4d(sQ + t * TILE + c * ATOM, &tmQ, q_full, c * 64, it.h[t], it.row[t], it.b);
-                for (int j = 0; ok && j < it.n; ++j, ++g) {
-                    const uint32_t s = g % ST, u = g / ST;
-                    const int row = it.tile(j) * 128;
-                    if (g >= ST && !(ok = tc::mbar_wait(&k_empty[s], (u - 1) & 1u, err, 92))) break;
-                    tc::mbar_arrive_expect_tx(&k_full[s], TILE);
+                        for (int c = 0; c < C::ATOMS; ++c)
+                            tc::tma_load_4d(sQ + t * TILE + c * ATOM, &tmQ, q_full, c * 64, it.h[t], it.row[t], it.b);
+                    for (int j = 0; ok && j < it.n; ++j, ++g) {
+                        const uint32_t s = g % ST, u = g / ST;
+                        const int row = it.tile(j) * 128;
+                        if (g >= ST && !(ok = tc::mbar_wait(&k_empty[s], (u - 1) & 1u, err, 92))) break;
+                        tc::mbar_arrive_expect_tx(&k_full[s], TILE);
 #pragma unroll
-                    for (int c = 0; c < C::ATOMS; ++c)
-                        tc::tma_load_4d(sK + s * TILE + c * ATOM, &tmK, &k_full[s], c * 64, it.kvh, row, it.b);
-                    if (g >= ST && !(ok = tc::mbar_wait(&v_empty[s], (u - 1) & 1u, err, 93))) break;
-                    tc::mbar_arrive_expect_tx(&v_full[s], TILE);
+                        for (int c = 0; c < C::ATOMS; ++c)
+                            tc::tma_load_4d(sK + s * TILE + c * ATOM, &tmK, &k_full[s], c * 64, it.kvh, row, it.b);
+                        if (g >= ST && !(ok = tc::mbar_wait(&v_empty[s], (u - 1) & 1u, err, 93))) break;
+                        tc::mbar_arrive_expect_tx(&v_full[s], TILE);
 #pragma unroll
-                    for (int c = 0; c < C::ATOMS; ++c)
-                        tc::tma_load_4d(sV + s * TILE + c * ATOM, &tmV, &v_full[s], c * 64, it.kvh, row, it.b);
-                    if (j == 0) ok = publish(k + 1);
+                        for (int c = 0; c < C::ATOMS; ++c)
+                            tc::tma_load_4d(sV + s * TILE + c * ATOM, &tmV, &v_full[s], c * 64, it.kvh, row, it.b);
+                        if (j == 0) ok = publish(k + 1);
+                    }
                 }
             }
-        }
-    } else if (warp >= 9) {
-        // ---------------- MMA issuers: one per tile, so that the tensor core always has the other's
-        // products queued while one waits or computes descriptors ----------------
-        if (lane == 0) {
-            constexpr uint32_t idO = tc::idesc_f16(128, D, BF16, true);
-            constexpr uint32_t idS = tc::idesc_f16(128, 0, BF16, false);
-            const int t = warp - 9;
-            const uint32_t tP = tmem + (uint32_t)t * 256, tO = tP + 128;
-            // a descriptor's address field counts 16 bytes: steps are added to it
-            const uint64_t dq = tc::desc_k_sw128(tc::smem_u32(sQ) + (uint32_t)t * TILE);
-            const uint64_t dk0 = tc::desc_k_sw128(tc::smem_u32(sK)), dv0 = tc::desc_mn_sw128(tc::smem_u32(sV), ATOM);
-            bool ok = true;
-            uint32_t np = 0;  // P tiles consumed
-            WinItem it;
-            auto wait_k = [&](uint32_t gj) { return tc::mbar_wait(&k_full[gj % ST], (gj / ST) & 1u, err, 94); };
-            auto wait_v = [&](uint32_t gj) { return tc::mbar_wait(&v_full[gj % ST], (gj / ST) & 1u, err, 95); };
-            // Turns: A's products of a step, then B's, and so on.  The other tile's products are in the
-            // queue while this thread waits for its own operands, and the two softmaxes stay half a step apart.
-            uint32_t turns = 0;
-            auto my_turn = [&]() {
-                const bool mine = (t == 0 && turns == 0) || tc::mbar_wait(&turn[t], (turns - (t == 0)) & 1u, err, 102);
-                ++turns;
-                return mine;
-            };
-            for (uint32_t k = 0; ok && next_item(k, false, it, ok); ++k) {
-                const int from = t == 0 ? 0 : it.dB, to = t == 0 ? it.nA : it.hasB ? it.n : 0;
-                int w = 0;
-                for (int j = -1; j < it.n; ++j) {
-                    const uint32_t gj = g + (uint32_t)j, s = gj % ST, s1 = (gj + 1) % ST;
-                    const bool pv = j >= from && j < to, qk = j + 1 >= from && j + 1 < to;
-                    const int steps = w >> 4;
-                    if (qk) w = it.width(a, t, j + 1);
-                    if (j + 1 < it.n) ok = (j >= 0 || tc::mbar_wait(q_full, k & 1u, err, 96)) && wait_k(gj + 1);
-                    if (j >= 0) ok = ok && wait_v(gj);
-                    if (pv) ok = ok && tc::mbar_wait(&p_lo[t], np & 1u, err, 97);
-                    ok = ok && my_turn();
-                    if (!ok) break;
-                    tc::fence_after_sync();
-                    if (pv) {
-                        const uint64_t dv = dv0 + s * (TILE >> 4);
-                        tc::mma_f16_ts(tO, tP, dv, idO, j > from ? 1u : 0u);
-#pragma unroll
-                        for (int kk = 1; kk < 4; ++kk)
-                            if (kk < steps) tc::mma_f16_ts(tO, tP + (uint32_t)kk * 8, dv + (uint32_t)kk * 128u, idO, 1u);
-                        if (!(ok = tc::mbar_wait(&p_hi[t], np & 1u, err, 101))) break;
-                        ++np;
+        } else if (warp <= 10) {
+            // ---------------- MMA issuers: one per tile, so that the tensor core always has the other's
+            // products queued while one waits or computes descriptors ----------------
+            if (lane == 0) {
+                constexpr uint32_t idO = tc::idesc_f16(128, D, BF16, true);
+                constexpr uint32_t idS = tc::idesc_f16(128, 0, BF16, false);
+                const int t = warp - 9;
+                const uint32_t tP = tmem + (uint32_t)t * 256, tO = tP + 128;
+                // a descriptor's address field counts 16 bytes: steps are added to it
+                const uint64_t dq = tc::desc_k_sw128(tc::smem_u32(sQ) + (uint32_t)t * TILE);
+                const uint64_t dk0 = tc::desc_k_sw128(tc::smem_u32(sK)), dv0 = tc::desc_mn_sw128(tc::smem_u32(sV), ATOM);
+                bool ok = true;
+                uint32_t np = 0;  // P tiles consumed
+                WinItem it;
+                auto wait_k = [&](uint32_t gj) { return tc::mbar_wait(&k_full[gj % ST], (gj / ST) & 1u, err, 94); };
+                auto wait_v = [&](uint32_t gj) { return tc::mbar_wait(&v_full[gj % ST], (gj / ST) & 1u, err, 95); };
+                // Turns: A's products of a step, then B's, and so on.  The other tile's products are in the
+                // queue while this thread waits for its own operands, and the two softmaxes stay half a step apart.
+                uint32_t turns = 0;
+                auto my_turn = [&]() {
+                    const bool mine = (t == 0 && turns == 0) || tc::mbar_wait(&turn[t], (turns - (t == 0)) & 1u, err, 102);
+                    ++turns;
+                    return mine;
+                };
+                for (uint32_t k = 0; ok && next_item(k, false, it, ok); ++k) {
+                    const int from = t == 0 ? 0 : it.dB, to = t == 0 ? it.nA : it.hasB ? it.n : 0;
+                    int w = 0;
+                    for (int j = -1; j < it.n; ++j) {
+                        const uint32_t gj = g + (uint32_t)j, s = gj % ST, s1 = (gj + 1) % ST;
+                        const bool pv = j >= from && j < to, qk = j + 1 >= from && j + 1 < to;
+                        const int steps = w >> 4;
+                        if (qk) w = it.width(a, t, j + 1);
+                        if (j + 1 < it.n) ok = (j >= 0 || tc::mbar_wait(q_full, k & 1u, err, 96)) && wait_k(gj + 1);
+                        if (j >= 0) ok = ok && wait_v(gj);
+                        if (pv) ok = ok && tc::mbar_wait(&p_lo[t], np & 1u, err, 97);
+                        ok = ok && my_turn();
+                        if (!ok) break;
                         tc::fence_after_sync();
+                        if (pv) {
+                            const uint64_t dv = dv0 + s * (TILE >> 4);
+                            tc::mma_f16_ts(tO, tP, dv, idO, j > from ? 1u : 0u);
 #pragma unroll
-                        for (int kk = 4; kk < 8; ++kk)
-                            if (kk < steps) tc::mma_f16_ts(tO, tP + (uint32_t)kk * 8, dv + (uint32_t)kk * 128u, idO, 1u);
-                        if (j + 1 == to) tc::mma_commit(&o_done[t]);
-                    }
-                    if (qk) {
-                        const uint64_t dk = dk0 + s1 * (TILE >> 4);
-                        const uint32_t id = idS | ((uint32_t)(w >> 3) << 17);
+                            for (int kk = 1; kk < 4; ++kk)
+                                if (kk < steps) tc::mma_f16_ts(tO, tP + (uint32_t)kk * 8, dv + (uint32_t)kk * 128u, idO, 1u);
+                            if (!(ok = tc::mbar_wait(&p_hi[t], np & 1u, err, 101))) break;
+                            ++np;
+                            tc::fence_after_sync();
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk) {
-                            const uint32_t off = ((uint32_t)(kk >> 2) * ATOM + (uint32_t)(kk & 3) * 32) >> 4;
-                            tc::mma_f16(tP, dq + off, dk + off, id, kk > 0 ? 1u : 0u);
+                            for (int kk = 4; kk < 8; ++kk)
+                                if (kk < steps) tc::mma_f16_ts(tO, tP + (uint32_t)kk * 8, dv + (uint32_t)kk * 128u, idO, 1u);
+                            if (j + 1 == to) tc::mma_commit(&o_done[t]);
                         }
-                        tc::mma_commit(&s_full[t]);
+                        if (qk) {
+                            const uint64_t dk = dk0 + s1 * (TILE >> 4);
+                            const uint32_t id = idS | ((uint32_t)(w >> 3) << 17);
+#pragma unroll
+                            for (int kk = 0; kk < D / 16; ++kk) {
+                                const uint32_t off = ((uint32_t)(kk >> 2) * ATOM + (uint32_t)(kk & 3) * 32) >> 4;
+                                tc::mma_f16(tP, dq + off, dk + off, id, kk > 0 ? 1u : 0u);
+                            }
+                            tc::mma_commit(&s_full[t]);
+                        }
+                        tc::mbar_arrive(&turn[t ^ 1]);
+                        // whatever this tile read of the step's K and V has been read once these arrive
+                        if (j >= 0) tc::mma_commit(&v_empty[s]);
+                        if (j + 1 < it.n) tc::mma_commit(&k_empty[s1]);
+                        if (j + 2 == it.n) tc::mma_commit(q_empty);
                     }
-                    tc::mbar_arrive(&turn[t ^ 1]);
-                    // whatever this tile read of the step's K and V has been read once these arrive
-                    if (j >= 0) tc::mma_commit(&v_empty[s]);
-                    if (j + 1 < it.n) tc::mma_commit(&k_empty[s1]);
-                    if (j + 2 == it.n) tc::mma_commit(q_empty);
+                    g += it.n;
                 }
-                g += it.n;
             }
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWinRegsMany));
         // ---------------- softmax and output: tile t, one query row per thread ----------------
         const int t = warp >> 2, rq = warp & 3;
         const uint32_t lane_base = (uint32_t)(rq * 32) << 16;
@@ -518,23 +529,30 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                 m = m_use;
                 const uint64_t nm2 = two(-m, -m);
                 uint64_t l2[2] = {0, 0};
+                auto weights = [&](auto masked) {  // columns past w are not read by the product
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t pk[16];
+                    for (int c = 0; c < 4; ++c) {
+                        if (!decltype(masked)::value || 32 * c < w) {
+                            uint32_t pk[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float2 x = one_each(fma2(two(__uint_as_float(v[32 * c + e]), __uint_as_float(v[32 * c + e + 1])), scale2, nm2));
-                        const float p0 = win_ex2(x.x), p1 = win_ex2(x.y);
-                        l2[(e >> 1) & 1] = add2(l2[(e >> 1) & 1], two(p0, p1));
-                        pk[e >> 1] = win_pack<BF16>(p0, p1);
+                            for (int e = 0; e < 32; e += 2) {
+                                const float2 x = one_each(
+                                    fma2(two(__uint_as_float(v[32 * c + e]), __uint_as_float(v[32 * c + e + 1])), scale2, nm2));
+                                const float p0 = win_ex2(x.x), p1 = win_ex2(x.y);
+                                l2[(e >> 1) & 1] = add2(l2[(e >> 1) & 1], two(p0, p1));
+                                pk[e >> 1] = win_pack<BF16>(p0, p1);
+                            }
+                            tc::tmem_st16(tS + (uint32_t)(16 * c), pk);
+                        }
+                        if (c & 1) {
+                            tc::tmem_wait_st();
+                            tc::fence_before_sync();
+                            tc::mbar_arrive(c == 1 ? &p_lo[t] : &p_hi[t]);
+                        }
                     }
-                    tc::tmem_st16(tS + (uint32_t)(16 * c), pk);
-                    if (c & 1) {
-                        tc::tmem_wait_st();
-                        tc::fence_before_sync();
-                        tc::mbar_arrive(c == 1 ? &p_lo[t] : &p_hi[t]);
-                    }
-                }
+                };
+                if (whole) weights(std::false_type());
+                else weights(std::true_type());
                 const float2 ls = one_each(add2(l2[0], l2[1]));
                 l = l * alpha + (ls.x + ls.y);
             }
