@@ -6,14 +6,16 @@
 // order, to positions 0 .. n-1.  The bytes are the scores once, and the kept
 // rows read and written (8 D bytes each): HBM bounds it, the choice is latency.
 //
-// Two launches.  The choice is one CTA per (sequence, kv head): the positions'
-// ordered keys in shared memory, the n-th best found 11 bits at a time from a
-// histogram, then every kept position's place by one scan, ties going to the
-// lowest positions.  Latency bounds it: the scores are a small part of the
-// bytes.  (A cluster of 8 CTAs per choice, histograms added through
-// distributed shared memory, took 20 us a cluster for 4096 scores: each of its
-// exchanges costs more than the reading it saves.)
-// The move is spread over the GPU.
+// The choice is one CTA per (sequence, kv head): the positions' ordered keys
+// in shared memory, the n-th best found 11 bits at a time from a histogram,
+// then every kept position's place by one scan, ties going to the lowest
+// positions.  Latency bounds it: the scores are a small part of the bytes.  (A
+// cluster of 8 CTAs per choice, histograms added through distributed shared
+// memory, took 20 us a cluster for 4096 scores, this 10: each of its exchanges
+// costs more than the reading it saves.)  The move is a second launch spread
+// over the GPU, or, where few bytes stay, the choosing CTA's own.  Measured: 16
+// x 32768 to 8192 (8 heads of 128, half): 201 us, the move 177 of them at 5.9
+// TB/s (92 % of the measured copy); 8 x up to 4096 to 1024: 20 us.
 //
 // Moving in place is safe without a second copy because kept position j comes
 // from kept[j] >= j and kept rises: a CTA takes rows in order of j in batches,
@@ -27,11 +29,12 @@
 namespace b2 {
 
 constexpr int kEvThreads = 1024;   // of a choice
-constexpr int kEvCached = 49152;   // keys of a choice kept in shared memory; the rest are read again
+constexpr int kEvCached = 45056;   // keys of a choice kept in shared memory; the rest are read again
 constexpr int kMvThreads = 256;    // of a move
 constexpr int kMvBatch = 4;        // 16-byte pieces in flight per thread
 constexpr int kMvRows = 128;       // rows looked up together; those of a CTA that moves into other blocks
 constexpr int kMvSlices = 8;       // column slices in place
+constexpr int64_t kFusedBytes = 128 << 10;
 
 struct EvictArgs {
     b2_paged_kv kv;
@@ -51,17 +54,74 @@ struct EvictArgs {
 constexpr uint32_t kEvStays = 0xffffffffu, kEvNan = 0xfffffffeu;
 __device__ __forceinline__ uint32_t rank_key(float f) { return f != f ? kEvNan : float_key(f + 0.f); }
 
-__global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const EvictArgs a) {
+// Moves rows j0 .. j1 - 1 of one (sequence, kv head), pieces first .. first +
+// width - 1 of each (16 bytes; K's, then V's), and their scores if `scores`.
+// The whole CTA of THREADS calls it.  One thread per row looks up where it
+// comes from and goes; the copies then take a few instructions per 16 bytes
+// (looking up per copy bounded the kernel by its arithmetic: 5.0 TB/s).
+template <int ROWS>
+struct MoveLists {
+    int64_t from[ROWS], to[ROWS];  // of the rows looked up together, in elements; from -1: nothing to move
+};
+template <int THREADS, int ROWS>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int kvh, int b, int j0, int j1, int first, int width,
+                                          bool scores, MoveLists<ROWS>& list) {
+    const int t = threadIdx.x;
+    const int* bt = a.kv.block_tables + (int64_t)b * a.kv.max_blocks;
+    const int* dt = a.dst ? a.dst + (int64_t)b * a.dst_blocks : bt;
+    const int* kept = a.kept + ((int64_t)b * a.nkv + kvh) * a.budget;
+    const int chunks = a.D / 8;
+    // thread t: piece first + t % width of rows t / width, t / width + rows, ..
+    const int rows = width > 0 ? THREADS / width : 0, r = width > 0 ? t / width : 0, piece = first + t - r * width;
+    uint4* base = static_cast<uint4*>(piece < chunks ? a.kv.k : a.kv.v) + (piece < chunks ? piece : piece - chunks);
+    for (int jb = j0; jb < j1; jb += ROWS) {
+        const int m = min(ROWS, j1 - jb);
+        int64_t sf = -1, st = -1;
+        float sv = 0.f;
+        if (t < m) {
+            const int j = jb + t, i = __ldcg(kept + j), ib = a.div.block(i), jb2 = a.div.block(j);
+            const int sb = bt[ib], db = dt[jb2];
+            const bool go = (unsigned)sb < (unsigned)a.kv.num_blocks && (unsigned)db < (unsigned)a.kv.num_blocks &&
+                            (a.dst || i != j);
+            const int ss = a.div.slot(i, ib), ds = a.div.slot(j, jb2);
+            list.from[t] = go ? sb * a.kv.stride_block + ss * a.kv.stride_slot + kvh * a.kv.stride_head : -1;
+            list.to[t] = db * a.kv.stride_block + ds * a.kv.stride_slot + kvh * a.kv.stride_head;
+            if (go && scores) {
+                sf = ((int64_t)sb * a.nkv + kvh) * a.kv.block_size + ss;
+                st = ((int64_t)db * a.nkv + kvh) * a.kv.block_size + ds;
+                sv = a.scores[sf];
+            }
+        }
+        __syncthreads();  // (in place it also parts the batch's score reads from its writes)
+        if (sf >= 0) a.scores[st] = sv;
+        for (int k0 = 0; k0 < m; k0 += rows * kMvBatch) {
+            if (rows == 0) break;
+            int64_t from[kMvBatch];
+            uint4 v[kMvBatch];
+#pragma unroll
+            for (int e = 0; e < kMvBatch; ++e) {
+                const int k = k0 + e * rows + r;
+                from[e] = r < rows && k < m ? list.from[k] : -1;
+                if (from[e] >= 0) v[e] = __ldcs(base + (from[e] >> 3));
+            }
+            if (!a.dst) __syncthreads();
+#pragma unroll
+            for (int e = 0; e < kMvBatch; ++e)
+                if (from[e] >= 0) __stcs(base + (list.to[k0 + e * rows + r] >> 3), v[e]);
+        }
+        __syncthreads();
+    }
+}
+
+// Fills kept for (kvh, b) of a sequence of L positions; the whole CTA of kEvThreads calls it.
+__device__ __forceinline__ void choose(const EvictArgs& a, int kvh, int b, int L) {
     extern __shared__ __align__(16) uint32_t s_key[];
     __shared__ int s_hist[2][2048];
     __shared__ int s_pick[2];  // the bin that holds the n-th best, positions above it
     __shared__ int s_sum[kEvThreads / 32];
     __shared__ int2 s_warp[kEvThreads / 32];
-    const int kvh = blockIdx.x, b = blockIdx.y, t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int bs = a.kv.block_size;
-    griddep_wait();
-    griddep_launch_dependents();
-    const int L = paged_len(a.kv, b), n = min(L, a.budget);
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int bs = a.kv.block_size, n = min(L, a.budget);
     const int* bt = a.kv.block_tables + (int64_t)b * a.kv.max_blocks;
     int* kept = a.kept + ((int64_t)b * a.nkv + kvh) * a.budget;
     if (L <= a.budget) {
@@ -215,74 +275,46 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const Evict
     }
 }
 
+// grid (kv heads, sequences).  FUSED: the CTA moves the rows as well.
+template <bool FUSED>
+__global__ void __launch_bounds__(kEvThreads, 1) evict_choose_kernel(const EvictArgs a) {
+    const int kvh = blockIdx.x, b = blockIdx.y;
+    griddep_wait();
+    griddep_launch_dependents();
+    const int L = paged_len(a.kv, b);
+    choose(a, kvh, b, L);
+    if constexpr (FUSED) {
+        __shared__ MoveLists<kEvThreads> list;
+        const int n = min(L, a.budget);
+        if (kvh == 0 && threadIdx.x == 0) a.new_lens[b] = n;
+        __syncthreads();  // the list is whole
+        move_rows<kEvThreads, kEvThreads>(a, kvh, b, 0, n, 0, a.D / 4, true, list);
+    }
+}
+
 // grid (kv heads; row ranges, or column slices in place; sequences): the heads
-// of one range run together, so that their rows' DRAM pages do.  One thread
-// per row looks up where it comes from and goes; the copies then take a few
-// instructions per 16 bytes (looking up per copy bounded the kernel by its
-// arithmetic: 5.0 TB/s).
+// of one range run together, so that their rows' DRAM pages do.
 __global__ void __launch_bounds__(kMvThreads, 4) evict_move_kernel(const EvictArgs a) {
-    __shared__ int64_t s_from[kMvRows], s_to[kMvRows];  // elements; from -1: nothing to move
+    __shared__ MoveLists<kMvRows> list;
     const int kvh = blockIdx.x, b = blockIdx.z, rank = blockIdx.y, parts = gridDim.y, t = threadIdx.x;
     griddep_wait();
     griddep_launch_dependents();
     // (new_lens may be the lengths themselves: the minimum below is the same before and after)
     const int L = paged_len(a.kv, b), n = min(L, a.budget);
     if (kvh == 0 && rank == 0 && t == 0) a.new_lens[b] = n;
-    const int* bt = a.kv.block_tables + (int64_t)b * a.kv.max_blocks;
-    const int* dt = a.dst ? a.dst + (int64_t)b * a.dst_blocks : bt;
-    const int* kept = a.kept + ((int64_t)b * a.nkv + kvh) * a.budget;
-    const int chunks = a.D / 8;  // 16-byte pieces of a row, K's then V's
-    int j0 = 0, j1 = n, first = 0, width = 2 * chunks;
+    const int pieces = a.D / 4;  // 16-byte pieces of a K and a V row
+    int j0 = 0, j1 = n, first = 0, width = pieces;
     bool scores = true;
     if (a.dst) {
         j0 = min(n, rank * kMvRows);
         j1 = min(n, j0 + kMvRows);
     } else {
-        width = (2 * chunks + parts - 1) / parts;
-        first = min(2 * chunks, rank * width);
-        width = min(width, 2 * chunks - first);
+        width = (pieces + parts - 1) / parts;
+        first = min(pieces, rank * width);
+        width = min(width, pieces - first);
         scores = rank == 0;
     }
-    // thread t: piece first + t % width of rows t / width, t / width + rows, ..
-    const int rows = width > 0 ? kMvThreads / width : 0, r = width > 0 ? t / width : 0, piece = first + t - r * width;
-    uint4* base = static_cast<uint4*>(piece < chunks ? a.kv.k : a.kv.v) + (piece < chunks ? piece : piece - chunks);
-    for (int jb = j0; jb < j1; jb += kMvRows) {
-        const int m = min(kMvRows, j1 - jb);
-        int64_t sf = -1, st = -1;
-        float sv = 0.f;
-        if (t < m) {
-            const int j = jb + t, i = __ldcg(kept + j), ib = a.div.block(i), jb2 = a.div.block(j);
-            const int sb = bt[ib], db = dt[jb2];
-            const bool go = (unsigned)sb < (unsigned)a.kv.num_blocks && (unsigned)db < (unsigned)a.kv.num_blocks &&
-                            (a.dst || i != j);
-            const int ss = a.div.slot(i, ib), ds = a.div.slot(j, jb2);
-            s_from[t] = go ? sb * a.kv.stride_block + ss * a.kv.stride_slot + kvh * a.kv.stride_head : -1;
-            s_to[t] = db * a.kv.stride_block + ds * a.kv.stride_slot + kvh * a.kv.stride_head;
-            if (go && scores) {
-                sf = ((int64_t)sb * a.nkv + kvh) * a.kv.block_size + ss;
-                st = ((int64_t)db * a.nkv + kvh) * a.kv.block_size + ds;
-                sv = a.scores[sf];
-            }
-        }
-        __syncthreads();  // (in place it also parts the batch's score reads from its writes)
-        if (sf >= 0) a.scores[st] = sv;
-        for (int k0 = 0; k0 < m; k0 += rows * kMvBatch) {
-            if (rows == 0) break;
-            int64_t from[kMvBatch];
-            uint4 v[kMvBatch];
-#pragma unroll
-            for (int e = 0; e < kMvBatch; ++e) {
-                const int k = k0 + e * rows + r;
-                from[e] = r < rows && k < m ? s_from[k] : -1;
-                if (from[e] >= 0) v[e] = __ldcs(base + (from[e] >> 3));
-            }
-            if (!a.dst) __syncthreads();
-#pragma unroll
-            for (int e = 0; e < kMvBatch; ++e)
-                if (from[e] >= 0) __stcs(base + (s_to[k0 + e * rows + r] >> 3), v[e]);
-        }
-        __syncthreads();
-    }
+    move_rows<kMvThreads, kMvRows>(a, kvh, b, j0, j1, first, width, scores, list);
 }
 
 }  // namespace b2
@@ -318,9 +350,20 @@ extern "C" int b2_paged_kv_evict(const b2_paged_kv* kv, float* scores, const int
     if (parts > 65535) return B2_ERR_UNSUPPORTED;
     a.quads = kv->block_size % 4 == 0 && aligned16(scores);
     cudaStream_t s = as_stream(stream);
+    const size_t smem = (size_t)a.cached * sizeof(uint32_t);
+    // One launch or two, by the bytes a (sequence, kv head) keeps.  At 64 KB (256 rows of 64, 2 heads) one launch takes
+    // 8.5 us on the device and 3.9 on the host, two take 7.9 and 6.3; at 128 KB 9.9 against 8.5 for 2 pairs, but 11.6
+    // against 14.4 for 128; at 256 KB (512 rows of 128, 8 pairs) 12.7 against 8.9.  Lengths written over the old ones
+    // need the second launch: other heads' CTAs still read them.
+    if (rows * 4 * D <= kFusedBytes && new_lens != kv->seq_lens) {
+        static bool fused[64];
+        B2_TRY(allow_smem(evict_choose_kernel<true>, kEvCached * 4, fused));
+        B2_TRY(launch(evict_choose_kernel<true>, dim3(nkv, batch), dim3(kEvThreads), smem, s, true, a));
+        return B2_OK;
+    }
     static bool done[64];
-    B2_TRY(allow_smem(evict_choose_kernel, kEvCached * 4, done));
-    B2_TRY(launch(evict_choose_kernel, dim3(nkv, batch), dim3(kEvThreads), (size_t)a.cached * sizeof(float), s, true, a));
+    B2_TRY(allow_smem(evict_choose_kernel<false>, kEvCached * 4, done));
+    B2_TRY(launch(evict_choose_kernel<false>, dim3(nkv, batch), dim3(kEvThreads), smem, s, true, a));
     B2_TRY(launch(evict_move_kernel, dim3(nkv, (unsigned)parts, batch), dim3(kMvThreads), 0, s, true, a));
     return B2_OK;
 }
