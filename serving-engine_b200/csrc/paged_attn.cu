@@ -37,6 +37,7 @@
 // instead of reading K again.
 #include <cmath>
 
+#include "mma.cuh"
 #include "paged.cuh"
 #include "workspace.cuh"
 
@@ -46,7 +47,6 @@ constexpr int kPgWarps = 4;
 constexpr int kPgThreads = kPgWarps * 32;
 constexpr int kPgStages = 3;
 constexpr int kPgScoreThreads = 128;
-constexpr int kPgMinUnits = 4;  // a range is at least this many units
 
 struct PagedArgs {
     const void* q;
@@ -82,9 +82,6 @@ struct PagedCfg {
     static constexpr int CTAS = DP == 256 ? 1 : 2;    // per SM
 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
 // Rows are read once: they leave the L2 first, and what the call reads again
 // (logits, partial results, tables) stays (8 x 4096 with weights: 30.4 us, 32.2
 // without).
@@ -104,42 +101,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(a)
-                 : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(a)
-                 : "memory");
-}
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float& c0, float& c1, float& c2, float& c3, uint32_t a0, uint32_t a1,
-                                         uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (BF16)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c0), "+f"(c1), "+f"(c2), "+f"(c3)
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(c0), "+f"(c1), "+f"(c2), "+f"(c3)
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack16(float a, float b) {
-    if constexpr (BF16) {
-        __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<uint32_t*>(&h);
-    } else {
-        return f2_to_h2(a, b);
-    }
-}
 // (a, b) as 16-bit values and what the rounding left, again in 16 bits
 template <bool BF16>
 __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
@@ -157,11 +118,6 @@ template <bool BF16>
 __device__ __forceinline__ void store4(void* p, int64_t i, float4 v, float scale) {
     const uint2 x = make_uint2(pack16<BF16>(v.x * scale, v.y * scale), pack16<BF16>(v.z * scale, v.w * scale));
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = x;
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 // What the newest token of a sequence of L tokens sees, in units of U
@@ -239,7 +195,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
         s.n = 0;
         if (lane < a.batch) s.of(a, lane);
         total = __reduce_add_sync(~0u, s.n) * heads;
-        upc = max(kPgMinUnits, (total + grid - 1) / grid);
+        upc = (total + grid - 1) / grid;
         int here = s.n * heads;
         if (can_piece) {
             int pick = -1;
@@ -293,7 +249,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
             return make_int2(incl - mine, incl);
         };
         int2 span = scan([&](int n) { return n * heads; });
-        upc = max(kPgMinUnits, (total + grid - 1) / grid);
+        upc = (total + grid - 1) / grid;
         if (can_piece) {
             const int size = size_of(tid & 7);
             int n = 0, pick = -1;

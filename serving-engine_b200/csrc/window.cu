@@ -32,6 +32,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "mma.cuh"
 #include "tc.cuh"
 
 namespace b2 {
@@ -46,65 +47,162 @@ struct WinArgs {
     int single;  // tiles are not paired
 };
 
-template <bool BF16>
-__device__ __forceinline__ float ld16f(const void* p, int64_t i) {
-    if constexpr (BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-    return __half2float(static_cast<const __half*>(p)[i]);
+// ---------------------------------------------------------------------------
+// mma.sync form: head_dim above 128, and rows that 16-byte copies cannot take
+// ---------------------------------------------------------------------------
+// A CTA takes 64 query rows of one head, 16 a warp, queries and outputs in
+// registers; the keys any of its rows sees come 32 at a time through shared
+// memory, first the sinks, then from the first row's window on.  Bound by
+// mma.sync and by the loads it does not overlap: 8192 tokens, window 2048, 32
+// heads of 128 take MMAMS ms this way (the tcgen05 form 0.27).
+constexpr int kWmRows = 64, kWmKeys = 32, kWmThreads = 128;
+
+// 8 elements from p, of which n exist; vec: p is 16-byte aligned
+__device__ __forceinline__ uint4 ld8(const uint16_t* p, int n, bool vec) {
+    uint4 r = make_uint4(0, 0, 0, 0);
+    if (vec && n >= 8) return *reinterpret_cast<const uint4*>(p);
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < n) w[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+    return r;
 }
 
-template <bool BF16>
-__device__ __forceinline__ void st16f(void* p, int64_t i, float v) {
-    if constexpr (BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-    else static_cast<__half*>(p)[i] = __float2half_rn(v);
-}
-
-// One warp per (query, head); lane l holds elements l, l + 32, .. of the
-// rows.  Any element alignment, D <= 256.
-template <bool BF16>
-__global__ void __launch_bounds__(256) window_rows_kernel(const WinArgs a) {
+// DP: head dim rounded up to 64, 128 or 256
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kWmThreads) window_mma_kernel(const WinArgs a, int vec) {
+    constexpr int ROW = DP * 2, CH = DP / 8;
+    extern __shared__ __align__(16) uint8_t smem[];  // K rows, V rows; 16-byte pieces swizzled by the row
     griddep_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t n = (int64_t)a.batch * a.S * a.nq;
-    for (int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; w < n;
-         w += ((int64_t)gridDim.x * blockDim.x) >> 5) {
-        const int h = (int)(w % a.nq);
-        const int i = (int)((w / a.nq) % a.S);
-        const int b = (int)(w / ((int64_t)a.nq * a.S));
-        const int pos = a.q_start + i;
-        const int len = a.seq_lens ? min(a.seq_lens[b], a.q_start + a.S) : a.q_start + a.S;
-        const int kvh = h / (a.nq / a.nkv);
-        float q[8], o[8], m = -INFINITY, l = 0.f;
+    griddep_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lr = lane >> 2, lc = lane & 3;
+    const uint32_t sk = smem_addr(smem), sv = sk + kWmKeys * ROW;
+    const int tiles = (a.S + kWmRows - 1) / kWmRows, T = a.q_start + a.S;
+    const int64_t items = (int64_t)a.batch * tiles * a.nq;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int h = (int)(item % a.nq), tile = tiles - 1 - (int)((item / a.nq) % tiles);
+        const int b = (int)(item / ((int64_t)a.nq * tiles)), kvh = h / (a.nq / a.nkv);
+        const int len = a.seq_lens ? max(0, min(a.seq_lens[b], T)) : T;
+        const int row0 = tile * kWmRows + warp * 16, p0 = a.q_start + tile * kWmRows;  // p0: position of the CTA's first row
+        const int pos[2] = {a.q_start + row0 + lr, a.q_start + row0 + lr + 8};
+        const uint16_t* K = static_cast<const uint16_t*>(a.k.data) + b * a.k.stride_b + kvh * a.k.stride_h;
+        const uint16_t* V = static_cast<const uint16_t*>(a.v.data) + b * a.v.stride_b + kvh * a.v.stride_h;
+        uint32_t qa[DP / 16][4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int d = lane + 32 * e;
-            q[e] = d < a.D ? ld16f<BF16>(a.q.data, b * a.q.stride_b + h * a.q.stride_h + i * a.q.stride_s + d) : 0.f;
-            o[e] = 0.f;
-        }
-        if (pos < len) {
-            const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-            const int64_t kb = b * a.k.stride_b + kvh * a.k.stride_h, vb = b * a.v.stride_b + kvh * a.v.stride_h;
-            for (int j = 0; j <= pos; ++j) {
-                if (j < lo && j >= a.sinks) j = lo;
-                float s = 0.f;
+        for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (lane + 32 * e < a.D) s = fmaf(q[e], ld16f<BF16>(a.k.data, kb + j * a.k.stride_s + lane + 32 * e), s);
-                s = warp_sum(s) * a.scale_log2;
-                const float m_new = fmaxf(m, s);
-                const float al = exp2f(m - m_new), p = exp2f(s - m_new);
-                m = m_new;
-                l = fmaf(l, al, p);
+            for (int e = 0; e < 4; ++e) {
+                const int row = row0 + lr + (e & 1) * 8, col = kk * 16 + lc * 2 + (e >> 1) * 8;
+                const uint16_t* q = static_cast<const uint16_t*>(a.q.data) + b * a.q.stride_b + h * a.q.stride_h +
+                                    (int64_t)row * a.q.stride_s + col;
+                qa[kk][e] = 0u;
+                if (row < a.S && col < a.D) qa[kk][e] = q[0];
+                if (row < a.S && col + 1 < a.D) qa[kk][e] |= (uint32_t)q[1] << 16;
+            }
+        float o[DP / 8][4] = {}, m[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f};
+        const int lo = a.window > 0 ? max(0, p0 - a.window + 1) : 0, hi = min(p0 + kWmRows, len);  // keys lo .. hi - 1
+        const int s0 = min(a.sinks, lo);
+        if (p0 < len) {
+            for (int j0 = s0 > 0 ? 0 : lo; j0 < hi; j0 = j0 < s0 && j0 + kWmKeys >= s0 ? lo : j0 + kWmKeys) {
+                const int n = min(kWmKeys, (j0 < s0 ? s0 : hi) - j0);
+                __syncthreads();
+                for (int i = threadIdx.x; i < kWmKeys * CH; i += kWmThreads) {
+                    const int r = i / CH, c = i - r * CH, off = r * ROW + ((c ^ (r & 7)) << 4);
+                    const int have = r < n ? a.D - c * 8 : 0;
+                    *reinterpret_cast<uint4*>(smem + off) = ld8(K + (int64_t)(j0 + r) * a.k.stride_s + c * 8, have, vec);
+                    *reinterpret_cast<uint4*>(smem + kWmKeys * ROW + off) =
+                        ld8(V + (int64_t)(j0 + r) * a.v.stride_s + c * 8, have, vec);
+                }
+                __syncthreads();
+                const int mi = lane >> 3, mr = lane & 7;
+                float s[4][4] = {};
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (lane + 32 * e < a.D)
-                        o[e] = fmaf(o[e], al, p * ld16f<BF16>(a.v.data, vb + j * a.v.stride_s + lane + 32 * e));
+                for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {  // 16 keys
+                        uint32_t kf[4];
+                        ldsm4(kf, sk + (g * 16 + (mi >> 1) * 8 + mr) * ROW + (((kk * 2 + (mi & 1)) ^ mr) << 4));
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            float* c = s[2 * g + x];
+                            mma16816<BF16>(c[0], c[1], c[2], c[3], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], kf[2 * x],
+                                           kf[2 * x + 1]);
+                        }
+                    }
+                float t[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = j0 + x * 8 + lc * 2 + (e & 1), p = pos[e >> 1];
+                        const bool sees = x * 8 + lc * 2 + (e & 1) < n && j <= p && p < len &&
+                                          (a.window == 0 || j > p - a.window || j < a.sinks);
+                        s[x][e] = sees ? s[x][e] * a.scale_log2 : -INFINITY;
+                        t[e >> 1] = fmaxf(t[e >> 1], s[x][e]);
+                    }
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    t[e] = fmaxf(t[e], __shfl_xor_sync(~0u, t[e], 1));
+                    t[e] = fmaxf(fmaxf(t[e], __shfl_xor_sync(~0u, t[e], 2)), m[e]);
+                    f[e] = ex2(m[e] - t[e]);
+                    m[e] = t[e];
+                    l[e] *= f[e];
+                }
+#pragma unroll
+                for (int x = 0; x < DP / 8; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[x][e] *= f[e >> 1];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    uint32_t pa[4];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float* c = s[2 * g + x];
+                        const float w0 = ex2(c[0] - m[0]), w1 = ex2(c[1] - m[0]), w2 = ex2(c[2] - m[1]), w3 = ex2(c[3] - m[1]);
+                        l[0] += w0 + w1;
+                        l[1] += w2 + w3;
+                        pa[2 * x] = pack16<BF16>(w0, w1);
+                        pa[2 * x + 1] = pack16<BF16>(w2, w3);
+                    }
+#pragma unroll
+                    for (int x = 0; x < DP / 16; ++x) {
+                        uint32_t vf[4];
+                        ldsm4t(vf, sv + (g * 16 + (mi & 1) * 8 + mr) * ROW + (((x * 2 + (mi >> 1)) ^ mr) << 4));
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            float* c = o[2 * x + y];
+                            mma16816<BF16>(c[0], c[1], c[2], c[3], pa[0], pa[1], pa[2], pa[3], vf[2 * y], vf[2 * y + 1]);
+                        }
+                    }
+                }
             }
         }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (lane + 32 * e < a.D) st16f<BF16>(a.out, w * a.D + lane + 32 * e, o[e] * inv);
+        for (int e = 0; e < 2; ++e) {
+            l[e] += __shfl_xor_sync(~0u, l[e], 1);
+            l[e] += __shfl_xor_sync(~0u, l[e], 2);
+            const float inv = l[e] > 0.f ? 1.f / l[e] : 0.f;
+            const int row = row0 + lr + 8 * e;
+            if (row >= a.S) continue;
+            uint16_t* out = static_cast<uint16_t*>(a.out) + (((int64_t)b * a.S + row) * a.nq + h) * a.D;
+#pragma unroll
+            for (int x = 0; x < DP / 8; ++x) {
+                const int col = x * 8 + lc * 2;
+                const uint32_t w = pack16<BF16>(o[x][2 * e] * inv, o[x][2 * e + 1] * inv);
+                if (col < a.D) out[col] = (uint16_t)w;
+                if (col + 1 < a.D) out[col + 1] = (uint16_t)(w >> 16);
+            }
+        }
     }
+}
+
+template <int DP, bool BF16>
+static int launch_window_mma(const WinArgs& a, int vec, cudaStream_t s) {
+    const int64_t items = (int64_t)a.batch * a.nq * (((int64_t)a.S + kWmRows - 1) / kWmRows);
+    const unsigned grid = (unsigned)(items < (1 << 30) ? items : 1 << 30);
+    B2_TRY(launch(window_mma_kernel<DP, BF16>, dim3(grid), dim3(kWmThreads), 2 * kWmKeys * DP * 2, s, true, a, vec));
+    return B2_OK;
 }
 
 // ---------------------------------------------------------------------------
@@ -132,23 +230,6 @@ struct WinCfg {
 // last one hands part of its share to the two whose threads hold a row of S.
 constexpr int kWinRegsFew = 104, kWinRegsMany = 200;
 static_assert(kWinRegsFew + 2 * kWinRegsMany <= 3 * 168, "more registers than the block is launched with");
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t win_pack(float a, float b) {
-    if constexpr (BF16) {
-        __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<uint32_t*>(&h);
-    } else {
-        return f2_to_h2(a, b);
-    }
-}
-
-// 2^x on the SFU: 2^-22 relative, far below the 16-bit rounding P gets next
-__device__ __forceinline__ float win_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // Bits below position n (none for n <= 0, all for n >= 32).
 __device__ __forceinline__ uint32_t below(int n) {
@@ -513,7 +594,7 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                 const float m_new = fmaxf(m, mx);
                 const bool resc = m_new > m + 8.f;
                 const float m_use = resc ? m_new : m;
-                const float alpha = win_ex2(m - m_use);
+                const float alpha = ex2(m - m_use);
                 if (j > from && __any_sync(0xffffffffu, resc)) {
                     // the P V before has completed (S, issued behind it, has)
 #pragma unroll 1
@@ -538,9 +619,9 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                             for (int e = 0; e < 32; e += 2) {
                                 const float2 x = one_each(
                                     fma2(two(__uint_as_float(v[32 * c + e]), __uint_as_float(v[32 * c + e + 1])), scale2, nm2));
-                                const float p0 = win_ex2(x.x), p1 = win_ex2(x.y);
+                                const float p0 = ex2(x.x), p1 = ex2(x.y);
                                 l2[(e >> 1) & 1] = add2(l2[(e >> 1) & 1], two(p0, p1));
-                                pk[e >> 1] = win_pack<BF16>(p0, p1);
+                                pk[e >> 1] = pack16<BF16>(p0, p1);
                             }
                             tc::tmem_st16(tS + (uint32_t)(16 * c), pk);
                         }
@@ -574,10 +655,10 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
 #pragma unroll
                     for (int q = 0; q < 8; ++q) {
                         uint4 x;
-                        x.x = win_pack<BF16>(__uint_as_float(o[8 * q + 0]) * inv_l, __uint_as_float(o[8 * q + 1]) * inv_l);
-                        x.y = win_pack<BF16>(__uint_as_float(o[8 * q + 2]) * inv_l, __uint_as_float(o[8 * q + 3]) * inv_l);
-                        x.z = win_pack<BF16>(__uint_as_float(o[8 * q + 4]) * inv_l, __uint_as_float(o[8 * q + 5]) * inv_l);
-                        x.w = win_pack<BF16>(__uint_as_float(o[8 * q + 6]) * inv_l, __uint_as_float(o[8 * q + 7]) * inv_l);
+                        x.x = pack16<BF16>(__uint_as_float(o[8 * q + 0]) * inv_l, __uint_as_float(o[8 * q + 1]) * inv_l);
+                        x.y = pack16<BF16>(__uint_as_float(o[8 * q + 2]) * inv_l, __uint_as_float(o[8 * q + 3]) * inv_l);
+                        x.z = pack16<BF16>(__uint_as_float(o[8 * q + 4]) * inv_l, __uint_as_float(o[8 * q + 5]) * inv_l);
+                        x.w = pack16<BF16>(__uint_as_float(o[8 * q + 6]) * inv_l, __uint_as_float(o[8 * q + 7]) * inv_l);
                         *reinterpret_cast<uint4*>(stage + lane * 128 + ((q ^ (lane & 7)) << 4)) = x;
                     }
                     tc::fence_proxy_async_smem();
@@ -694,10 +775,11 @@ extern "C" int b2_window_prefill_gqa(b2_kv_view q, b2_kv_view k, b2_kv_view v, v
         if (D <= 64) return bf16 ? launch_window_tc<64, true>(a, s) : launch_window_tc<64, false>(a, s);
         return bf16 ? launch_window_tc<128, true>(a, s) : launch_window_tc<128, false>(a, s);
     }
-    const int64_t warps = q_len * nq * batch;
-    int64_t blocks = (warps + 7) / 8;
-    if (blocks > (int64_t)sm_count() * 64) blocks = (int64_t)sm_count() * 64;
-    B2_TRY(launch(bf16 ? window_rows_kernel<true> : window_rows_kernel<false>, dim3((unsigned)blocks), dim3(256), 0,
-                  as_stream(stream), true, a));
-    return B2_OK;
+    // 16-byte loads where every row is aligned for them
+    auto rows16 = [](const b2_kv_view& x) { return aligned16(x.data) && !((x.stride_b | x.stride_h | x.stride_s) & 7); };
+    const int vec = rows16(k) && rows16(v);
+    cudaStream_t s = as_stream(stream);
+    if (D <= 64) return bf16 ? launch_window_mma<64, true>(a, vec, s) : launch_window_mma<64, false>(a, vec, s);
+    if (D <= 128) return bf16 ? launch_window_mma<128, true>(a, vec, s) : launch_window_mma<128, false>(a, vec, s);
+    return bf16 ? launch_window_mma<256, true>(a, vec, s) : launch_window_mma<256, false>(a, vec, s);
 }
