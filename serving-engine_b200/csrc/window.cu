@@ -54,7 +54,7 @@ struct WinArgs {
 // registers; the keys any of its rows sees come 32 at a time through shared
 // memory, first the sinks, then from the first row's window on.  Bound by
 // mma.sync and by the loads it does not overlap: 8192 tokens, window 2048, 32
-// heads of 128 take MMAMS ms this way (the tcgen05 form 0.27).
+// heads of 128 take 2.35 ms this way (the tcgen05 form 0.26).
 constexpr int kWmRows = 64, kWmKeys = 32, kWmThreads = 128;
 
 // 8 elements from p, of which n exist; vec: p is 16-byte aligned
@@ -318,8 +318,10 @@ struct WinItem {
     }
 };
 
-// The pairs of all sequences and kv heads, dealt round robin to the CTAs; a
-// sequence's later (longer) rows first.
+// The pairs of all sequences and kv heads, a sequence's later (longer) rows
+// first, dealt to the CTAs back and forth: without a window the first CTA of a
+// round would otherwise always get its longest pair (8192 tokens, 32 heads: 591
+// us dealt one way, 551 back and forth).
 struct WinList {
     int b = 0, len = 0, count = 0, np = 0;  // of the sequence: tiles and pairs per kv head
     int64_t before = 0;                     // items of sequences before b
@@ -426,7 +428,8 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                 WinItem it, ahead;
                 auto publish = [&](uint32_t k) -> bool {
                     if (k >= 2 && !tc::mbar_wait(&i_empty[k & 1], ((k >> 1) - 1) & 1u, err, 104)) return false;
-                    if (!list.get(a, blockIdx.x + (int64_t)k * gridDim.x, ahead)) ahead.n = 0;
+                    const uint32_t c = k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+                if (!list.get(a, (int64_t)k * gridDim.x + c, ahead)) ahead.n = 0;
                     s_item[k & 1] = ahead;
                     tc::mbar_arrive(&i_full[k & 1]);
                     return true;
