@@ -375,7 +375,9 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(i_empty + 2);
     __shared__ WinItem s_item[2];       // n 0: no more
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // a value that is the same in all lanes, told to the compiler
+    auto same = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };
+    const int warp = same(threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         tc::mbar_init(q_full, 1);
         tc::mbar_init(q_empty, 2);
@@ -400,7 +402,7 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = same(*tmem_slot);
 
     griddep_wait();
     griddep_launch_dependents();
@@ -462,60 +464,66 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                 }
             }
         } else if (warp <= 10) {
-            // ---------------- MMA issuers: one per tile, so that the tensor core always has the other's
-            // products queued while one waits or computes descriptors ----------------
-            if (lane == 0) {
-                constexpr uint32_t idO = tc::idesc_f16(128, D, BF16, true);
-                constexpr uint32_t idS = tc::idesc_f16(128, 0, BF16, false);
-                const int t = warp - 9;
-                const uint32_t tP = tmem + (uint32_t)t * 256, tO = tP + 128;
-                // a descriptor's address field counts 16 bytes: steps are added to it
-                const uint64_t dq = tc::desc_k_sw128(tc::smem_u32(sQ) + (uint32_t)t * TILE);
-                const uint64_t dk0 = tc::desc_k_sw128(tc::smem_u32(sK)), dv0 = tc::desc_mn_sw128(tc::smem_u32(sV), ATOM);
-                bool ok = true;
-                uint32_t np = 0;  // P tiles consumed
-                WinItem it;
-                auto wait_k = [&](uint32_t gj) { return tc::mbar_wait(&k_full[gj % ST], (gj / ST) & 1u, err, 94); };
-                auto wait_v = [&](uint32_t gj) { return tc::mbar_wait(&v_full[gj % ST], (gj / ST) & 1u, err, 95); };
-                // Turns: A's products of a step, then B's, and so on.  The other tile's products are in the
-                // queue while this thread waits for its own operands, and the two softmaxes stay half a step apart.
-                uint32_t turns = 0;
-                auto my_turn = [&]() {
-                    const bool mine = (t == 0 && turns == 0) || tc::mbar_wait(&turn[t], (turns - (t == 0)) & 1u, err, 102);
-                    ++turns;
-                    return mine;
-                };
-                for (uint32_t k = 0; ok && next_item(k, false, it, ok); ++k) {
-                    const int from = t == 0 ? 0 : it.dB, to = t == 0 ? it.nA : it.hasB ? it.n : 0;
-                    int w = 0;
-                    for (int j = -1; j < it.n; ++j) {
-                        const uint32_t gj = g + (uint32_t)j, s = gj % ST, s1 = (gj + 1) % ST;
-                        const bool pv = j >= from && j < to, qk = j + 1 >= from && j + 1 < to;
-                        const int steps = w >> 4;
-                        if (qk) w = it.width(a, t, j + 1);
-                        if (j + 1 < it.n) ok = (j >= 0 || tc::mbar_wait(q_full, k & 1u, err, 96)) && wait_k(gj + 1);
-                        if (j >= 0) ok = ok && wait_v(gj);
-                        if (pv) ok = ok && tc::mbar_wait(&p_lo[t], np & 1u, err, 97);
-                        ok = ok && my_turn();
-                        if (!ok) break;
-                        tc::fence_after_sync();
-                        if (pv) {
-                            const uint64_t dv = dv0 + s * (TILE >> 4);
+            // ---------------- MMA issuers: one warp per tile, so that the tensor core always has the other's
+            // products queued while one waits or computes descriptors.  The whole warp runs the control flow.
+            constexpr uint32_t idO = tc::idesc_f16(128, D, BF16, true);
+            constexpr uint32_t idS = tc::idesc_f16(128, 0, BF16, false);
+            const int t = warp - 9;
+            const uint32_t tP = tmem + (uint32_t)t * 256, tO = tP + 128;
+            // a descriptor's address field counts 16 bytes: steps are added to it
+            const uint64_t dq = tc::desc_k_sw128(tc::smem_u32(sQ) + (uint32_t)t * TILE);
+            const uint64_t dk0 = tc::desc_k_sw128(tc::smem_u32(sK)), dv0 = tc::desc_mn_sw128(tc::smem_u32(sV), ATOM);
+            bool ok = true;
+            uint32_t np = 0;  // P tiles consumed
+            auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+                return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, err, where)) != 0;
+            };
+            // Turns: A's products of a step, then B's, and so on.  The other tile's products are in the
+            // queue while this warp waits for its own operands, and the two softmaxes stay half a step apart.
+            uint32_t turns = 0;
+            auto my_turn = [&]() {
+                const bool mine = (t == 0 && turns == 0) || wait(&turn[t], (turns - (t == 0)) & 1u, 102);
+                ++turns;
+                return mine;
+            };
+            WinItem it;
+            for (uint32_t k = 0; ok && next_item(k, true, it, ok); ++k) {
+                const int from = same(t == 0 ? 0 : it.dB), to = same(t == 0 ? it.nA : it.hasB ? it.n : 0), n = same(it.n);
+                int w = 0;
+                for (int j = -1; j < n; ++j) {
+                    const uint32_t gj = g + (uint32_t)j, s = gj % ST, s1 = (gj + 1) % ST;
+                    const bool pv = j >= from && j < to, qk = j + 1 >= from && j + 1 < to;
+                    const int steps = w >> 4;
+                    if (qk) w = same(it.width(a, t, j + 1));
+                    if (j + 1 < n)
+                        ok = (j >= 0 || wait(q_full, k & 1u, 96)) && wait(&k_full[s1], ((gj + 1) / ST) & 1u, 94);
+                    if (j >= 0) ok = ok && wait(&v_full[s], (gj / ST) & 1u, 95);
+                    if (pv) ok = ok && wait(&p_lo[t], np & 1u, 97);
+                    ok = ok && my_turn();
+                    if (!ok) break;
+                    tc::fence_after_sync();
+                    if (pv) {
+                        const uint64_t dv = dv0 + s * (TILE >> 4);
+                        if (tc::elect_one()) {
                             tc::mma_f16_ts(tO, tP, dv, idO, j > from ? 1u : 0u);
 #pragma unroll
                             for (int kk = 1; kk < 4; ++kk)
                                 if (kk < steps) tc::mma_f16_ts(tO, tP + (uint32_t)kk * 8, dv + (uint32_t)kk * 128u, idO, 1u);
-                            if (!(ok = tc::mbar_wait(&p_hi[t], np & 1u, err, 101))) break;
-                            ++np;
-                            tc::fence_after_sync();
+                        }
+                        if (!(ok = wait(&p_hi[t], np & 1u, 101))) break;
+                        ++np;
+                        tc::fence_after_sync();
+                        if (tc::elect_one()) {
 #pragma unroll
                             for (int kk = 4; kk < 8; ++kk)
                                 if (kk < steps) tc::mma_f16_ts(tO, tP + (uint32_t)kk * 8, dv + (uint32_t)kk * 128u, idO, 1u);
                             if (j + 1 == to) tc::mma_commit(&o_done[t]);
                         }
-                        if (qk) {
-                            const uint64_t dk = dk0 + s1 * (TILE >> 4);
-                            const uint32_t id = idS | ((uint32_t)(w >> 3) << 17);
+                    }
+                    if (qk) {
+                        const uint64_t dk = dk0 + s1 * (TILE >> 4);
+                        const uint32_t id = idS | ((uint32_t)(w >> 3) << 17);
+                        if (tc::elect_one()) {
 #pragma unroll
                             for (int kk = 0; kk < D / 16; ++kk) {
                                 const uint32_t off = ((uint32_t)(kk >> 2) * ATOM + (uint32_t)(kk & 3) * 32) >> 4;
@@ -523,14 +531,17 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                             }
                             tc::mma_commit(&s_full[t]);
                         }
+                    }
+                    if (tc::elect_one()) {
                         tc::mbar_arrive(&turn[t ^ 1]);
                         // whatever this tile read of the step's K and V has been read once these arrive
                         if (j >= 0) tc::mma_commit(&v_empty[s]);
-                        if (j + 1 < it.n) tc::mma_commit(&k_empty[s1]);
-                        if (j + 2 == it.n) tc::mma_commit(q_empty);
+                        if (j + 1 < n) tc::mma_commit(&k_empty[s1]);
+                        if (j + 2 == n) tc::mma_commit(q_empty);
                     }
-                    g += it.n;
+                    __syncwarp();
                 }
+                g += (uint32_t)n;
             }
         }
     } else {
