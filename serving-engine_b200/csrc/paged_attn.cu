@@ -32,9 +32,17 @@
 // weights costs no accuracy next to the output's own rounding.
 //
 // Weights (scores): the logits go to the workspace as they are computed (G
-// floats beside 4 D bytes of row), and a second kernel turns them into
-// weights with the joined max and sum: G/(2 D) more traffic than the rows,
-// instead of reading K again.
+// floats beside the 4 D bytes of a position's rows, written and read once), and
+// a second kernel turns them into weights with the joined max and sum, instead
+// of reading K again.
+//
+// Measured (4 D bytes per visible position and kv head, and the scores' 8):
+// 32 sequences of up to 32768, 8 kv heads of 128: 545 us, 6.7 TB/s (the
+// measured copy is 6.47); window 1024 of 16384: 27 us, 4.9 TB/s; 8 of up to
+// 4096 with weights: 29 us, 3.7 TB/s; one of 131001 with weights: 121 us, 4.5
+// TB/s; 301 tokens of a small model: 7 us.  The short ones are bound by the
+// chain length -> tables -> rows -> merge -> join (8.5 k cycles before the
+// first product, 3 to 6 k after the last).
 #include <cmath>
 
 #include "mma.cuh"

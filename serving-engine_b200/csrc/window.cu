@@ -16,19 +16,25 @@
 // an order in which the tiles of A, and those of B, are each consecutive.
 //   S_t = Q_t K^T   M = 128 queries, N = keys of the tile, in TMEM
 //   O_t += P_t V    P_t, 16-bit, over S_t's columns in TMEM (A operand)
-// with one MMA issuer per tile, taking turns: PV_A, S_A', PV_B, S_B' per key
-// tile.  The turns keep the two softmaxes half a step apart (without them both
-// run, then both wait: 3.6 k cycles a step with, 4.6 k without), and an issuer
-// does its waiting and addressing while the other's products are queued (one
-// issuer for both tiles: 4.4 k).  Across pairs nothing drains: the next pair's
-// Q, K and V are requested as soon as their buffers are read.
+// with one MMA issuer warp per tile, taking turns: PV_A, S_A', PV_B, S_B' per
+// key tile.  The turns keep the two softmaxes half a step apart (without them
+// both run, then both wait: 83 us for a chunk of 512 after 5500 at 64 heads, 74
+// with), and an issuer does its waiting and addressing while the other's
+// products are queued.  Across pairs nothing drains: the next pair's Q, K and V
+// are requested as soon as their buffers are read.
 // Online softmax in the log2 domain, one query row per thread; the reference
 // max moves only when a row's max exceeds it by more than 8, so O is rescaled
 // rarely and P stays below 2^8.  P is handed over in two halves of 64 keys, so
 // that P V starts while the second half's exponentials run.  Masks only in
 // tiles that a row of the warp does not see whole.  P is rounded to 16 bits
 // for the product (its row sum is not): one more rounding the size of the
-// output's own.  Outputs leave through shared memory as whole 128-byte lines.
+// output's own.  Outputs leave by TMA from shared memory.
+//
+// A step of two tiles and 128 keys takes 3.1 k cycles at head dim 128: 2.0 k of
+// products, and the chain S, softmax (2.0 k), P V, S around them.  Measured:
+// 8192 tokens, window 2048, 32 heads of 128, bf16: 237 us, 1017 TFLOP/s of
+// visible pairs (62 % of the measured burst rate); in a long run the chip's
+// power bounds it (990 W, 1.7 GHz).  Without a window: 502 us, 1095 TFLOP/s.
 #include <cmath>
 #include <type_traits>
 
@@ -54,7 +60,7 @@ struct WinArgs {
 // registers; the keys any of its rows sees come 32 at a time through shared
 // memory, first the sinks, then from the first row's window on.  Bound by
 // mma.sync and by the loads it does not overlap: 8192 tokens, window 2048, 32
-// heads of 128 take 2.35 ms this way (the tcgen05 form 0.26).
+// heads of 128 take 2.35 ms this way (the tcgen05 form 0.24).
 constexpr int kWmRows = 64, kWmKeys = 32, kWmThreads = 128;
 
 // 8 elements from p, of which n exist; vec: p is 16-byte aligned
@@ -222,6 +228,10 @@ struct WinCfg {
     // above half an SM's shared memory: one CTA, with all 512 TMEM columns, per SM
     static constexpr size_t NEED = OFF_BAR + 512 + 1024;
     static constexpr size_t SMEM = NEED > 122880 ? NEED : 122880;
+    // Every SHARE-th pair of exponentials of a tile without masks goes to the FMA pipe: at head dim 64 the SFU (16 a
+    // cycle and SM) is what a tile takes longest over (8192 tokens, window 2048, 32 heads: 187 us, 198 without); at
+    // 128 the products are, and the chip's power, and it gains nothing (240 us, 237 without)
+    static constexpr int SHARE = D == 64 ? 4 : 0;
     // warps 0-7 softmax, 8 TMA, 9 and 10 MMA of tile A and of tile B, 11 idle (a warpgroup gives up registers as a whole)
     static constexpr int THREADS = 384;
 };
@@ -256,6 +266,24 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+
+// 2^x of two numbers on the FMA pipe: x = n + f with n the nearest integer
+// (found by adding 1.5 * 2^23, which leaves it in the low mantissa bits), 2^f
+// on [-1/2, 1/2] by a degree-4 polynomial (least squares of the relative error
+// at Chebyshev nodes: 2.7e-6, far below the 16-bit rounding P gets next), n
+// added to the exponent.  x is finite; below -126 it counts as -126.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+    const uint64_t y = two(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+    const uint64_t t = add2(y, two(12582912.f, 12582912.f));
+    const uint64_t f = fma2(add2(t, two(-12582912.f, -12582912.f)), two(-1.f, -1.f), y);
+    uint64_t r = fma2(two(0.00956051f, 0.00956051f), f, two(0.05591704f, 0.05591704f));
+    r = fma2(r, f, two(0.24024981f, 0.24024981f));
+    r = fma2(r, f, two(0.69312197f, 0.69312197f));
+    r = fma2(r, f, two(0.99999919f, 0.99999919f));
+    const float2 p = one_each(r), n = one_each(t);
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(n.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(n.y) << 23)));
 }
 
 // One pair of query tiles and the key tiles it visits.  The tiles of a kv head
@@ -321,7 +349,7 @@ struct WinItem {
 // The pairs of all sequences and kv heads, a sequence's later (longer) rows
 // first, dealt to the CTAs back and forth: without a window the first CTA of a
 // round would otherwise always get its longest pair (8192 tokens, 32 heads: 591
-// us dealt one way, 551 back and forth).
+// us dealt one way, 551 back and forth, before the issuers were made quicker).
 struct WinList {
     int b = 0, len = 0, count = 0, np = 0;  // of the sequence: tiles and pairs per kv head
     int64_t before = 0;                     // items of sequences before b
@@ -633,9 +661,12 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                             for (int e = 0; e < 32; e += 2) {
                                 const float2 x = one_each(
                                     fma2(two(__uint_as_float(v[32 * c + e]), __uint_as_float(v[32 * c + e + 1])), scale2, nm2));
-                                const float p0 = ex2(x.x), p1 = ex2(x.y);
-                                l2[(e >> 1) & 1] = add2(l2[(e >> 1) & 1], two(p0, p1));
-                                pk[e >> 1] = pack16<BF16>(p0, p1);
+                                float2 p;
+                                if (!decltype(masked)::value && C::SHARE && (e >> 1) % (C::SHARE ? C::SHARE : 1) == C::SHARE - 1)
+                                    p = ex2_fma(x);
+                                else p = make_float2(ex2(x.x), ex2(x.y));
+                                l2[(e >> 1) & 1] = add2(l2[(e >> 1) & 1], two(p.x, p.y));
+                                pk[e >> 1] = pack16<BF16>(p.x, p.y);
                             }
                             tc::tmem_st16(tS + (uint32_t)(16 * c), pk);
                         }
