@@ -27,6 +27,13 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
                  : "r"(a)
                  : "memory");
 }
+// The 8 x 8 matrix of 16-bit values that the warp holds, lane l row l / 4 and
+// columns 2 (l % 4) and the next, with rows and columns exchanged.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 template <bool BF16>
 __device__ __forceinline__ void mma16816(float& c0, float& c1, float& c2, float& c3, uint32_t a0, uint32_t a1,
                                          uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

@@ -24,12 +24,15 @@
 // its own ring of shared-memory stages (cp.async, no barrier between warps),
 // with its own running max and sum; the warps meet once per segment.  Rows
 // come through the block table 16 bytes per lane, rows that are not visible
-// are filled with zeros and never read.  Products on mma.sync m16n8k16 (heads
-// as M, fp32 accumulation): the 2 x 16 x D MACs per position are far below its
-// rate at this memory speed, and it takes any row addresses, where tensor-map
-// copies would need one map per layout and whole swizzle atoms per block.  P
-// is split into a 16-bit value and a 16-bit remainder, so that rounding the
-// weights costs no accuracy next to the output's own rounding.
+// are filled with zeros and never read.  Products on mma.sync m16n8k16, fp32
+// accumulation: far below its rate at this memory speed, and it takes any row
+// addresses, where tensor-map copies would need one map per layout and whole
+// swizzle atoms per block.  Positions, then head-dim elements, are the 16 rows
+// of a product and the heads its 8 columns (S = K Q^T, O = V^T P): heads as
+// rows would leave half of every product empty, at twice the products (and the
+// chip is at its power limit here: 566 us for 32 x 32768 in a long run, 528
+// this way).  P is split into a 16-bit value and a 16-bit remainder, so that
+// rounding the weights costs no accuracy next to the output's own rounding.
 //
 // Weights (scores): the logits go to the workspace as they are computed (G
 // floats beside the 4 D bytes of a position's rows, written and read once), and
@@ -37,9 +40,9 @@
 // of reading K again.
 //
 // Measured (4 D bytes per visible position and kv head, and the scores' 8):
-// 32 sequences of up to 32768, 8 kv heads of 128: 545 us, 6.7 TB/s (the
-// measured copy is 6.47); window 1024 of 16384: 27 us, 4.9 TB/s; 8 of up to
-// 4096 with weights: 29 us, 3.7 TB/s; one of 131001 with weights: 121 us, 4.5
+// 32 sequences of up to 32768, 8 kv heads of 128: 521 us, 7.0 TB/s (the
+// measured copy is 6.47); window 1024 of 16384: 26 us, 5.1 TB/s; 8 of up to
+// 4096 with weights: 28 us, 3.9 TB/s; one of 131001 with weights: 119 us, 4.6
 // TB/s; 301 tokens of a small model: 7 us.  The short ones are bound by the
 // chain length -> tables -> rows -> merge -> join (8.5 k cycles before the
 // first product, 3 to 6 k after the last).
@@ -403,28 +406,40 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
 #pragma unroll
     for (int s = 0; s < kPgStages - 1; ++s) issue(s);
 
-    // ---- consumer
-    uint32_t qa[DP / 16][GH ? 4 : 2];
-    float o[DP / 8][GH ? 4 : 2], m0, m1, l0, l1;
+    // ---- consumer.  Positions are the rows of S, head-dim elements those of O: lane (lr, lc) holds positions lr and
+    // lr + 8, then outputs lr and lr + 8, of heads 2 lc and 2 lc + 1 (and those + 8)
+    constexpr int NT = GH ? 2 : 1;  // 8 heads each
+    const int lr = lane >> 2, lc = lane & 3;
+    uint32_t qb[DP / 16][NT][2];
+    float o[DP / 16][NT][4], m[NT][2], l[NT][2];
     float* logits = nullptr;  // where this lane's of the segment go
     auto start = [&]() {  // a new segment (or the rest of one): its queries, nothing summed yet
         const int h0 = at.head0(a), nh = at.heads(a);
         const uint16_t* q = static_cast<const uint16_t*>(a.q) + at.b * a.ldq + (int64_t)h0 * a.D;
-        const int r = lane >> 2, k = (lane & 3) * 2;
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
 #pragma unroll
-            for (int e = 0; e < (GH ? 4 : 2); ++e) {
-                const int row = GH ? r + (e & 1) * 8 : r, col = kk * 16 + k + (GH ? e >> 1 : e) * 8;
-                qa[kk][e] = row < nh && col < a.D ? *reinterpret_cast<const uint32_t*>(q + (int64_t)row * a.D + col) : 0u;
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = n * 8 + lr, col = kk * 16 + e * 8 + lc * 2;
+                    qb[kk][n][e] =
+                        row < nh && col < a.D ? *reinterpret_cast<const uint32_t*>(q + (int64_t)row * a.D + col) : 0u;
+                }
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[x][n][e] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m[n][e] = -INFINITY;
+                l[n][e] = 0.f;
             }
-#pragma unroll
-        for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < (GH ? 4 : 2); ++e) o[n][e] = 0.f;
-        m0 = m1 = -INFINITY;
-        l0 = l1 = 0.f;
-        if (a.logits) logits = a.logits + ((int64_t)at.b * a.nq + h0 + (lane >> 2)) * a.cap + warp * TP + (lane & 3) * 2;
+        if (a.logits) logits = a.logits + ((int64_t)at.b * a.nq + h0 + lc * 2) * a.cap + warp * TP + lr;
     };
 
     start();
@@ -438,99 +453,87 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
         if (there) {
 #pragma unroll
             for (int t = 0; t < TP / 16; ++t) {
-                // S = Q K^T: 16 heads x 16 positions
-                float s[2][4] = {};
+                // S = K Q^T: 16 positions x 8 (or 16) heads, even and odd steps of the head dim in sums of their own
+                float s[NT][4] = {}, s2[NT][4] = {};
                 const uint32_t kb = st + t * 16 * C::ROW, vb = kb + TP * C::ROW;
                 const int mi = lane >> 3, mr = lane & 7;
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
                     uint32_t kf[4];
-                    ldsm4(kf, kb + ((mi >> 1) * 8 + mr) * C::ROW + (((kk * 2 + (mi & 1)) ^ mr) << 4));
+                    ldsm4(kf, kb + ((mi & 1) * 8 + mr) * C::ROW + (((kk * 2 + (mi >> 1)) ^ mr) << 4));
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        if constexpr (GH)
-                            mma16816<BF16>(s[n][0], s[n][1], s[n][2], s[n][3], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3],
-                                           kf[2 * n], kf[2 * n + 1]);
-                        else
-                            mma16816<BF16>(s[n][0], s[n][1], s[n][2], s[n][3], qa[kk][0], 0u, qa[kk][1], 0u, kf[2 * n],
-                                           kf[2 * n + 1]);
+                    for (int n = 0; n < NT; ++n) {
+                        float* c = kk & 1 ? s2[n] : s[n];
+                        mma16816<BF16>(c[0], c[1], c[2], c[3], kf[0], kf[1], kf[2], kf[3], qb[kk][n][0], qb[kk][n][1]);
                     }
                 }
-                const int col = (lane & 3) * 2;
                 const uint32_t tm = there >> (t * 16);
+                const bool see[2] = {((tm >> lr) & 1) != 0, ((tm >> (lr + 8)) & 1) != 0};
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[n][e] = (tm >> (n * 8 + col + (e & 1))) & 1 ? s[n][e] * a.scale_log2 : -INFINITY;
+                    for (int e = 0; e < 4; ++e) s[n][e] = see[e >> 1] ? (s[n][e] + s2[n][e]) * a.scale_log2 : -INFINITY;
                 if (a.logits) {
                     const int nh = at.heads(a);
                     float* lg = logits + at.u * U + t * 16;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        if ((lane >> 2) < nh) *reinterpret_cast<float2*>(lg + n * 8) = make_float2(s[n][0], s[n][1]);
-                        if (GH && (lane >> 2) + 8 < nh)
-                            *reinterpret_cast<float2*>(lg + 8 * (int64_t)a.cap + n * 8) = make_float2(s[n][2], s[n][3]);
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (n * 8 + lc * 2 + (e & 1) < nh) lg[(int64_t)(n * 8 + (e & 1)) * a.cap + (e >> 1) * 8] = s[n][e];
+                }
+                // running max of the heads; finite, so that exp2(-inf - m) is 0
+                float top[NT][2];
+                bool moved = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = fmaxf(s[n][e], s[n][2 + e]);
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+                        top[n][e] = fmaxf(fmaxf(m[n][e], x), -1e30f);
+                        moved |= top[n][e] > m[n][e];
                     }
-                }
-                // running max of the rows; finite, so that exp2(-inf - m) is 0
-                float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-                t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, 1));
-                t0 = fmaxf(t0, __shfl_xor_sync(~0u, t0, 2));
-                const float n0 = fmaxf(fmaxf(m0, t0), -1e30f);
-                float t1 = 0.f, n1 = 0.f;
-                bool moved = n0 > m0;
-                if constexpr (GH) {
-                    t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-                    t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, 1));
-                    t1 = fmaxf(t1, __shfl_xor_sync(~0u, t1, 2));
-                    n1 = fmaxf(fmaxf(m1, t1), -1e30f);
-                    moved |= n1 > m1;
-                }
                 if (__any_sync(~0u, moved)) {
-                    const float a0 = ex2(m0 - n0), a1 = GH ? ex2(m1 - n1) : 0.f;
-                    l0 *= a0;
-                    l1 *= a1;
 #pragma unroll
-                    for (int n = 0; n < DP / 8; ++n) {
-                        o[n][0] *= a0;
-                        o[n][1] *= a0;
-                        if constexpr (GH) {
-                            o[n][2] *= a1;
-                            o[n][3] *= a1;
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float f = ex2(m[n][e] - top[n][e]);
+                            m[n][e] = top[n][e];
+                            l[n][e] *= f;
+#pragma unroll
+                            for (int x = 0; x < DP / 16; ++x) {
+                                o[x][n][e] *= f;
+                                o[x][n][2 + e] *= f;
+                            }
                         }
-                    }
-                    m0 = n0;
-                    m1 = n1;
                 }
-                uint32_t ph[4] = {}, pl[4] = {};
+                // the weights as value + remainder, turned from (position, head) to (head, position) pairs
+                uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const float p0 = ex2(s[n][0] - m0), p1 = ex2(s[n][1] - m0);
-                    l0 += p0 + p1;
-                    split16<BF16>(p0, p1, ph[2 * n], pl[2 * n]);
-                    if constexpr (GH) {
-                        const float p2 = ex2(s[n][2] - m1), p3 = ex2(s[n][3] - m1);
-                        l1 += p2 + p3;
-                        split16<BF16>(p2, p3, ph[2 * n + 1], pl[2 * n + 1]);
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float p0 = ex2(s[n][2 * k] - m[n][0]), p1 = ex2(s[n][2 * k + 1] - m[n][1]);
+                        l[n][0] += p0;
+                        l[n][1] += p1;
+                        split16<BF16>(p0, p1, ph[n][k], pl[n][k]);
+                        ph[n][k] = transpose8x8(ph[n][k]);
+                        pl[n][k] = transpose8x8(pl[n][k]);
                     }
-                }
-                // O += P V, the weights as value + remainder
+                // O += V^T P
 #pragma unroll
-                for (int n = 0; n < DP / 16; ++n) {
+                for (int x = 0; x < DP / 16; ++x) {
                     uint32_t vf[4];
-                    ldsm4t(vf, vb + ((mi & 1) * 8 + mr) * C::ROW + (((n * 2 + (mi >> 1)) ^ mr) << 4));
+                    ldsm4t(vf, vb + ((mi >> 1) * 8 + mr) * C::ROW + (((x * 2 + (mi & 1)) ^ mr) << 4));
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float* d = o[2 * n + h];
-                        if constexpr (GH) {
-                            mma16816<BF16>(d[0], d[1], d[2], d[3], ph[0], ph[1], ph[2], ph[3], vf[2 * h], vf[2 * h + 1]);
-                            mma16816<BF16>(d[0], d[1], d[2], d[3], pl[0], pl[1], pl[2], pl[3], vf[2 * h], vf[2 * h + 1]);
-                        } else {
-                            float z2 = 0.f, z3 = 0.f;
-                            mma16816<BF16>(d[0], d[1], z2, z3, ph[0], 0u, ph[2], 0u, vf[2 * h], vf[2 * h + 1]);
-                            mma16816<BF16>(d[0], d[1], z2, z3, pl[0], 0u, pl[2], 0u, vf[2 * h], vf[2 * h + 1]);
-                        }
+                    for (int n = 0; n < NT; ++n) {
+                        float* c = o[x][n];
+                        mma16816<BF16>(c[0], c[1], c[2], c[3], vf[0], vf[1], vf[2], vf[3], ph[n][0], ph[n][1]);
+                        mma16816<BF16>(c[0], c[1], c[2], c[3], vf[0], vf[1], vf[2], vf[3], pl[n][0], pl[n][1]);
                     }
                 }
             }
@@ -540,49 +543,50 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
 
         const bool done = at.u == at.s.n - 1;
         if (done || r == r1 - 1) {
-            // ---- the warps meet: max and sum of each row, then the outputs, in warp order
-            l0 += __shfl_xor_sync(~0u, l0, 1);
-            l0 += __shfl_xor_sync(~0u, l0, 2);
-            l1 += __shfl_xor_sync(~0u, l1, 1);
-            l1 += __shfl_xor_sync(~0u, l1, 2);
-            if ((lane & 3) == 0) {
-                s_m[warp][lane >> 2] = m0;
-                s_l[warp][lane >> 2] = l0;
-                if (GH) {
-                    s_m[warp][(lane >> 2) + 8] = m1;
-                    s_l[warp][(lane >> 2) + 8] = l1;
+            // ---- the warps meet: max and sum of each head, then the outputs, in warp order
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    l[n][e] += __shfl_xor_sync(~0u, l[n][e], 4);
+                    l[n][e] += __shfl_xor_sync(~0u, l[n][e], 8);
+                    l[n][e] += __shfl_xor_sync(~0u, l[n][e], 16);
+                    if (lr == 0) {
+                        s_m[warp][n * 8 + lc * 2 + e] = m[n][e];
+                        s_l[warp][n * 8 + lc * 2 + e] = l[n][e];
+                    }
                 }
-            }
             __syncthreads();
-            float w[GH ? 2 : 1];
+            float w[NT][2];
 #pragma unroll
-            for (int e = 0; e < (GH ? 2 : 1); ++e) {
-                const int row = (lane >> 2) + 8 * e;
-                float M = -1e30f;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int v = 0; v < kPgWarps; ++v) M = fmaxf(M, s_m[v][row]);
-                w[e] = ex2(s_m[warp][row] - M);
-                if (warp == 0 && (lane & 3) == 0) {
-                    float Ls = 0.f;
+                for (int e = 0; e < 2; ++e) {
+                    const int row = n * 8 + lc * 2 + e;
+                    float M = -1e30f;
 #pragma unroll
-                    for (int v = 0; v < kPgWarps; ++v) Ls = fmaf(s_l[v][row], ex2(s_m[v][row] - M), Ls);
-                    s_ml[row] = make_float2(M, Ls);
+                    for (int v = 0; v < kPgWarps; ++v) M = fmaxf(M, s_m[v][row]);
+                    w[n][e] = ex2(s_m[warp][row] - M);
+                    if (warp == 0 && lr == 0) {
+                        float Ls = 0.f;
+#pragma unroll
+                        for (int v = 0; v < kPgWarps; ++v) Ls = fmaf(s_l[v][row], ex2(s_m[v][row] - M), Ls);
+                        s_ml[row] = make_float2(M, Ls);
+                    }
                 }
-            }
 #pragma unroll 1
             for (int turn = 0; turn < kPgWarps / C::NB; ++turn) {
                 if (warp / C::NB == turn) {
                     float* buf = s_o + (warp % C::NB) * G * C::LDO;
 #pragma unroll
-                    for (int n = 0; n < DP / 8; ++n)
+                    for (int x = 0; x < DP / 16; ++x)
 #pragma unroll
-                        for (int e = 0; e < (GH ? 2 : 1); ++e) {
-                            float2* d = reinterpret_cast<float2*>(buf + ((lane >> 2) + 8 * e) * C::LDO + n * 8 + (lane & 3) * 2);
-                            float2 v = turn ? *d : make_float2(0.f, 0.f);
-                            v.x = fmaf(o[n][2 * e], w[e], v.x);
-                            v.y = fmaf(o[n][2 * e + 1], w[e], v.y);
-                            *d = v;
-                        }
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float* d = buf + (n * 8 + lc * 2 + (e & 1)) * C::LDO + x * 16 + lr + (e >> 1) * 8;
+                                *d = fmaf(o[x][n][e], w[n][e & 1], turn ? *d : 0.f);
+                            }
                 }
                 __syncthreads();
             }
