@@ -208,7 +208,9 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
         total = __reduce_add_sync(~0u, s.n) * heads;
         upc = (total + grid - 1) / grid;
         int here = s.n * heads;
-        if (can_piece) {
+        if (can_piece && total <= grid) {
+            pieced = true;  // a CTA for every unit
+        } else if (can_piece) {
             int pick = -1;
 #pragma unroll
             for (int k = 7; k >= 0; --k)
