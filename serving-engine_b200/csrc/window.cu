@@ -436,13 +436,12 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
     griddep_launch_dependents();
 
     uint32_t g = 0;  // key tiles of the pairs before this one
-    // Pair k as the producer found it: into `it`, false after the last one.  lanes: the whole warp calls it.
-    auto next_item = [&](uint32_t k, bool lanes, WinItem& it, bool& ok) -> bool {
-        ok = tc::mbar_wait(&i_full[k & 1], (k >> 1) & 1u, err, 103);
-        if (lanes) ok = __all_sync(0xffffffffu, ok);
+    // Pair k as the producer found it: into `it`, false after the last one.  The whole warp calls it.
+    auto next_item = [&](uint32_t k, WinItem& it, bool& ok) -> bool {
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(&i_full[k & 1], (k >> 1) & 1u, err, 103));
         if (!ok) return false;
         it = s_item[k & 1];
-        if (lanes) __syncwarp();
+        __syncwarp();
         if (lane == 0) tc::mbar_arrive(&i_empty[k & 1]);
         return it.n > 0;
     };
@@ -459,7 +458,7 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                 auto publish = [&](uint32_t k) -> bool {
                     if (k >= 2 && !tc::mbar_wait(&i_empty[k & 1], ((k >> 1) - 1) & 1u, err, 104)) return false;
                     const uint32_t c = k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-                if (!list.get(a, (int64_t)k * gridDim.x + c, ahead)) ahead.n = 0;
+                    if (!list.get(a, (int64_t)k * gridDim.x + c, ahead)) ahead.n = 0;
                     s_item[k & 1] = ahead;
                     tc::mbar_arrive(&i_full[k & 1]);
                     return true;
@@ -515,7 +514,7 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                 return mine;
             };
             WinItem it;
-            for (uint32_t k = 0; ok && next_item(k, true, it, ok); ++k) {
+            for (uint32_t k = 0; ok && next_item(k, it, ok); ++k) {
                 const int from = same(t == 0 ? 0 : it.dB), to = same(t == 0 ? it.nA : it.hasB ? it.n : 0), n = same(it.n);
                 int w = 0;
                 for (int j = -1; j < n; ++j) {
@@ -582,7 +581,7 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
         bool ok = true;
         uint32_t cs = 0, co = 0;  // S tiles and outputs of this tile so far
         WinItem it;
-        for (uint32_t k = 0; ok && next_item(k, true, it, ok); ++k) {
+        for (uint32_t k = 0; ok && next_item(k, it, ok); ++k) {
             const int from = t == 0 ? 0 : it.dB, to = t == 0 ? it.nA : it.hasB ? it.n : 0;
             const int wp = it.p[t] + rq * 32;  // position of the warp's first row
             const int pos = wp + lane < it.len ? wp + lane : -1;
@@ -708,7 +707,8 @@ __global__ void __launch_bounds__(WinCfg<D>::THREADS, 1)
                     }
                     tc::fence_proxy_async_smem();
                     __syncwarp();
-                    if (ok && lane == 0 && c < a.D) tc::tma_store_4d(&tmO, stage, c, it.h[t], it.row[t] + rq * 32, it.b);
+                    const int row = it.row[t] + rq * 32;
+                    if (ok && lane == 0 && c < a.D && row < a.S) tc::tma_store_4d(&tmO, stage, c, it.h[t], row, it.b);
                 }
             }
             g += it.n;
