@@ -80,6 +80,21 @@ def test_prefill_masks(cuda, window, sinks):
     prefill_case(5, 1, 700, 0, 2, 1, 64, "fp16", window, sinks)
 
 
+@pytest.mark.parametrize("nq,nkv", [(32, 8), (28, 4), (36, 36), (33, 11), (40, 1)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (64, 200), (300, 4), (512, 130), (129, 129)])
+def test_prefill_more_tiles_than_sms(cuda, nq, nkv, window, sinks):
+    """Pairs of tiles: two heads at the same rows, or (odd groups) the next rows; several pairs per CTA."""
+    prefill_case(13, 1, 700, 0, nq, nkv, 128, "bf16", window, sinks)
+    prefill_case(14, 2, 401, 77, nq, nkv, 64, "fp16", window, sinks, lens=[478, 300])
+
+
+def test_prefill_many_ragged_sequences(cuda):
+    rng = np.random.default_rng(5)
+    lens = [int(x) for x in rng.integers(0, 260, 70)]
+    prefill_case(15, 70, 260, 0, 6, 2, 64, "bf16", 50, 3, lens=lens)
+    prefill_case(16, 70, 200, 60, 3, 1, 128, "fp16", 0, 0, lens=lens)
+
+
 @pytest.mark.parametrize("S,start", [(1, 0), (1, 500), (1, 511), (5, 123), (128, 128), (200, 333), (300, 1),
                                      (130, 1200)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (64, 4), (257, 130)])
@@ -341,6 +356,50 @@ def test_decode_in_a_graph_follows_lengths_and_tables(cuda):
         graph.replay()
         want, mag, _, _ = R.paged_decode(q, c.k, c.v, c.tables, lens, 0, 0)
         close(out, want, mag, "fp16")
+
+
+def test_all_three_in_one_graph(cuda):
+    """Prefill, decode and eviction captured together and replayed on new contents."""
+    c = Cache(42, [300, 200], 16, 2, 64, "bf16")
+    g = gen(43)
+    q, k, v = (randn(g, 1, 200, h, 64).bfloat16() for h in (4, 2, 2))
+    out, q1, o1 = torch.empty_like(q), randn(g, 2, 4, 64).bfloat16(), torch.empty(2, 4, 64, dtype=torch.bfloat16, device="cuda")
+    kept = torch.empty(2, 2, 64, dtype=torch.int32, device="cuda")
+    ws = b2.Workspace(b2.paged_decode_workspace_bytes(2, 4, 2, 64, c.tables.shape[1] * 16, True))
+
+    def calls():
+        b2.window_prefill_gqa(q, k, v, out, window=30, sinks=2)
+        b2.paged_decode_gqa(q1, c.kv, o1, scores=c.scores, ws=ws)
+        b2.paged_kv_evict(c.kv, c.scores, 64, kept, c.seq_lens, sinks=2, recent=10)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        calls()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls()
+    for seed in (1, 2):
+        d = Cache(44 + seed, [300, 200], 16, 2, 64, "bf16")
+        for t in (c.k, c.v, c.scores, c.seq_lens, c.tables):
+            src = d.k if t is c.k else d.v if t is c.v else d.scores if t is c.scores else d.seq_lens if t is c.seq_lens else d.tables
+            t.copy_(src)
+        q.copy_(randn(gen(seed), 1, 200, 4, 64))
+        graph.replay()
+        torch.cuda.synchronize()
+        close(out, *R.window_prefill(q, k, v, None, 30, 2), "bf16")
+        want, mag, score, add = R.paged_decode(q1, d.k, d.v, d.tables, [300, 200], 0, 0, d.scores)
+        close(o1, want, mag, "bf16")
+        assert c.seq_lens.tolist() == [64, 64]
+        # the choice goes by the scores the decode call left, which the reference gives to within their rounding
+        for b in range(2):
+            for h in range(2):
+                i = kept[b, h].long()
+                assert i[:2].tolist() == [0, 1] and i[-10:].tolist() == list(range([300, 200][b] - 10, [300, 200][b]))
+                at = lambda p: score[d.tables[b].long()[p // 16], h, p % 16]  # noqa: E731
+                mid = torch.arange(2, [300, 200][b] - 10, device="cuda")
+                out_of = mid[~torch.isin(mid, i)]
+                assert at(i[2:-10]).min() >= at(out_of).max() - 1e-4
 
 
 def test_decode_workspace_too_small(cuda):
