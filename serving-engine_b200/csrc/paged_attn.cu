@@ -37,12 +37,14 @@
 // Weights (scores): the logits go to the workspace as they are computed (G
 // floats beside the 4 D bytes of a position's rows, written and read once), and
 // a second kernel turns them into weights with the joined max and sum, instead
-// of reading K again.
+// of reading K again.  (An L2 policy that keeps the logits until then gains 4 us
+// of 117 for 131001 tokens, but they stay there after the call: a tensor of 96
+// MB that is read over and over next takes 31 us a time instead of 25.)
 //
 // Measured (4 D bytes per visible position and kv head, and the scores' 8):
 // 32 sequences of up to 32768, 8 kv heads of 128: 521 us, 7.0 TB/s (the
 // measured copy is 6.47); window 1024 of 16384: 26 us, 5.1 TB/s; 8 of up to
-// 4096 with weights: 28 us, 3.9 TB/s; one of 131001 with weights: 119 us, 4.6
+// 4096 with weights: 27 us, 4.0 TB/s; one of 131001 with weights: 117 us, 4.7
 // TB/s; 301 tokens of a small model: 7 us.  The short ones are bound by the
 // chain length -> tables -> rows -> merge -> join (8.5 k cycles before the
 // first product, 3 to 6 k after the last).
@@ -667,34 +669,25 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
 }
 
 // One thread per 4 stored logit columns: the weights their positions get from
-// the group's heads, in head order, onto their scores.
+// the group's heads, in head order, onto their scores.  Slots and scores are
+// read while the kernel before still runs (8 x 4096: 27.0 us with, 28.2
+// without; one sequence of 4000: 13.0 and 14.2), 4 heads at a time keep 8 CTAs
+// on an SM (131001 tokens: 116.4 us; 8 heads at a time and 5 CTAs: 117.3).
 template <int U>
-__global__ void __launch_bounds__(kPgScoreThreads) paged_scores_kernel(const PagedArgs a) {
-    griddep_wait();
-    griddep_launch_dependents();
+__global__ void __launch_bounds__(kPgScoreThreads, 8) paged_scores_kernel(const PagedArgs a) {
+    // Until the logits are there: what the kernel before only reads.  (It starts this one behind its own wait, so
+    // what came before it is complete.)
     const int kvh = blockIdx.y, b = blockIdx.z;
     Seen<U> s;
     s.of(a, b);
     const int i = (blockIdx.x * blockDim.x + threadIdx.x) * 4, u = i / U;
-    if (u >= s.n) return;
-    // the first 8 heads' logits are on their way while the positions' slots are looked up
-    const int h0 = b * a.nq + kvh * a.group;
-    const float* lg = a.logits + (int64_t)h0 * a.cap + i;
-    float4 x[8];
-    float2 st[8];
-#pragma unroll
-    for (int h = 0; h < 8; ++h)
-        if (h < a.group) {
-            x[h] = __ldcg(reinterpret_cast<const float4*>(lg + (int64_t)h * a.cap));
-            st[h] = a.stats[h0 + h];
-        }
     const int pos0 = s.base(u) + i - u * U, bs = a.kv.block_size;
     float* sc[4];
     float w[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         sc[e] = nullptr;
-        if (!s.sees(u, pos0 + e)) continue;
+        if (u >= s.n || !s.sees(u, pos0 + e)) continue;
         const int at = a.div.block(pos0 + e), blk = a.kv.block_tables[(int64_t)b * a.kv.max_blocks + at];
         if ((unsigned)blk < (unsigned)a.kv.num_blocks)
             sc[e] = a.scores + ((int64_t)blk * a.nkv + kvh) * bs + a.div.slot(pos0 + e, at);
@@ -703,6 +696,19 @@ __global__ void __launch_bounds__(kPgScoreThreads) paged_scores_kernel(const Pag
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (sc[e] && pos0 + e != s.L - 1) old[e] = *sc[e];
+    griddep_wait();
+    griddep_launch_dependents();
+    if (u >= s.n) return;
+    const int h0 = b * a.nq + kvh * a.group;
+    const float* lg = a.logits + (int64_t)h0 * a.cap + i;
+    float4 x[4];
+    float2 st[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+        if (h < a.group) {
+            x[h] = __ldcg(reinterpret_cast<const float4*>(lg + (int64_t)h * a.cap));
+            st[h] = a.stats[h0 + h];
+        }
     auto add = [&](float4 l, float2 ml) {
         const float inv = ml.y > 0.f ? 1.f / ml.y : 0.f;
         w[0] = fmaf(ex2(l.x - ml.x), inv, w[0]);
@@ -711,9 +717,10 @@ __global__ void __launch_bounds__(kPgScoreThreads) paged_scores_kernel(const Pag
         w[3] = fmaf(ex2(l.w - ml.x), inv, w[3]);
     };
 #pragma unroll
-    for (int h = 0; h < 8; ++h)
+    for (int h = 0; h < 4; ++h)
         if (h < a.group) add(x[h], st[h]);
-    for (int h = 8; h < a.group; ++h)
+#pragma unroll 4
+    for (int h = 4; h < a.group; ++h)
         add(__ldcg(reinterpret_cast<const float4*>(lg + (int64_t)h * a.cap)), a.stats[h0 + h]);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -737,8 +744,9 @@ static PagedSizes paged_sizes(int batch, int nq, int nkv, int D, int64_t max_pos
     z.hg = (group + 15) / 16;
     z.gs = (group + z.hg - 1) / z.hg;
     z.grid = sm_count() * (D > 128 ? 1 : 2);
-    // whole units of up to 128 positions over the sinks and over the window, whose first may begin 15 early
-    z.cap = (max_positions + 2 * 127 + 15 + 3) & ~int64_t(3);
+    // whole units of up to 128 positions over the sinks and over the window, whose first may begin 15 early; rows of
+    // whole 128-byte lines
+    z.cap = (max_positions + 2 * 127 + 15 + 31) & ~int64_t(31);
     z.parts = (size_t)2 * z.grid * z.gs * D * sizeof(float);
     z.pml = (size_t)2 * z.grid * z.gs * sizeof(float2);
     z.stats = scored ? ((size_t)batch * nq * sizeof(float2) + 15) & ~size_t(15) : 0;
