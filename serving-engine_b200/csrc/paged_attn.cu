@@ -187,9 +187,17 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
     const int c = blockIdx.x;
     const int heads = a.nkv * a.hg;
 
-    // chunks of a row past D are never copied: they stay zero
-    if (a.D < DP)
-        for (int i = tid; i < C::OFF_O / 16; i += kPgThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    // Chunks of a row past D are never copied, but the products read them: zeros, whatever an earlier kernel left
+    // there.  A warp clears those of its own ring, which no other warp touches and its copies never write.
+    if (a.D < DP) {
+        const int pads = C::CH - a.D / 8;
+        uint8_t* rows = smem + warp * kPgStages * C::STAGE;
+        for (int i = lane; i < kPgStages * 2 * TP * pads; i += 32) {
+            const int r = i / pads, ch = a.D / 8 + i - r * pads;
+            *reinterpret_cast<uint4*>(rows + r * C::ROW + ((ch ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+    }
     griddep_wait();
     griddep_launch_dependents();
 
