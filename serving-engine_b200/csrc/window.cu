@@ -795,7 +795,7 @@ extern "C" int b2_window_prefill_gqa(b2_kv_view q, b2_kv_view k, b2_kv_view v, v
     if (q_len <= 0 || batch <= 0) return B2_OK;
     B2_REQUIRE(q.data && k.data && v.data && out && q_start >= 0 && nq > 0 && nkv > 0 && nq % nkv == 0 && D > 0 &&
                window >= 0 && sinks >= 0);
-    if (D > 256 || q_len + q_start > (1 << 30) || q.stride_d != 1 || k.stride_d != 1 || v.stride_d != 1)
+    if (D > 256 || q_len > (1 << 30) || q_start > (1 << 30) - q_len || q.stride_d != 1 || k.stride_d != 1 || v.stride_d != 1)
         return B2_ERR_UNSUPPORTED;
     WinArgs a = {};
     a.q = q;

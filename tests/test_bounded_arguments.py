@@ -1,0 +1,13 @@
+"""Bounded-cache attention without a GPU: arguments at the edges of their types
+and tensors that no kernel may be given."""
+import pytest
+
+import b2engine as b2
+from test_bounded import prefill
+
+
+@pytest.mark.parametrize("S,start", [(4, 2 ** 63 - 2), (2 ** 63 - 1, 2 ** 63 - 1), (2 ** 62, 2 ** 62), (2 ** 30, 1),
+                                     (1, 2 ** 30)])
+def test_prefill_refuses_more_positions_than_it_counts(S, start):
+    assert prefill(S=S, start=start) == -2
+    assert prefill(S=S, start=start, D=160) == -2
