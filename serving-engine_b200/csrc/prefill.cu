@@ -831,9 +831,11 @@ extern "C" int b2_flash_prefill_gqa_ex(const void* q, const void* k, const void*
 extern "C" int b2_workspace_create(size_t bytes, b2_workspace** out) {
     B2_REQUIRE(out && bytes > 0);
     *out = nullptr;
+    // one allocation: the lent bytes, then the counters
+    constexpr size_t extra = 255 + kWsCounters * sizeof(int);
+    if (bytes > SIZE_MAX - extra) return (int)cudaErrorMemoryAllocation;
     b2_workspace* w = new (std::nothrow) b2_workspace();
     if (!w) return B2_ERR_INVALID;
-    // one allocation: the lent bytes, then the counters
     const size_t lent = (bytes + 255) & ~size_t(255);
     cudaError_t e = cudaMalloc(&w->ptr, lent + kWsCounters * sizeof(int));
     if (e == cudaSuccess) {

@@ -11,3 +11,11 @@ from test_bounded import prefill
 def test_prefill_refuses_more_positions_than_it_counts(S, start):
     assert prefill(S=S, start=start) == -2
     assert prefill(S=S, start=start, D=160) == -2
+
+
+@pytest.mark.parametrize("nbytes", [2 ** 64 - 1, 2 ** 64 - 256, 2 ** 64 - 16384])
+def test_workspace_refuses_sizes_that_wrap(nbytes):
+    """The lent bytes are rounded up and the counters' follow: cudaErrorMemoryAllocation, not a small workspace."""
+    with pytest.raises(b2.B2Error) as e:
+        b2.Workspace(nbytes)
+    assert e.value.status == 2
