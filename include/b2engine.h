@@ -170,9 +170,10 @@ int b2_flash_prefill_gqa_ex(const void* q, const void* k, const void* v, void* o
  * one, so that those never allocate (no counterpart in the reference, whose
  * only internal workspaces are the sampler's).  b2_workspace_create
  * allocates `bytes` of device memory on the current device (and a small
- * cleared area for arrival counters that every call leaves cleared); it
- * synchronises the legacy default stream.  The handle may be reused by any
- * number of calls on that device that do not overlap in time. */
+ * cleared area for arrival counters that every call leaves cleared); it waits
+ * for its own clearing, not for work queued on the caller's streams.  The
+ * handle may be reused by any number of calls on that device that do not
+ * overlap in time. */
 typedef struct b2_workspace b2_workspace;
 int b2_workspace_create(size_t bytes, b2_workspace** out);
 int b2_workspace_destroy(b2_workspace* ws);

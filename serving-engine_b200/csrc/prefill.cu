@@ -840,8 +840,14 @@ extern "C" int b2_workspace_create(size_t bytes, b2_workspace** out) {
     cudaError_t e = cudaMalloc(&w->ptr, lent + kWsCounters * sizeof(int));
     if (e == cudaSuccess) {
         w->counters = reinterpret_cast<int*>(static_cast<char*>(w->ptr) + lent);
-        e = cudaMemset(w->counters, 0, kWsCounters * sizeof(int));
-        if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
+        // cleared on a stream of its own: the caller's queued work is not waited for
+        cudaStream_t s;
+        e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+        if (e == cudaSuccess) {
+            e = cudaMemsetAsync(w->counters, 0, kWsCounters * sizeof(int), s);
+            if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+            cudaStreamDestroy(s);
+        }
     }
     if (e != cudaSuccess) {
         cudaFree(w->ptr);
