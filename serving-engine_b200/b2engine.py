@@ -215,13 +215,12 @@ def _torch():
     return _TORCH
 
 
-def _stream_of(stream) -> int | None:
-    """stream_ptr without building a torch.cuda.Stream object (3.3 us a call)."""
+def _stream_of(stream, dev) -> int | None:
+    """stream_ptr of device dev without building a torch.cuda.Stream object (3.3 us a call)."""
     if stream is not None:
         return stream
-    c = _torch()._C
     try:
-        return c._cuda_getCurrentRawStream(c._cuda_getDevice())
+        return _torch()._C._cuda_getCurrentRawStream(dev)
     except AttributeError:
         return stream_ptr()
 
@@ -262,6 +261,7 @@ class Workspace:
         h = vp()
         call("b2_workspace_create", max(1, int(nbytes)), C.byref(h))
         self.h = h
+        self.device = _torch().cuda.current_device()
 
     @property
     def nbytes(self) -> int:
@@ -291,10 +291,22 @@ def _is_bf16(t) -> int:
     raise ValueError(f"expected a float16 or bfloat16 tensor, got {t.dtype}")
 
 
-def _need(t, name, dtype, shape):
+def _device_of(t, name) -> int:
+    """Index of the GPU that t is on, which has to be the current one: the call launches there."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{name} must be on a GPU, got {t.device}")
+    if dev != _torch()._C._cuda_getDevice():
+        raise ValueError(f"{name} is on {t.device}, which is not the current device")
+    return dev
+
+
+def _need(t, name, dtype, shape, dev):
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape}, "
                          f"got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the other tensors are not")
 
 
 def _view(t) -> KVView:
@@ -314,13 +326,16 @@ def window_prefill_gqa(q, k, v, out, window=0, sinks=0, seq_lens=None, stream=No
     kb, T, nkv, kd = k.shape
     if k.shape != v.shape or kb != B or kd != D or T < S or k.dtype != dtype or v.dtype != dtype:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
-    _need(out, "out", dtype, shape)
+    dev = _device_of(q, "q")
+    if k.get_device() != dev or v.get_device() != dev:
+        raise ValueError(f"q, k and v are on {q.device}, {k.device} and {v.device}")
+    _need(out, "out", dtype, shape, dev)
     lens = None
     if seq_lens is not None:
-        _need(seq_lens, "seq_lens", _torch().int32, (B,))
+        _need(seq_lens, "seq_lens", _torch().int32, (B,), dev)
         lens = seq_lens.data_ptr()
     call("b2_window_prefill_gqa", _view(q), _view(k), _view(v), out.data_ptr(), lens, S, T - S, nq, nkv, D, B, window,
-         sinks, _is_bf16(q), _stream_of(stream))
+         sinks, _is_bf16(q), _stream_of(stream, dev))
     return out
 
 
@@ -339,8 +354,11 @@ class PagedKV:
         if block_tables.dim() != 2:
             raise ValueError("block_tables must be [batch, max_blocks]")
         B, mb = block_tables.shape
-        _need(block_tables, "block_tables", torch.int32, (B, mb))
-        _need(seq_lens, "seq_lens", torch.int32, (B,))
+        self.device = k.get_device()
+        if v.get_device() != self.device:
+            raise ValueError(f"k and v are on {k.device} and {v.device}")
+        _need(block_tables, "block_tables", torch.int32, (B, mb), self.device)
+        _need(seq_lens, "seq_lens", torch.int32, (B,), self.device)
         self.k, self.v, self.block_tables, self.seq_lens = k, v, block_tables, seq_lens
         self.batch, self.nkv, self.head_dim, self.dtype = B, k.shape[2], k.shape[3], k.dtype
         self.num_blocks, self.block_size = k.shape[0], k.shape[1]
@@ -365,13 +383,18 @@ def paged_decode_gqa(q, kv: PagedKV, out, window=0, sinks=0, scores=None, ws: Wo
     if B != kv.batch or D != kv.head_dim or q.dtype != kv.dtype or sd != 1 or sh != D:
         raise ValueError(f"q {q.dtype} {tuple(q.shape)} does not fit the cache ({kv.batch} sequences, "
                          f"head_dim {kv.head_dim}, {kv.dtype})")
-    _need(out, "out", kv.dtype, shape)
+    dev = _device_of(q, "q")
+    if kv.device != dev:
+        raise ValueError(f"q is on {q.device}, the cache on {kv.k.device}")
+    if ws is not None and ws.device != dev:
+        raise ValueError(f"q is on {q.device}, the workspace on cuda:{ws.device}")
+    _need(out, "out", kv.dtype, shape, dev)
     sc = None
     if scores is not None:
-        _need(scores, "scores", _torch().float32, kv.scores_shape)
+        _need(scores, "scores", _torch().float32, kv.scores_shape, dev)
         sc = scores.data_ptr()
     call("b2_paged_decode_gqa", q.data_ptr(), ldq, kv.ref, out.data_ptr(), sc, B, nq, kv.nkv, D, window, sinks,
-         ws.h if ws is not None else None, _stream_of(stream))
+         ws.h if ws is not None else None, _stream_of(stream, dev))
     return out
 
 
@@ -383,16 +406,17 @@ def paged_kv_evict(kv: PagedKV, scores, budget, kept, new_lens, sinks=0, recent=
     max_dst_blocks]).  kept int32 [B, nkv, budget] (-1 past a sequence's new
     length), new_lens int32 [B] (may be kv.seq_lens)."""
     torch = _torch()
-    _need(scores, "scores", torch.float32, kv.scores_shape)
-    _need(kept, "kept", torch.int32, (kv.batch, kv.nkv, budget))
-    _need(new_lens, "new_lens", torch.int32, (kv.batch,))
+    dev = _device_of(kv.k, "the cache")
+    _need(scores, "scores", torch.float32, kv.scores_shape, dev)
+    _need(kept, "kept", torch.int32, (kv.batch, kv.nkv, budget), dev)
+    _need(new_lens, "new_lens", torch.int32, (kv.batch,), dev)
     mdb, dst = 0, None
     if dst_tables is not None:
         mdb = dst_tables.shape[1]
-        _need(dst_tables, "dst_tables", torch.int32, (kv.batch, mdb))
+        _need(dst_tables, "dst_tables", torch.int32, (kv.batch, mdb), dev)
         dst = dst_tables.data_ptr()
     call("b2_paged_kv_evict", kv.ref, scores.data_ptr(), dst, mdb, kv.batch, kv.nkv, kv.head_dim, budget, sinks, recent,
-         kept.data_ptr(), new_lens.data_ptr(), _stream_of(stream))
+         kept.data_ptr(), new_lens.data_ptr(), _stream_of(stream, dev))
 
 
 class Sampler:
