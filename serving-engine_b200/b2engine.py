@@ -309,6 +309,15 @@ def _need(t, name, dtype, shape, dev):
         raise ValueError(f"{name} is on {t.device}, the other tensors are not")
 
 
+def _clamp(n, most) -> int:
+    """n as a C integer of at most `most`, past which a count of positions means the same; -1 for all below 0 (ctypes
+    would drop the upper bits)."""
+    return n if 0 <= n <= most else most if n > 0 else -1
+
+
+_MOST32, _MOST64 = 2 ** 31 - 1, 2 ** 63 - 1
+
+
 def _view(t) -> KVView:
     b, s, h, d = t.stride()
     return KVView(t.data_ptr(), b, h, s, d)
@@ -334,8 +343,8 @@ def window_prefill_gqa(q, k, v, out, window=0, sinks=0, seq_lens=None, stream=No
     if seq_lens is not None:
         _need(seq_lens, "seq_lens", _torch().int32, (B,), dev)
         lens = seq_lens.data_ptr()
-    call("b2_window_prefill_gqa", _view(q), _view(k), _view(v), out.data_ptr(), lens, S, T - S, nq, nkv, D, B, window,
-         sinks, _is_bf16(q), _stream_of(stream, dev))
+    call("b2_window_prefill_gqa", _view(q), _view(k), _view(v), out.data_ptr(), lens, S, T - S, nq, nkv, D, B,
+         _clamp(window, _MOST64), _clamp(sinks, _MOST64), _is_bf16(q), _stream_of(stream, dev))
     return out
 
 
@@ -393,8 +402,8 @@ def paged_decode_gqa(q, kv: PagedKV, out, window=0, sinks=0, scores=None, ws: Wo
     if scores is not None:
         _need(scores, "scores", _torch().float32, kv.scores_shape, dev)
         sc = scores.data_ptr()
-    call("b2_paged_decode_gqa", q.data_ptr(), ldq, kv.ref, out.data_ptr(), sc, B, nq, kv.nkv, D, window, sinks,
-         ws.h if ws is not None else None, _stream_of(stream, dev))
+    call("b2_paged_decode_gqa", q.data_ptr(), ldq, kv.ref, out.data_ptr(), sc, B, nq, kv.nkv, D,
+         _clamp(window, _MOST32), _clamp(sinks, _MOST32), ws.h if ws is not None else None, _stream_of(stream, dev))
     return out
 
 
@@ -415,8 +424,8 @@ def paged_kv_evict(kv: PagedKV, scores, budget, kept, new_lens, sinks=0, recent=
         mdb = dst_tables.shape[1]
         _need(dst_tables, "dst_tables", torch.int32, (kv.batch, mdb), dev)
         dst = dst_tables.data_ptr()
-    call("b2_paged_kv_evict", kv.ref, scores.data_ptr(), dst, mdb, kv.batch, kv.nkv, kv.head_dim, budget, sinks, recent,
-         kept.data_ptr(), new_lens.data_ptr(), _stream_of(stream, dev))
+    call("b2_paged_kv_evict", kv.ref, scores.data_ptr(), dst, mdb, kv.batch, kv.nkv, kv.head_dim, budget,
+         _clamp(sinks, _MOST32), _clamp(recent, _MOST32), kept.data_ptr(), new_lens.data_ptr(), _stream_of(stream, dev))
 
 
 class Sampler:
