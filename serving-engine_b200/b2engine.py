@@ -357,7 +357,10 @@ class PagedKV:
 
     def __init__(self, k, v, block_tables, seq_lens):
         torch = _torch()
-        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
+        # the stride of a dimension of one may be anything and is never used
+        strides = lambda t: [t.shape[3] if n == 1 else s for n, s in zip(t.shape[:3], t.stride())]  # noqa: E731
+        if k.dim() != 4 or k.shape != v.shape or strides(k) != strides(v) or k.dtype != v.dtype or \
+                k.stride(3) != 1 or v.stride(3) != 1:
             raise ValueError("k and v must be [num_blocks, block_size, nkv, D] of one type with the same strides and "
                              "contiguous rows")
         if block_tables.dim() != 2:
@@ -372,8 +375,8 @@ class PagedKV:
         self.batch, self.nkv, self.head_dim, self.dtype = B, k.shape[2], k.shape[3], k.dtype
         self.num_blocks, self.block_size = k.shape[0], k.shape[1]
         self.scores_shape = (self.num_blocks, self.nkv, self.block_size)
-        self.c = PagedKVStruct(k.data_ptr(), v.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), k.stride(0),
-                               k.stride(1), k.stride(2), k.shape[0], k.shape[1], mb, _is_bf16(k))
+        self.c = PagedKVStruct(k.data_ptr(), v.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(), *strides(k),
+                               k.shape[0], k.shape[1], mb, _is_bf16(k))
         self.ref = C.addressof(self.c)
 
 
@@ -389,7 +392,9 @@ def paged_decode_gqa(q, kv: PagedKV, out, window=0, sinks=0, scores=None, ws: Wo
     shape = q.shape
     B, nq, D = shape
     ldq, sh, sd = q.stride()
-    if B != kv.batch or D != kv.head_dim or q.dtype != kv.dtype or sd != 1 or sh != D:
+    if B == 1:
+        ldq = nq * D  # (whatever the view says: there is no next row)
+    if B != kv.batch or D != kv.head_dim or q.dtype != kv.dtype or sd != 1 or (sh != D and nq != 1):
         raise ValueError(f"q {q.dtype} {tuple(q.shape)} does not fit the cache ({kv.batch} sequences, "
                          f"head_dim {kv.head_dim}, {kv.dtype})")
     dev = _device_of(q, "q")
