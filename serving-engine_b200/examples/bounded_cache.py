@@ -27,6 +27,9 @@ class BoundedLayer:
 
     def __init__(self, batch, nq, nkv, head_dim, capacity, budget, sinks=4, recent=64, window=0, block_size=16,
                  dtype=torch.bfloat16):
+        if not 0 < budget < capacity or sinks < 0 or recent < 0 or sinks + recent > budget:
+            raise ValueError(f"a capacity of {capacity} needs a budget below it that holds the sinks and the recent "
+                             f"rows, got {budget}, {sinks} and {recent}")
         blocks = -(-capacity // block_size)
         self.capacity, self.budget, self.sinks, self.recent, self.window = capacity, budget, sinks, recent, window
         self.block_size, self.nq = block_size, nq
