@@ -278,7 +278,8 @@ int b2_append_kv_cache(const void* src_k, const void* src_v, void* dst_k, void* 
  * the tokens of each sequence counted from position 0, or NULL for q_start +
  * q_len everywhere; query rows at positions >= seq_lens[b] give zeros, and
  * K/V rows there may hold anything, NaN included.  K and V rows of positions
- * below seq_lens[b] must be finite.  fp16, or bf16 when bf16 != 0.
+ * below seq_lens[b] must be finite (a NaN in a K row leaves every output that
+ * sees the row NaN or infinite).  fp16, or bf16 when bf16 != 0.
  * head_dim up to 128 (a multiple of 8, 16-byte-aligned rows) runs on the
  * tcgen05 tensor cores; other head_dim up to 256 and other alignments on a
  * CUDA-core kernel.  Allocates nothing. */

@@ -272,9 +272,16 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // (found by adding 1.5 * 2^23, which leaves it in the low mantissa bits), 2^f
 // on [-1/2, 1/2] by a degree-4 polynomial (least squares of the relative error
 // at Chebyshev nodes: 2.7e-6, far below the 16-bit rounding P gets next), n
-// added to the exponent.  x is finite; below -126 it counts as -126.
+// added to the exponent.  Below -126 x counts as -126.  NaN (which fmaxf would
+// take for -126 too) gives the largest float: infinity as a 16-bit weight, so
+// that it shows in the output.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
-    const uint64_t y = two(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+    const uint64_t y = two(max_nan(x.x, -126.f), max_nan(x.y, -126.f));
     const uint64_t t = add2(y, two(12582912.f, 12582912.f));
     const uint64_t f = fma2(add2(t, two(-12582912.f, -12582912.f)), two(-1.f, -1.f), y);
     uint64_t r = fma2(two(0.00956051f, 0.00956051f), f, two(0.05591704f, 0.05591704f));
