@@ -281,8 +281,10 @@ int b2_append_kv_cache(const void* src_k, const void* src_v, void* dst_k, void* 
  * below seq_lens[b] must be finite (a NaN in a K row leaves every output that
  * sees the row NaN or infinite).  fp16, or bf16 when bf16 != 0.
  * head_dim up to 128 (a multiple of 8, 16-byte-aligned rows) runs on the
- * tcgen05 tensor cores; other head_dim up to 256 and other alignments on a
- * CUDA-core kernel.  Allocates nothing. */
+ * tcgen05 tensor cores; other head_dim up to 256, other alignments and
+ * broadcast views (a stride of 0) run on mma.sync, some ten times slower.  Both
+ * round the weights to the 16-bit type for the product with V.  q_start + q_len
+ * is at most 2^30.  Allocates nothing. */
 int b2_window_prefill_gqa(b2_kv_view q, b2_kv_view k, b2_kv_view v, void* out, const int* seq_lens, int64_t q_len,
                           int64_t q_start, int num_q_heads, int num_kv_heads, int head_dim, int batch,
                           int64_t window, int64_t sinks, int bf16, void* stream);
@@ -323,7 +325,11 @@ typedef struct b2_paged_kv {
  * blocks): the weight that the group's query heads together give to each
  * visible position is added to its score; the newest position's score starts
  * from nothing (its slot may hold anything).  Sequences of one call must not
- * share blocks then.  One writer per score: the same bits every run.
+ * share blocks then, and batch and num_kv_heads are at most 65535.  One writer
+ * per score: the same bits every run.
+ *
+ * The window counts rows held: after an eviction that is no longer the distance
+ * in tokens.
  *
  * The positions of all (sequence, kv head) pairs are cut into equal shares,
  * one per resident CTA; a pair cut between CTAs is joined from partial
@@ -354,8 +360,8 @@ size_t b2_paged_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_he
  * positions in order, -1 past n; new_lens (int32 [batch], may be
  * kv->seq_lens) receives n.  K rows keep the position encoding they were
  * written with.  Entries of either table outside [0, num_blocks) are neither
- * read nor written through.  In place, sequences must not share blocks.
- * Allocates nothing. */
+ * read nor written through.  In place, sequences must not share blocks.  batch
+ * and num_kv_heads are at most 65535.  Allocates nothing. */
 int b2_paged_kv_evict(const b2_paged_kv* kv, float* scores, const int* dst_tables, int max_dst_blocks, int batch,
                       int num_kv_heads, int head_dim, int budget, int sinks, int recent, int* kept, int* new_lens,
                       void* stream);

@@ -30,8 +30,8 @@
 // swizzle atoms per block.  Positions, then head-dim elements, are the 16 rows
 // of a product and the heads its 8 columns (S = K Q^T, O = V^T P): heads as
 // rows would leave half of every product empty, at twice the products (and the
-// chip is at its power limit here: 566 us for 32 x 32768 in a long run, 528
-// this way).  P is split into a 16-bit value and a 16-bit remainder, so that
+// chip is at its power limit here: 566 us for 32 x 32768 in a long run of graph
+// replays, 528 this way).  P is split into a 16-bit value and a 16-bit remainder, so that
 // rounding the weights costs no accuracy next to the output's own rounding.
 //
 // Weights (scores): the logits go to the workspace as they are computed (G
@@ -41,13 +41,15 @@
 // of 117 for 131001 tokens, but they stay there after the call: a tensor of 96
 // MB that is read over and over next takes 31 us a time instead of 25.)
 //
-// Measured (4 D bytes per visible position and kv head, and the scores' 8):
-// 32 sequences of up to 32768, 8 kv heads of 128: 521 us, 7.0 TB/s (the
-// measured copy is 6.47); window 1024 of 16384: 26 us, 5.1 TB/s; 8 of up to
-// 4096 with weights: 27 us, 4.0 TB/s; one of 131001 with weights: 117 us, 4.7
-// TB/s; 301 tokens of a small model: 7 us.  The short ones are bound by the
-// chain length -> tables -> rows -> merge -> join (8.5 k cycles before the
-// first product, 3 to 6 k after the last).
+// Measured (4 D bytes per visible position and kv head, and the scores' 8),
+// called in a row: 32 sequences of up to 32768, 8 kv heads of 128: 550 us, 6.7
+// TB/s (the measured copy is 6.47; 521 us in the shortest graph replay, 537 in
+// most); window 1024 of 16384: 27 us, 5.0 TB/s; 8 of up to 4096 with weights: 28
+// us, 3.9 TB/s; one of 131001 with weights: 119 us, 4.6 TB/s; 301 tokens of a
+// small model: 6.5 us.  The short ones are bound by the chain length -> tables
+// -> rows -> merge -> join (8.5 k cycles before the first product, 3 to 6 k
+// after the last).  A head_dim below 64, 128 or 256 costs what that costs (8 of
+// up to 4096: 26 us at 80 and 96, 25 at 128, 46 at 192, 45 at 256).
 #include <cmath>
 
 #include "mma.cuh"
@@ -87,7 +89,7 @@ struct PagedCfg {
     static constexpr int ROW = DP * 2;                // bytes of a row
     static constexpr int CH = DP / 8;                 // 16-byte chunks of a row
     static constexpr int STAGE = 2 * TP * ROW;        // K and V rows of a warp's tile
-    static constexpr int G = GH ? 16 : 8;             // rows kept of the 16 of an MMA
+    static constexpr int G = GH ? 16 : 8;             // heads of a segment, a row each in the warps' meeting
     static constexpr int NB = GH ? 1 : 2;             // buffers of the warps' meeting
     static constexpr int LDO = DP + 4;
     static constexpr int OFF_O = kPgWarps * kPgStages * STAGE;

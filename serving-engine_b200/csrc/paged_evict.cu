@@ -3,8 +3,10 @@
 //
 // Per (sequence, kv head): n = min(length, budget) positions stay -- the first
 // `sinks`, the last `recent`, and the best scores between them -- and move, in
-// order, to positions 0 .. n-1.  The bytes are the scores once, and the kept
-// rows read and written (8 D bytes each): HBM bounds it, the choice is latency.
+// order, to positions 0 .. n-1.  The bytes are the scores once (those past the
+// 45056 that a CTA keeps in shared memory five times, one table entry and one
+// score at a time), and the kept rows read and written (8 D bytes each): HBM
+// bounds it, the choice is latency.
 //
 // The choice is one CTA per (sequence, kv head): the positions' ordered keys
 // in shared memory, the n-th best found 11 bits at a time from a histogram,
@@ -15,7 +17,9 @@
 // costs more than the reading it saves.)  The move is a second launch spread
 // over the GPU, or, where few bytes stay, the choosing CTA's own.  Measured: 16
 // x 32768 to 8192 (8 heads of 128, half): 201 us, the move 177 of them at 5.9
-// TB/s (92 % of the measured copy); 8 x up to 4096 to 1024: 20 us.
+// TB/s (92 % of the measured copy); 8 x up to 4096 to 1024: 20 us.  Few long
+// sequences leave most SMs idle in the choice: 1 x 32768 to 8192 40 us, 1 x
+// 131072 230 (events around single calls, some 4 us above calls in a row).
 //
 // Moving in place is safe without a second copy because kept position j comes
 // from kept[j] >= j and kept rises: a CTA takes rows in order of j in batches,
@@ -23,7 +27,9 @@
 // at or above that batch's own start, where no earlier batch has written.  So
 // in place the CTAs of a (sequence, kv head) split the columns of the rows
 // (whole 32-byte sectors where a row has them), each taking all rows in order;
-// into other blocks they split the rows.
+// into other blocks they split the rows.  In place, timed singly: 16 x
+// 32768 to 8192 321 us, 8 x 4096 to 1024 30, 1 x 32768 to 8192 128 (8 CTAs per
+// sequence and head, each through all rows with a barrier per batch).
 #include "paged.cuh"
 
 namespace b2 {

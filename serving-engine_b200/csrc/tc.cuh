@@ -168,10 +168,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// One lane of a converged warp, the same one each time.  Code that issues
-// tcgen05.mma under it, with the rest of the warp beside it, lets the compiler
-// keep descriptors in the uniform registers the instruction takes: issued from
-// a single-lane branch each one costs some 90 cycles of moving them there.
+// One lane of a converged warp, the same one each time.  A tcgen05.mma issued
+// under it, with the rest of the warp beside it, takes 72 cycles by clock stamps
+// (M 128, N 128, K 16), one issued from a single-lane branch 92: presumably the
+// compiler then has to move descriptors into the uniform registers that the
+// instruction takes.
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}" : "=r"(p));

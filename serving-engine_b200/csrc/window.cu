@@ -18,8 +18,8 @@
 //   O_t += P_t V    P_t, 16-bit, over S_t's columns in TMEM (A operand)
 // with one MMA issuer warp per tile, taking turns: PV_A, S_A', PV_B, S_B' per
 // key tile.  The turns keep the two softmaxes half a step apart (without them
-// both run, then both wait: 83 us for a chunk of 512 after 5500 at 64 heads, 74
-// with), and an issuer does its waiting and addressing while the other's
+// both run, then both wait: 83 us for a chunk of 512 after 5500 at 64 heads when
+// it took 74 with them), and an issuer does its waiting and addressing while the other's
 // products are queued.  Across pairs nothing drains: the next pair's Q, K and V
 // are requested as soon as their buffers are read.
 // Online softmax in the log2 domain, one query row per thread; the reference
@@ -31,10 +31,14 @@
 // output's own.  Outputs leave by TMA from shared memory.
 //
 // A step of two tiles and 128 keys takes 3.1 k cycles at head dim 128: 2.0 k of
-// products, and the chain S, softmax (2.0 k), P V, S around them.  Measured:
-// 8192 tokens, window 2048, 32 heads of 128, bf16: 237 us, 1017 TFLOP/s of
-// visible pairs (62 % of the measured burst rate); in a long run the chip's
-// power bounds it (990 W, 1.7 GHz).  Without a window: 502 us, 1095 TFLOP/s.
+// products, and the chain S, softmax (2.0 k), P V, S around them, which is what
+// a step lasts: P lies over S, so that the next S waits for P V.  Measured, 8192
+// tokens, window 2048, 32 heads of 128, bf16: 260 us called in a row for long
+// (927 TFLOP/s of visible pairs; the chip at 990 W and 1.7 GHz), 235 to 243 in
+// graph replays, 224 in a short run at 1.97 GHz (1077 TFLOP/s, 66 % of the
+// measured burst rate).  Without a window: 502 us in graph replays, 1095
+// TFLOP/s.  Head dims between 64 and 128 cost what 128 costs (80 and 96: 218
+// us in a short run).
 #include <cmath>
 #include <type_traits>
 
@@ -60,7 +64,8 @@ struct WinArgs {
 // registers; the keys any of its rows sees come 32 at a time through shared
 // memory, first the sinks, then from the first row's window on.  Bound by
 // mma.sync and by the loads it does not overlap: 8192 tokens, window 2048, 32
-// heads of 128 take 2.35 ms this way (the tcgen05 form 0.24).
+// heads of 128 take 2.35 ms this way (the tcgen05 form 0.24), of 256 3.6 ms, of
+// 160, padded to 256, 5.0 ms.
 constexpr int kWmRows = 64, kWmKeys = 32, kWmThreads = 128;
 
 // 8 elements from p, of which n exist; vec: p is 16-byte aligned

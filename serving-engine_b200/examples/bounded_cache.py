@@ -8,7 +8,10 @@ that every row has an attention weight; from there on each new token is one
 paged decode call that also accumulates weights, and whenever a sequence
 reaches its capacity the cache is cut back to its budget: sinks, the most
 recent rows, and the rows with the most weight.  Rows keep the position
-encoding they were written with, so q and k come in already rotated."""
+encoding they were written with, so q and k come in already rotated.  A decode
+window counts the rows held: once something above `recent` has been evicted it
+reaches further back in tokens than its number says.  Rows are written by plain
+indexing, one sequence at a time; a server would append them in one kernel."""
 from __future__ import annotations
 
 import os
