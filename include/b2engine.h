@@ -366,6 +366,53 @@ int b2_paged_kv_evict(const b2_paged_kv* kv, float* scores, const int* dst_table
                       int num_kv_heads, int head_dim, int budget, int sinks, int recent, int* kept, int* new_lens,
                       void* stream);
 
+/* A paged K/V cache of one layer held in 4 bits: blocks of block_size (a
+ * multiple of 16) positions in one dense byte pool, stride_block bytes apart,
+ * with block tables and lengths as in b2_paged_kv.  A K or V row of one token
+ * and kv head is held in groups of 64 channels, each as m + u*s with 4-bit
+ * codes u, m = half(min), s = half((max - m) / 15) and u = (x - m) / s rounded
+ * to even and clamped to 0..15.  m and s are cut to half's finite range; a
+ * group that holds a NaN or an infinity comes back as NaN.  16 positions of a
+ * kv head are a tile of b2_kv4_tile_bytes(head_dim) bytes, K and V together; a
+ * block is [num_kv_heads][block_size/16][tile].  head_dim is a multiple of 8
+ * up to 256; rows are padded to 64, 96, 128, 192 or 256 channels (72 bytes per
+ * row of 128).  bf16 says what type the rows that go in and come out have. */
+typedef struct b2_paged_kv4 {
+    void* pool;
+    const int* block_tables;
+    const int* seq_lens;
+    int64_t stride_block;
+    int num_blocks;
+    int block_size;
+    int max_blocks;
+    int bf16; /* 0: half rows, else bf16 */
+} b2_paged_kv4;
+
+/* Bytes of a tile (16 positions of one kv head, K and V); 0 for a head_dim
+ * that the cache does not take. */
+size_t b2_kv4_tile_bytes(int head_dim);
+
+/* b2_paged_decode_gqa over a cache held in 4 bits: q and out have the type
+ * that kv->bf16 says.  No scores.  blocks != NULL: as in
+ * b2_paged_decode_gqa_blocks (window 0 then).  ws as there, of
+ * b2_paged_kv4_decode_workspace_bytes(...) bytes, or NULL.  Sums, softmax
+ * statistics and outputs in progress are 32-bit; codes enter the products
+ * exactly. */
+int b2_paged_kv4_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv4* kv, const int* blocks, int listed,
+                            void* out, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window,
+                            int sinks, b2_workspace* ws, void* stream);
+size_t b2_paged_kv4_decode_workspace_bytes(int num_q_heads, int num_kv_heads, int head_dim);
+
+/* b2_paged_decode_gqa in which each (sequence, kv head) sees the positions of
+ * the listed blocks of its sequence alone, below seq_lens[b]: blocks is device
+ * int32 [batch][num_kv_heads][listed], indexes into the sequence's row of the
+ * block tables.  Entries outside [0, max_blocks) or past the sequence's end
+ * add nothing (pad with -1); a block listed twice counts twice.  Same
+ * workspace. */
+int b2_paged_decode_gqa_blocks(const void* q, int64_t ldq, const b2_paged_kv* kv, const int* blocks, int listed,
+                               void* out, int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                               b2_workspace* ws, void* stream);
+
 /* ---------------------------------------------------------------------------
  * Sampler  (replaces engine::SamplerGPU, src/runtime/sampler.h:10-65)
  * ------------------------------------------------------------------------- */

@@ -37,6 +37,11 @@ class PagedKVStruct(C.Structure):
                 ("max_blocks", i32), ("bf16", i32)]
 
 
+class PagedKV4Struct(C.Structure):
+    _fields_ = [("pool", vp), ("block_tables", vp), ("seq_lens", vp), ("stride_block", i64), ("num_blocks", i32),
+                ("block_size", i32), ("max_blocks", i32), ("bf16", i32)]
+
+
 class TokenizerInfo(C.Structure):
     _fields_ = [("vocab_size", i64), ("n_ids", i64), ("n_merges", i64), ("pre_tokenizer", i32), ("nfc", i32),
                 ("ignore_merges", i32), ("chat_format", i32), ("bos_id", i32), ("eos_id", i32), ("n_stop", i32),
@@ -80,6 +85,10 @@ _SIGS = {
     "b2_window_prefill_gqa": (i32, [KVView, KVView, KVView, vp, vp, i64, i64, i32, i32, i32, i32, i64, i64, i32, vp]),
     "b2_paged_decode_gqa": (i32, [vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
     "b2_paged_decode_workspace_bytes": (C.c_size_t, [i32, i32, i32, i32, i64, i32]),
+    "b2_paged_decode_gqa_blocks": (i32, [vp, i64, vp, vp, i32, vp, i32, i32, i32, i32, vp, vp]),
+    "b2_kv4_tile_bytes": (C.c_size_t, [i32]),
+    "b2_paged_kv4_decode_gqa": (i32, [vp, i64, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
+    "b2_paged_kv4_decode_workspace_bytes": (C.c_size_t, [i32, i32, i32]),
     "b2_paged_kv_evict": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
     "b2_swiglu": (i32, [vp, vp, vp, i64, vp]),
     "b2_matmul_transB": (i32, [vp, vp, vp, i32, i32, i32, vp]),
@@ -380,15 +389,65 @@ class PagedKV:
         self.ref = C.addressof(self.c)
 
 
+def kv4_pool(num_blocks, block_size, nkv, head_dim):
+    """An empty pool of a cache held in 4 bits on the current GPU: uint8
+    [num_blocks, nkv, block_size / 16, tile]."""
+    tile = int(lib().b2_kv4_tile_bytes(head_dim))
+    if tile == 0 or block_size <= 0 or block_size % 16:
+        raise ValueError(f"a 4-bit cache takes a head_dim that is a multiple of 8 up to 256 and blocks of a multiple of "
+                         f"16 positions, got {head_dim} and {block_size}")
+    return _torch().zeros(num_blocks, nkv, block_size // 16, tile, dtype=_torch().uint8, device="cuda")
+
+
+class PagedKV4:
+    """One layer's paged K/V cache held in 4 bits (b2_paged_kv4): pool uint8
+    [num_blocks, nkv, block_size / 16, tile] as kv4_pool makes it (blocks may be
+    further apart), block_tables int32 [B, max_blocks] and seq_lens int32 [B];
+    dtype is that of the rows that go in and come out.  Holds references to the
+    tensors, copies nothing."""
+
+    def __init__(self, pool, block_tables, seq_lens, head_dim, dtype):
+        torch = _torch()
+        tile = int(lib().b2_kv4_tile_bytes(head_dim))
+        if tile == 0:
+            raise ValueError(f"head_dim must be a multiple of 8 up to 256, got {head_dim}")
+        if pool.dim() != 4 or pool.dtype != torch.uint8 or pool.shape[3] != tile or \
+                (pool.numel() and not pool[0].is_contiguous()):
+            raise ValueError(f"pool must be uint8 [num_blocks, nkv, block_size / 16, {tile}] with dense blocks, got "
+                             f"{pool.dtype} {tuple(pool.shape)}")
+        if block_tables.dim() != 2:
+            raise ValueError("block_tables must be [batch, max_blocks]")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"expected float16 or bfloat16 rows, got {dtype}")
+        B, mb = block_tables.shape
+        self.device = pool.get_device()
+        _need(block_tables, "block_tables", torch.int32, (B, mb), self.device)
+        _need(seq_lens, "seq_lens", torch.int32, (B,), self.device)
+        self.pool, self.block_tables, self.seq_lens = pool, block_tables, seq_lens
+        self.batch, self.nkv, self.head_dim, self.dtype = B, pool.shape[1], head_dim, dtype
+        self.num_blocks, self.block_size = pool.shape[0], 16 * pool.shape[2]
+        dense = pool.shape[1] * pool.shape[2] * tile
+        self.c = PagedKV4Struct(pool.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
+                                dense if pool.shape[0] == 1 else pool.stride(0), pool.shape[0], self.block_size, mb,
+                                int(dtype == torch.bfloat16))
+        self.ref = C.addressof(self.c)
+
+
 def paged_decode_workspace_bytes(batch, nq, nkv, head_dim, max_positions, scored=False) -> int:
-    return int(lib().b2_paged_decode_workspace_bytes(batch, nq, nkv, head_dim, max_positions, int(scored)))
+    """Enough for paged_decode_gqa over either kind of cache, with or without a list of blocks."""
+    return max(int(lib().b2_paged_decode_workspace_bytes(batch, nq, nkv, head_dim, max_positions, int(scored))),
+               int(lib().b2_paged_kv4_decode_workspace_bytes(nq, nkv, head_dim)))
 
 
-def paged_decode_gqa(q, kv: PagedKV, out, window=0, sinks=0, scores=None, ws: Workspace | None = None, stream=None):
-    """Attention of the newest token of each sequence over its paged rows.  q
-    [B, nq, D] (rows of heads contiguous), out [B, nq, D] contiguous; scores
-    (float32 [num_blocks, nkv, block_size], optional) accumulates every
-    visible position's weight and needs a workspace."""
+def paged_decode_gqa(q, kv, out, window=0, sinks=0, scores=None, ws: Workspace | None = None, stream=None,
+                     blocks=None):
+    """Attention of the newest token of each sequence over its paged rows, a
+    PagedKV's or a PagedKV4's.  q [B, nq, D] (rows of heads contiguous), out
+    [B, nq, D] contiguous; scores (float32 [num_blocks, nkv, block_size],
+    optional, PagedKV only) accumulates every visible position's weight and
+    needs a workspace.  blocks (int32 [B, nkv, n], optional, without window and
+    scores): the blocks of its sequence that each K/V head sees, as
+    paged_block_select gives them; -1 is none."""
     shape = q.shape
     B, nq, D = shape
     ldq, sh, sd = q.stride()
@@ -399,16 +458,33 @@ def paged_decode_gqa(q, kv: PagedKV, out, window=0, sinks=0, scores=None, ws: Wo
                          f"head_dim {kv.head_dim}, {kv.dtype})")
     dev = _device_of(q, "q")
     if kv.device != dev:
-        raise ValueError(f"q is on {q.device}, the cache on {kv.k.device}")
+        raise ValueError(f"q is on {q.device}, the cache on cuda:{kv.device}")
     if ws is not None and ws.device != dev:
         raise ValueError(f"q is on {q.device}, the workspace on cuda:{ws.device}")
     _need(out, "out", kv.dtype, shape, dev)
+    n, lst = 0, None
+    if blocks is not None:
+        if window or sinks or scores is not None:
+            raise ValueError("a list of blocks goes without window, sinks and scores")
+        n = blocks.shape[-1]
+        _need(blocks, "blocks", _torch().int32, (B, kv.nkv, n), dev)
+        lst = blocks.data_ptr()
+    wsh, st = ws.h if ws is not None else None, _stream_of(stream, dev)
+    if isinstance(kv, PagedKV4):
+        if scores is not None:
+            raise ValueError("a cache held in 4 bits keeps no scores")
+        call("b2_paged_kv4_decode_gqa", q.data_ptr(), ldq, kv.ref, lst, n, out.data_ptr(), B, nq, kv.nkv, D,
+             _clamp(window, _MOST32), _clamp(sinks, _MOST32), wsh, st)
+        return out
+    if blocks is not None:
+        call("b2_paged_decode_gqa_blocks", q.data_ptr(), ldq, kv.ref, lst, n, out.data_ptr(), B, nq, kv.nkv, D, wsh, st)
+        return out
     sc = None
     if scores is not None:
         _need(scores, "scores", _torch().float32, kv.scores_shape, dev)
         sc = scores.data_ptr()
     call("b2_paged_decode_gqa", q.data_ptr(), ldq, kv.ref, out.data_ptr(), sc, B, nq, kv.nkv, D,
-         _clamp(window, _MOST32), _clamp(sinks, _MOST32), ws.h if ws is not None else None, _stream_of(stream, dev))
+         _clamp(window, _MOST32), _clamp(sinks, _MOST32), wsh, st)
     return out
 
 

@@ -8,17 +8,7 @@
 // The work is one read of the visible K and V rows: 4 D bytes per (position,
 // kv head) for up to 4 D G flops (G heads of the group), so HBM bounds it.
 //
-// Split.  A (sequence, kv head, group of up to 16 heads) is a segment of
-// units of U positions.  Every CTA of a grid that is resident at once takes an
-// equal share of the units, in one of two ways.  Pieces: every segment is cut
-// into pieces of the same size, one per CTA, when a size within an eighth (or
-// two units) of the even share gives no more pieces than CTAs -- one segment
-// end per CTA.  Stream-K otherwise: all units end to end, cut evenly, whatever
-// the lengths -- up to three segment ends per CTA but no idle ones.
-// A CTA that covers a segment writes its outputs; a segment cut between
-// CTAs leaves a partial (max, sum, unnormalised output) per piece in the
-// workspace, and the CTA that arrives last at the segment's counter adds the
-// pieces in order (same bits whoever is last).
+// Split: paged_split.cuh, segments of up to 16 heads.
 //
 // Inside a CTA each of 4 warps streams its own quarter of every unit through
 // its own ring of shared-memory stages (cp.async, no barrier between warps),
@@ -52,31 +42,20 @@
 // up to 4096: 26 us at 80 and 96, 25 at 128, 46 at 192, 45 at 256).
 #include <cmath>
 
-#include "mma.cuh"
-#include "paged.cuh"
-#include "workspace.cuh"
+#include "paged_split.cuh"
 
 namespace b2 {
 
-constexpr int kPgWarps = 4;
-constexpr int kPgThreads = kPgWarps * 32;
 constexpr int kPgStages = 3;
 constexpr int kPgScoreThreads = 128;
 
-struct PagedArgs {
+struct PagedArgs : SplitArgs {
     const void* q;
     int64_t ldq;
     b2_paged_kv kv;
-    BlockDiv div;
-    void* out;
     float* scores;
-    int batch, nq, nkv, D, group, hg, gs, window, sinks;
     float scale_log2;
     int whole;      // blocks are whole groups of 16 positions
-    float* parts;   // [2 * grid][gs][D], unnormalised partial outputs
-    float2* pml;    // [2 * grid][gs], their (max, sum)
-    int* counters;  // [grid], null: segments are not cut
-    float2* stats;  // [batch][nq], the joined (max, sum); scores only
     float* logits;  // [batch][nq][cap]; scores only
     int cap;
 };
@@ -97,25 +76,6 @@ struct PagedCfg {
     static constexpr int CTAS = DP == 256 ? 1 : 2;    // per SM
 };
 
-// Rows are read once: they leave the L2 first, and what the call reads again
-// (logits, partial results, tables) stays (8 x 4096 with weights: 30.4 us, 32.2
-// without).
-__device__ __forceinline__ uint64_t read_once() {
-    uint64_t policy;
-    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-    return policy;
-}
-// 16 bytes, or 16 zero bytes without reading src
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there, uint64_t policy) {
-    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src),
-                 "r"(there ? 16 : 0), "l"(policy)
-                 : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 // (a, b) as 16-bit values and what the rounding left, again in 16 bits
 template <bool BF16>
 __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
@@ -129,65 +89,17 @@ __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t
     }
     lo = pack16<BF16>(a - f.x, b - f.y);
 }
-template <bool BF16>
-__device__ __forceinline__ void store4(void* p, int64_t i, float4 v, float scale) {
-    const uint2 x = make_uint2(pack16<BF16>(v.x * scale, v.y * scale), pack16<BF16>(v.z * scale, v.w * scale));
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = x;
-}
-
-// What the newest token of a sequence of L tokens sees, in units of U
-// positions: ns units over the first s0 positions, then units from w0 (lo
-// rounded down to 16) on, of which positions lo .. L-1 count.  A sequence
-// that sees nothing still has one unit, which writes its zeros.
-template <int U>
-struct Seen {
-    int L, lo, s0, ns, w0, n;
-    __device__ __forceinline__ void of(const PagedArgs& a, int b) {
-        L = paged_len(a.kv, b);
-        lo = a.window > 0 ? max(0, L - a.window) : 0;
-        s0 = min(a.sinks, lo);
-        ns = (s0 + U - 1) / U;
-        w0 = lo & ~15;
-        n = max(1, ns + (L - w0 + U - 1) / U);
-    }
-    __device__ __forceinline__ int base(int u) const { return u < ns ? u * U : w0 + (u - ns) * U; }
-    __device__ __forceinline__ bool sees(int u, int pos) const { return u < ns ? pos < s0 : pos >= lo && pos < L; }
-};
-
-// A place in the list of all units: head group g of kv head kvh of sequence b,
-// unit u of that segment.
-template <int U>
-struct Place {
-    int b, kvh, g, u;
-    Seen<U> s;
-    __device__ __forceinline__ void next(const PagedArgs& a) {
-        if (++u < s.n) return;
-        u = 0;
-        if (++g < a.hg) return;
-        g = 0;
-        if (++kvh < a.nkv) return;
-        kvh = 0;
-        if (++b < a.batch) s.of(a, b);
-    }
-    // First query head of the segment, and how many it has.
-    __device__ __forceinline__ int head0(const PagedArgs& a) const { return kvh * a.group + g * a.gs; }
-    __device__ __forceinline__ int heads(const PagedArgs& a) const { return min(a.gs, a.group - g * a.gs); }
-};
-
-template <int DP, bool GH, bool BF16>
+template <int DP, bool GH, bool BF16, bool LIST>
 __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn_kernel(const PagedArgs a) {
     using C = PagedCfg<DP, GH>;
     constexpr int U = C::U, TP = C::TP, G = C::G;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int s_scan[kPgWarps], s_count[kPgWarps][8];
-    __shared__ int s_b, s_before, s_last;
+    __shared__ SplitShared s_split;
     __shared__ uint32_t s_there[kPgWarps][kPgStages];
     __shared__ float s_m[kPgWarps][16], s_l[kPgWarps][16];
     __shared__ float2 s_ml[16];
     float* s_o = reinterpret_cast<float*>(smem + C::OFF_O);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int c = blockIdx.x;
-    const int heads = a.nkv * a.hg;
 
     // Chunks of a row past D are never copied, but the products read them: zeros, whatever an earlier kernel left
     // there.  A warp clears those of its own ring, which no other warp touches and its copies never write.
@@ -204,163 +116,32 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
     griddep_launch_dependents();
 
     // ---- this CTA's range of units, and the place where it starts
-    const int grid = (int)gridDim.x;
-    int total, upc, first;   // units of all segments (or pieces); units per CTA; what this CTA starts with
-    bool pieced = false;     // equal pieces: first counts pieces, else units
-    int fb, fbefore;         // the sequence it lies in, what lies before that
-    const bool can_piece = a.counters && (int64_t)a.batch * heads <= grid;
-    // the k-th candidate for the size of equal pieces; those up to an eighth or two units above the even share are taken
-    auto size_of = [&](int k) { return upc + k * ((upc + 63) / 64); };
-    auto near = [&](int k) { return k * ((upc + 63) / 64) <= max(2, upc / 8); };
-    if (a.batch <= 32) {
-        // every warp by itself, lane b for sequence b
-        Seen<U> s;
-        s.n = 0;
-        if (lane < a.batch) s.of(a, lane);
-        total = __reduce_add_sync(~0u, s.n) * heads;
-        upc = (total + grid - 1) / grid;
-        int here = s.n * heads;
-        if (can_piece && total <= grid) {
-            pieced = true;  // a CTA for every unit
-        } else if (can_piece) {
-            int pick = -1;
-#pragma unroll
-            for (int k = 7; k >= 0; --k)
-                if (near(k) && (int)__reduce_add_sync(~0u, (unsigned)(s.n + size_of(k) - 1) / (unsigned)size_of(k)) * heads <= grid)
-                    pick = k;
-            if (pick >= 0) {
-                pieced = true;
-                upc = size_of(pick);
-                here = (int)((unsigned)(s.n + upc - 1) / (unsigned)upc) * heads;
-            }
-        }
-        int incl = here;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(~0u, incl, o);
-            if (lane >= o) incl += v;
-        }
-        total = __shfl_sync(~0u, incl, 31);
-        first = pieced ? c : c * upc;
-        if (first >= total) return;
-        fb = __ffs(__ballot_sync(~0u, incl > first)) - 1;
-        fbefore = __shfl_sync(~0u, incl - here, fb);
-    } else {
-        const int per = (a.batch + kPgThreads - 1) / kPgThreads;
-        const int b0 = min(a.batch, tid * per), b1 = min(a.batch, b0 + per);
-        // Sum of count(units) over the sequences before this thread's own and with them, and over all.
-        auto scan = [&](auto count) -> int2 {
-            int mine = 0;
-            for (int b = b0; b < b1; ++b) {
-                Seen<U> s;
-                s.of(a, b);
-                mine += count(s.n);
-            }
-            int incl = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(~0u, incl, o);
-                if (lane >= o) incl += v;
-            }
-            __syncthreads();
-            if (lane == 31) s_scan[warp] = incl;
-            __syncthreads();
-            total = 0;
-#pragma unroll
-            for (int w = 0; w < kPgWarps; ++w) {
-                if (w < warp) incl += s_scan[w];
-                total += s_scan[w];
-            }
-            return make_int2(incl - mine, incl);
-        };
-        int2 span = scan([&](int n) { return n * heads; });
-        upc = (total + grid - 1) / grid;
-        if (can_piece) {
-            const int size = size_of(tid & 7);
-            int n = 0, pick = -1;
-            for (int b = tid >> 3; b < a.batch; b += kPgThreads / 8) {
-                Seen<U> s;
-                s.of(a, b);
-                n += (s.n + size - 1) / size * heads;
-            }
-            n += __shfl_xor_sync(~0u, n, 8);
-            n += __shfl_xor_sync(~0u, n, 16);
-            if (lane < 8) s_count[warp][lane] = n;
-            __syncthreads();
-            for (int k = 7; k >= 0; --k) {
-                int all = 0;
-#pragma unroll
-                for (int w = 0; w < kPgWarps; ++w) all += s_count[w][k];
-                if (all <= grid && near(k)) pick = k;
-            }
-            if (pick >= 0) {
-                pieced = true;
-                upc = size_of(pick);
-                span = scan([&](int n) { return (n + upc - 1) / upc * heads; });
-            }
-        }
-        first = pieced ? c : c * upc;
-        if (first >= total) return;
-        if (first >= span.x && first < span.y) {  // one thread
-            int b = b0, before = span.x;
-            for (;; ++b) {
-                Seen<U> s;
-                s.of(a, b);
-                const int here = (pieced ? (s.n + upc - 1) / upc : s.n) * heads;
-                if (first < before + here) break;
-                before += here;
-            }
-            s_b = b;
-            s_before = before;
-        }
-        __syncthreads();
-        fb = s_b;
-        fbefore = s_before;
-    }
-    Place<U> at;
-    at.b = fb;
-    at.s.of(a, at.b);
-    int r0, r1;         // units, counted from the first one of the segment or of all
-    int cf, pieces;     // first CTA of the segment and how many share it (pieces only)
-    {
-        pieces = pieced ? (at.s.n + upc - 1) / upc : at.s.n;
-        const int hh = (first - fbefore) / pieces, rest = first - fbefore - hh * pieces;
-        cf = c - rest;
-        at.u = pieced ? rest * upc : rest;
-        at.kvh = hh / a.hg;
-        at.g = hh - at.kvh * a.hg;
-        r0 = pieced ? at.u : first;
-        r1 = min(pieced ? at.s.n : total, r0 + upc);
-    }
-    if (!a.counters) {  // whole segments only: those that begin in the range
-        if (at.u > 0) {
-            r0 += at.s.n - at.u;
-            at.u = at.s.n - 1;
-            at.next(a);
-        }
-        if (r0 >= r1) return;
-        // the end moves to the end of the segment that holds unit r1 - 1
-        Place<U> e = at;
-        int r = r0;
-        while (r < r1) {
-            r += e.s.n;
-            e.u = e.s.n - 1;
-            e.next(a);
-        }
-        r1 = r;
-    }
+    Share w;
+    Place<U, LIST> at;
+    if (!split_units(a, s_split, w, at)) return;
+    const int r0 = w.r0, r1 = w.r1;
 
     // ---- producer: rows of the next unit into a stage.  The table entries of the two next units are on their way:
     // lane l's is that of row l % TP of the unit (-1: not visible), with the rest of the row's offset
-    Place<U> pp = at;
+    Place<U, LIST> pp = at;
     int pr = r0, pf = r0, pid[2];  // units requested, units looked up
     int64_t add[2];
     auto lookup = [&](int k) {
         pid[k] = -1;
         if (pf < r1) {
-            const int pos = pp.s.base(pp.u) + warp * TP + (lane & (TP - 1)), blk = a.div.block(pos);
-            if (pp.s.sees(pp.u, pos)) pid[k] = a.kv.block_tables[(int64_t)pp.b * a.kv.max_blocks + blk];
-            add[k] = (int64_t)a.div.slot(pos, blk) * a.kv.stride_slot + (int64_t)pp.kvh * a.kv.stride_head;
+            const int pos = pp.s.base(pp.u) + warp * TP + (lane & (TP - 1));
+            int blk = a.div.block(pos);
+            const int slot = a.div.slot(pos, blk);
+            bool sees = pp.s.sees(pp.u, pos);
+            if constexpr (LIST) {  // blk counts entries of the list
+                sees = false;
+                if (blk < a.listed) {
+                    blk = a.blocks[((int64_t)pp.b * a.nkv + pp.kvh) * a.listed + blk];
+                    sees = (unsigned)blk < (unsigned)a.max_blocks && slot < pp.s.L - blk * a.block_size;
+                }
+            }
+            if (sees) pid[k] = a.block_tables[(int64_t)pp.b * a.max_blocks + blk];
+            add[k] = (int64_t)slot * a.kv.stride_slot + (int64_t)pp.kvh * a.kv.stride_head;
             ++pf;
             pp.next(a);
         }
@@ -370,7 +151,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
     const int chunk = lane % C::CH;
     auto issue = [&](int stage) {
         if (pr < r1) {
-            const bool there = (unsigned)pid[0] < (unsigned)a.kv.num_blocks;
+            const bool there = (unsigned)pid[0] < (unsigned)a.num_blocks;
             const int64_t off = (int64_t)pid[0] * a.kv.stride_block + add[0];
             const uint32_t mask = __ballot_sync(~0u, there);
             if (lane == 0) s_there[warp][stage] = mask;
@@ -571,7 +352,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
                     }
                 }
             __syncthreads();
-            float w[NT][2];
+            float wt[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -580,7 +361,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
                     float M = -1e30f;
 #pragma unroll
                     for (int v = 0; v < kPgWarps; ++v) M = fmaxf(M, s_m[v][row]);
-                    w[n][e] = ex2(s_m[warp][row] - M);
+                    wt[n][e] = ex2(s_m[warp][row] - M);
                     if (warp == 0 && lr == 0) {
                         float Ls = 0.f;
 #pragma unroll
@@ -599,12 +380,11 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 float* d = buf + (n * 8 + lc * 2 + (e & 1)) * C::LDO + x * 16 + lr + (e >> 1) * 8;
-                                *d = fmaf(o[x][n][e], w[n][e & 1], turn ? *d : 0.f);
+                                *d = fmaf(o[x][n][e], wt[n][e & 1], turn ? *d : 0.f);
                             }
                 }
                 __syncthreads();
             }
-            const int h0 = at.head0(a), nh = at.heads(a);
             auto sum = [&](int row, int d) -> float4 {
                 float4 v = *reinterpret_cast<const float4*>(s_o + row * C::LDO + d);
                 if (C::NB == 2) {
@@ -613,61 +393,8 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
                 }
                 return v;
             };
-            const int64_t oat = ((int64_t)at.b * a.nq + h0) * a.D;
-            const int seg0 = r - at.u;  // first unit of the segment
-            const int quads = a.D / 4;
-            if (done && piece0 == seg0) {
-                for (int i = tid; i < nh * quads; i += kPgThreads) {
-                    const int row = i / quads, d = (i - row * quads) * 4;
-                    const float Ls = s_ml[row].y;
-                    store4<BF16>(a.out, oat + row * a.D + d, sum(row, d), Ls > 0.f ? 1.f / Ls : 0.f);
-                }
-                if (a.stats && tid < nh) a.stats[(int64_t)at.b * a.nq + h0 + tid] = s_ml[tid];
-            } else {
-                const int slot = 2 * c + (piece0 == seg0 ? 1 : 0);
-                float* part = a.parts + (int64_t)slot * a.gs * a.D;
-                for (int i = tid; i < nh * quads; i += kPgThreads) {
-                    const int row = i / quads, d = (i - row * quads) * 4;
-                    *reinterpret_cast<float4*>(part + row * a.D + d) = sum(row, d);
-                }
-                if (tid < nh) a.pml[(int64_t)slot * a.gs + tid] = s_ml[tid];
-                if (!pieced) {
-                    cf = seg0 / upc;
-                    pieces = (seg0 + at.s.n - 1) / upc - cf + 1;
-                }
-                __syncthreads();
-                if (tid == 0) {  // (the barrier orders the CTA's writes before this thread's fence)
-                    __threadfence();
-                    s_last = atomicAdd(a.counters + cf, 1) == pieces - 1;
-                    __threadfence();
-                }
-                __syncthreads();
-                if (s_last) {
-                    // ---- last of the segment's CTAs: its pieces in order.  Piece p is in slot 2 (cf + p), the first
-                    // one in the slot after
-                    if (tid == 0) a.counters[cf] = 0;
-                    const float2* ml0 = a.pml + (int64_t)2 * cf * a.gs;
-                    const float* part0 = a.parts + (int64_t)2 * cf * a.gs * a.D;
-                    for (int i = tid; i < nh * quads; i += kPgThreads) {
-                        const int row = i / quads, d = (i - row * quads) * 4;
-                        float M = -1e30f, Ls = 0.f;
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                        for (int p = 0; p < pieces; ++p) {
-                            const int64_t sl = (int64_t)(2 * p + (p == 0)) * a.gs + row;
-                            const float4 x = __ldcg(reinterpret_cast<const float4*>(part0 + sl * a.D + d));
-                            const float2 ml = __ldcg(&ml0[sl]);
-                            const float m = fmaxf(M, ml.x), f = ex2(M - m), w = ex2(ml.x - m);
-                            M = m;
-                            Ls = fmaf(Ls, f, ml.y * w);
-                            v = make_float4(fmaf(v.x, f, x.x * w), fmaf(v.y, f, x.y * w), fmaf(v.z, f, x.z * w),
-                                            fmaf(v.w, f, x.w * w));
-                        }
-                        store4<BF16>(a.out, oat + row * a.D + d, v, Ls > 0.f ? 1.f / Ls : 0.f);
-                        if (a.stats && d == 0) a.stats[(int64_t)at.b * a.nq + h0 + row] = make_float2(M, Ls);
-                    }
-                }
-            }
+            finish_piece(a, s_split, w, at, r, piece0, s_ml, sum,
+                         [&](int64_t i, float4 v, float scale) { store4<BF16>(a.out, i, v, scale); });
             __syncthreads();
             at.next(a);
             piece0 = r + 1;
@@ -691,15 +418,15 @@ __global__ void __launch_bounds__(kPgScoreThreads, 8) paged_scores_kernel(const 
     Seen<U> s;
     s.of(a, b);
     const int i = (blockIdx.x * blockDim.x + threadIdx.x) * 4, u = i / U;
-    const int pos0 = s.base(u) + i - u * U, bs = a.kv.block_size;
+    const int pos0 = s.base(u) + i - u * U, bs = a.block_size;
     float* sc[4];
     float w[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         sc[e] = nullptr;
         if (u >= s.n || !s.sees(u, pos0 + e)) continue;
-        const int at = a.div.block(pos0 + e), blk = a.kv.block_tables[(int64_t)b * a.kv.max_blocks + at];
-        if ((unsigned)blk < (unsigned)a.kv.num_blocks)
+        const int at = a.div.block(pos0 + e), blk = a.block_tables[(int64_t)b * a.max_blocks + at];
+        if ((unsigned)blk < (unsigned)a.num_blocks)
             sc[e] = a.scores + ((int64_t)blk * a.nkv + kvh) * bs + a.div.slot(pos0 + e, at);
     }
     float old[4] = {0.f, 0.f, 0.f, 0.f};
@@ -764,10 +491,10 @@ static PagedSizes paged_sizes(int batch, int nq, int nkv, int D, int64_t max_pos
     return z;
 }
 
-template <int DP, bool GH, bool BF16>
+template <int DP, bool GH, bool BF16, bool LIST>
 static int paged_launch(const PagedArgs& a, const PagedSizes& z, cudaStream_t s) {
     using C = PagedCfg<DP, GH>;
-    auto kern = paged_attn_kernel<DP, GH, BF16>;
+    auto kern = paged_attn_kernel<DP, GH, BF16, LIST>;
     static bool done[64];
     B2_TRY(allow_smem(kern, C::BYTES, done));
     B2_TRY(launch(kern, dim3(z.grid), dim3(kPgThreads), C::BYTES, s, true, a));
@@ -778,32 +505,31 @@ static int paged_launch(const PagedArgs& a, const PagedSizes& z, cudaStream_t s)
     return B2_OK;
 }
 
-template <int DP>
+template <int DP, bool LIST>
 static int paged_dispatch(const PagedArgs& a, const PagedSizes& z, cudaStream_t s) {
-    if (a.kv.bf16) return a.gs > 8 ? paged_launch<DP, true, true>(a, z, s) : paged_launch<DP, false, true>(a, z, s);
-    return a.gs > 8 ? paged_launch<DP, true, false>(a, z, s) : paged_launch<DP, false, false>(a, z, s);
+    if (a.kv.bf16)
+        return a.gs > 8 ? paged_launch<DP, true, true, LIST>(a, z, s) : paged_launch<DP, false, true, LIST>(a, z, s);
+    return a.gs > 8 ? paged_launch<DP, true, false, LIST>(a, z, s) : paged_launch<DP, false, false, LIST>(a, z, s);
+}
+template <bool LIST>
+static int paged_dispatch(const PagedArgs& a, const PagedSizes& z, cudaStream_t s) {
+    if (a.D <= 64) return paged_dispatch<64, LIST>(a, z, s);
+    if (a.D <= 128) return paged_dispatch<128, LIST>(a, z, s);
+    return paged_dispatch<256, LIST>(a, z, s);
 }
 
-}  // namespace b2
-
-extern "C" size_t b2_paged_decode_workspace_bytes(int batch, int nq, int nkv, int D, int64_t max_positions,
-                                                  int scored) {
-    if (batch <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || D <= 0 || max_positions < 0) return 0;
-    const b2::PagedSizes z = b2::paged_sizes(batch, nq, nkv, D, max_positions, scored != 0);
-    return z.parts + z.pml + z.stats + z.logits;
-}
-
-extern "C" int b2_paged_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv* kv, void* out, float* scores,
-                                   int batch, int nq, int nkv, int D, int window, int sinks, b2_workspace* ws,
-                                   void* stream) {
-    using namespace b2;
+// Checks and arguments of both entry points: blocks null, or the listed blocks of each (sequence, kv head).
+static int paged_call(const void* q, int64_t ldq, const b2_paged_kv* kv, void* out, float* scores, const int* blocks,
+                      int listed, int batch, int nq, int nkv, int D, int window, int sinks, b2_workspace* ws,
+                      void* stream) {
     if (batch <= 0) return B2_OK;
     B2_REQUIRE(q && out && nq > 0 && nkv > 0 && nq % nkv == 0 && window >= 0 && sinks >= 0);
     const int rc = check_paged(kv, nkv, D);
     if (rc != B2_OK) return rc;
     if (!aligned16(q) || !aligned16(out) || (ldq & 7)) return B2_ERR_UNSUPPORTED;
     if (scores && !ws) return B2_ERR_WORKSPACE;
-    const int64_t span = (int64_t)kv->max_blocks * kv->block_size;
+    const int64_t span = (int64_t)(blocks ? listed : kv->max_blocks) * kv->block_size;
+    if (span > (1 << 30)) return B2_ERR_UNSUPPORTED;
     const int64_t most = window > 0 && (int64_t)window + sinks < span ? (int64_t)window + sinks : span;
     const PagedSizes z = paged_sizes(batch, nq, nkv, D, most, scores != nullptr);
     // units are counted in 32 bits; the scores' grid has (nkv, batch) as (y, z)
@@ -814,7 +540,14 @@ extern "C" int b2_paged_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv
     a.q = q;
     a.ldq = ldq;
     a.kv = *kv;
+    a.block_tables = kv->block_tables;
+    a.seq_lens = kv->seq_lens;
+    a.num_blocks = kv->num_blocks;
+    a.block_size = kv->block_size;
+    a.max_blocks = kv->max_blocks;
     a.div = block_div(kv->block_size);
+    a.blocks = blocks;
+    a.listed = listed;
     a.out = out;
     a.scores = scores;
     a.batch = batch;
@@ -839,7 +572,28 @@ extern "C" int b2_paged_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv
         a.counters = ws->counters;
     }
     cudaStream_t s = as_stream(stream);
-    if (D <= 64) return paged_dispatch<64>(a, z, s);
-    if (D <= 128) return paged_dispatch<128>(a, z, s);
-    return paged_dispatch<256>(a, z, s);
+    return blocks ? paged_dispatch<true>(a, z, s) : paged_dispatch<false>(a, z, s);
+}
+
+}  // namespace b2
+
+extern "C" size_t b2_paged_decode_workspace_bytes(int batch, int nq, int nkv, int D, int64_t max_positions,
+                                                  int scored) {
+    if (batch <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || D <= 0 || max_positions < 0) return 0;
+    const b2::PagedSizes z = b2::paged_sizes(batch, nq, nkv, D, max_positions, scored != 0);
+    return z.parts + z.pml + z.stats + z.logits;
+}
+
+extern "C" int b2_paged_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv* kv, void* out, float* scores,
+                                   int batch, int nq, int nkv, int D, int window, int sinks, b2_workspace* ws,
+                                   void* stream) {
+    return b2::paged_call(q, ldq, kv, out, scores, nullptr, 0, batch, nq, nkv, D, window, sinks, ws, stream);
+}
+
+extern "C" int b2_paged_decode_gqa_blocks(const void* q, int64_t ldq, const b2_paged_kv* kv, const int* blocks,
+                                          int listed, void* out, int batch, int nq, int nkv, int D, b2_workspace* ws,
+                                          void* stream) {
+    if (batch <= 0) return B2_OK;
+    B2_REQUIRE(blocks && listed > 0);
+    return b2::paged_call(q, ldq, kv, out, nullptr, blocks, listed, batch, nq, nkv, D, 0, 0, ws, stream);
 }
