@@ -17,19 +17,27 @@
 // queries for K (channels whose codes come out smaller are multiplied by 16)
 // and into the end for V, where it depends on the output's channel alone.
 //   scores   s_i = sum_g s_ig (sum_d q_d u_id) + m_ig (sum_d q_d): one product
-//            per group into its own sums, then one multiply-add each.
-//   outputs  o_d = sum_i (p_i s_ig) u_id + sum_i p_i m_ig: the weights times the
-//            scale are the operand, split into a half and the half of what the
-//            rounding left, so that it costs no accuracy beside the output's
-//            own rounding; the second sum is kept in 32 bits per group.
+//            per group into its own sums, then one multiply-add each; the second
+//            terms are a product too, of the scale words as they are stored with
+//            the sums of q as half and remainder.
+//   outputs  o_d = sum_i (p_i s_ig) (u_id - 8) + sum_i p_i (m_ig + 8 s_ig): the
+//            weights times the scale are the operand, split into a half and the
+//            half of what the rounding left, so that they cost no accuracy
+//            beside the output's own rounding; the second sum is kept in 32 bits
+//            per group.  Less 8, because sums of codes of one sign would be far
+//            larger than the output that is left of them (at 131001 tokens the
+//            rounding of the sums would show in the output: 5e-4 instead of
+//            1.7e-4 of it): a product with a constant -8 is where each unit's
+//            sums start.
 // Queries are scaled by a power of two into the middle of the halves' range
-// (bf16 ones are then exact in half), the weights times the scale by one that
-// follows the largest scale seen so far, like the running max of the softmax.
+// (bf16 ones are then exact in half), the weights by one that follows the
+// largest scale seen so far, like the running max of the softmax.
 //
-// Layout of the products: heads are the rows of S = Q K^T and the columns of O
-// = V^T P, so a lane's S values are its fragment of P as they are.  Up to 4
-// heads (H = 4) stand twice in the rows: the second copy becomes the
-// remainders, the other 4 columns of the same product.
+// Layout of the products: positions, then channels, are the 16 rows and the
+// heads the 8 columns.  Up to 4 heads (H = 4) stand twice in the columns: the
+// second copy becomes the remainders, in the same product.  (Heads as the rows
+// of S take twice the products and, since half of each operand's registers are
+// then zeros that have to be put there, 456 instructions a tile instead of 340.)
 //
 // Split: paged_split.cuh.  Each of 4 warps streams tiles of 16 positions (kv4.cuh)
 // through its own ring of shared-memory stages (cp.async).
@@ -58,7 +66,7 @@ struct Kv4Cfg {
     static constexpr int TILE = kv4_tile(DP);
     static constexpr int T = DP <= 128 ? 2 : 1;        // tiles per warp and unit
     static constexpr int U = kPgWarps * T * 16;        // positions per unit
-    static constexpr int STAGES = 2;
+    static constexpr int STAGES = DP <= 128 ? 3 : 2;
     static constexpr int STAGE = T * TILE;
     static constexpr int LDO = DP + 4;
     static constexpr int OFF_O = kPgWarps * STAGES * STAGE;
@@ -96,6 +104,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
+__device__ __forceinline__ void mma_f16_k8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0, const float* c) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%8,%9,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(b0), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 // two 32-bit numbers in a register pair: one instruction for both
 __device__ __forceinline__ uint64_t pair(float a, float b) {
     uint64_t r;
@@ -107,19 +121,9 @@ __device__ __forceinline__ float2 two(uint64_t p) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
     return r;
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
@@ -131,10 +135,10 @@ template <int DP, int H, bool LIST>
 __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kernel(const Kv4Args a) {
     using C = Kv4Cfg<DP, H>;
     constexpr int U = C::U, T = C::T, W = C::W, NG = C::NG;
-    constexpr int R = H == 16 ? 2 : 1;  // rows of S per lane: head lr (H = 4: lr % 4), and head lr + 8
+    constexpr int NT = H == 16 ? 2 : 1;  // products side by side, 8 heads each
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ SplitShared s_split;
-    __shared__ int s_vis[kPgWarps][C::STAGES][T];  // visible rows of a tile, first | end << 8; 0: none
+    __shared__ __align__(4) uint16_t s_vis[kPgWarps][C::STAGES][T];  // visible rows of a tile, first | end << 8; 0: none
     __shared__ float s_m[kPgWarps][16], s_l[kPgWarps][16];
     __shared__ float2 s_ml[16];
     float* s_o = reinterpret_cast<float*>(smem + C::OFF_O);
@@ -149,84 +153,94 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
     if (!split_units(a, s_split, w, at)) return;
     const int r0 = w.r0, r1 = w.r1;
 
-    // ---- producer: tiles of the next unit into a stage.  The table entries of the two next units are on their way,
-    // lane t's that of tile t
+    // ---- producer: tiles of the next unit into a stage.  Where they are is looked up for up to 32 tiles of the warp at a
+    // time, one per lane, a batch before it is needed (looked up unit by unit, that alone was 100 of 380 instructions a
+    // tile)
+    constexpr int BATCH = 32 / T;            // units of a batch, all of one segment
     Place<U, LIST> pp = at;
-    int pr = r0, pf = r0, pid[2], vis[2];  // units requested, units looked up
-    int64_t off[2];
-    auto lookup = [&](int k) {
-        pid[k] = -1;
-        vis[k] = 0;
-        off[k] = 0;
-        if (pf < r1) {
-            const int pos = pp.s.base(pp.u) + (warp * T + lane) * 16;
+    int pr = r0, pf = r0;                    // units requested, units looked up
+    int used = 0, count = 0, next = 0;       // units of the current batch: requested, all; units of the next batch
+    int pid = -1, vis2 = 0, vis = 0;         // table entry and visible rows (first | end << 8) of the next batch; current
+    int64_t off = 0, from = -1;              // in the block, next batch; in the pool (-1: nothing), current one
+    auto lookup = [&]() {
+        pid = -1;
+        vis2 = 0;
+        next = min(BATCH, min(pp.s.n - pp.u, r1 - pf));
+        if (next <= 0) return;
+        const int u = pp.u + lane / T;
+        if (lane < next * T) {
+            const int pos = pp.s.base(u) + (warp * T + lane % T) * 16;
             int blk = a.div.block(pos), v0 = 0, v1 = 0;
             const int slot = a.div.slot(pos, blk);
-            if (lane < T) {
-                if constexpr (LIST) {  // blk counts entries of the list
-                    if (blk < a.listed) {
-                        blk = a.blocks[((int64_t)pp.b * a.nkv + pp.kvh) * a.listed + blk];
-                        if ((unsigned)blk < (unsigned)a.max_blocks) v1 = min(16, pp.s.L - blk * a.block_size - slot);
-                    }
-                } else if (pp.u < pp.s.ns) {
-                    v1 = min(16, pp.s.s0 - pos);
-                } else {
-                    v0 = max(0, pp.s.lo - pos);
-                    v1 = min(16, pp.s.L - pos);
+            if constexpr (LIST) {  // blk counts entries of the list
+                if (blk < a.listed) {
+                    blk = a.blocks[((int64_t)pp.b * a.nkv + pp.kvh) * a.listed + blk];
+                    if ((unsigned)blk < (unsigned)a.max_blocks) v1 = min(16, pp.s.L - blk * a.block_size - slot);
                 }
-                if (v0 < v1) {
-                    pid[k] = a.block_tables[(int64_t)pp.b * a.max_blocks + blk];
-                    vis[k] = v0 | v1 << 8;
-                    off[k] = pp.kvh * a.head_bytes + (int64_t)(slot >> 4) * C::TILE;
-                }
+            } else if (u < pp.s.ns) {
+                v1 = min(16, pp.s.s0 - pos);
+            } else {
+                v0 = max(0, pp.s.lo - pos);
+                v1 = min(16, pp.s.L - pos);
             }
-            ++pf;
-            pp.next(a);
+            if (v0 < v1) {
+                pid = a.block_tables[(int64_t)pp.b * a.max_blocks + blk];
+                vis2 = v0 | v1 << 8;
+                off = pp.kvh * a.head_bytes + (int64_t)(slot >> 4) * C::TILE;
+            }
         }
+        pf += next;
+        pp.u += next - 1;
+        pp.next(a);
     };
     const uint64_t policy = read_once();
     uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
+    const uint32_t ring_at = smem_addr(ring) + lane * 16;
+    const uint8_t* const pool = a.pool + lane * 16;
     auto issue = [&](int stage) {
         if (pr < r1) {
-            const bool mine = (unsigned)pid[0] < (unsigned)a.num_blocks;
-            const int64_t from = (int64_t)pid[0] * a.stride_block + off[0];
-            if (lane < T) s_vis[warp][stage][lane] = mine ? vis[0] : 0;
+            if (used == count) {
+                const bool there = (unsigned)pid < (unsigned)a.num_blocks;
+                from = there ? pid * a.stride_block + off : -1;
+                vis = there ? vis2 : 0;
+                count = next;
+                used = 0;
+                lookup();
+            }
+            const int v = __shfl_sync(~0u, vis, used * T + lane % T);
+            if (lane < T) s_vis[warp][stage][lane] = (uint16_t)v;
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                const int64_t f = __shfl_sync(~0u, from, t);
-                if (__shfl_sync(~0u, (int)mine, t)) {
-                    const uint8_t* src = a.pool + f + lane * 16;
-                    const uint32_t dst = smem_addr(ring + stage * C::STAGE + t * C::TILE + lane * 16);
+                const int64_t f = __shfl_sync(~0u, from, used * T + t);
+                if (f >= 0) {
+                    const uint32_t dst = ring_at + stage * C::STAGE + t * C::TILE;
 #pragma unroll
                     for (int i = 0; i < (C::TILE + 511) / 512; ++i)
-                        if (i < C::TILE / 512 || lane * 16 < C::TILE % 512) cp16(dst + i * 512, src + i * 512, true, policy);
+                        if (i < C::TILE / 512 || lane * 16 < C::TILE % 512)
+                            cp16(dst + i * 512, pool + f + i * 512, true, policy);
                 }
             }
+            ++used;
             ++pr;
-            pid[0] = pid[1];
-            vis[0] = vis[1];
-            off[0] = off[1];
-            lookup(1);
         }
         cp_commit();
     };
-    lookup(0);
-    lookup(1);
+    lookup();
 #pragma unroll
     for (int s = 0; s < C::STAGES; ++s) issue(s);
 
-    // ---- consumer
-    uint32_t qa[W][2][R][2];         // fragments of Q: word, step, row, half
-    float mq[NG][R], fq[R];          // sums of q over a group, and the factor of the products, both with the log2 scale
-    float o[W][2][R][4], m[R];
-    uint64_t l[R], am[R][NG];        // even and odd positions apart
-    int E;                           // scales of V below 2^E so far: weights are 2^(14 - E) times theirs
+    // ---- consumer.  Lane (lr, lc) holds positions lr and lr + 8, then channels 32 x + 4 lr .. + 3, of heads 2 lc and
+    // 2 lc + 1 (of each 8; H = 4: modulo 4)
+    uint32_t qb[W][2][NT][2], mb[NT][2];         // fragments of Q and of its sums over the groups
+    float fq[NT][2];                             // from scores as they come out of the products to base-2 logits
+    float o[W][2][NT][4], m[NT][2], l[NT][2], am[NT][2][NG];
+    int E;                                       // scales of V below 2^E so far: weights are 2^(14 - E) times theirs
     auto start = [&]() {  // a new segment (or the rest of one): its queries, nothing summed yet
         const int h0 = at.head0(a), nh = at.heads(a);
         const uint16_t* q = static_cast<const uint16_t*>(a.q) + at.b * a.ldq + (int64_t)h0 * a.D;
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int row = (H == 4 ? lr & 3 : lr) + 8 * r;
+        for (int n = 0; n < NT; ++n) {
+            const int row = (H == 4 ? lr & 3 : lr) + 8 * n;
             uint4 raw[W];
             float top = 0.f;
             auto eight = [&](const uint4& x, float (&f)[8]) {
@@ -250,35 +264,41 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
             }
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-            // the largest |q| to 2^9 .. 2^10, times 16 still inside half; elements 2^-34 below it are lost
-            const int e = top > 0.f && top < INFINITY ? min(120, 9 - ((int)(__float_as_uint(top) >> 23) - 127)) : 0;
+            // the largest |q| to 2^5 .. 2^6: times 16, and summed over a group, still inside half.  Elements 2^-30 below
+            // it are lost
+            const int e = top > 0.f && top < INFINITY ? min(120, 5 - ((int)(__float_as_uint(top) >> 23) - 127)) : 0;
             const float sc = pow2(e);
-            fq[r] = a.scale_log2 * pow2(20) * pow2(-e);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) mq[g][r] = 0.f;
+            float sums[NG] = {};
 #pragma unroll
             for (int j = 0; j < W; ++j) {
                 float f[8];
                 eight(raw[j], f);
-                float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum += f[i], f[i] *= sc;
-                mq[j / 2][r] += sum;
-                qa[j][0][r][0] = f2_to_h2(f[0] * 16.f, f[4] * 16.f);
-                qa[j][0][r][1] = f2_to_h2(f[1], f[5]);
-                qa[j][1][r][0] = f2_to_h2(f[2] * 16.f, f[6] * 16.f);
-                qa[j][1][r][1] = f2_to_h2(f[3], f[7]);
+                for (int i = 0; i < 8; ++i) f[i] *= sc, sums[j / 2] += f[i];
+                qb[j][0][n][0] = f2_to_h2(f[0] * 16.f, f[4] * 16.f);
+                qb[j][0][n][1] = f2_to_h2(f[1], f[5]);
+                qb[j][1][n][0] = f2_to_h2(f[2] * 16.f, f[6] * 16.f);
+                qb[j][1][n][1] = f2_to_h2(f[3], f[7]);
             }
+            // rows 2 g + 1 of this operand meet m of group g, rows 2 g its s
+            mb[n][0] = mb[n][1] = 0u;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                float x = mq[g][r];
+                float x = sums[g];
                 x += __shfl_xor_sync(~0u, x, 1);
                 x += __shfl_xor_sync(~0u, x, 2);
-                mq[g][r] = x * a.scale_log2;
-                am[r][g] = 0;
+                const uint32_t hi = f2_to_h2(0.f, x), lo = f2_to_h2(0.f, x - h2_to_f2(hi).y);
+                if (lc == g) mb[n][0] = hi, mb[n][1] = lo;
             }
-            m[r] = -INFINITY;
-            l[r] = 0;
+            const float f = a.scale_log2 * pow2(-e);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                fq[n][h] = __shfl_sync(~0u, f, (lc * 2 + h) * 4);
+                m[n][h] = -INFINITY;
+                l[n][h] = 0.f;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) am[n][h][g] = 0.f;
+            }
         }
         E = -15;  // the first tile raises it
 #pragma unroll
@@ -286,167 +306,190 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int r = 0; r < R; ++r)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[x][h][r][e] = 0.f;
+                    for (int e = 0; e < 4; ++e) o[x][h][n][e] = 0.f;
     };
 
     start();
     int piece0 = r0;  // where the current piece of a segment began
+    int stage = 0;
     for (int r = r0; r < r1; ++r) {
-        const int stage = (r - r0) % C::STAGES;
         cp_wait<C::STAGES - 1>();
         __syncwarp();
-        int seen[T], any = 0;
-#pragma unroll
-        for (int t = 0; t < T; ++t) any |= seen[t] = s_vis[warp][stage][t];
+        uint32_t seen;
+        if constexpr (T == 2)
+            seen = *reinterpret_cast<const uint32_t*>(s_vis[warp][stage]);
+        else
+            seen = s_vis[warp][stage][0];
         const uint8_t* const unit = ring + stage * C::STAGE;
-        if (__any_sync(~0u, any)) {
+        if (__any_sync(~0u, seen != 0u)) {
             constexpr float zero[4] = {0.f, 0.f, 0.f, 0.f};
-            // S of positions 2 lc, 2 lc + 1 (pp = 0) and those + 8 (pp = 1) of each tile, and the scales of V there
-            uint64_t x[T][R][2];
-            uint32_t vm[T][4 * NG];
+            float x[T][NT][4];        // scores of (lr, 2 lc), (lr, 2 lc + 1), (lr + 8, ..)
+            uint32_t vm[T][2][NG];    // scale words of V at positions lr and lr + 8
 #pragma unroll
             for (int t = 0; t < T; ++t) {
                 const uint8_t* tile = unit + t * C::TILE;
-                uint32_t meta[4 * NG];
-                lds(meta, tile + 16 * DP + lc * 16 * NG);
-                lds(vm[t], tile + 16 * DP + 64 * NG + lc * 16 * NG);
+                const uint8_t* meta = tile + 16 * DP + kv4_slot(lr) * (4 * NG);  // (position lr + 8: two slots on)
+                uint32_t kw[2][W], km[2][NG];
 #pragma unroll
                 for (int pp = 0; pp < 2; ++pp) {
-                    float acc[NG][4];
-                    uint32_t kw[W];
-                    lds(kw, tile + (lr + 8 * pp) * (DP / 2) + lc * (4 * W));
-#pragma unroll
-                    for (int j = 0; j < W; ++j) {
-                        const uint32_t u = kw[j], v = u >> 8;
-                        float(&c)[4] = acc[j / 2];
-                        mma_f16(c, qa[j][0][0][0], R == 2 ? qa[j][0][R - 1][0] : 0u, qa[j][0][0][1],
-                                R == 2 ? qa[j][0][R - 1][1] : 0u, u & 0x000f000fu, u & 0x00f000f0u, j & 1 ? c : zero);
-                        mma_f16(c, qa[j][1][0][0], R == 2 ? qa[j][1][R - 1][0] : 0u, qa[j][1][0][1],
-                                R == 2 ? qa[j][1][R - 1][1] : 0u, v & 0x000f000fu, v & 0x00f000f0u, c);
-                    }
-                    uint64_t y[R];
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) {
-                        const float2 a0 = h2_to_f2(meta[2 * pp * NG + g]), a1 = h2_to_f2(meta[(2 * pp + 1) * NG + g]);
-                        const uint64_t sc = pair(a0.x, a1.x), mn = pair(a0.y, a1.y);
-#pragma unroll
-                        for (int k = 0; k < R; ++k) {
-                            const uint64_t c = pair(acc[g][2 * k], acc[g][2 * k + 1]), q2 = pair(mq[g][k], mq[g][k]);
-                            x[t][k][pp] = g ? fma2(sc, c, x[t][k][pp]) : mul2(sc, c);
-                            y[k] = g ? fma2(mn, q2, y[k]) : mul2(mn, q2);
-                        }
-                    }
-#pragma unroll
-                    for (int k = 0; k < R; ++k) x[t][k][pp] = fma2(x[t][k][pp], pair(fq[k], fq[k]), y[k]);
+                    lds(kw[pp], tile + (lr + 8 * pp) * (DP / 2) + lc * (4 * W));
+                    lds(km[pp], meta + pp * (8 * NG));
+                    lds(vm[t][pp], meta + 64 * NG + pp * (8 * NG));
                 }
-                if (seen[t] != 16 << 8) {  // rows that are not visible hold anything
-                    const int v0 = seen[t] & 255, v1 = seen[t] >> 8;
+                const uint8_t* own = meta + (lc < NG ? lc : 0) * 4;
+                const uint32_t w0 = *reinterpret_cast<const uint32_t*>(own),
+                               w1 = *reinterpret_cast<const uint32_t*>(own + 8 * NG);
+                float acc[NT][NG][4], y[NT][4];
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    const uint32_t u0 = kw[0][j], u1 = kw[1][j], v0 = u0 >> 8, v1 = u1 >> 8;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float(&c)[4] = acc[n][j / 2];
+                        mma_f16(c, u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u, qb[j][0][n][0],
+                                qb[j][0][n][1], j & 1 ? c : zero);
+                        mma_f16(c, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qb[j][1][n][0],
+                                qb[j][1][n][1], c);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma_f16_k8(y[n], w0, w1, mb[n][0], zero);
+                    mma_f16_k8(y[n], w0, w1, mb[n][1], y[n]);
+                }
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
 #pragma unroll
                     for (int pp = 0; pp < 2; ++pp) {
-                        const int p = pp * 8 + 2 * lc;
-                        const bool there[2] = {p >= v0 && p < v1, p + 1 >= v0 && p + 1 < v1};
+                        const float sc = h2_to_f2(km[pp][g]).x;
 #pragma unroll
-                        for (int k = 0; k < R; ++k) {
-                            const float2 y = two(x[t][k][pp]);
-                            x[t][k][pp] = pair(there[0] ? y.x : -INFINITY, there[1] ? y.y : -INFINITY);
-                        }
+                        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int g = 0; g < 2 * NG; ++g) vm[t][2 * pp * NG + g] = there[g / NG] ? vm[t][2 * pp * NG + g] : 0u;
+                            for (int h = 0; h < 2; ++h) {
+                                const int i = 2 * pp + h;
+                                x[t][n][i] = g ? fmaf(sc, acc[n][g][i], x[t][n][i]) : sc * acc[n][g][i];
+                            }
+                    }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[t][n][i] = fmaf(x[t][n][i], 1048576.f, y[n][i]);
+            }
+            if (seen != (T == 2 ? 0x10001000u : 0x1000u)) {  // rows that are not visible hold anything
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    const int v0 = seen >> (16 * t) & 255, v1 = seen >> (16 * t + 8) & 255;
+#pragma unroll
+                    for (int pp = 0; pp < 2; ++pp) {
+                        const bool there = lr + 8 * pp >= v0 && lr + 8 * pp < v1;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) x[t][n][2 * pp + h] = there ? x[t][n][2 * pp + h] : -INFINITY;
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) vm[t][pp][g] = there ? vm[t][pp][g] : 0u;
                     }
                 }
             }
-            // running max of the heads, finite, so that exp2(-inf - m) is 0, and the largest scale of V (NaN and
-            // infinities do not count)
-            float top[R];
-            uint32_t big = vm[0][0];
+            // does a score pass its head's running max, or a scale of V 2^E?  (NaN and infinities do not count)
+            float top[NT][2];
+            uint32_t big = vm[0][0][0];
+            bool moved = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float y = fmaxf(x[0][n][h], x[0][n][2 + h]);
+#pragma unroll
+                    for (int t = 1; t < T; ++t) y = fmaxf(y, fmaxf(x[t][n][h], x[t][n][2 + h]));
+                    top[n][h] = y;
+                    moved |= y > m[n][h];
+                }
 #pragma unroll
             for (int t = 0; t < T; ++t)
 #pragma unroll
-                for (int i = 0; i < 4 * NG; ++i) big = hmax2(big, vm[t][i]);
-            big = hmax2(big, __shfl_xor_sync(~0u, big, 1));
-            big = hmax2(big, __shfl_xor_sync(~0u, big, 2)) & 0xffffu;
+                for (int i = 0; i < 2 * NG; ++i) big = hmax2(big, vm[t][i / NG][i % NG]);
+            big &= 0xffffu;
             if (big > 0x7bffu) big = 0u;
-            bool moved = (int)big >= (E + 15) * 1024;
-#pragma unroll
-            for (int k = 0; k < R; ++k) {
-                float y = -1e30f;
-#pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    const float2 a0 = two(x[t][k][0]), a1 = two(x[t][k][1]);
-                    y = fmaxf(y, fmaxf(fmaxf(a0.x, a0.y), fmaxf(a1.x, a1.y)));
-                }
-                y = fmaxf(y, __shfl_xor_sync(~0u, y, 1));
-                y = fmaxf(y, __shfl_xor_sync(~0u, y, 2));
-                top[k] = fmaxf(m[k], y);
-                moved |= top[k] > m[k];
-            }
+            moved |= (int)big >= (E + 15) * 1024;
             if (__any_sync(~0u, moved)) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) big = max(big, __shfl_xor_sync(~0u, big, d));
                 const int En = (int)big >= (E + 15) * 1024 ? max(1, (int)(big >> 10)) - 13 : E;
 #pragma unroll
-                for (int k = 0; k < R; ++k) {
-                    const float f = ex2(m[k] - top[k] + (float)(E - En));
-                    m[k] = top[k];
-                    l[k] = mul2(l[k], pair(f, f));
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) am[k][g] = mul2(am[k][g], pair(f, f));
-                    const float f0 = __shfl_sync(~0u, f, lc * 8), f1 = __shfl_sync(~0u, f, lc * 8 + 4);
+                    for (int h = 0; h < 2; ++h) {
+                        float y = fmaxf(m[n][h], top[n][h]);
 #pragma unroll
-                    for (int v = 0; v < W; ++v)
+                        for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(~0u, y, d));
+                        const float f = ex2(fmaf(m[n][h] - y, fq[n][h], (float)(E - En)));
+                        m[n][h] = y;
+                        l[n][h] *= f;
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            o[v][h][k][0] *= f0, o[v][h][k][1] *= f1;
-                            o[v][h][k][2] *= f0, o[v][h][k][3] *= f1;
-                        }
-                }
+                        for (int g = 0; g < NG; ++g) am[n][h][g] *= f;
+#pragma unroll
+                        for (int v = 0; v < W; ++v)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                o[v][k][n][h] *= f;
+                                o[v][k][n][2 + h] *= f;
+                            }
+                    }
                 E = En;
             }
             // the weights, 2^(14 - E) times theirs
 #pragma unroll
-            for (int k = 0; k < R; ++k) {
-                const float less = (float)(14 - E) - m[k];
-                const uint64_t by = pair(less, less);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int t = 0; t < T; ++t)
+                for (int h = 0; h < 2; ++h) {
+                    const float less = fmaf(-m[n][h], fq[n][h], (float)(14 - E));
 #pragma unroll
-                    for (int pp = 0; pp < 2; ++pp) {
-                        const float2 y = two(add2(x[t][k][pp], by));
-                        x[t][k][pp] = pair(ex2(y.x), ex2(y.y));
-                        l[k] = add2(l[k], x[t][k][pp]);
-                    }
-            }
-            // O += V^T (P s), group by group, with codes less 8
-            const uint64_t eight = pair(8.f, 8.f);
+                    for (int t = 0; t < T; ++t)
+#pragma unroll
+                        for (int pp = 0; pp < 2; ++pp) {
+                            float& p = x[t][n][2 * pp + h];
+                            p = ex2(fmaf(p, fq[n][h], less));
+                            l[n][h] += p;
+                        }
+                }
+            // O += V^T (P s), group by group, with codes less 8; the weights as half and remainder, turned from
+            // (position, head) to (head, position) pairs
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                uint32_t hi[T][R][2], lo[T][R][2];
-                float less[R][4];
+                uint32_t hi[T][NT][2], lo[T][NT][2];
+                float less[NT][4];
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
 #pragma unroll
                     for (int pp = 0; pp < 2; ++pp) {
-                        const float2 a0 = h2_to_f2(vm[t][2 * pp * NG + g]), a1 = h2_to_f2(vm[t][(2 * pp + 1) * NG + g]);
-                        const uint64_t sc = pair(a0.x, a1.x), mid = fma2(eight, sc, pair(a0.y, a1.y));
+                        const float2 sm = h2_to_f2(vm[t][pp][g]);
+                        const float mid = fmaf(8.f, sm.x, sm.y);
 #pragma unroll
-                        for (int k = 0; k < R; ++k) {
-                            am[k][g] = fma2(x[t][k][pp], mid, am[k][g]);
-                            const uint64_t ws = mul2(x[t][k][pp], sc);
-                            const float2 a = two(ws);
-                            hi[t][k][pp] = f2_to_h2(a.x, a.y);
-                            const float2 b = h2_to_f2(hi[t][k][pp]), rest = two(add2(ws, pair(-b.x, -b.y)));
-                            lo[t][k][pp] = f2_to_h2(rest.x, rest.y);
-                            if (H == 4) hi[t][k][pp] = lr >= 4 ? lo[t][k][pp] : hi[t][k][pp];
+                        for (int n = 0; n < NT; ++n) {
+                            const float p0 = x[t][n][2 * pp], p1 = x[t][n][2 * pp + 1];
+                            am[n][0][g] = fmaf(p0, mid, am[n][0][g]);
+                            am[n][1][g] = fmaf(p1, mid, am[n][1][g]);
+                            uint32_t u, r;
+                            split16<false>(p0 * sm.x, p1 * sm.x, u, r);
+                            if (H == 4) {
+                                hi[t][n][pp] = transpose8x8(lc < 2 ? u : r);
+                            } else {
+                                hi[t][n][pp] = transpose8x8(u);
+                                lo[t][n][pp] = transpose8x8(r);
+                            }
                         }
                     }
                     // -8 units in the rows of either nibble: what the products of the codes start from
 #pragma unroll
-                    for (int k = 0; k < R; ++k) {
-                        mma_f16(less[k], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, hi[t][k][0], hi[t][k][1],
-                                t ? less[k] : zero);
+                    for (int n = 0; n < NT; ++n) {
+                        mma_f16(less[n], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, hi[t][n][0], hi[t][n][1],
+                                t ? less[n] : zero);
                         if (H > 4)
-                            mma_f16(less[k], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, lo[t][k][0], lo[t][k][1],
-                                    less[k]);
+                            mma_f16(less[n], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, lo[t][n][0], lo[t][n][1],
+                                    less[n]);
                     }
                 }
 #pragma unroll
@@ -455,24 +498,24 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
 #pragma unroll
                     for (int t = 0; t < T; ++t) lds(vw[t], unit + t * C::TILE + 8 * DP + (v * 32 + lane) * 8);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float c[R][4];
+                    for (int k = 0; k < 2; ++k) {
+                        float c[NT][4];
 #pragma unroll
                         for (int t = 0; t < T; ++t) {
-                            const uint32_t u0 = vw[t][0] >> (8 * h), u1 = vw[t][1] >> (8 * h);
+                            const uint32_t u0 = vw[t][0] >> (8 * k), u1 = vw[t][1] >> (8 * k);
                             const uint32_t b0 = u0 & 0x000f000fu, b1 = u0 & 0x00f000f0u, b2 = u1 & 0x000f000fu,
                                            b3 = u1 & 0x00f000f0u;
 #pragma unroll
-                            for (int k = 0; k < R; ++k) {
-                                mma_f16(c[k], b0, b1, b2, b3, hi[t][k][0], hi[t][k][1], t ? c[k] : less[k]);
-                                if (H > 4) mma_f16(c[k], b0, b1, b2, b3, lo[t][k][0], lo[t][k][1], c[k]);
+                            for (int n = 0; n < NT; ++n) {
+                                mma_f16(c[n], b0, b1, b2, b3, hi[t][n][0], hi[t][n][1], t ? c[n] : less[n]);
+                                if (H > 4) mma_f16(c[n], b0, b1, b2, b3, lo[t][n][0], lo[t][n][1], c[n]);
                             }
                         }
 #pragma unroll
-                        for (int k = 0; k < R; ++k) {
-                            float(&d)[4] = o[v][h][k];
-                            const float2 y0 = two(add2(pair(d[0], d[1]), pair(c[k][0], c[k][1])));
-                            const float2 y1 = two(add2(pair(d[2], d[3]), pair(c[k][2], c[k][3])));
+                        for (int n = 0; n < NT; ++n) {
+                            float(&d)[4] = o[v][k][n];
+                            const float2 y0 = two(add2(pair(d[0], d[1]), pair(c[n][0], c[n][1])));
+                            const float2 y1 = two(add2(pair(d[2], d[3]), pair(c[n][2], c[n][3])));
                             d[0] = y0.x, d[1] = y0.y, d[2] = y1.x, d[3] = y1.y;
                         }
                     }
@@ -481,27 +524,28 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
         }
         __syncwarp();
         issue(stage);
+        stage = stage + 1 == C::STAGES ? 0 : stage + 1;
 
         const bool done = at.u == at.s.n - 1;
         if (done || r == r1 - 1) {
             // ---- the warps meet: max and sum of each head, then the outputs, in warp order
-            float mids[R][NG];
 #pragma unroll
-            for (int k = 0; k < R; ++k) {
-                auto all = [&](uint64_t p) -> float {
-                    float v = two(p).x + two(p).y;
-                    v += __shfl_xor_sync(~0u, v, 1);
-                    v += __shfl_xor_sync(~0u, v, 2);
-                    return v;
-                };
-                const float total = all(l[k]);
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int g = 0; g < NG; ++g) mids[k][g] = all(am[k][g]);
-                if (lc == 0 && lr + 8 * k < H) {
-                    s_m[warp][lr + 8 * k] = m[k] + (float)(E - 14);
-                    s_l[warp][lr + 8 * k] = total;
+                for (int h = 0; h < 2; ++h) {
+                    auto all = [&](float v) -> float {
+                        v += __shfl_xor_sync(~0u, v, 4);
+                        v += __shfl_xor_sync(~0u, v, 8);
+                        return v + __shfl_xor_sync(~0u, v, 16);
+                    };
+                    l[n][h] = all(l[n][h]);
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) am[n][h][g] = all(am[n][h][g]);
+                    if (lr == 0 && lc * 2 + h + 8 * n < H) {
+                        s_m[warp][lc * 2 + h + 8 * n] = fmaf(m[n][h], fq[n][h], (float)(E - 14));
+                        s_l[warp][lc * 2 + h + 8 * n] = l[n][h];
+                    }
                 }
-            }
             __syncthreads();
             if (tid < H) {
                 float M = -1e30f, Ls = 0.f;
@@ -511,28 +555,26 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                 for (int v = 0; v < kPgWarps; ++v) Ls = fmaf(s_l[v][tid], ex2(s_m[v][tid] - M), Ls);
                 s_ml[tid] = make_float2(M, Ls);
             }
-            float wt[R][2], mn[R][NG][2];
+            float wt[NT][2];
 #pragma unroll
-            for (int k = 0; k < R; ++k)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = (H == 4 ? (lc * 2 + e) & 3 : lc * 2 + e) + 8 * k;
+                for (int h = 0; h < 2; ++h) {
+                    const int row = (H == 4 ? (lc * 2 + h) & 3 : lc * 2 + h) + 8 * n;
                     float M = -1e30f;
 #pragma unroll
                     for (int v = 0; v < kPgWarps; ++v) M = fmaxf(M, s_m[v][row]);
-                    wt[k][e] = ex2(s_m[warp][row] - M);
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) mn[k][g][e] = __shfl_sync(~0u, mids[k][g], (lc * 2 + e) * 4);
+                    wt[n][h] = ex2(s_m[warp][row] - M);
                 }
             // rows of codes in the low nibble of a byte hold sums 16 times smaller
-            const float k0 = pow2(24), k1 = pow2(20);
+            constexpr float k0 = 16777216.f, k1 = 1048576.f;
             if (H == 4) {
 #pragma unroll
                 for (int x = 0; x < W; ++x)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int k = 0; k < 2; ++k)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[x][h][0][e] += __shfl_xor_sync(~0u, o[x][h][0][e], 2);
+                        for (int e = 0; e < 4; ++e) o[x][k][0][e] += __shfl_xor_sync(~0u, o[x][k][0][e], 2);
             }
 #pragma unroll 1
             for (int turn = 0; turn < kPgWarps / 2; ++turn) {
@@ -541,16 +583,16 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
 #pragma unroll
                     for (int x = 0; x < W; ++x)
 #pragma unroll
-                        for (int k = 0; k < R; ++k)
+                        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                float4* d = reinterpret_cast<float4*>(buf + (k * 8 + lc * 2 + e) * C::LDO + x * 32 + lr * 4);
+                            for (int h = 0; h < 2; ++h) {
+                                float4* d = reinterpret_cast<float4*>(buf + (n * 8 + lc * 2 + h) * C::LDO + x * 32 + lr * 4);
                                 const float4 old = turn ? *d : make_float4(0.f, 0.f, 0.f, 0.f);
-                                const float n = mn[k][x / 2][e], f = wt[k][e];
-                                *d = make_float4(fmaf(fmaf(o[x][0][k][e], k0, n), f, old.x),
-                                                 fmaf(fmaf(o[x][0][k][2 + e], k1, n), f, old.y),
-                                                 fmaf(fmaf(o[x][1][k][e], k0, n), f, old.z),
-                                                 fmaf(fmaf(o[x][1][k][2 + e], k1, n), f, old.w));
+                                const float mid = am[n][h][x / 2], f = wt[n][h];
+                                *d = make_float4(fmaf(fmaf(o[x][0][n][h], k0, mid), f, old.x),
+                                                 fmaf(fmaf(o[x][0][n][2 + h], k1, mid), f, old.y),
+                                                 fmaf(fmaf(o[x][1][n][h], k0, mid), f, old.z),
+                                                 fmaf(fmaf(o[x][1][n][2 + h], k1, mid), f, old.w));
                             }
                 }
                 __syncthreads();
