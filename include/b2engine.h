@@ -413,6 +413,81 @@ int b2_paged_decode_gqa_blocks(const void* q, int64_t ldq, const b2_paged_kv* kv
                                void* out, int batch, int num_q_heads, int num_kv_heads, int head_dim,
                                b2_workspace* ws, void* stream);
 
+/* The rows of new tokens into a paged cache, with the position rotation of
+ * their queries and keys on the way; one launch.  k and v are [batch][S]
+ * [num_kv_heads][head_dim] views of the cache's type (stride_b, stride_s,
+ * stride_h; rows contiguous and 16-byte aligned), q and q_out (both or neither)
+ * the same of num_q_heads; q_out may be q.  counts (device int32 [batch], NULL:
+ * S each) says how many of a sequence's S rows are new tokens; the others are
+ * neither read nor written.  seq_lens counts them already: row i of n goes to
+ * position seq_lens[b] - n + i, as long as that is at least 0, inside the
+ * table's row and the entry inside [0, num_blocks).
+ *
+ * Rotation: the first rotary_dim channels (a multiple of 8, 0: none) in pairs
+ * (i, i + rotary_dim/2) by position * inv_freq[i]; inv_freq is read on the host
+ * during the call (rotary_dim/2 numbers).  The position is the row's in the
+ * cache, or counts up from positions[b] (device int32 [batch]) where that is
+ * given: after an eviction the two differ.  Angles are reduced in 64 bits.
+ *
+ * Sequences of one call must not share the blocks that they write.  Allocates
+ * nothing; graph-capturable.  S at most 2^30, batch at most 65535. */
+int b2_paged_kv_append(const b2_paged_kv* kv, b2_kv_view k, b2_kv_view v, const b2_kv_view* q, const b2_kv_view* q_out,
+                       const double* inv_freq, int rotary_dim, const int* counts, const int* positions, int batch,
+                       int64_t S, int num_q_heads, int num_kv_heads, int head_dim, void* stream);
+/* The same into a cache held in 4 bits.  Keys are rotated in 64 bits and every
+ * code is the one of exact arithmetic (m and s by way of 32 bits). */
+int b2_paged_kv4_append(const b2_paged_kv4* kv, b2_kv_view k, b2_kv_view v, const b2_kv_view* q,
+                        const b2_kv_view* q_out, const double* inv_freq, int rotary_dim, const int* counts,
+                        const int* positions, int batch, int64_t S, int num_q_heads, int num_kv_heads, int head_dim,
+                        void* stream);
+
+/* The newest rows of each sequence out of a cache held in 4 bits, as 16-bit
+ * rows (for the attention of a prompt's next chunk, say): the last n =
+ * min(counts[b], T, seq_lens[b]) positions (counts NULL: T), in order, into
+ * rows 0 .. n-1 of k_out and v_out, [batch][T][num_kv_heads][head_dim] views as
+ * above.  Other rows, and those whose table entry is outside [0, num_blocks),
+ * are left as they were. */
+int b2_paged_kv4_read(const b2_paged_kv4* kv, b2_kv_view k_out, b2_kv_view v_out, const int* counts, int batch,
+                      int64_t T, int num_kv_heads, int head_dim, void* stream);
+
+/* Channel-wise bounds of the keys of each block, for the choice below: codes is
+ * int8 [num_blocks][num_kv_heads][2][head_dim] (lower bounds, upper ones; 16-byte
+ * aligned), scale float [num_blocks][num_kv_heads], a power of two: code *
+ * scale bounds every key that the block holds (as a 32-bit number).  Written
+ * for the blocks that the last newest[b] positions of each sequence lie in
+ * (device int32 [batch]; NULL: all its blocks), over all rows below seq_lens[b].
+ * A block that holds a NaN or an infinity gets codes 0 and an infinite scale.
+ * Blocks shared by sequences have to be full in all of them.  One launch;
+ * allocates nothing. */
+int b2_paged_block_bounds(const b2_paged_kv* kv, const int* newest, void* codes, float* scale, int batch,
+                          int num_kv_heads, int head_dim, void* stream);
+int b2_paged_kv4_block_bounds(const b2_paged_kv4* kv, const int* newest, void* codes, float* scale, int batch,
+                              int num_kv_heads, int head_dim, void* stream);
+
+/* The n blocks of each sequence that a new token looks at, per kv head: the
+ * first `first`, the last `last` (first + last <= n) and, of those between, the
+ * ones with the largest score (equal scores: the lowest block).  blocks (int32
+ * [batch][num_kv_heads][n]) receives indexes into the sequence's row of the
+ * block tables, ascending, -1 past the last; all blocks when there are at most
+ * n.  q as in b2_paged_decode_gqa (no alignment needed), bf16 its type.
+ *
+ * score = float(sum_d hi_d P_d + lo_d N_d) * scale over the bounds' codes,
+ * where P_d and N_d are the sums of the positive and of the negative q_hd over
+ * the group's heads, rounded (to even) to whole multiples of the least power of
+ * two that 32767 multiples of cover the largest of them: whole numbers, so the
+ * choice does not depend on the order of any sum.  Up to that rounding and a
+ * positive factor it is an upper bound of the sum of the group's logits.  q with
+ * a NaN or an infinity scores 0 everywhere; blocks of infinite scale rank first;
+ * those whose table entry is outside [0, num_blocks) rank last.
+ *
+ * ws needs b2_paged_block_select_workspace_bytes(...) bytes.  One launch;
+ * allocates nothing.  batch and num_kv_heads at most 65535. */
+int b2_paged_block_select(const void* q, int64_t ldq, int bf16, const int* block_tables, const int* seq_lens,
+                          int num_blocks, int block_size, int max_blocks, const void* codes, const float* scale,
+                          int* blocks, int n, int first, int last, int batch, int num_q_heads, int num_kv_heads,
+                          int head_dim, b2_workspace* ws, void* stream);
+size_t b2_paged_block_select_workspace_bytes(int batch, int num_kv_heads, int max_blocks);
+
 /* ---------------------------------------------------------------------------
  * Sampler  (replaces engine::SamplerGPU, src/runtime/sampler.h:10-65)
  * ------------------------------------------------------------------------- */

@@ -89,6 +89,14 @@ _SIGS = {
     "b2_kv4_tile_bytes": (C.c_size_t, [i32]),
     "b2_paged_kv4_decode_gqa": (i32, [vp, i64, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
     "b2_paged_kv4_decode_workspace_bytes": (C.c_size_t, [i32, i32, i32]),
+    "b2_paged_kv_append": (i32, [vp, KVView, KVView, vp, vp, vp, i32, vp, vp, i32, i64, i32, i32, i32, vp]),
+    "b2_paged_kv4_append": (i32, [vp, KVView, KVView, vp, vp, vp, i32, vp, vp, i32, i64, i32, i32, i32, vp]),
+    "b2_paged_kv4_read": (i32, [vp, KVView, KVView, vp, i32, i64, i32, i32, vp]),
+    "b2_paged_block_bounds": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
+    "b2_paged_kv4_block_bounds": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
+    "b2_paged_block_select": (i32, [vp, i64, i32, vp, vp, i32, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
+                                    vp, vp]),
+    "b2_paged_block_select_workspace_bytes": (C.c_size_t, [i32, i32, i32]),
     "b2_paged_kv_evict": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
     "b2_swiglu": (i32, [vp, vp, vp, i64, vp]),
     "b2_matmul_transB": (i32, [vp, vp, vp, i32, i32, i32, vp]),
@@ -435,8 +443,8 @@ class PagedKV4:
 
 def paged_decode_workspace_bytes(batch, nq, nkv, head_dim, max_positions, scored=False) -> int:
     """Enough for paged_decode_gqa over either kind of cache, with or without a list of blocks."""
-    return max(int(lib().b2_paged_decode_workspace_bytes(batch, nq, nkv, head_dim, max_positions, int(scored))),
-               int(lib().b2_paged_kv4_decode_workspace_bytes(nq, nkv, head_dim)))
+    n = int(lib().b2_paged_decode_workspace_bytes(batch, nq, nkv, head_dim, max_positions, int(scored)))
+    return max(n, int(lib().b2_paged_kv4_decode_workspace_bytes(nq, nkv, head_dim))) if n else 0
 
 
 def paged_decode_gqa(q, kv, out, window=0, sinks=0, scores=None, ws: Workspace | None = None, stream=None,
@@ -507,6 +515,163 @@ def paged_kv_evict(kv: PagedKV, scores, budget, kept, new_lens, sinks=0, recent=
         dst = dst_tables.data_ptr()
     call("b2_paged_kv_evict", kv.ref, scores.data_ptr(), dst, mdb, kv.batch, kv.nkv, kv.head_dim, budget,
          _clamp(sinks, _MOST32), _clamp(recent, _MOST32), kept.data_ptr(), new_lens.data_ptr(), _stream_of(stream, dev))
+
+
+class Rope:
+    """Inverse frequencies of a rotary position encoding, on the host: pairs
+    (i, i + rotary_dim / 2) of the first rotary_dim channels (a multiple of 8) turn by
+    position * inv_freq[i], theta ** (-2 i / rotary_dim) where none are given."""
+
+    def __init__(self, rotary_dim, theta=10000.0, inv_freq=None):
+        if rotary_dim <= 0 or rotary_dim % 8 or rotary_dim > 256:
+            raise ValueError(f"rotary_dim must be a multiple of 8 up to 256, got {rotary_dim}")
+        if inv_freq is None:
+            inv_freq = [float(theta) ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+        if len(inv_freq) != rotary_dim // 2:
+            raise ValueError(f"{rotary_dim // 2} inverse frequencies are needed, got {len(inv_freq)}")
+        self.rotary_dim = rotary_dim
+        self.inv_freq = (C.c_double * len(inv_freq))(*[float(f) for f in inv_freq])
+        self.ref = C.addressof(self.inv_freq)
+
+
+def _rows(t, name, B, S, D, dtype, dev):
+    """View of [B, S, heads, D] rows."""
+    if t.dim() != 4 or t.shape[0] != B or t.shape[1] != S or t.shape[3] != D or t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} [{B}, {S}, heads, {D}], got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the cache on cuda:{dev}")
+    b, s, h, d = t.stride()
+    # the stride of a dimension of one may be anything and is never used
+    return KVView(t.data_ptr(), b if B > 1 else 0, h if t.shape[2] > 1 else 0, s if S > 1 else 0, d if D > 1 else 1)
+
+
+def paged_kv_append(kv, k, v, q=None, q_out=None, rope: Rope | None = None, counts=None, positions=None, stream=None):
+    """Rotate the queries and keys of new tokens and write their K and V rows
+    into a PagedKV or PagedKV4.  k and v [B, S, nkv, D], q [B, S, nq, D] and q_out
+    of q's shape (q itself, the default, or another): any strides with contiguous
+    16-byte-aligned rows.  kv.seq_lens already counts the new tokens: the last of
+    them goes to position seq_lens - 1.  counts (int32 [B], optional): how many
+    of a sequence's S rows are new tokens; positions (int32 [B], optional): the
+    position in the encoding of each one's first, where that is not its place in
+    the cache.  Without rope nothing is rotated.  Returns q_out."""
+    dev = _device_of(k, "k")
+    if kv.device != dev:
+        raise ValueError(f"k is on {k.device}, the cache on cuda:{kv.device}")
+    if k.dim() != 4 or k.shape[2] != kv.nkv or v.shape != k.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit a cache of {kv.nkv} heads of {kv.head_dim}")
+    B, S, D = kv.batch, k.shape[1], kv.head_dim
+    kview, vview = _rows(k, "k", B, S, D, kv.dtype, dev), _rows(v, "v", B, S, D, kv.dtype, dev)
+    qr = qor = None
+    nq = 0
+    if q is not None:
+        if q_out is None:
+            q_out = q
+        if q_out.shape != q.shape:
+            raise ValueError(f"q_out {tuple(q_out.shape)} must have q's shape {tuple(q.shape)}")
+        qview, qoview = _rows(q, "q", B, S, D, kv.dtype, dev), _rows(q_out, "q_out", B, S, D, kv.dtype, dev)
+        nq, qr, qor = q.shape[2], C.addressof(qview), C.addressof(qoview)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    cp = pp = None
+    if counts is not None:
+        _need(counts, "counts", _torch().int32, (B,), dev)
+        cp = counts.data_ptr()
+    if positions is not None:
+        _need(positions, "positions", _torch().int32, (B,), dev)
+        pp = positions.data_ptr()
+    call("b2_paged_kv4_append" if isinstance(kv, PagedKV4) else "b2_paged_kv_append", kv.ref, kview, vview, qr, qor,
+         rope.ref if rope is not None else None, rope.rotary_dim if rope is not None else 0, cp, pp, B, S, nq, kv.nkv, D,
+         _stream_of(stream, dev))
+    return q_out
+
+
+def paged_kv_read(kv: PagedKV4, k_out, v_out, counts=None, stream=None):
+    """The newest rows of each sequence of a PagedKV4 as 16-bit rows: its last
+    min(counts, T, length) positions, in order, into k_out and v_out [B, T, nkv, D]
+    (any strides with contiguous 16-byte-aligned rows; other rows are left as they
+    were)."""
+    if not isinstance(kv, PagedKV4):
+        raise ValueError("only a cache held in 4 bits is read back: a PagedKV's rows are its tensors")
+    dev = _device_of(k_out, "k_out")
+    if kv.device != dev:
+        raise ValueError(f"k_out is on {k_out.device}, the cache on cuda:{kv.device}")
+    if k_out.dim() != 4 or k_out.shape[2] != kv.nkv or v_out.shape != k_out.shape:
+        raise ValueError(f"k_out {tuple(k_out.shape)} and v_out {tuple(v_out.shape)} do not fit a cache of {kv.nkv} heads "
+                         f"of {kv.head_dim}")
+    B, T, D = kv.batch, k_out.shape[1], kv.head_dim
+    kview, vview = _rows(k_out, "k_out", B, T, D, kv.dtype, dev), _rows(v_out, "v_out", B, T, D, kv.dtype, dev)
+    cp = None
+    if counts is not None:
+        _need(counts, "counts", _torch().int32, (B,), dev)
+        cp = counts.data_ptr()
+    call("b2_paged_kv4_read", kv.ref, kview, vview, cp, B, T, kv.nkv, D, _stream_of(stream, dev))
+
+
+class BlockBounds:
+    """Bounds of the keys of every block of a paged cache, in 8 bits: codes int8
+    [num_blocks, nkv, 2, D] (lower, upper) times scale float32 [num_blocks, nkv].
+    Made on the current GPU, or over the caller's tensors."""
+
+    def __init__(self, num_blocks=None, nkv=None, head_dim=None, codes=None, scale=None):
+        torch = _torch()
+        if codes is None:
+            codes = torch.zeros(num_blocks, nkv, 2, head_dim, dtype=torch.int8, device="cuda")
+            scale = torch.ones(num_blocks, nkv, dtype=torch.float32, device="cuda")
+        self.device = codes.get_device()
+        if codes.dim() != 4 or codes.shape[2] != 2:
+            raise ValueError(f"codes must be [num_blocks, nkv, 2, head_dim], got {tuple(codes.shape)}")
+        _need(codes, "codes", torch.int8, codes.shape, self.device)
+        _need(scale, "scale", torch.float32, codes.shape[:2], self.device)
+        self.codes, self.scale = codes, scale
+
+    def _fit(self, kv, dev):
+        if self.device != dev or kv.device != dev:
+            raise ValueError("the bounds, the cache and q must be on the current GPU")
+        if self.codes.shape != (kv.num_blocks, kv.nkv, 2, kv.head_dim):
+            raise ValueError(f"bounds {tuple(self.codes.shape)} do not fit the cache ({kv.num_blocks} blocks, {kv.nkv} heads "
+                             f"of {kv.head_dim})")
+
+
+def paged_block_bounds(kv, bounds: BlockBounds, newest=None, stream=None):
+    """Bring the bounds of a PagedKV's or PagedKV4's blocks up to date: of those
+    that the last newest[b] positions of each sequence lie in (int32 [B];
+    default: all its blocks)."""
+    dev = _device_of(bounds.codes, "codes")
+    bounds._fit(kv, dev)
+    np_ = None
+    if newest is not None:
+        _need(newest, "newest", _torch().int32, (kv.batch,), dev)
+        np_ = newest.data_ptr()
+    call("b2_paged_kv4_block_bounds" if isinstance(kv, PagedKV4) else "b2_paged_block_bounds", kv.ref, np_,
+         bounds.codes.data_ptr(), bounds.scale.data_ptr(), kv.batch, kv.nkv, kv.head_dim, _stream_of(stream, dev))
+
+
+def paged_block_select_workspace_bytes(batch, nkv, max_blocks) -> int:
+    return int(lib().b2_paged_block_select_workspace_bytes(batch, nkv, max_blocks))
+
+
+def paged_block_select(q, kv, bounds: BlockBounds, blocks, first=1, last=1, ws: Workspace | None = None, stream=None):
+    """Choose the blocks that one new token per sequence looks at: blocks int32
+    [B, nkv, n] receives, per K/V head, the first `first`, the last `last` and the
+    best-scored of those between, ascending, -1 past the last.  q [B, nq, D] as
+    in paged_decode_gqa, whose `blocks` this fills."""
+    B, nq, D = q.shape
+    ldq, sh, sd = q.stride()
+    if B == 1:
+        ldq = nq * D
+    if B != kv.batch or D != kv.head_dim or q.dtype != kv.dtype or sd != 1 or (sh != D and nq != 1):
+        raise ValueError(f"q {q.dtype} {tuple(q.shape)} does not fit the cache ({kv.batch} sequences, "
+                         f"head_dim {kv.head_dim}, {kv.dtype})")
+    dev = _device_of(q, "q")
+    bounds._fit(kv, dev)
+    if ws is not None and ws.device != dev:
+        raise ValueError(f"q is on {q.device}, the workspace on cuda:{ws.device}")
+    n = blocks.shape[-1]
+    _need(blocks, "blocks", _torch().int32, (B, kv.nkv, n), dev)
+    call("b2_paged_block_select", q.data_ptr(), ldq, _is_bf16(q), kv.block_tables.data_ptr(), kv.seq_lens.data_ptr(),
+         kv.num_blocks, kv.block_size, kv.block_tables.shape[1], bounds.codes.data_ptr(), bounds.scale.data_ptr(),
+         blocks.data_ptr(), n, first, last, B, nq, kv.nkv, D, ws.h if ws is not None else None, _stream_of(stream, dev))
+    return blocks
 
 
 class Sampler:
