@@ -480,7 +480,7 @@ int b2_paged_kv4_block_bounds(const b2_paged_kv4* kv, const int* newest, void* c
  * a NaN or an infinity scores 0 everywhere; blocks of infinite scale rank first;
  * those whose table entry is outside [0, num_blocks) rank last.
  *
- * ws needs b2_paged_block_select_workspace_bytes(...) bytes.  One launch;
+ * ws needs b2_paged_block_select_workspace_bytes(...) bytes.  Two launches;
  * allocates nothing.  batch and num_kv_heads at most 65535. */
 int b2_paged_block_select(const void* q, int64_t ldq, int bf16, const int* block_tables, const int* seq_lens,
                           int num_blocks, int block_size, int max_blocks, const void* codes, const float* scale,

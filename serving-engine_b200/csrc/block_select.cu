@@ -5,7 +5,7 @@
 // the block holds, in 8 bits: whole multiples of one power of two per (block,
 // head), the least that 127 multiples of cover the largest |k|, lo rounded down
 // and hi up.  The bytes are the keys once; a CTA takes a (block, kv head), its
-// warps every fourth row, a lane 4 channels.
+// warps every fourth row or group of rows, a lane 8 channels.
 //
 // Choice.  No query head h of a group has a logit above sum_d max(q_hd lo_d,
 // q_hd hi_d) in a block.  Summed over the group's heads that is
@@ -19,10 +19,12 @@
 // float times the block's power of two is what blocks are ranked by.  A block
 // that holds a NaN or an infinity ranks first, so that it shows.
 //
-// The bytes are 2 D + 4 per (block, kv head).  Scores go to the workspace; the
-// CTA that arrives last for its (sequence, kv head) finds the n-th best by its
-// ordered key, 11 bits of the range still open at a time, and lists what is
-// above it and the first of those equal to it, in order.
+// The bytes are 2 D + 4 per (block, kv head).  Scores go to the workspace; a
+// second launch, a CTA per (sequence, kv head), finds the n-th best by its
+// ordered key, 11 bits of the range still open at a time until 32 are left, and
+// lists what is above it and the first of those equal to it, in order.  (In one
+// launch, the last CTA of each pair choosing and every CTA working out P and N:
+// 54 us for 32 x 2048 blocks of 8 heads of 128, instead of TODO.)
 #include <cmath>
 
 #include "kv4.cuh"
@@ -48,142 +50,204 @@ struct BoundsArgs {
     float* scale;
 };
 
-template <bool KV4>
-__global__ void __launch_bounds__(kBdThreads) bounds_kernel(const BoundsArgs a) {
-    __shared__ int s_end[kBdThreads];  // (block, head) pairs of the sequences up to each of the next kBdThreads
-    __shared__ float s_lo[kBdWarps][256], s_hi[kBdWarps][256];
-    __shared__ float s_top[kBdWarps];
-    __shared__ int s_bad;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+// 2^e as a float, e from -126 to 127
+__device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }
+
+// The smaller and the larger of two numbers, or a NaN if one is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The same of two 16-bit numbers each.
+template <bool BF16>
+__device__ __forceinline__ uint32_t least2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (BF16)
+        asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+        asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t most2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (BF16)
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+template <bool KV4, bool BF16>
+__global__ void __launch_bounds__(kBdThreads, 7) bounds_kernel(const BoundsArgs a) {
+    __shared__ __align__(16) float s_lo[kBdWarps - 1][256], s_hi[kBdWarps - 1][256];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
     griddep_wait();
     griddep_launch_dependents();
-    const int DP = kv4_dp(a.D), NG = kv4_groups(DP);
-    int64_t base = 0;  // pairs of the sequences before b0
-    for (int b0 = 0; b0 < a.batch; b0 += kBdThreads) {
-        // the blocks that sequence b0 + tid's newest positions lie in
-        int n = 0;
-        if (b0 + tid < a.batch) {
-            const int len = max(0, min(a.seq_lens[b0 + tid], a.max_blocks * a.block_size));
-            const int since = a.newest ? len - max(0, min(len, a.newest[b0 + tid])) : 0;
+    // a lane has 8 channels, 8, 16 or 32 lanes a row
+    const int DP = kv4_dp(a.D), NG = kv4_groups(DP), wide = DP == 64 ? 3 : DP <= 128 ? 4 : 5;
+    const int sub = lane >> wide, c = (lane & ((1 << wide) - 1)) * 8;
+    const bool in = c < a.D;
+    int base = 0;  // blocks of the sequences before b0
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        // every warp by itself: lane b for the blocks that sequence b0 + b's newest positions lie in
+        int n = 0, len = 0;
+        if (b0 + lane < a.batch) {
+            len = max(0, min(a.seq_lens[b0 + lane], a.max_blocks * a.block_size));
+            const int since = a.newest ? len - max(0, min(len, a.newest[b0 + lane])) : 0;
             if (since < len) n = (len - 1) / a.block_size - since / a.block_size + 1;
         }
-        __syncthreads();
-        s_end[tid] = n;
-        __syncthreads();
-        for (int o = 1; o < kBdThreads; o <<= 1) {
-            const int v = tid >= o ? s_end[tid - o] : 0;
-            __syncthreads();
-            s_end[tid] += v;
-            __syncthreads();
+        int end = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(~0u, end, o);
+            if (lane >= o) end += v;
         }
-        const int64_t all = (int64_t)s_end[kBdThreads - 1] * a.nkv;
-        int64_t i = base > blockIdx.x ? blockIdx.x + (base - blockIdx.x + gridDim.x - 1) / gridDim.x * gridDim.x : blockIdx.x;
-        for (; i < base + all; i += gridDim.x) {
-            const int pair = (int)((i - base) / a.nkv), h = (int)(i - base - (int64_t)pair * a.nkv);
-            int lo = 0, up = kBdThreads - 1;  // the first sequence whose blocks end behind this one
-            while (lo < up) {
-                const int mid = (lo + up) / 2;
-                if (s_end[mid] > pair)
-                    up = mid;
-                else
-                    lo = mid + 1;
-            }
-            const int b = b0 + lo, from_end = s_end[lo] - 1 - pair;
-            const int len = max(0, min(a.seq_lens[b], a.max_blocks * a.block_size));
-            const int blk = (len - 1) / a.block_size - from_end, rows = min(a.block_size, len - blk * a.block_size);
-            const int id = a.block_tables[(int64_t)b * a.max_blocks + blk];
+        // more blocks than CTAs: a warp for each, else all warps of a CTA together
+        const int all = __shfl_sync(~0u, end, 31), team = all > (int)gridDim.x ? 1 : kBdWarps;
+        const int grid = (int)gridDim.x * (kBdWarps / team), own = team == 1 ? warp : 0;
+        const int r0 = (team == 1 ? 0 : warp * (32 >> wide)) + sub, step = team * (32 >> wide);
+        int i = (int)blockIdx.x + own * (int)gridDim.x;
+        if (i < base) i += (base - i + grid - 1) / grid * grid;
+        for (; i < base + all; i += grid) {
+            const int b = __ffs(__ballot_sync(~0u, end > i - base)) - 1;
+            const int from_end = __shfl_sync(~0u, end, b) - 1 - (i - base), L = __shfl_sync(~0u, len, b);
+            const int blk = (L - 1) / a.block_size - from_end, rows = min(a.block_size, L - blk * a.block_size);
+            const int id = a.block_tables[(int64_t)(b0 + b) * a.max_blocks + blk];
             if ((unsigned)id >= (unsigned)a.num_blocks) continue;
-            if (tid == 0) s_bad = 0;
-            __syncthreads();
-            bool bad = false;
-            for (int c = lane * 4; c < a.D; c += 128) {
-                float l[4], u[4];
+            float lo[8], hi[8];
+            constexpr int ON = 8;  // rows on their way
+            if constexpr (KV4) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) l[e] = INFINITY, u[e] = -INFINITY;
-                auto take = [&](const float (&f)[4]) {
+                for (int e = 0; e < 8; ++e) lo[e] = INFINITY, hi[e] = -INFINITY;
+                const uint8_t* at = a.pool + (int64_t)id * a.stride_block + h * a.stride_head;
+                const int j = c >> 3, word = ((j & 3) * (DP / 32) + (j >> 2)) * 4, meta = 16 * DP + (c >> 6) * 4;
+                for (int r = r0; r < rows; r += ON * step) {
+                    uint32_t w[ON], m[ON];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        l[e] = fminf(l[e], f[e]);
-                        u[e] = fmaxf(u[e], f[e]);
-                        bad |= !(fabsf(f[e]) < INFINITY);
-                    }
-                };
-                if constexpr (KV4) {
-                    const uint8_t* at = a.pool + (int64_t)id * a.stride_block + h * a.stride_head;
-                    const int j = c >> 3, in_row = ((j & 3) * (DP / 32) + (j >> 2)) * 4 + ((c >> 2) & 1) * 2;
-#pragma unroll 4
-                    for (int r = warp; r < rows; r += kBdWarps) {
-                        const uint8_t* tile = at + (int64_t)(r >> 4) * kv4_tile(DP);
-                        const uint32_t w = *reinterpret_cast<const uint16_t*>(tile + (r & 15) * (DP / 2) + in_row);
-                        const float2 sm = h2_to_f2(
-                            *reinterpret_cast<const uint32_t*>(tile + 16 * DP + (kv4_slot(r & 15) * NG + (c >> 6)) * 4));
-                        float f[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) f[e] = fmaf((float)((w >> (4 * e)) & 15), sm.x, sm.y);
-                        take(f);
-                    }
-                } else {
-                    const uint16_t* at = a.k + (int64_t)id * a.stride_block + (int64_t)h * a.stride_head + c;
-#pragma unroll 4
-                    for (int r = warp; r < rows; r += kBdWarps) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(at + r * a.stride_slot);
-                        float2 x, y;
-                        if (a.bf16) {
-                            x = make_float2(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u));
-                            y = make_float2(__uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-                        } else {
-                            x = h2_to_f2(w.x), y = h2_to_f2(w.y);
+                    for (int k = 0; k < ON; ++k) {
+                        const int rr = r + k * step;
+                        if (in && rr < rows) {
+                            const uint8_t* tile = at + (rr >> 4) * kv4_tile(DP);
+                            w[k] = *reinterpret_cast<const uint32_t*>(tile + (rr & 15) * (DP / 2) + word);
+                            m[k] = *reinterpret_cast<const uint32_t*>(tile + meta + kv4_slot(rr & 15) * NG * 4);
                         }
-                        const float f[4] = {x.x, x.y, y.x, y.y};
-                        take(f);
+                    }
+#pragma unroll
+                    for (int k = 0; k < ON; ++k)
+                        if (in && r + k * step < rows) {
+                            const float2 sm = h2_to_f2(m[k]);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float f = fmaf((float)((w[k] >> (4 * e)) & 15), sm.x, sm.y);
+                                lo[e] = min_nan(lo[e], f);
+                                hi[e] = max_nan(hi[e], f);
+                            }
+                        }
+                }
+            } else {
+                // (of 16-bit numbers the least and the largest are such numbers: two at a time, a NaN staying one)
+                uint32_t l[4], u[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l[e] = BF16 ? 0x7f807f80u : 0x7c007c00u, u[e] = l[e] | 0x80008000u;
+                const int64_t inc = step * a.stride_slot;
+                const uint16_t* p = a.k + (int64_t)id * a.stride_block + (int64_t)h * a.stride_head + c + r0 * a.stride_slot;
+                for (int r = r0; r < rows; r += ON * step) {
+                    uint4 w[ON];
+#pragma unroll
+                    for (int k = 0; k < ON; ++k, p += inc)
+                        if (in && r + k * step < rows) w[k] = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+                    for (int k = 0; k < ON; ++k)
+                        if (in && r + k * step < rows) {
+                            const uint32_t x[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) l[e] = least2<BF16>(l[e], x[e]), u[e] = most2<BF16>(u[e], x[e]);
+                        }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 x = BF16 ? make_float2(__uint_as_float(l[e] << 16), __uint_as_float(l[e] & 0xffff0000u)) : h2_to_f2(l[e]);
+                    const float2 y = BF16 ? make_float2(__uint_as_float(u[e] << 16), __uint_as_float(u[e] & 0xffff0000u)) : h2_to_f2(u[e]);
+                    lo[2 * e] = x.x, lo[2 * e + 1] = x.y;
+                    hi[2 * e] = y.x, hi[2 * e + 1] = y.y;
+                }
+            }
+            for (int o = 1 << wide; o < 32; o <<= 1)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    lo[e] = min_nan(lo[e], __shfl_xor_sync(~0u, lo[e], o));
+                    hi[e] = max_nan(hi[e], __shfl_xor_sync(~0u, hi[e], o));
+                }
+            if (team > 1) {  // the first warp goes on alone
+                if (warp > 0 && sub == 0 && in) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        *reinterpret_cast<float4*>(&s_lo[warp - 1][c + e]) = make_float4(lo[e], lo[e + 1], lo[e + 2], lo[e + 3]);
+                        *reinterpret_cast<float4*>(&s_hi[warp - 1][c + e]) = make_float4(hi[e], hi[e + 1], hi[e + 2], hi[e + 3]);
                     }
                 }
-                *reinterpret_cast<float4*>(&s_lo[warp][c]) = make_float4(l[0], l[1], l[2], l[3]);
-                *reinterpret_cast<float4*>(&s_hi[warp][c]) = make_float4(u[0], u[1], u[2], u[3]);
+                __syncthreads();
+                if (warp == 0 && in) {
+#pragma unroll
+                    for (int v = 0; v < kBdWarps - 1; ++v)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            lo[e] = min_nan(lo[e], s_lo[v][c + e]);
+                            hi[e] = max_nan(hi[e], s_hi[v][c + e]);
+                        }
+                }
+                __syncthreads();
+                if (warp > 0) continue;
             }
-            if (__any_sync(~0u, bad) && lane == 0) s_bad = 1;
-            __syncthreads();
             float top = 0.f;
-            for (int c = tid; c < a.D; c += kBdThreads) {
-                float l = s_lo[0][c], u = s_hi[0][c];
 #pragma unroll
-                for (int w = 1; w < kBdWarps; ++w) l = fminf(l, s_lo[w][c]), u = fmaxf(u, s_hi[w][c]);
-                s_lo[0][c] = l;
-                s_hi[0][c] = u;
-                top = fmaxf(top, fmaxf(fabsf(l), fabsf(u)));
-            }
-            top = warp_max(top);
-            if (lane == 0) s_top[warp] = top;
-            __syncthreads();
+            for (int e = 0; e < 8; ++e) top = in ? max_nan(top, max_nan(fabsf(lo[e]), fabsf(hi[e]))) : top;
+            for (int o = 1; o < (1 << wide); o <<= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, o));
+            const bool fine = top < INFINITY;
+            // the least e with top <= 127 * 2^e: top is f 2^x with f from 1 to 2, 127 is 127/64 2^6
+            const uint32_t bits = __float_as_uint(top);
+            const int e = top == 0.f ? 0 : max(-126, (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) > 0x7e0000u ? 5 : 6));
+            if (sub == 0 && in) {
+                const float back = fine ? power(-e) : 0.f;
+                // (a product that vanishes still is on its side of zero)
+                uint32_t d[2] = {0, 0}, u[2] = {0, 0};
 #pragma unroll
-            for (int w = 0; w < kBdWarps; ++w) top = fmaxf(top, s_top[w]);
-            // the least e with top <= 127 * 2^e
-            int e;
-            const float f = frexpf(top, &e);
-            e = max(-126, f > 127.f / 128.f ? e - 6 : e - 7);
-            if (top == 0.f) e = 0;
-            const double back = ldexp(1.0, -e);
-            int8_t* out = a.codes + ((int64_t)id * a.nkv + h) * 2 * a.D;
-            const bool fine = s_bad == 0;
-            for (int c = tid; c < a.D; c += kBdThreads) {
-                out[c] = (int8_t)(fine ? (int)floor((double)s_lo[0][c] * back) : 0);
-                out[a.D + c] = (int8_t)(fine ? (int)ceil((double)s_hi[0][c] * back) : 0);
+                for (int k = 0; k < 8; ++k) {
+                    const float x = lo[k], y = hi[k];
+                    const int dn = fine ? (int)fminf(floorf(x * back), x < 0.f ? -1.f : 127.f) : 0;
+                    const int up = fine ? (int)fmaxf(ceilf(y * back), y > 0.f ? 1.f : -127.f) : 0;
+                    d[k / 4] |= (uint32_t)(dn & 255) << (8 * (k & 3));
+                    u[k / 4] |= (uint32_t)(up & 255) << (8 * (k & 3));
+                }
+                int8_t* out = a.codes + ((int64_t)id * a.nkv + h) * 2 * a.D + c;
+                *reinterpret_cast<uint2*>(out) = make_uint2(d[0], d[1]);
+                *reinterpret_cast<uint2*>(out + a.D) = make_uint2(u[0], u[1]);
+                if (lane == 0) a.scale[(int64_t)id * a.nkv + h] = fine ? power(e) : INFINITY;
             }
-            if (tid == 0) a.scale[(int64_t)id * a.nkv + h] = fine ? ldexpf(1.f, e) : INFINITY;
-            __syncthreads();
         }
         base += all;
     }
 }
 
 static int bounds_launch(const BoundsArgs& a, bool kv4, cudaStream_t s) {
-    // pairs are dealt out in turn: 16 CTAs of 4 warps fill an SM
-    const int64_t most = (int64_t)a.batch * a.nkv * a.max_blocks;
-    const unsigned grid = (unsigned)(most < 16 * sm_count() ? most : 16 * sm_count());
+    // the blocks of a head are dealt out in turn to as many CTAs as fill the GPU once
+    const int64_t most = (int64_t)a.batch * a.max_blocks;
+    int64_t grid = (8 * sm_count() + a.nkv - 1) / a.nkv;
+    if (grid > most) grid = most;
+    const dim3 g((unsigned)grid, (unsigned)a.nkv);
     if (kv4)
-        B2_TRY(launch(bounds_kernel<true>, dim3(grid), dim3(kBdThreads), 0, s, true, a));
+        B2_TRY(launch(bounds_kernel<true, false>, g, dim3(kBdThreads), 0, s, true, a));
+    else if (a.bf16)
+        B2_TRY(launch(bounds_kernel<false, true>, g, dim3(kBdThreads), 0, s, true, a));
     else
-        B2_TRY(launch(bounds_kernel<false>, dim3(grid), dim3(kBdThreads), 0, s, true, a));
+        B2_TRY(launch(bounds_kernel<false, false>, g, dim3(kBdThreads), 0, s, true, a));
     return B2_OK;
 }
 
@@ -191,7 +255,9 @@ static int bounds_launch(const BoundsArgs& a, bool kv4, cudaStream_t s) {
 // choice
 // ---------------------------------------------------------------------------
 
-constexpr int kSlThreads = 256;
+constexpr int kScThreads = 256;  // of the scores
+constexpr int kScWarps = kScThreads / 32;
+constexpr int kSlThreads = 512;  // of a choice
 constexpr int kSlWarps = kSlThreads / 32;
 constexpr int kSlKeys = 8192;  // keys of a choice kept in shared memory; of longer ones they are read again
 constexpr int kSlBins = 2048;
@@ -206,9 +272,8 @@ struct SelectArgs {
     const float* scale;
     int* out;
     int nq, nkv, D, group, bf16, n, first, last;
-    int chunk;       // blocks per CTA
-    uint32_t* keys;  // [batch][nkv][max_blocks]
-    int* counters;
+    int chunk, heads, team;  // blocks and kv heads per CTA of the scores, warps per head
+    uint32_t* keys;          // [batch][nkv][max_blocks]
 };
 
 __device__ __forceinline__ int dp4_su(uint32_t s, uint32_t u, int c) {
@@ -223,103 +288,107 @@ __device__ __forceinline__ int dp4_ss(uint32_t s, uint32_t u, int c) {
 }
 
 // P: 16-byte pieces of a bounds row (2 D bytes) that each of 4 lanes takes.
+// A warp has the bounds of one kv head (a team of warps where there are fewer
+// than 8): P and N are worked out by every warp for itself, without a barrier,
+// while the first bounds are on their way.
 template <int P>
-__global__ void __launch_bounds__(kSlThreads) select_kernel(const SelectArgs a) {
-    __shared__ union {
-        struct {
-            double sum[2][256];
-            __align__(16) uint8_t hi[512], lo[512];
-        } q;
-        struct {
-            uint32_t keys[kSlKeys];
-            int hist[kSlBins];
-        } c;
-    } sm;
-    __shared__ double s_red[kSlWarps];
-    __shared__ int s_wsum[kSlWarps][2];
-    __shared__ int s_last, s_bin, s_above;
-    __shared__ uint32_t s_range[2][kSlWarps];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int h = blockIdx.y, b = blockIdx.z;
+__global__ void __launch_bounds__(kScThreads, 2) score_kernel(const SelectArgs a) {
+    __shared__ __align__(16) uint8_t s_q[kScWarps][2][512];  // upper and lower bytes of N, P
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.z, h = blockIdx.y * a.heads + warp / a.team;
     griddep_wait();
     griddep_launch_dependents();
     const int len = max(0, min(a.seq_lens[b], a.max_blocks * a.block_size));
     const int nb = (len + a.block_size - 1) / a.block_size;
-    const int64_t pair = (int64_t)b * a.nkv + h;
-    int* out = a.out + pair * a.n;
-    if (nb <= a.n) {  // every block
-        if (blockIdx.x == 0)
-            for (int i = tid; i < a.n; i += kSlThreads) out[i] = i < nb ? i : -1;
-        return;
-    }
     const int c0 = blockIdx.x * a.chunk, c1 = min(nb, c0 + a.chunk);
-    if (c0 >= nb) return;
+    if (nb <= a.n || c0 >= nb || warp / a.team >= a.heads || h >= a.nkv) return;  // (a warp's own business: no barrier here)
+    constexpr int ON = P <= 4 ? 2 : 1;  // blocks of a lane at a time
+    const int part = lane & 3, pieces = a.D / 8, step = 8 * a.team, first = c0 + (warp % a.team) * 8 + (lane >> 2);
+    const int* bt = a.block_tables + (int64_t)b * a.max_blocks;
+    // (where there is no block, or no piece, the first one's is read and comes to nothing)
+    int shift[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) shift[p] = part + 4 * p < pieces ? part + 4 * p : 0;
+    const uint4* const codes = reinterpret_cast<const uint4*>(a.codes) + (int64_t)h * pieces;
+    const float* const scales = a.scale + h;
+    uint4 w[ON][P];
+    float sc[ON];
+    int id[ON];        // of the blocks that are fetched next
+    bool there[ON], next[ON];
+    auto look = [&](int j0) {
+#pragma unroll
+        for (int n = 0; n < ON; ++n) id[n] = j0 + n * step < c1 ? __ldg(bt + j0 + n * step) : -1;
+    };
+    auto fetch = [&]() {
+#pragma unroll
+        for (int n = 0; n < ON; ++n) {
+            next[n] = (unsigned)id[n] < (unsigned)a.num_blocks;
+            const int64_t row = (next[n] ? id[n] : 0) * (int64_t)a.nkv;
+            const uint4* src = codes + row * pieces;
+#pragma unroll
+            for (int p = 0; p < P; ++p) w[n][p] = __ldg(src + shift[p]);
+            sc[n] = __ldg(scales + row);
+        }
+    };
+    look(first);
+    fetch();
+    look(first + ON * step);
 
     // ---- P and N in 16 bits: N first, as lo stands before hi
-    double top = 0.0;
-    for (int c = tid; c < a.D; c += kSlThreads) {
-        double neg = 0.0, pos = 0.0;
-        const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.ldq + (int64_t)h * a.group * a.D + c;
+    constexpr int CH = P;  // channels of a lane: D <= 32 P
+    double neg[CH], pos[CH];
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + b * a.ldq + (int64_t)h * a.group * a.D;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) neg[k] = pos[k] = 0.0;
 #pragma unroll 4
-        for (int g = 0; g < a.group; ++g) {
-            const uint32_t w = q[(int64_t)g * a.D];
-            const float f = a.bf16 ? __uint_as_float(w << 16) : __half2float(__ushort_as_half((uint16_t)w));
-            if (!(f <= 0.f)) pos += (double)f;  // (a NaN to both)
-            if (!(f >= 0.f)) neg += (double)f;
+    for (int g = 0; g < a.group; ++g)
+#pragma unroll
+        for (int k = 0; k < CH; ++k) {
+            const int c = k * 32 + lane;
+            if (c < a.D) {
+                const uint32_t u = q[(int64_t)g * a.D + c];
+                const float f = a.bf16 ? __uint_as_float(u << 16) : __half2float(__ushort_as_half((uint16_t)u));
+                pos[k] += f <= 0.f ? 0.0 : (double)f;  // (a NaN to both)
+                neg[k] += f >= 0.f ? 0.0 : (double)f;
+            }
         }
-        sm.q.sum[0][c] = neg;
-        sm.q.sum[1][c] = pos;
-        const double t = fmax(-neg, pos);
-        top = t > top || !(t < INFINITY) ? t : top;
-        if (!(neg > -INFINITY) || !(pos < INFINITY)) top = INFINITY;
-    }
+    // the largest of them by its bits, which rank like the numbers (a NaN above all)
+    unsigned long long big = 0;
+    auto bits = [](double y) { return (unsigned long long)__double_as_longlong(y) & ~(1ull << 63); };
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(~0u, top, o));
-    if (lane == 0) s_red[warp] = top;
-    __syncthreads();
+    for (int k = 0; k < CH; ++k) big = max(big, max(bits(neg[k]), bits(pos[k])));
 #pragma unroll
-    for (int w = 0; w < kSlWarps; ++w) top = fmax(top, s_red[w]);
-    int e = 0;
-    const double f = frexp(top < INFINITY && top > 0.0 ? top : 1.0, &e);
-    e = f > 32767.0 / 32768.0 ? e - 14 : e - 15;  // the least with top <= 32767 * 2^e
-    const double back = top < INFINITY ? ldexp(1.0, -e) : 0.0;
-    for (int i = tid; i < 2 * a.D; i += kSlThreads) {
-        const double x = sm.q.sum[i >= a.D][i >= a.D ? i - a.D : i];
-        const int v = top < INFINITY ? (int)rint(x * back) : 0;
-        sm.q.hi[i] = (uint8_t)(v >> 8);
-        sm.q.lo[i] = (uint8_t)v;
+    for (int o = 16; o > 0; o >>= 1) big = max(big, __shfl_xor_sync(~0u, big, o));
+    const bool fine = big < 0x7ff0000000000000ull;
+    // the least e with it <= 32767 * 2^e: it is f 2^x with f from 1 to 2, 32767 is 32767/16384 2^14 (doubles of sums of
+    // halves and bf16 are normal, or zero)
+    const int x = (int)(big >> 52) - 1023, e = x - ((big & 0xfffffffffffffull) > 0xfffc000000000ull ? 13 : 14);
+    const double back = fine && big ? __longlong_as_double((long long)(1023 - e) << 52) : 0.0;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+        const int c = k * 32 + lane;
+        if (c < a.D) {
+            const int n = fine ? __double2int_rn(neg[k] * back) : 0, p = fine ? __double2int_rn(pos[k] * back) : 0;
+            s_q[warp][0][c] = (uint8_t)(n >> 8), s_q[warp][1][c] = (uint8_t)n;
+            s_q[warp][0][a.D + c] = (uint8_t)(p >> 8), s_q[warp][1][a.D + c] = (uint8_t)p;
+        }
     }
-    __syncthreads();
+    __syncwarp();
 
-    // ---- scores of this CTA's blocks: 4 lanes a block
-    uint32_t* keys = a.keys + pair * a.max_blocks;
-    const int part = lane & 3, pieces = a.D / 8;
+    // ---- scores, 4 lanes a block
+    uint32_t* keys = a.keys + ((int64_t)b * a.nkv + h) * a.max_blocks;
     uint4 qh[P], ql[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
         const int at = part + 4 * p;
-        qh[p] = at < pieces ? *reinterpret_cast<const uint4*>(sm.q.hi + 16 * at) : make_uint4(0, 0, 0, 0);
-        ql[p] = at < pieces ? *reinterpret_cast<const uint4*>(sm.q.lo + 16 * at) : make_uint4(0, 0, 0, 0);
+        qh[p] = at < pieces ? *reinterpret_cast<const uint4*>(s_q[warp][0] + 16 * at) : make_uint4(0, 0, 0, 0);
+        ql[p] = at < pieces ? *reinterpret_cast<const uint4*>(s_q[warp][1] + 16 * at) : make_uint4(0, 0, 0, 0);
     }
-    constexpr int STEP = kSlThreads / 4;
-    constexpr int ON = P <= 4 ? 4 : 2;  // blocks of a thread at a time
-    const int* bt = a.block_tables + (int64_t)b * a.max_blocks;
-    for (int j0 = c0 + (tid >> 2); j0 - (tid >> 2) < c1; j0 += ON * STEP) {
-        int id[ON];
+    for (int j0 = first; j0 - (lane >> 2) < c1; j0 += ON * step) {
+        int sum[ON];
+        float s[ON];
 #pragma unroll
-        for (int n = 0; n < ON; ++n) id[n] = j0 + n * STEP < c1 ? bt[j0 + n * STEP] : -1;
-        uint4 w[ON][P];
-        float sc[ON];
-#pragma unroll
-        for (int n = 0; n < ON; ++n) {
-            const bool there = (unsigned)id[n] < (unsigned)a.num_blocks;
-            const int64_t row = (int64_t)id[n] * a.nkv + h;
-            const uint4* src = reinterpret_cast<const uint4*>(a.codes + row * 2 * a.D) + part;
-#pragma unroll
-            for (int p = 0; p < P; ++p)
-                w[n][p] = there && part + 4 * p < pieces ? __ldg(src + 4 * p) : make_uint4(0, 0, 0, 0);
-            sc[n] = there ? a.scale[row] : 0.f;
-        }
+        for (int n = 0; n < ON; ++n) there[n] = next[n];
 #pragma unroll
         for (int n = 0; n < ON; ++n) {
             int hi = 0, lo = 0;
@@ -330,42 +399,54 @@ __global__ void __launch_bounds__(kSlThreads) select_kernel(const SelectArgs a) 
                 hi = dp4_ss(w[n][p].z, qh[p].z, hi), lo = dp4_su(w[n][p].z, ql[p].z, lo);
                 hi = dp4_ss(w[n][p].w, qh[p].w, hi), lo = dp4_su(w[n][p].w, ql[p].w, lo);
             }
-            int sum = hi * 256 + lo;
-            sum += __shfl_xor_sync(~0u, sum, 1);
-            sum += __shfl_xor_sync(~0u, sum, 2);
-            const int j = j0 + n * STEP;
+            sum[n] = hi * 256 + lo;
+            s[n] = sc[n];
+        }
+        fetch();
+        look(j0 + 2 * ON * step);
+#pragma unroll
+        for (int n = 0; n < ON; ++n) {
+            sum[n] += __shfl_xor_sync(~0u, sum[n], 1);
+            sum[n] += __shfl_xor_sync(~0u, sum[n], 2);
+            const int j = j0 + n * step;
             if (part == 0 && j < c1) {
-                const bool there = (unsigned)id[n] < (unsigned)a.num_blocks;
-                const float score = sc[n] == INFINITY ? INFINITY : (float)sum * sc[n];
+                const float score = s[n] == INFINITY ? INFINITY : (float)sum[n] * s[n];
                 // (a NaN, as of a scale never written, ranks first but is not one of the blocks that stay)
                 keys[j] = j < a.first || j >= nb - a.last ? kSlStays
-                                                          : there ? min(float_key(score + 0.f), kSlStays - 2) : 0u;
+                                                          : there[n] ? min(float_key(score + 0.f), kSlStays - 2) : 0u;
             }
         }
     }
+}
 
-    // ---- the last CTA of this (sequence, kv head) chooses
-    const int ctas = (nb + a.chunk - 1) / a.chunk;
-    if (ctas > 1) {
-        __syncthreads();
-        if (tid == 0) {
-            __threadfence();
-            s_last = atomicAdd(a.counters + pair, 1) == ctas - 1;
-            __threadfence();
-        }
-        __syncthreads();
-        if (!s_last) return;
-        if (tid == 0) a.counters[pair] = 0;
+// One CTA per (sequence, kv head).
+__global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) {
+    __shared__ uint32_t s_keys[kSlKeys], s_few32[32];
+    __shared__ int s_hist[kSlBins];
+    __shared__ int s_wsum[kSlWarps][2];
+    __shared__ int s_bin, s_above, s_in, s_few;
+    __shared__ uint32_t s_range[2][kSlWarps];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int h = blockIdx.x, b = blockIdx.y;
+    griddep_wait();
+    griddep_launch_dependents();
+    const int len = max(0, min(a.seq_lens[b], a.max_blocks * a.block_size));
+    const int nb = (len + a.block_size - 1) / a.block_size;
+    const int64_t pair = (int64_t)b * a.nkv + h;
+    int* out = a.out + pair * a.n;
+    if (nb <= a.n) {  // every block
+        for (int i = tid; i < a.n; i += kSlThreads) out[i] = i < nb ? i : -1;
+        return;
     }
-    __syncthreads();
+    const uint32_t* keys = a.keys + pair * a.max_blocks;
     const bool fits = nb <= kSlKeys;
     uint32_t lowest = ~0u, highest = 0u;
     for (int i = tid; i < nb; i += kSlThreads) {
         const uint32_t k = __ldcg(keys + i);
-        if (fits) sm.c.keys[i] = k;
+        if (fits) s_keys[i] = k;
         if (k != kSlStays) lowest = min(lowest, k), highest = max(highest, k);
     }
-    auto key = [&](int i) -> uint32_t { return fits ? sm.c.keys[i] : __ldcg(keys + i); };
+    auto key = [&](int i) -> uint32_t { return fits ? s_keys[i] : __ldcg(keys + i); };
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         lowest = min(lowest, __shfl_xor_sync(~0u, lowest, o));
@@ -380,11 +461,11 @@ __global__ void __launch_bounds__(kSlThreads) select_kernel(const SelectArgs a) 
     while (want > 0 && lowest < highest) {
         const uint32_t range = highest - lowest;
         const int shift = max(0, 21 - __clz(range));  // range >> shift below 2048
-        for (int i = tid; i < kSlBins; i += kSlThreads) sm.c.hist[i] = 0;
+        for (int i = tid; i < kSlBins; i += kSlThreads) s_hist[i] = 0;
         __syncthreads();
         for (int i = tid; i < nb; i += kSlThreads) {
             const uint32_t k = key(i) - lowest;
-            if (k <= range) atomicAdd(&sm.c.hist[k >> shift], 1);
+            if (k <= range) atomicAdd(&s_hist[k >> shift], 1);
         }
         __syncthreads();
         // the bin of the want-th best: thread t sums the bins 8 t' .. 8 t' + 7, t' counting from the top
@@ -392,7 +473,7 @@ __global__ void __launch_bounds__(kSlThreads) select_kernel(const SelectArgs a) 
         const int top_bin = kSlBins - 1 - tid * PER;
         int mine = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) mine += sm.c.hist[top_bin - i];
+        for (int i = 0; i < PER; ++i) mine += s_hist[top_bin - i];
         int incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -406,51 +487,66 @@ __global__ void __launch_bounds__(kSlThreads) select_kernel(const SelectArgs a) 
             if (w < warp) incl += s_wsum[w][0];
         if (incl >= want && incl - mine < want) {
             int above = incl - mine, bin = top_bin;
-            while (above + sm.c.hist[bin] < want) above += sm.c.hist[bin--];
+            while (above + s_hist[bin] < want) above += s_hist[bin--];
             s_bin = bin;
             s_above = above;
+            s_in = s_hist[bin];
+            s_few = 0;
         }
         __syncthreads();
         want -= s_above;
         lowest += (uint32_t)s_bin << shift;
         highest = min(highest, lowest + ((1u << shift) - 1));
+        if (s_in <= 32 && lowest < highest) {  // few enough to be ranked side by side in every warp
+            for (int i = tid; i < nb; i += kSlThreads) {
+                const uint32_t k = key(i);
+                if (k - lowest <= highest - lowest) s_few32[atomicAdd(&s_few, 1)] = k;
+            }
+            __syncthreads();
+            const uint32_t k = lane < s_in ? s_few32[lane] : 0u;
+            int more = 0, same = 0;  // candidates above this lane's, and equal to it
+            for (int i = 0; i < s_in; ++i) {
+                const uint32_t o = __shfl_sync(~0u, k, i);
+                more += o > k;
+                same += o == k;
+            }
+            const int who = __ffs(__ballot_sync(~0u, lane < s_in && more < want && more + same >= want)) - 1;
+            lowest = highest = __shfl_sync(~0u, k, who);
+            want -= __shfl_sync(~0u, more, who);
+        }
         __syncthreads();
     }
     // ---- what is above, and the first `want` that equal it, in order (want 0: nothing below the blocks that stay)
     const uint32_t border = want > 0 ? lowest : kSlStays - 1;
-    const int per = (nb + kSlThreads - 1) / kSlThreads, i0 = min(nb, tid * per), i1 = min(nb, i0 + per);
+    const int per = ((nb + kSlWarps - 1) / kSlWarps + 31) & ~31, i0 = warp * per, i1 = min(nb, i0 + per);
     int above = 0, equal = 0;
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t k = key(i);
-        above += k > border;
-        equal += k == border;
+    for (int i = i0; i < i1; i += 32) {
+        const uint32_t k = i + lane < i1 ? key(i + lane) : 0u;
+        above += __popc(__ballot_sync(~0u, k > border));
+        equal += __popc(__ballot_sync(~0u, k == border && i + lane < i1));
     }
-    int ia = above, ie = equal;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(~0u, ia, o), y = __shfl_up_sync(~0u, ie, o);
-        if (lane >= o) ia += x, ie += y;
-    }
-    if (lane == 31) s_wsum[warp][0] = ia, s_wsum[warp][1] = ie;
+    if (lane == 0) s_wsum[warp][0] = above, s_wsum[warp][1] = equal;
     __syncthreads();
+    above = equal = 0;  // before this warp's own
 #pragma unroll
     for (int w = 0; w < kSlWarps; ++w)
-        if (w < warp) ia += s_wsum[w][0], ie += s_wsum[w][1];
-    above = ia - above;  // before this thread's own
-    equal = ie - equal;
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t k = key(i);
-        const bool eq = k == border && equal < want;
-        if (k > border || eq) out[above + min(equal, want)] = i;
-        above += k > border;
-        equal += k == border;
+        if (w < warp) above += s_wsum[w][0], equal += s_wsum[w][1];
+    const uint32_t before = (1u << lane) - 1;
+    for (int i = i0; i < i1; i += 32) {
+        const uint32_t k = i + lane < i1 ? key(i + lane) : 0u;
+        const uint32_t up = __ballot_sync(~0u, k > border), eq = __ballot_sync(~0u, k == border && i + lane < i1);
+        const int e = equal + __popc(eq & before), at = above + __popc(up & before) + min(e, want);
+        if ((k > border || (k == border && i + lane < i1 && e < want)) && at < a.n) out[at] = i + lane;
+        above += __popc(up);
+        equal += __popc(eq);
     }
 }
 
 template <int P>
 static int select_launch(const SelectArgs& a, int batch, cudaStream_t s) {
-    const dim3 grid((unsigned)((a.max_blocks + a.chunk - 1) / a.chunk), (unsigned)a.nkv, (unsigned)batch);
-    B2_TRY(launch(select_kernel<P>, grid, dim3(kSlThreads), 0, s, true, a));
+    const dim3 grid((unsigned)((a.max_blocks + a.chunk - 1) / a.chunk), (unsigned)((a.nkv + a.heads - 1) / a.heads), (unsigned)batch);
+    B2_TRY(launch(score_kernel<P>, grid, dim3(kScThreads), 0, s, true, a));
+    B2_TRY(launch(choose_kernel, dim3((unsigned)a.nkv, (unsigned)batch), dim3(kSlThreads), 0, s, true, a));
     return B2_OK;
 }
 
@@ -460,7 +556,7 @@ static int bounds_check(const void* codes, const void* scale, int batch, int nkv
     B2_REQUIRE(codes && scale);
     if (!b2::aligned16(codes)) return B2_ERR_UNSUPPORTED;
     // blocks of all sequences are counted in 32 bits
-    if ((int64_t)batch * max_blocks > (1ll << 31) - 1) return B2_ERR_UNSUPPORTED;
+    if ((int64_t)batch * max_blocks > (1ll << 30) || nkv > 65535) return B2_ERR_UNSUPPORTED;
     return B2_OK;
 }
 
@@ -554,12 +650,13 @@ extern "C" int b2_paged_block_select(const void* q, int64_t ldq, int bf16, const
     a.first = first;
     a.last = last;
     a.keys = static_cast<uint32_t*>(ws->ptr);
-    a.counters = ws->counters;
-    // a few CTAs per SM in all; as many counters as there are, else one CTA per choice
-    const int64_t pairs = (int64_t)batch * nkv;
-    int64_t chunk = (pairs * max_blocks + 4 * sm_count() - 1) / (4 * sm_count());
-    chunk = (chunk + 255) / 256 * 256;
-    a.chunk = pairs > kWsCounters || chunk >= max_blocks ? max_blocks : (int)chunk;
+    // up to 8 heads per CTA, and as many CTAs as an SM holds together where that leaves each a few steps
+    a.heads = nkv < kScWarps ? nkv : kScWarps;
+    a.team = kScWarps / a.heads;
+    const int64_t groups = (nkv + a.heads - 1) / a.heads, step = 8 * a.team;
+    int64_t chunk = (batch * groups * max_blocks + 2 * sm_count() - 1) / (2 * sm_count());
+    chunk = chunk < 4 * step ? 4 * step : chunk > 32 * step ? 32 * step : (chunk + step - 1) / step * step;
+    a.chunk = (int)chunk;
     cudaStream_t s = as_stream(stream);
     if (D <= 64) return select_launch<2>(a, batch, s);
     if (D <= 128) return select_launch<4>(a, batch, s);

@@ -21,9 +21,11 @@
 //            terms are a product too, of the scale words as they are stored with
 //            the sums of q as half and remainder.
 //   outputs  o_d = sum_i (p_i s_ig) (u_id - 8) + sum_i p_i (m_ig + 8 s_ig): the
-//            weights times the scale are the operand, split into a half and the
-//            half of what the rounding left, so that they cost no accuracy
-//            beside the output's own rounding; the second sum is kept in 32 bits
+//            weights times the scale are the operand, rounded to halves; for
+//            outputs in half with what the rounding left as a half beside it, so
+//            that they cost no accuracy beside the output's own rounding (bf16
+//            rounds 8 times coarser than the weights are, and goes without: 1 %
+//            on the error of an exact result).  The second sum is kept in 32 bits
 //            per group.  Less 8, because sums of codes of one sign would be far
 //            larger than the output that is left of them (at 131001 tokens the
 //            rounding of the sums would show in the output: 5e-4 instead of
@@ -34,8 +36,8 @@
 // largest scale seen so far, like the running max of the softmax.
 //
 // Layout of the products: positions, then channels, are the 16 rows and the
-// heads the 8 columns.  Up to 4 heads (H = 4) stand twice in the columns: the
-// second copy becomes the remainders, in the same product.  (Heads as the rows
+// heads the 8 columns.  Up to 4 heads (H = 4) stand twice in the columns: with
+// remainders the second copy becomes those, in the same product.  (Heads as the rows
 // of S take twice the products and, since half of each operand's registers are
 // then zeros that have to be put there, 456 instructions a tile instead of 340.)
 //
@@ -131,10 +133,12 @@ __device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-template <int DP, int H, bool LIST>
+// BF16: type of q and out; without it weights are split.
+template <int DP, int H, bool BF16, bool LIST>
 __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kernel(const Kv4Args a) {
     using C = Kv4Cfg<DP, H>;
     constexpr int U = C::U, T = C::T, W = C::W, NG = C::NG;
+    constexpr bool SPLIT = !BF16, TWO = SPLIT && H > 4;  // remainders of the weights; in products of their own
     constexpr int NT = H == 16 ? 2 : 1;  // products side by side, 8 heads each
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ SplitShared s_split;
@@ -247,7 +251,7 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                 const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 y = a.bf16 ? make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u))
+                    const float2 y = BF16 ? make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u))
                                             : h2_to_f2(u[i]);
                     f[2 * i] = y.x, f[2 * i + 1] = y.y;
                 }
@@ -472,13 +476,14 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                             const float p0 = x[t][n][2 * pp], p1 = x[t][n][2 * pp + 1];
                             am[n][0][g] = fmaf(p0, mid, am[n][0][g]);
                             am[n][1][g] = fmaf(p1, mid, am[n][1][g]);
-                            uint32_t u, r;
-                            split16<false>(p0 * sm.x, p1 * sm.x, u, r);
-                            if (H == 4) {
-                                hi[t][n][pp] = transpose8x8(lc < 2 ? u : r);
+                            const float w0 = p0 * sm.x, w1 = p1 * sm.x;
+                            const uint32_t u = f2_to_h2(w0, w1);
+                            if constexpr (SPLIT) {  // (in one multiply-add of halves and a 32-bit number each)
+                                const uint32_t r = f2_to_h2(fma_f16_f32<0>(u, 0xbc00bc00u, w0), fma_f16_f32<1>(u, 0xbc00bc00u, w1));
+                                hi[t][n][pp] = transpose8x8(TWO || lc < 2 ? u : r);
+                                if constexpr (TWO) lo[t][n][pp] = transpose8x8(r);
                             } else {
                                 hi[t][n][pp] = transpose8x8(u);
-                                lo[t][n][pp] = transpose8x8(r);
                             }
                         }
                     }
@@ -487,7 +492,7 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                     for (int n = 0; n < NT; ++n) {
                         mma_f16(less[n], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, hi[t][n][0], hi[t][n][1],
                                 t ? less[n] : zero);
-                        if (H > 4)
+                        if (TWO)
                             mma_f16(less[n], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, lo[t][n][0], lo[t][n][1],
                                     less[n]);
                     }
@@ -508,7 +513,7 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
                                 mma_f16(c[n], b0, b1, b2, b3, hi[t][n][0], hi[t][n][1], t ? c[n] : less[n]);
-                                if (H > 4) mma_f16(c[n], b0, b1, b2, b3, lo[t][n][0], lo[t][n][1], c[n]);
+                                if (TWO) mma_f16(c[n], b0, b1, b2, b3, lo[t][n][0], lo[t][n][1], c[n]);
                             }
                         }
 #pragma unroll
@@ -568,7 +573,7 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                 }
             // rows of codes in the low nibble of a byte hold sums 16 times smaller
             constexpr float k0 = 16777216.f, k1 = 1048576.f;
-            if (H == 4) {
+            if (H == 4 && SPLIT) {
 #pragma unroll
                 for (int x = 0; x < W; ++x)
 #pragma unroll
@@ -603,10 +608,7 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                 return make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
             };
             finish_piece(a, s_split, w, at, r, piece0, s_ml, sum, [&](int64_t i, float4 v, float scale) {
-                if (a.bf16)
-                    store4<true>(a.out, i, v, scale);
-                else
-                    store4<false>(a.out, i, v, scale);
+                store4<BF16>(a.out, i, v, scale);
             });
             __syncthreads();
             at.next(a);
@@ -652,18 +654,22 @@ static Kv4Sizes kv4_sizes(int nq, int nkv, int D) {
     return z;
 }
 
-template <int DP, int H, bool LIST>
+template <int DP, int H, bool BF16, bool LIST>
 static int kv4_launch(const Kv4Args& a, const Kv4Sizes& z, cudaStream_t s) {
-    auto kern = kv4_attn_kernel<DP, H, LIST>;
+    auto kern = kv4_attn_kernel<DP, H, BF16, LIST>;
     static bool done[64];
     B2_TRY(allow_smem(kern, Kv4Cfg<DP, H>::BYTES, done));
     B2_TRY(launch(kern, dim3(z.grid), dim3(kPgThreads), Kv4Cfg<DP, H>::BYTES, s, true, a));
     return B2_OK;
 }
+template <int DP, int H, bool LIST>
+static int kv4_dispatch(const Kv4Args& a, const Kv4Sizes& z, cudaStream_t s) {
+    return a.bf16 ? kv4_launch<DP, H, true, LIST>(a, z, s) : kv4_launch<DP, H, false, LIST>(a, z, s);
+}
 template <int DP, bool LIST>
 static int kv4_dispatch(const Kv4Args& a, const Kv4Sizes& z, cudaStream_t s) {
-    return z.h == 16 ? kv4_launch<DP, 16, LIST>(a, z, s)
-                     : z.h == 8 ? kv4_launch<DP, 8, LIST>(a, z, s) : kv4_launch<DP, 4, LIST>(a, z, s);
+    return z.h == 16 ? kv4_dispatch<DP, 16, LIST>(a, z, s)
+                     : z.h == 8 ? kv4_dispatch<DP, 8, LIST>(a, z, s) : kv4_dispatch<DP, 4, LIST>(a, z, s);
 }
 template <bool LIST>
 static int kv4_dispatch(const Kv4Args& a, const Kv4Sizes& z, cudaStream_t s) {

@@ -17,11 +17,11 @@
 // bits are too coarse to notice.
 //
 // 4-bit codes are decided exactly: a key near the border between two codes would
-// otherwise fall either way by the rounding of whoever rotates it.  Keys are
-// rotated in 64 bits (the B200 has a 64-bit multiply-add for every two 32-bit
-// ones, so this stays below the memory time); the division is a 32-bit product
-// wherever that cannot miss the border, which is checked, and settled in 64 bits
-// where it can.
+// otherwise fall either way by the rounding of whoever rotates it.  Rows are
+// quantised in 32 bits with a bound on what that is off by; where the minimum,
+// the scale or a code could round otherwise within it (1 row in 100 or so) the
+// warp does them again in 64 bits.  (All of it in 64 bits: 540 instructions for
+// 8 channels a lane instead of 200, 101 us for 8192 tokens instead of TODO.)
 #include <cmath>
 
 #include "kv4.cuh"
@@ -39,9 +39,9 @@ struct AppendArgs {
     int64_t pool_block, head_bytes;
     const int *block_tables, *seq_lens, *counts, *positions;
     int num_blocks, block_size, max_blocks;
-    int S, nq, nkv, D, rot, tokens, shares, bf16;
+    int S, nq, nkv, D, rot, tokens, shares, q_shares, bf16;
     int per;              // items of a row
-    BlockDiv by_item;
+    BlockDiv by_kvh;
     double turns[128];    // f_i / 2 pi
 };
 
@@ -55,11 +55,16 @@ template <>
 struct Chunk<4> {
     using T = uint2;
 };
-__device__ __forceinline__ float2 unpack2(uint32_t x, bool bf16) {
-    return bf16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) : h2_to_f2(x);
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+    return BF16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) : h2_to_f2(x);
 }
-__device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
-    return bf16 ? pack16<true>(a, b) : pack16<false>(a, b);
+
+// The larger, or a NaN if one is.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
 // How many new rows sequence b has, and where the first one goes.
@@ -68,29 +73,17 @@ __device__ __forceinline__ int2 new_rows(const int* seq_lens, const int* counts,
     return make_int2(n, seq_lens[b] - n);
 }
 
-// u of (x - m) / s: d = x - m, r = 32-bit 1 / s
-__device__ __forceinline__ int code_of(double d, float df, double s, float r) {
-    const float t = df * r;
-    float u = rintf(t);
-    if (fabsf(t - u) > 0.4998f && t < 16.f) {
-        // (the product is off by less than 16 * 2^-22: elsewhere its rounding is right)
-        const double left = d - (double)u * s;
-        if (left > 0.5 * s || (left == 0.5 * s && ((int)u & 1))) u += 1.f;
-        if (left < -0.5 * s || (left == -0.5 * s && ((int)u & 1))) u -= 1.f;
-    }
-    return (int)fminf(fmaxf(u, 0.f), 15.f);
-}
-
 // KV4: rows of 4 bits.  VEC: channels per load, 8, or 4 where half the rotated
 // channels are no multiple of 8.
-template <bool KV4, int VEC>
-__global__ void __launch_bounds__(kApThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+template <bool KV4, int VEC, bool BF16>
+__global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const __grid_constant__ AppendArgs a) {
     using Vec = typename Chunk<VEC>::T;
-    __shared__ float2 s_cs[kApTokens][128];
-    __shared__ double2 s_cs64[KV4 ? kApTokens : 1][128];
+    __shared__ __align__(16) float2 s_cs[kApTokens][128];
     __shared__ int64_t s_row[kApTokens];  // where a token's rows go: element offset of head 0, or byte offset of its tile
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int b = blockIdx.z, share = blockIdx.y, t0 = blockIdx.x * a.tokens;
+    // rows of 4 bits have CTAs of their own, behind those of the queries
+    const bool rows4 = KV4 && (int)blockIdx.y >= a.q_shares;
+    const int b = blockIdx.z, share = blockIdx.y - (rows4 ? a.q_shares : 0), t0 = blockIdx.x * a.tokens;
     griddep_wait();
     griddep_launch_dependents();
     const int2 rows = new_rows(a.seq_lens, a.counts, b, a.S);
@@ -117,169 +110,244 @@ __global__ void __launch_bounds__(kApThreads) append_kernel(const __grid_constan
         const int t = i / half, e = i - t * half;
         double turn = (double)(first + t) * a.turns[e];
         turn -= rint(turn);
-        if (KV4) {
-            double sn, cn;
-            sincospi(2.0 * turn, &sn, &cn);
-            s_cs64[t][e] = make_double2(cn, sn);
-            s_cs[t][e] = make_float2((float)cn, (float)sn);
-        } else {
-            float sn, cn;
-            sincospif((float)(2.0 * turn), &sn, &cn);
-            s_cs[t][e] = make_float2(cn, sn);
-        }
+        float sn, cn;
+        sincospif((float)(2.0 * turn), &sn, &cn);
+        s_cs[t][e] = make_float2(cn, sn);
     }
     __syncthreads();
 
     const int q0 = a.nq * share / a.shares, q1 = a.nq * (share + 1) / a.shares;
     const int k0 = a.nkv * share / a.shares, k1 = a.nkv * (share + 1) / a.shares;
-    const int heads = (a.q.data ? q1 - q0 : 0) + (KV4 ? 0 : 2 * (k1 - k0));
-    // ---- rows of 16 bits: an item is two chunks of VEC channels that are rotated together, or two to be copied
-    const int items = nt * heads * a.per;
-    constexpr int ON = 4;
-    for (int i0 = tid; i0 < items; i0 += ON * kApThreads) {
-        Vec x[ON], y[ON];
-        const uint16_t* src[ON];
-        uint16_t* dst[ON];
-        int c0[ON], c1[ON], tok[ON];  // channels of the two chunks; c1 < 0: none
-        bool turn[ON];
+    // ---- rows of 16 bits: an item is two chunks of VEC channels that are rotated together, or two to be copied.  A
+    // thread has the same item of every rows-th row
+    if (!rows4) {
+        const int nqh = a.q.data ? q1 - q0 : 0, nkh = KV4 ? 0 : k1 - k0, heads = nqh + 2 * nkh;
+        const int rows = kApThreads / a.per, row0 = tid / a.per, e = tid - row0 * a.per, pairs = a.rot / (2 * VEC);
+        const bool turns = e < pairs;
+        const int c0 = turns ? e * VEC : a.rot + (e - pairs) * 2 * VEC, c1 = turns ? half + c0 : c0 + VEC;
+        const bool both = c1 < a.D;
+        const int all = row0 < rows ? nt * heads : 0;
+        constexpr int ON = 4;  // rows of a thread on their way
+        int tok = heads ? row0 / heads : 0, h = row0 - tok * heads;
+        for (int r = row0; r < all; r += ON * rows) {
+            Vec x[ON], y[ON];
+            uint16_t* dst[ON];
+            int at[ON];  // token whose angles turn the row; -1: a copy
 #pragma unroll
-        for (int n = 0; n < ON; ++n) {
-            const int i = i0 + n * kApThreads;
-            dst[n] = nullptr;
-            if (i >= items) continue;
-            const int r = a.by_item.block(i), e = a.by_item.slot(i, r);
-            tok[n] = r / heads;
-            int h = r - tok[n] * heads;
-            const int s = t0 + tok[n];
-            turn[n] = e < a.rot / (2 * VEC);
-            c0[n] = turn[n] ? e * VEC : a.rot + (e - a.rot / (2 * VEC)) * 2 * VEC;
-            c1[n] = turn[n] ? half + e * VEC : c0[n] + VEC;
-            if (c1[n] >= a.D) c1[n] = -1;
-            const int nqh = a.q.data ? q1 - q0 : 0;
-            if (h < nqh) {
-                h += q0;
-                src[n] = static_cast<const uint16_t*>(a.q.data) + b * a.q.stride_b + s * a.q.stride_s + h * a.q.stride_h;
-                dst[n] = static_cast<uint16_t*>(const_cast<void*>(a.q_out.data)) + b * a.q_out.stride_b +
-                         s * a.q_out.stride_s + h * a.q_out.stride_h;
-            } else {
-                h -= nqh;
-                const bool key = h < k1 - k0;
-                h = k0 + (key ? h : h - (k1 - k0));
-                const b2_kv_view& w = key ? a.k : a.v;
-                src[n] = static_cast<const uint16_t*>(w.data) + b * w.stride_b + s * w.stride_s + h * w.stride_h;
-                if (!key) turn[n] = false;
-                if (s_row[tok[n]] >= 0)
-                    dst[n] = static_cast<uint16_t*>(key ? a.kv.k : a.kv.v) + s_row[tok[n]] + (int64_t)h * a.kv.stride_head;
-            }
-            if (!dst[n]) continue;
-            x[n] = *reinterpret_cast<const Vec*>(src[n] + c0[n]);
-            if (c1[n] >= 0) y[n] = *reinterpret_cast<const Vec*>(src[n] + c1[n]);
-        }
-#pragma unroll
-        for (int n = 0; n < ON; ++n) {
-            if (!dst[n]) continue;
-            if (turn[n]) {
-                uint32_t* xs = reinterpret_cast<uint32_t*>(&x[n]);
-                uint32_t* ys = reinterpret_cast<uint32_t*>(&y[n]);
-#pragma unroll
-                for (int j = 0; j < VEC / 2; ++j) {
-                    const float2 u = unpack2(xs[j], a.bf16), w = unpack2(ys[j], a.bf16);
-                    const float2 t = s_cs[tok[n]][c0[n] + 2 * j], v = s_cs[tok[n]][c0[n] + 2 * j + 1];
-                    xs[j] = pack2(u.x * t.x - w.x * t.y, u.y * v.x - w.y * v.y, a.bf16);
-                    ys[j] = pack2(w.x * t.x + u.x * t.y, w.y * v.x + u.y * v.y, a.bf16);
+            for (int n = 0; n < ON; ++n) {
+                dst[n] = nullptr;
+                if (r + n * rows < all) {
+                    const int s = t0 + tok;
+                    const uint16_t* src;
+                    at[n] = turns ? tok : -1;
+                    if (h < nqh) {
+                        const int64_t o = b * a.q.stride_b + s * a.q.stride_s + (q0 + h) * a.q.stride_h;
+                        src = static_cast<const uint16_t*>(a.q.data) + o;
+                        dst[n] = static_cast<uint16_t*>(const_cast<void*>(a.q_out.data)) + b * a.q_out.stride_b +
+                                 s * a.q_out.stride_s + (q0 + h) * a.q_out.stride_h;
+                    } else {
+                        const bool key = h < nqh + nkh;
+                        const int hh = k0 + h - nqh - (key ? 0 : nkh);
+                        const b2_kv_view& w = key ? a.k : a.v;
+                        src = static_cast<const uint16_t*>(w.data) + b * w.stride_b + s * w.stride_s + hh * w.stride_h;
+                        if (!key) at[n] = -1;
+                        if (s_row[tok] >= 0)
+                            dst[n] = static_cast<uint16_t*>(key ? a.kv.k : a.kv.v) + s_row[tok] + hh * a.kv.stride_head;
+                    }
+                    if (dst[n]) {
+                        x[n] = *reinterpret_cast<const Vec*>(src + c0);
+                        if (both) y[n] = *reinterpret_cast<const Vec*>(src + c1);
+                    }
+                    h += rows;
+                    while (h >= heads) h -= heads, ++tok;
                 }
             }
-            *reinterpret_cast<Vec*>(dst[n] + c0[n]) = x[n];
-            if (c1[n] >= 0) *reinterpret_cast<Vec*>(dst[n] + c1[n]) = y[n];
+#pragma unroll
+            for (int n = 0; n < ON; ++n) {
+                if (!dst[n]) continue;
+                if (at[n] >= 0) {
+                    uint32_t* xs = reinterpret_cast<uint32_t*>(&x[n]);
+                    uint32_t* ys = reinterpret_cast<uint32_t*>(&y[n]);
+#pragma unroll
+                    for (int j = 0; j < VEC / 2; ++j) {
+                        const float2 u = unpack2<BF16>(xs[j]), w = unpack2<BF16>(ys[j]);
+                        const float4 t = *reinterpret_cast<const float4*>(&s_cs[at[n]][c0 + 2 * j]);
+                        xs[j] = pack16<BF16>(u.x * t.x - w.x * t.y, u.y * t.z - w.y * t.w);
+                        ys[j] = pack16<BF16>(w.x * t.x + u.x * t.y, w.y * t.z + u.y * t.w);
+                    }
+                }
+                *reinterpret_cast<Vec*>(dst[n] + c0) = x[n];
+                if (both) *reinterpret_cast<Vec*>(dst[n] + c1) = y[n];
+            }
         }
     }
-    if (!KV4) return;
+    if (!rows4) return;
 
-    // ---- rows of 4 bits: lane l holds channels 4 l .. 4 l + 3 of 128 at a time, 16 lanes a group; two rows at once
-    // where a row has 64
+    // ---- rows of 4 bits: a lane holds 8 channels, 8 lanes a group, 8, 16 or 32 lanes a row
     const int DP = kv4_dp(a.D), NG = kv4_groups(DP), kvh = k1 - k0;
-    const bool twin = DP == 64;
-    const int sub = twin ? lane >> 4 : 0, c4 = (twin ? lane & 15 : lane) * 4;
+    const int wide = DP == 64 ? 3 : DP <= 128 ? 4 : 5, at_once = 32 >> wide;
+    const int sub = lane >> wide, c = (lane & ((1 << wide) - 1)) * 8;
     const int nr = nt * kvh;  // rows of K, then of V
-    for (int r0 = warp * (twin ? 2 : 1); r0 < 2 * nr; r0 += kApThreads / 32 * (twin ? 2 : 1)) {
+    const bool in = c < a.D, turned = c < a.rot;
+    const bool empty = (c & ~63) >= a.D;  // a group of padding alone
+    // K is rotated with the sign of the sine taken to the partner: whole chunks of 4 channels have one sign
+    const bool low0 = c < half, low1 = c + 4 < half;
+    const int e0 = low0 ? c : c - half, e1 = low1 ? c + 4 : c + 4 - half;  // pairs of channels c and c + 4
+    const int g0 = low0 ? c + half : c - half, g1 = low1 ? c + 4 + half : c + 4 - half;  // and their partners
+    constexpr int STEP = kApThreads / 32;
+    const BlockDiv by_kvh = a.by_kvh;
+    // a row and the partners of its channels: the next row's are on their way while one is worked on
+    struct Row {
+        int tok, h;
+        bool key;
+        uint4 own;
+        uint2 other[2];
+    };
+    auto fetch = [&](int r0) {
+        Row w;
         const int r = min(r0 + sub, 2 * nr - 1);
-        const bool key = r < nr;
-        const int rr = key ? r : r - nr, tok = rr / kvh, h = k0 + rr - tok * kvh;
+        w.key = r < nr;
+        const int rr = w.key ? r : r - nr;
+        w.tok = a.shares == 1 ? by_kvh.block(rr) : rr / kvh;
+        w.h = k0 + rr - w.tok * kvh;
+        const b2_kv_view& v = w.key ? a.k : a.v;
+        const uint16_t* src = static_cast<const uint16_t*>(v.data) + b * v.stride_b + (int64_t)(t0 + w.tok) * v.stride_s +
+                              w.h * v.stride_h;
+        w.own = in ? *reinterpret_cast<const uint4*>(src + c) : make_uint4(0, 0, 0, 0);
+        w.other[0] = w.other[1] = make_uint2(0, 0);
+        if (w.key && turned) {
+            if (VEC == 8) {
+                const uint4 x = *reinterpret_cast<const uint4*>(src + g0);
+                w.other[0] = make_uint2(x.x, x.y), w.other[1] = make_uint2(x.z, x.w);
+            } else {
+                w.other[0] = *reinterpret_cast<const uint2*>(src + g0);
+                w.other[1] = *reinterpret_cast<const uint2*>(src + g1);
+            }
+        }
+        return w;
+    };
+    Row ahead = fetch(warp * at_once);
+    for (int r0 = warp * at_once; r0 < 2 * nr; r0 += STEP * at_once) {
+        const Row row = ahead;
+        if (r0 + STEP * at_once < 2 * nr) ahead = fetch(r0 + STEP * at_once);
+        const bool key = row.key;
+        const int tok = row.tok, h = row.h;
+        const uint4 own = row.own;
+        const uint2 other[2] = {row.other[0], row.other[1]};
         const int64_t at = s_row[tok];
-        const b2_kv_view& w = key ? a.k : a.v;
-        const uint16_t* src = static_cast<const uint16_t*>(w.data) + b * w.stride_b + (int64_t)(t0 + tok) * w.stride_s +
-                              h * w.stride_h;
-        const bool mine = at >= 0 && r0 + sub < 2 * nr;
+        float f[8];
+        auto unpack = [&](uint2 x, float* v) {
+            const float2 p0 = unpack2<BF16>(x.x), p1 = unpack2<BF16>(x.y);
+            v[0] = p0.x, v[1] = p0.y, v[2] = p1.x, v[3] = p1.y;
+        };
+        unpack(make_uint2(own.x, own.y), f);
+        unpack(make_uint2(own.z, own.w), f + 4);
+        float off = 0.f;  // what f is off by, at most
+        if (key && turned) {
+            const uint32_t n0 = low0 ? 0x80008000u : 0u, n1 = (VEC == 8 ? low0 : low1) ? 0x80008000u : 0u;
+            float g[8];
+            unpack(make_uint2(other[0].x ^ n0, other[0].y ^ n0), g);
+            unpack(make_uint2(other[1].x ^ n1, other[1].y ^ n1), g + 4);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float4 t = *reinterpret_cast<const float4*>(&s_cs[tok][VEC == 8 || i < 4 ? e0 + i : e1 + i - 4]);
+                off = fmaxf(off, fmaxf(fabsf(f[i]) + fabsf(g[i]), fabsf(f[i + 1]) + fabsf(g[i + 1])));
+                f[i] = fmaf(f[i], t.x, g[i] * t.y);
+                f[i + 1] = fmaf(f[i + 1], t.z, g[i + 1] * t.w);
+            }
+            off *= 0x1p-21f;  // sine and cosine within 2^-22 (the angle's rounding to 32 bits among it), two roundings
+        }
+        float lo = f[0], hi = f[0], most = fabsf(f[0]);
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+            lo = fminf(lo, f[i]);
+            hi = fmaxf(hi, f[i]);
+            most = fmax_nan(most, fabsf(f[i]));
+        }
+        if (!in) lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
+            most = fmax_nan(most, __shfl_xor_sync(~0u, most, o));
+            off = fmaxf(off, __shfl_xor_sync(~0u, off, o));
+        }
+        const bool fine = most < INFINITY;
+        auto to_half = [](float x) { return __half2float(__float2half_rn(fminf(fmaxf(x, -65504.f), 65504.f))); };
+        float m = to_half(lo);
+        // the span is off by off + 2^-24 (hi - m), as a 15th of it two roundings more
+        const float span = (hi - m) * (1.f / 15.f), wrong = off * (1.f / 15.f) + span * 0x1p-22f;
+        float s = to_half(fmaxf(span, 0.f));
+        bool sure = to_half(lo - off) == to_half(lo + off) && to_half(fmaxf(span - wrong, 0.f)) == to_half(fmaxf(span + wrong, 0.f));
+        // u as the nearest whole number to t: adding 1.5 * 2^23 leaves it in the low bits
+        constexpr float MAGIC = 12582912.f;
+        const float rs = s > 0.f ? __frcp_rn(s) : 0.f;
+        uint32_t codes = 0;
+        float worst = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float t = fminf(fmaxf((f[i] - m) * rs, 0.f), 15.f), v = t + MAGIC;
+            worst = fmaxf(worst, fabsf(t - (v - MAGIC)));
+            codes += __float_as_uint(v) << (4 * i);
+        }
+        codes -= 0x4b400000u * 0x11111111u;
+        // t is off by (off + 2^-23 most) / s and 2^-22 of itself: nearer to a half than that, it may round otherwise
+        if (!in) worst = 0.f;
+        sure = sure && worst < 0.5f - ((off + most * 0x1p-23f) * rs + 0x1p-18f);
+        if (__any_sync(~0u, !(sure || !fine || empty))) {
+            // in 64 bits
+            double x[8];
+            auto four = [&](uint2 own4, uint2 oth, bool low, int e, double* y) {
+                float u[4], g[4];
+                unpack(own4, u);
+                unpack(oth, g);
+                const int64_t pos = first + tok;
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) {
+                    y[i] = u[i];
+                    if (key && turned) {
+                        double turn = (double)pos * a.turns[e + i], sn, cn;
+                        turn -= rint(turn);
+                        sincospi(2.0 * turn, &sn, &cn);
+                        y[i] = fma((double)u[i], cn, (low ? -(double)g[i] : (double)g[i]) * sn);
+                    }
+                }
+            };
+            four(make_uint2(own.x, own.y), other[0], low0, e0, x);
+            four(make_uint2(own.z, own.w), other[1], VEC == 8 ? low0 : low1, VEC == 8 ? e0 + 4 : e1, x + 4);
+            double l = in ? x[0] : INFINITY, u = in ? x[0] : -INFINITY;
+            for (int i = 1; i < 8; ++i)
+                if (in) l = x[i] < l ? x[i] : l, u = x[i] > u ? x[i] : u;
+            for (int o = 1; o < 8; o <<= 1) {
+                const double y = __shfl_xor_sync(~0u, l, o), z = __shfl_xor_sync(~0u, u, o);
+                l = y < l ? y : l;
+                u = z > u ? z : u;
+            }
+            m = to_half((float)l);
+            s = to_half(fmaxf((float)((u - (double)m) / 15.0), 0.f));
+            codes = 0;
+            for (int i = 0; i < 8; ++i) {
+                const double t = s > 0.f ? rint((x[i] - (double)m) / (double)s) : 0.0;
+                codes |= (uint32_t)(t < 0.0 ? 0.0 : t > 15.0 ? 15.0 : t) << (4 * i);
+            }
+        }
+        if (at < 0 || r0 + sub >= 2 * nr || c >= DP) continue;
+        if (!in || !fine) codes = 0;
         const int p = (int)(at & 15);
         uint8_t* tile = a.pool + (at >> 4) + h * a.head_bytes;
-        for (int c = c4; c < (DP + 127) / 128 * 128; c += 128) {
-            const bool in = c < a.D;
-            double x[4] = {0, 0, 0, 0};
-            float f[4] = {0.f, 0.f, 0.f, 0.f};
-            if (in) {
-                auto four = [&](int ch, float (&v)[4]) {
-                    const uint2 u = *reinterpret_cast<const uint2*>(src + ch);
-                    const float2 p0 = unpack2(u.x, a.bf16), p1 = unpack2(u.y, a.bf16);
-                    v[0] = p0.x, v[1] = p0.y, v[2] = p1.x, v[3] = p1.y;
-                };
-                four(c, f);
-                if (key && c < a.rot) {  // (half the rotated channels are a multiple of 4)
-                    const bool low = c < half;
-                    float g[4];
-                    four(low ? c + half : c - half, g);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const double2 t = s_cs64[tok][(low ? c : c - half) + i];
-                        x[i] = fma((double)f[i], t.x, (low ? -(double)g[i] : (double)g[i]) * t.y);
-                        f[i] = (float)x[i];
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = f[i];
-                }
-            }
-            // least and largest of the group; the least only as a half of its 32-bit value is needed
-            float lo = INFINITY;
-            double hi = -INFINITY;
-            bool fine = true;
-            if (in) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    lo = fminf(lo, f[i]);
-                    hi = x[i] > hi ? x[i] : hi;
-                    fine = fine && fabsf(f[i]) < INFINITY;
-                }
-            }
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) {
-                lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
-                const double y = __shfl_xor_sync(~0u, hi, o);
-                hi = y > hi ? y : hi;
-            }
-            const uint32_t odd = __ballot_sync(~0u, !fine);
-            fine = ((odd >> (lane & 16)) & 0xffffu) == 0;
-            __half m = __float2half_rn(fminf(fmaxf(lo, -65504.f), 65504.f));
-            double span = (hi - (double)__half2float(m)) / 15.0;
-            span = span > 65504.0 ? 65504.0 : span > 0.0 ? span : 0.0;
-            __half s = __float2half_rn((float)span);
-            if (!fine) m = s = __ushort_as_half(0x7fff);
-            if (fine && hi < lo) m = s = __ushort_as_half(0);  // a group of padding alone
-            const float sf = __half2float(s), mf = __half2float(m);
-            uint32_t codes = 0;
-            if (in && sf > 0.f) {
-                const float rs = __frcp_rn(sf);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    codes |= code_of(x[i] - (double)mf, key ? (float)(x[i] - (double)mf) : f[i] - mf, (double)sf, rs) << (4 * i);
-            }
-            if (!mine || c >= DP) continue;
-            const int j = c >> 3, x32 = c >> 5, r8 = (c & 31) >> 2;
-            const int place = key ? p * (DP / 2) + ((j & 3) * (DP / 32) + (j >> 2)) * 4 + ((c >> 2) & 1) * 2
-                                  : 8 * DP + ((x32 * 8 + r8) * 4 + ((p & 7) >> 1)) * 8 + (p >> 3) * 4 + (p & 1) * 2;
-            *reinterpret_cast<uint16_t*>(tile + place) = (uint16_t)codes;
-            if ((c & 63) == 0)
-                *reinterpret_cast<__half2*>(tile + 16 * DP + (key ? 0 : 64 * NG) + (kv4_slot(p) * NG + (c >> 6)) * 4) =
-                    __halves2half2(s, m);
+        if (key) {
+            const int j = c >> 3;
+            *reinterpret_cast<uint32_t*>(tile + p * (DP / 2) + ((j & 3) * (DP / 32) + (j >> 2)) * 4) = codes;
+        } else {
+            uint8_t* to = tile + 8 * DP + (((c >> 5) * 8 + ((c & 31) >> 2)) * 4 + ((p & 7) >> 1)) * 8 + (p >> 3) * 4 + (p & 1) * 2;
+            *reinterpret_cast<uint16_t*>(to) = (uint16_t)codes;
+            *reinterpret_cast<uint16_t*>(to + 32) = (uint16_t)(codes >> 16);
+        }
+        if ((c & 63) == 0) {
+            __half2 sm = __floats2half2_rn(s, m);
+            if (!fine) sm = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff));
+            if (empty) sm = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+            *reinterpret_cast<__half2*>(tile + 16 * DP + (key ? 0 : 64 * NG) + (kv4_slot(p) * NG + (c >> 6)) * 4) = sm;
         }
     }
 }
@@ -294,7 +362,7 @@ struct ReadArgs {
 
 // A warp per tile of 16 positions and kv head; its lanes read what they read in
 // the attention's products (kv4.cuh) and write 16 bytes of K, 8 of V at a time.
-template <int DP>
+template <int DP, bool BF16>
 __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
     constexpr int W = DP / 32, NG = kv4_groups(DP);
     griddep_wait();
@@ -345,8 +413,8 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = fmaf((float)((kw[pp][j] >> (4 * e)) & 15), sm.x, sm.y);
             *reinterpret_cast<uint4*>(ko + (int64_t)(pos - first) * a.k.stride_s + c) =
-                make_uint4(pack2(f[0], f[1], a.bf16), pack2(f[2], f[3], a.bf16), pack2(f[4], f[5], a.bf16),
-                           pack2(f[6], f[7], a.bf16));
+                make_uint4(pack16<BF16>(f[0], f[1]), pack16<BF16>(f[2], f[3]), pack16<BF16>(f[4], f[5]),
+                           pack16<BF16>(f[6], f[7]));
         }
     }
 #pragma unroll
@@ -363,7 +431,7 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) f[e] = fmaf((float)((u >> (4 * e)) & 15), sm.x, sm.y);
             *reinterpret_cast<uint2*>(vo + (int64_t)(pos - first) * a.v.stride_s + c) =
-                make_uint2(pack2(f[0], f[1], a.bf16), pack2(f[2], f[3], a.bf16));
+                make_uint2(pack16<BF16>(f[0], f[1]), pack16<BF16>(f[2], f[3]));
         }
     }
 }
@@ -403,20 +471,29 @@ static int append_args(AppendArgs& a, const b2_kv_view* q, const b2_kv_view* q_o
     a.shares = 1;
     while (a.shares < nkv && a.shares < 8 && ctas * a.shares * 2 <= sm_count()) a.shares *= 2;
     if (a.shares > nkv) a.shares = nkv;
+    a.q_shares = q ? a.shares : 0;
     return B2_OK;
 }
 
 template <bool KV4>
 static int append_launch(AppendArgs& a, int batch, cudaStream_t s) {
     const int vec = (a.rot / 2) % 8 == 0 ? 8 : 4;
+    a.by_kvh = block_div(a.nkv);
     a.per = a.rot / (2 * vec) + (a.D - a.rot + 2 * vec - 1) / (2 * vec);
-    a.by_item = block_div(a.per);
-    const dim3 grid((unsigned)((a.S + a.tokens - 1) / a.tokens), (unsigned)a.shares, (unsigned)batch);
-    if (vec == 8)
-        B2_TRY(launch(append_kernel<KV4, 8>, grid, dim3(kApThreads), 0, s, true, a));
+    const dim3 grid((unsigned)((a.S + a.tokens - 1) / a.tokens), (unsigned)(KV4 ? a.q_shares + a.shares : a.shares), (unsigned)batch);
+    if (a.bf16)
+        B2_TRY(vec == 8 ? launch(append_kernel<KV4, 8, true>, grid, dim3(kApThreads), 0, s, true, a)
+                        : launch(append_kernel<KV4, 4, true>, grid, dim3(kApThreads), 0, s, true, a));
     else
-        B2_TRY(launch(append_kernel<KV4, 4>, grid, dim3(kApThreads), 0, s, true, a));
+        B2_TRY(vec == 8 ? launch(append_kernel<KV4, 8, false>, grid, dim3(kApThreads), 0, s, true, a)
+                        : launch(append_kernel<KV4, 4, false>, grid, dim3(kApThreads), 0, s, true, a));
     return B2_OK;
+}
+
+template <int DP>
+static cudaError_t read_launch(const ReadArgs& a, dim3 grid, cudaStream_t s) {
+    return a.bf16 ? launch(kv4_read_kernel<DP, true>, grid, dim3(128), 0, s, true, a)
+                  : launch(kv4_read_kernel<DP, false>, grid, dim3(128), 0, s, true, a);
 }
 
 }  // namespace b2
@@ -492,11 +569,11 @@ extern "C" int b2_paged_kv4_read(const b2_paged_kv4* kv, b2_kv_view k_out, b2_kv
     const dim3 grid((unsigned)((most + 30) / 16 / 4 + 1), (unsigned)nkv, (unsigned)batch);
     cudaStream_t s = as_stream(stream);
     switch (kv4_dp(D)) {
-        case 64: B2_TRY(launch(kv4_read_kernel<64>, grid, dim3(128), 0, s, true, a)); break;
-        case 96: B2_TRY(launch(kv4_read_kernel<96>, grid, dim3(128), 0, s, true, a)); break;
-        case 128: B2_TRY(launch(kv4_read_kernel<128>, grid, dim3(128), 0, s, true, a)); break;
-        case 192: B2_TRY(launch(kv4_read_kernel<192>, grid, dim3(128), 0, s, true, a)); break;
-        default: B2_TRY(launch(kv4_read_kernel<256>, grid, dim3(128), 0, s, true, a)); break;
+        case 64: B2_TRY(read_launch<64>(a, grid, s)); break;
+        case 96: B2_TRY(read_launch<96>(a, grid, s)); break;
+        case 128: B2_TRY(read_launch<128>(a, grid, s)); break;
+        case 192: B2_TRY(read_launch<192>(a, grid, s)); break;
+        default: B2_TRY(read_launch<256>(a, grid, s)); break;
     }
     return B2_OK;
 }

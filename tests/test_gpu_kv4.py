@@ -8,7 +8,11 @@ terms, the groups, the minima), each off by at most 2^-23 of the largest partial
 sum, which is below M = sum_d |q_d| 3 max|k| / sqrt(D), since m and 15 s of a
 group are each at most 3 max|k| together: 2^-18 M.  That changes every weight by
 that relative amount and their sum likewise, 2^-17 M A with A = sum_j p_j |v_j|;
-the exponential and the split of the weights add less than 2^-20 A.  Outputs add
+the exponential and the split of the weights add less than 2^-20 A; for outputs
+in bf16 the weights are rounded to halves instead, 2^-11 of each weight times its
+scale at most, which moves an output by 2^-11 sum_j p_j |v_j - mid_j| <= 2^-11 A'
+with A' below 3 max|v| / 2 (a group's codes less 8 times its scale are at most half
+its range, |m| + 15 s <= 3 max|v|).  Outputs add
 up 16 positions at a time, n / 16 + 64 additions (the joins among them) off by at
 most 2^-23 of 3 max|v|."""
 import math
@@ -33,7 +37,8 @@ def close(got, want, mag, q, k, v, n):
     fin = lambda x: x[torch.isfinite(x)].abs().max().item() if torch.isfinite(x).any() else 0.0  # noqa: E731
     u = torch.finfo(got.dtype).eps / 2
     M = q.double().abs().sum(-1, keepdim=True) * 3 * fin(k) / math.sqrt(q.shape[-1])
-    tol = u * want.abs() + (2.0 ** -17 * M + 2.0 ** -20) * mag + (n / 16 + 64) * 2.0 ** -23 * 3 * fin(v) + 2.0 ** -25
+    half = 2.0 ** -11 * 1.5 * fin(v) if got.dtype == torch.bfloat16 else 0.0
+    tol = u * want.abs() + half + (2.0 ** -17 * M + 2.0 ** -20) * mag + (n / 16 + 64) * 2.0 ** -23 * 3 * fin(v) + 2.0 ** -25
     assert torch.isfinite(got).all()
     err = (got.double() - want).abs()
     assert (err <= tol).all(), (int((err > tol).sum()), float((err - tol).max()), (err > tol).nonzero()[0].tolist())
