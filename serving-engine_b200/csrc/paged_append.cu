@@ -9,7 +9,7 @@
 //   / 15), u = (x - m) / s rounded to even and clamped to 0 .. 15
 //
 // One read of q, k and v and one write of q and the rows: HBM bounds long
-// prompts, latency single tokens.  A CTA takes up to 8 consecutive tokens of a
+// prompts, latency single tokens.  A CTA takes up to 16 consecutive tokens of a
 // sequence (all heads, or a share of them where there are few tokens), so the
 // angles are worked out once per token and not per head.  The angle is kept as
 // turns: position times f / 2 pi in 64 bits, its whole part dropped, so that far
@@ -23,14 +23,18 @@
 // warp does them again in 64 bits.  (All of it in 64 bits: 540 instructions for
 // 8 channels a lane instead of 200, 101 us for 8192 tokens instead of TODO.)
 #include <cmath>
+#include <type_traits>
 
 #include "kv4.cuh"
 #include "mma.cuh"
 
 namespace b2 {
 
+using namespace packed;
+
 constexpr int kApThreads = 256;
-constexpr int kApTokens = 8;
+constexpr int kApTokens = 16;
+constexpr int64_t kNoRow = INT64_MIN;  // a token whose rows have no place
 
 struct AppendArgs {
     b2_kv_view q, k, v, q_out;
@@ -41,7 +45,6 @@ struct AppendArgs {
     int num_blocks, block_size, max_blocks;
     int S, nq, nkv, D, rot, tokens, shares, q_shares, bf16;
     int per;              // items of a row
-    BlockDiv by_kvh;
     double turns[128];    // f_i / 2 pi
 };
 
@@ -67,6 +70,8 @@ __device__ __forceinline__ float fmax_nan(float a, float b) {
     return r;
 }
 
+__device__ __forceinline__ uint64_t pair(float2 x) { return pair(x.x, x.y); }
+
 // How many new rows sequence b has, and where the first one goes.
 __device__ __forceinline__ int2 new_rows(const int* seq_lens, const int* counts, int b, int S) {
     const int n = counts ? max(0, min(S, counts[b])) : S;
@@ -76,10 +81,11 @@ __device__ __forceinline__ int2 new_rows(const int* seq_lens, const int* counts,
 // KV4: rows of 4 bits.  VEC: channels per load, 8, or 4 where half the rotated
 // channels are no multiple of 8.
 template <bool KV4, int VEC, bool BF16>
-__global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_constant__ AppendArgs a) {
     using Vec = typename Chunk<VEC>::T;
-    __shared__ __align__(16) float2 s_cs[kApTokens][128];
-    __shared__ int64_t s_row[kApTokens];  // where a token's rows go: element offset of head 0, or byte offset of its tile
+    __shared__ float4 s_cs[kApTokens][64];  // of two pairs of channels: cosines, sines
+    __shared__ int64_t s_row[kApTokens];  // where a token's rows go: element offset of its first head, or byte offset of its tile
+    __shared__ int s_in[KV4 ? kApTokens : 1][3];  // in the tile: K row, V units, scales
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // rows of 4 bits have CTAs of their own, behind those of the queries
     const bool rows4 = KV4 && (int)blockIdx.y >= a.q_shares;
@@ -91,15 +97,20 @@ __global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const _
     if (nt <= 0) return;
     if (tid < nt) {
         const int64_t pos = (int64_t)rows.y + t0 + tid;
-        int64_t at = -1;
+        int64_t at = kNoRow;
         if (pos >= 0 && pos < (int64_t)a.max_blocks * a.block_size) {
             const int blk = (int)pos / a.block_size, slot = (int)pos - blk * a.block_size;
             const int id = a.block_tables[(int64_t)b * a.max_blocks + blk];
             if ((unsigned)id < (unsigned)a.num_blocks) {
-                if (KV4)
-                    at = ((int64_t)id * a.pool_block + (int64_t)(slot >> 4) * kv4_tile(kv4_dp(a.D))) * 16 + (slot & 15);
-                else
-                    at = (int64_t)id * a.kv.stride_block + (int64_t)slot * a.kv.stride_slot;
+                if (KV4) {
+                    const int DP = kv4_dp(a.D), p = slot & 15;
+                    at = (int64_t)id * a.pool_block + (int64_t)(slot >> 4) * kv4_tile(DP);
+                    s_in[tid][0] = p * (DP / 2);
+                    s_in[tid][1] = 8 * DP + ((p & 7) >> 1) * 8 + (p >> 3) * 4 + (p & 1) * 2;
+                    s_in[tid][2] = 16 * DP + kv4_slot(p) * kv4_groups(DP) * 4;
+                } else
+                    at = (int64_t)id * a.kv.stride_block + (int64_t)slot * a.kv.stride_slot +
+                         (a.nkv * share / a.shares) * a.kv.stride_head;
             }
         }
         s_row[tid] = at;
@@ -111,74 +122,90 @@ __global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const _
         double turn = (double)(first + t) * a.turns[e];
         turn -= rint(turn);
         float sn, cn;
-        sincospif((float)(2.0 * turn), &sn, &cn);
-        s_cs[t][e] = make_float2(cn, sn);
+        if (rows4) {  // rounded from 64 bits: within 2^-25 (a quarter of the rows that have to be done again)
+            double sd, cd;
+            sincospi(2.0 * turn, &sd, &cd);
+            sn = (float)sd, cn = (float)cd;
+        } else {
+            sincospif((float)(2.0 * turn), &sn, &cn);
+        }
+        float* cs = reinterpret_cast<float*>(&s_cs[t][e >> 1]) + (e & 1);
+        cs[0] = cn;
+        cs[2] = sn;
     }
     __syncthreads();
 
     const int q0 = a.nq * share / a.shares, q1 = a.nq * (share + 1) / a.shares;
     const int k0 = a.nkv * share / a.shares, k1 = a.nkv * (share + 1) / a.shares;
-    // ---- rows of 16 bits: an item is two chunks of VEC channels that are rotated together, or two to be copied.  A
-    // thread has the same item of every rows-th row
+    // ---- rows of 16 bits: a thread has two chunks of VEC channels that are rotated together, or two to be copied, of one
+    // token (its angles stay in registers) and goes through heads
     if (!rows4) {
-        const int nqh = a.q.data ? q1 - q0 : 0, nkh = KV4 ? 0 : k1 - k0, heads = nqh + 2 * nkh;
-        const int rows = kApThreads / a.per, row0 = tid / a.per, e = tid - row0 * a.per, pairs = a.rot / (2 * VEC);
+        const int pairs = a.rot / (2 * VEC), e = tid % a.per, lead = tid / a.per, fit = kApThreads / a.per;
         const bool turns = e < pairs;
         const int c0 = turns ? e * VEC : a.rot + (e - pairs) * 2 * VEC, c1 = turns ? half + c0 : c0 + VEC;
         const bool both = c1 < a.D;
-        const int all = row0 < rows ? nt * heads : 0;
-        constexpr int ON = 4;  // rows of a thread on their way
-        int tok = heads ? row0 / heads : 0, h = row0 - tok * heads;
-        for (int r = row0; r < all; r += ON * rows) {
-            Vec x[ON], y[ON];
-            uint16_t* dst[ON];
-            int at[ON];  // token whose angles turn the row; -1: a copy
-#pragma unroll
-            for (int n = 0; n < ON; ++n) {
-                dst[n] = nullptr;
-                if (r + n * rows < all) {
-                    const int s = t0 + tok;
-                    const uint16_t* src;
-                    at[n] = turns ? tok : -1;
-                    if (h < nqh) {
-                        const int64_t o = b * a.q.stride_b + s * a.q.stride_s + (q0 + h) * a.q.stride_h;
-                        src = static_cast<const uint16_t*>(a.q.data) + o;
-                        dst[n] = static_cast<uint16_t*>(const_cast<void*>(a.q_out.data)) + b * a.q_out.stride_b +
-                                 s * a.q_out.stride_s + (q0 + h) * a.q_out.stride_h;
-                    } else {
-                        const bool key = h < nqh + nkh;
-                        const int hh = k0 + h - nqh - (key ? 0 : nkh);
-                        const b2_kv_view& w = key ? a.k : a.v;
-                        src = static_cast<const uint16_t*>(w.data) + b * w.stride_b + s * w.stride_s + hh * w.stride_h;
-                        if (!key) at[n] = -1;
-                        if (s_row[tok] >= 0)
-                            dst[n] = static_cast<uint16_t*>(key ? a.kv.k : a.kv.v) + s_row[tok] + hh * a.kv.stride_head;
-                    }
-                    if (dst[n]) {
-                        x[n] = *reinterpret_cast<const Vec*>(src + c0);
-                        if (both) y[n] = *reinterpret_cast<const Vec*>(src + c1);
-                    }
-                    h += rows;
-                    while (h >= heads) h -= heads, ++tok;
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < ON; ++n) {
-                if (!dst[n]) continue;
-                if (at[n] >= 0) {
-                    uint32_t* xs = reinterpret_cast<uint32_t*>(&x[n]);
-                    uint32_t* ys = reinterpret_cast<uint32_t*>(&y[n]);
+        const int tp = min(nt, fit), groups = fit / tp, mine = lead % tp, group = lead / tp;  // tokens, and threads for each
+        // rows of `heads` heads from h0 on; TURN: rotated.  Into the cache where `to` is null
+        auto all_of = [&](auto turn, const b2_kv_view& view, int h0, int heads, uint16_t* to, int64_t to_s, int64_t to_h) {
+            constexpr bool TURN = decltype(turn)::value;
+            constexpr int ON = 4;  // rows of a thread on their way
+            for (int tok = mine; tok < nt && group < groups; tok += tp) {
+                uint16_t* dst = to ? to + tok * to_s : static_cast<uint16_t*>(TURN ? a.kv.k : a.kv.v) + s_row[tok];
+                if (!to && s_row[tok] == kNoRow) continue;
+                const uint16_t* src = static_cast<const uint16_t*>(view.data) + b * view.stride_b +
+                                      (int64_t)(t0 + tok) * view.stride_s + (h0 + group) * view.stride_h + c0;
+                dst += group * to_h + c0;
+                const int64_t step = groups * view.stride_h, to_step = groups * to_h;
+                const int next = c1 - c0;
+                uint64_t cn[VEC / 2], sn[VEC / 2], ns[VEC / 2];
+                if (TURN && turns) {
 #pragma unroll
                     for (int j = 0; j < VEC / 2; ++j) {
-                        const float2 u = unpack2<BF16>(xs[j]), w = unpack2<BF16>(ys[j]);
-                        const float4 t = *reinterpret_cast<const float4*>(&s_cs[at[n]][c0 + 2 * j]);
-                        xs[j] = pack16<BF16>(u.x * t.x - w.x * t.y, u.y * t.z - w.y * t.w);
-                        ys[j] = pack16<BF16>(w.x * t.x + u.x * t.y, w.y * t.z + u.y * t.w);
+                        const float4 t = s_cs[tok][(c0 >> 1) + j];
+                        cn[j] = pair(t.x, t.y), sn[j] = pair(t.z, t.w), ns[j] = pair(-t.z, -t.w);
                     }
                 }
-                *reinterpret_cast<Vec*>(dst[n] + c0) = x[n];
-                if (both) *reinterpret_cast<Vec*>(dst[n] + c1) = y[n];
+                for (int h = group; h < heads; h += ON * groups) {
+                    Vec x[ON], y[ON];
+#pragma unroll
+                    for (int n = 0; n < ON; ++n) {
+                        if (h + n * groups < heads) {
+                            x[n] = *reinterpret_cast<const Vec*>(src);
+                            if (both) y[n] = *reinterpret_cast<const Vec*>(src + next);
+                        }
+                        src += step;
+                    }
+#pragma unroll
+                    for (int n = 0; n < ON; ++n) {
+                        if (h + n * groups < heads) {
+                            if (TURN && turns) {
+                                uint32_t* xs = reinterpret_cast<uint32_t*>(&x[n]);
+                                uint32_t* ys = reinterpret_cast<uint32_t*>(&y[n]);
+#pragma unroll
+                                for (int j = 0; j < VEC / 2; ++j) {
+                                    const uint64_t u = pair(unpack2<BF16>(xs[j])), w = pair(unpack2<BF16>(ys[j]));
+                                    const float2 p = two(fma2(w, ns[j], mul2(u, cn[j]))), q = two(fma2(u, sn[j], mul2(w, cn[j])));
+                                    xs[j] = pack16<BF16>(p.x, p.y);
+                                    ys[j] = pack16<BF16>(q.x, q.y);
+                                }
+                            }
+                            *reinterpret_cast<Vec*>(dst) = x[n];
+                            if (both) *reinterpret_cast<Vec*>(dst + next) = y[n];
+                        }
+                        dst += to_step;
+                    }
+                }
             }
+        };
+        if (q1 > q0)
+            all_of(std::true_type{}, a.q, q0, q1 - q0,
+                   static_cast<uint16_t*>(const_cast<void*>(a.q_out.data)) + b * a.q_out.stride_b + t0 * a.q_out.stride_s +
+                       q0 * a.q_out.stride_h,
+                   a.q_out.stride_s, a.q_out.stride_h);
+        if (!KV4 && k1 > k0) {
+            // (heads are counted from k0 in the cache too)
+            all_of(std::true_type{}, a.k, k0, k1 - k0, nullptr, 0, a.kv.stride_head);
+            all_of(std::false_type{}, a.v, k0, k1 - k0, nullptr, 0, a.kv.stride_head);
         }
     }
     if (!rows4) return;
@@ -187,7 +214,7 @@ __global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const _
     const int DP = kv4_dp(a.D), NG = kv4_groups(DP), kvh = k1 - k0;
     const int wide = DP == 64 ? 3 : DP <= 128 ? 4 : 5, at_once = 32 >> wide;
     const int sub = lane >> wide, c = (lane & ((1 << wide) - 1)) * 8;
-    const int nr = nt * kvh;  // rows of K, then of V
+    const int nr = nt * kvh;  // rows of K, and of V
     const bool in = c < a.D, turned = c < a.rot;
     const bool empty = (c & ~63) >= a.D;  // a group of padding alone
     // K is rotated with the sign of the sine taken to the partner: whole chunks of 4 channels have one sign
@@ -195,46 +222,53 @@ __global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const _
     const int e0 = low0 ? c : c - half, e1 = low1 ? c + 4 : c + 4 - half;  // pairs of channels c and c + 4
     const int g0 = low0 ? c + half : c - half, g1 = low1 ? c + 4 + half : c + 4 - half;  // and their partners
     constexpr int STEP = kApThreads / 32;
-    const BlockDiv by_kvh = a.by_kvh;
+    // this lane's places in a K row, among a position's V units, among its scales
+    const int in_k = (((c >> 3) & 3) * (DP / 32) + (c >> 5)) * 4, in_v = ((c >> 5) * 8 + ((c & 31) >> 2)) * 32, in_s = (c >> 6) * 4;
+    auto rows_of = [&](auto is_key) {
+    constexpr bool key = decltype(is_key)::value;
+    const b2_kv_view& view = key ? a.k : a.v;
+    const uint16_t* const base = static_cast<const uint16_t*>(view.data) + b * view.stride_b + t0 * view.stride_s + k0 * view.stride_h;
     // a row and the partners of its channels: the next row's are on their way while one is worked on
     struct Row {
-        int tok, h;
-        bool key;
         uint4 own;
         uint2 other[2];
     };
-    auto fetch = [&](int r0) {
+    const int dt = STEP * at_once / kvh, dh = STEP * at_once - dt * kvh;  // from a row to the lane's next one
+    int tok = (warp * at_once + sub) / kvh, h = warp * at_once + sub - tok * kvh;
+    const uint16_t* src = base + (int64_t)tok * view.stride_s + h * view.stride_h + c;
+    const int64_t step = dt * view.stride_s + dh * view.stride_h, wrap = view.stride_s - kvh * view.stride_h;
+    uint8_t* pool = a.pool + (k0 + h) * a.head_bytes;  // of the lane's head
+    const int64_t pool_step = dh * a.head_bytes, pool_wrap = kvh * a.head_bytes;
+    auto fetch = [&](int r, const uint16_t* p) {
         Row w;
-        const int r = min(r0 + sub, 2 * nr - 1);
-        w.key = r < nr;
-        const int rr = w.key ? r : r - nr;
-        w.tok = a.shares == 1 ? by_kvh.block(rr) : rr / kvh;
-        w.h = k0 + rr - w.tok * kvh;
-        const b2_kv_view& v = w.key ? a.k : a.v;
-        const uint16_t* src = static_cast<const uint16_t*>(v.data) + b * v.stride_b + (int64_t)(t0 + w.tok) * v.stride_s +
-                              w.h * v.stride_h;
-        w.own = in ? *reinterpret_cast<const uint4*>(src + c) : make_uint4(0, 0, 0, 0);
+        const bool there = in && r < nr;
+        w.own = there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
         w.other[0] = w.other[1] = make_uint2(0, 0);
-        if (w.key && turned) {
+        if (key && turned && there) {
             if (VEC == 8) {
-                const uint4 x = *reinterpret_cast<const uint4*>(src + g0);
+                const uint4 x = *reinterpret_cast<const uint4*>(p + (g0 - c));
                 w.other[0] = make_uint2(x.x, x.y), w.other[1] = make_uint2(x.z, x.w);
             } else {
-                w.other[0] = *reinterpret_cast<const uint2*>(src + g0);
-                w.other[1] = *reinterpret_cast<const uint2*>(src + g1);
+                w.other[0] = *reinterpret_cast<const uint2*>(p + (g0 - c));
+                w.other[1] = *reinterpret_cast<const uint2*>(p + (g1 - c));
             }
         }
         return w;
     };
-    Row ahead = fetch(warp * at_once);
-    for (int r0 = warp * at_once; r0 < 2 * nr; r0 += STEP * at_once) {
+    Row ahead = fetch(warp * at_once + sub, src);
+    for (int r0 = warp * at_once; r0 < nr; r0 += STEP * at_once) {
         const Row row = ahead;
-        if (r0 + STEP * at_once < 2 * nr) ahead = fetch(r0 + STEP * at_once);
-        const bool key = row.key;
-        const int tok = row.tok, h = row.h;
+        const int row_tok = min(tok, nt - 1);
+        uint8_t* const head = pool;
+        src += step;
+        h += dh;
+        tok += dt;
+        pool += pool_step;
+        if (h >= kvh) h -= kvh, ++tok, src += wrap, pool -= pool_wrap;
+        ahead = fetch(r0 + sub + STEP * at_once, src);
         const uint4 own = row.own;
         const uint2 other[2] = {row.other[0], row.other[1]};
-        const int64_t at = s_row[tok];
+        const int64_t at = s_row[row_tok];
         float f[8];
         auto unpack = [&](uint2 x, float* v) {
             const float2 p0 = unpack2<BF16>(x.x), p1 = unpack2<BF16>(x.y);
@@ -242,7 +276,6 @@ __global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const _
         };
         unpack(make_uint2(own.x, own.y), f);
         unpack(make_uint2(own.z, own.w), f + 4);
-        float off = 0.f;  // what f is off by, at most
         if (key && turned) {
             const uint32_t n0 = low0 ? 0x80008000u : 0u, n1 = (VEC == 8 ? low0 : low1) ? 0x80008000u : 0u;
             float g[8];
@@ -250,12 +283,11 @@ __global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const _
             unpack(make_uint2(other[1].x ^ n1, other[1].y ^ n1), g + 4);
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                const float4 t = *reinterpret_cast<const float4*>(&s_cs[tok][VEC == 8 || i < 4 ? e0 + i : e1 + i - 4]);
-                off = fmaxf(off, fmaxf(fabsf(f[i]) + fabsf(g[i]), fabsf(f[i + 1]) + fabsf(g[i + 1])));
-                f[i] = fmaf(f[i], t.x, g[i] * t.y);
-                f[i + 1] = fmaf(f[i + 1], t.z, g[i + 1] * t.w);
+                const float4 t = s_cs[row_tok][(VEC == 8 || i < 4 ? e0 + i : e1 + i - 4) >> 1];
+                const float2 y = two(fma2(pair(make_float2(f[i], f[i + 1])), pair(make_float2(t.x, t.y)),
+                                          mul2(pair(make_float2(g[i], g[i + 1])), pair(make_float2(t.z, t.w)))));
+                f[i] = y.x, f[i + 1] = y.y;
             }
-            off *= 0x1p-21f;  // sine and cosine within 2^-22 (the angle's rounding to 32 bits among it), two roundings
         }
         float lo = f[0], hi = f[0], most = fabsf(f[0]);
 #pragma unroll
@@ -270,30 +302,63 @@ __global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const _
             lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
             hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
             most = fmax_nan(most, __shfl_xor_sync(~0u, most, o));
-            off = fmaxf(off, __shfl_xor_sync(~0u, off, o));
         }
         const bool fine = most < INFINITY;
-        auto to_half = [](float x) { return __half2float(__float2half_rn(fminf(fmaxf(x, -65504.f), 65504.f))); };
-        float m = to_half(lo);
-        // the span is off by off + 2^-24 (hi - m), as a 15th of it two roundings more
-        const float span = (hi - m) * (1.f / 15.f), wrong = off * (1.f / 15.f) + span * 0x1p-22f;
-        float s = to_half(fmaxf(span, 0.f));
-        bool sure = to_half(lo - off) == to_half(lo + off) && to_half(fmaxf(span - wrong, 0.f)) == to_half(fmaxf(span + wrong, 0.f));
-        // u as the nearest whole number to t: adding 1.5 * 2^23 leaves it in the low bits
+        // what f is off by, at most: sine and cosine 2^-25 each, a product 2^-24 |x2|, the sum 2^-24 of itself.  Turning
+        // keeps x1^2 + x2^2, so with M the larger of what the two become |x1| + |x2| <= 2 M and |x2| <= 1.42 M: 2^-22 M
+        float off = 0.f;
+        if (key && a.rot) {
+            off = most;
+            for (int o = 8; o < (1 << wide); o <<= 1) off = fmax_nan(off, __shfl_xor_sync(~0u, off, o));
+            off *= 0x1p-22f;
+        }
+        auto to_half = [](float x) { return __half2float(__float2half_rn(x)); };
+        auto finite_half = [&](float x) { return to_half(fminf(fmaxf(x, -65504.f), 65504.f)); };
+        float m = finite_half(lo);
+        // the span is off by off + 2^-24 (hi - m), as a 15th of it by two roundings more
+        const float span = fmaxf((hi - m) * (1.f / 15.f), 0.f), wrong = fmaf(off, 1.f / 15.f, span * 0x1p-22f);
+        float s = to_half(fminf(span, 65504.f));
+        bool sure = to_half(span - wrong) == to_half(span + wrong);
+        if (key) sure = sure && to_half(lo - off) == to_half(lo + off);
+        sure = sure && most < 65000.f;
+        // u as the nearest whole number to t = (f - m) / s, cut to 0 .. 15: a 15th of it is cut to 0 .. 1 by its
+        // multiply-add; adding 1.5 * 2^23 then leaves the whole number in the low bits
         constexpr float MAGIC = 12582912.f;
-        const float rs = s > 0.f ? __frcp_rn(s) : 0.f;
+        const float rs = s > 0.f ? __frcp_rn(s) : 0.f, r15 = rs * (1.f / 15.f), m15 = -m * r15;
         uint32_t codes = 0;
         float worst = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float t = fminf(fmaxf((f[i] - m) * rs, 0.f), 15.f), v = t + MAGIC;
-            worst = fmaxf(worst, fabsf(t - (v - MAGIC)));
+            const float t = __saturatef(fmaf(f[i], r15, m15)), v = fmaf(t, 15.f, MAGIC);
+            worst = fmaxf(worst, fabsf(fmaf(t, 15.f, MAGIC - v)));
             codes += __float_as_uint(v) << (4 * i);
         }
         codes -= 0x4b400000u * 0x11111111u;
-        // t is off by (off + 2^-23 most) / s and 2^-22 of itself: nearer to a half than that, it may round otherwise
+        // t is off by (off + 2^-21 most) / s and 2^-18: nearer to a half than that, it may round otherwise
         if (!in) worst = 0.f;
-        sure = sure && worst < 0.5f - ((off + most * 0x1p-23f) * rs + 0x1p-18f);
+        bool near = !(worst < 0.5f - (fmaf(most, 0x1p-21f, off) * rs + 0x1p-18f));
+        if (__any_sync(~0u, near && fine && off == 0.f)) {
+            // numbers of 8 or 11 bits often lie half way exactly (1 group in 30 of bf16): what is left of f - m is exact in
+            // 32 bits then, where f - m is
+            bool exact = true;
+            uint32_t fixed = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = f[i] - m, back = d - f[i];
+                exact = exact && (f[i] - (d - back)) == (m + back);
+                float u = fminf(fmaxf(rintf(d * rs), 0.f), 15.f);
+                const float left = fmaf(-u, s, d);
+                const bool odd = (int)u & 1;
+                if (left > 0.5f * s || (left == 0.5f * s && odd)) u += 1.f;
+                if (left < -0.5f * s || (left == -0.5f * s && odd)) u -= 1.f;
+                fixed |= (uint32_t)fminf(fmaxf(u, 0.f), 15.f) << (4 * i);
+            }
+            if (off == 0.f) {
+                codes = s > 0.f ? fixed : 0u;
+                near = near && !exact;
+            }
+        }
+        sure = sure && !near;
         if (__any_sync(~0u, !(sure || !fine || empty))) {
             // in 64 bits
             double x[8];
@@ -301,7 +366,7 @@ __global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const _
                 float u[4], g[4];
                 unpack(own4, u);
                 unpack(oth, g);
-                const int64_t pos = first + tok;
+                const int64_t pos = first + row_tok;
 #pragma unroll 1
                 for (int i = 0; i < 4; ++i) {
                     y[i] = u[i];
@@ -323,23 +388,21 @@ __global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const _
                 l = y < l ? y : l;
                 u = z > u ? z : u;
             }
-            m = to_half((float)l);
-            s = to_half(fmaxf((float)((u - (double)m) / 15.0), 0.f));
+            m = finite_half((float)l);
+            s = finite_half(fmaxf((float)((u - (double)m) / 15.0), 0.f));
             codes = 0;
             for (int i = 0; i < 8; ++i) {
                 const double t = s > 0.f ? rint((x[i] - (double)m) / (double)s) : 0.0;
                 codes |= (uint32_t)(t < 0.0 ? 0.0 : t > 15.0 ? 15.0 : t) << (4 * i);
             }
         }
-        if (at < 0 || r0 + sub >= 2 * nr || c >= DP) continue;
+        if (at == kNoRow || r0 + sub >= nr || c >= DP) continue;
         if (!in || !fine) codes = 0;
-        const int p = (int)(at & 15);
-        uint8_t* tile = a.pool + (at >> 4) + h * a.head_bytes;
+        uint8_t* tile = head + at;
         if (key) {
-            const int j = c >> 3;
-            *reinterpret_cast<uint32_t*>(tile + p * (DP / 2) + ((j & 3) * (DP / 32) + (j >> 2)) * 4) = codes;
+            *reinterpret_cast<uint32_t*>(tile + s_in[row_tok][0] + in_k) = codes;
         } else {
-            uint8_t* to = tile + 8 * DP + (((c >> 5) * 8 + ((c & 31) >> 2)) * 4 + ((p & 7) >> 1)) * 8 + (p >> 3) * 4 + (p & 1) * 2;
+            uint8_t* to = tile + s_in[row_tok][1] + in_v;
             *reinterpret_cast<uint16_t*>(to) = (uint16_t)codes;
             *reinterpret_cast<uint16_t*>(to + 32) = (uint16_t)(codes >> 16);
         }
@@ -347,8 +410,13 @@ __global__ void __launch_bounds__(kApThreads, KV4 ? 3 : 4) append_kernel(const _
             __half2 sm = __floats2half2_rn(s, m);
             if (!fine) sm = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff));
             if (empty) sm = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-            *reinterpret_cast<__half2*>(tile + 16 * DP + (key ? 0 : 64 * NG) + (kv4_slot(p) * NG + (c >> 6)) * 4) = sm;
+            *reinterpret_cast<__half2*>(tile + s_in[row_tok][2] + (key ? 0 : 64 * NG) + in_s) = sm;
         }
+    }
+    };
+    if (nr > 0) {
+        rows_of(std::true_type{});
+        rows_of(std::false_type{});
     }
 }
 
@@ -466,7 +534,7 @@ static int append_args(AppendArgs& a, const b2_kv_view* q, const b2_kv_view* q_o
     for (int i = 0; i < rot / 2; ++i) a.turns[i] = inv_freq[i] / 6.283185307179586476925286766559;
     // whole tokens while they fill the GPU, shares of the heads else
     a.tokens = S < kApTokens ? (int)S : kApTokens;
-    while (a.tokens > 1 && (S + a.tokens - 1) / a.tokens * batch < 2 * sm_count()) a.tokens /= 2;
+    while (a.tokens > 1 && (S + a.tokens - 1) / a.tokens * batch < 3 * sm_count()) a.tokens /= 2;
     const int64_t ctas = (S + a.tokens - 1) / a.tokens * batch;
     a.shares = 1;
     while (a.shares < nkv && a.shares < 8 && ctas * a.shares * 2 <= sm_count()) a.shares *= 2;
@@ -478,7 +546,6 @@ static int append_args(AppendArgs& a, const b2_kv_view* q, const b2_kv_view* q_o
 template <bool KV4>
 static int append_launch(AppendArgs& a, int batch, cudaStream_t s) {
     const int vec = (a.rot / 2) % 8 == 0 ? 8 : 4;
-    a.by_kvh = block_div(a.nkv);
     a.per = a.rot / (2 * vec) + (a.D - a.rot + 2 * vec - 1) / (2 * vec);
     const dim3 grid((unsigned)((a.S + a.tokens - 1) / a.tokens), (unsigned)(KV4 ? a.q_shares + a.shares : a.shares), (unsigned)batch);
     if (a.bf16)
