@@ -431,12 +431,13 @@ int b2_paged_decode_gqa_blocks(const void* q, int64_t ldq, const b2_paged_kv* kv
  *
  * Sequences of one call must not share the blocks that they write.  Allocates
  * nothing; graph-capturable.  S at most 2^30, batch at most 65535. */
-int b2_paged_kv_append(const b2_paged_kv* kv, b2_kv_view k, b2_kv_view v, const b2_kv_view* q, const b2_kv_view* q_out,
-                       const double* inv_freq, int rotary_dim, const int* counts, const int* positions, int batch,
-                       int64_t S, int num_q_heads, int num_kv_heads, int head_dim, void* stream);
+int b2_paged_kv_append(const b2_paged_kv* kv, const b2_kv_view* k, const b2_kv_view* v, const b2_kv_view* q,
+                       const b2_kv_view* q_out, const double* inv_freq, int rotary_dim, const int* counts,
+                       const int* positions, int batch, int64_t S, int num_q_heads, int num_kv_heads, int head_dim,
+                       void* stream);
 /* The same into a cache held in 4 bits.  Keys are rotated in 64 bits and every
  * code is the one of exact arithmetic (m and s by way of 32 bits). */
-int b2_paged_kv4_append(const b2_paged_kv4* kv, b2_kv_view k, b2_kv_view v, const b2_kv_view* q,
+int b2_paged_kv4_append(const b2_paged_kv4* kv, const b2_kv_view* k, const b2_kv_view* v, const b2_kv_view* q,
                         const b2_kv_view* q_out, const double* inv_freq, int rotary_dim, const int* counts,
                         const int* positions, int batch, int64_t S, int num_q_heads, int num_kv_heads, int head_dim,
                         void* stream);
@@ -447,8 +448,8 @@ int b2_paged_kv4_append(const b2_paged_kv4* kv, b2_kv_view k, b2_kv_view v, cons
  * rows 0 .. n-1 of k_out and v_out, [batch][T][num_kv_heads][head_dim] views as
  * above.  Other rows, and those whose table entry is outside [0, num_blocks),
  * are left as they were. */
-int b2_paged_kv4_read(const b2_paged_kv4* kv, b2_kv_view k_out, b2_kv_view v_out, const int* counts, int batch,
-                      int64_t T, int num_kv_heads, int head_dim, void* stream);
+int b2_paged_kv4_read(const b2_paged_kv4* kv, const b2_kv_view* k_out, const b2_kv_view* v_out, const int* counts,
+                      int batch, int64_t T, int num_kv_heads, int head_dim, void* stream);
 
 /* Channel-wise bounds of the keys of each block, for the choice below: codes is
  * int8 [num_blocks][num_kv_heads][2][head_dim] (lower bounds, upper ones; 16-byte

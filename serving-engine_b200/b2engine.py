@@ -8,6 +8,8 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
+import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libb2engine.so")
@@ -89,9 +91,9 @@ _SIGS = {
     "b2_kv4_tile_bytes": (C.c_size_t, [i32]),
     "b2_paged_kv4_decode_gqa": (i32, [vp, i64, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
     "b2_paged_kv4_decode_workspace_bytes": (C.c_size_t, [i32, i32, i32]),
-    "b2_paged_kv_append": (i32, [vp, KVView, KVView, vp, vp, vp, i32, vp, vp, i32, i64, i32, i32, i32, vp]),
-    "b2_paged_kv4_append": (i32, [vp, KVView, KVView, vp, vp, vp, i32, vp, vp, i32, i64, i32, i32, i32, vp]),
-    "b2_paged_kv4_read": (i32, [vp, KVView, KVView, vp, i32, i64, i32, i32, vp]),
+    "b2_paged_kv_append": (i32, [vp, vp, vp, vp, vp, vp, i32, vp, vp, i32, i64, i32, i32, i32, vp]),
+    "b2_paged_kv4_append": (i32, [vp, vp, vp, vp, vp, vp, i32, vp, vp, i32, i64, i32, i32, i32, vp]),
+    "b2_paged_kv4_read": (i32, [vp, vp, vp, vp, i32, i64, i32, i32, vp]),
     "b2_paged_block_bounds": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
     "b2_paged_kv4_block_bounds": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
     "b2_paged_block_select": (i32, [vp, i64, i32, vp, vp, i32, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
@@ -372,6 +374,8 @@ class PagedKV:
     through .transpose(1, 2)), block_tables int32 [B, max_blocks] and
     seq_lens int32 [B].  Holds references to the tensors, copies nothing."""
 
+    four = False
+
     def __init__(self, k, v, block_tables, seq_lens):
         torch = _torch()
         # the stride of a dimension of one may be anything and is never used
@@ -413,6 +417,8 @@ class PagedKV4:
     further apart), block_tables int32 [B, max_blocks] and seq_lens int32 [B];
     dtype is that of the rows that go in and come out.  Holds references to the
     tensors, copies nothing."""
+
+    four = True
 
     def __init__(self, pool, block_tables, seq_lens, head_dim, dtype):
         torch = _torch()
@@ -478,7 +484,7 @@ def paged_decode_gqa(q, kv, out, window=0, sinks=0, scores=None, ws: Workspace |
         _need(blocks, "blocks", _torch().int32, (B, kv.nkv, n), dev)
         lst = blocks.data_ptr()
     wsh, st = ws.h if ws is not None else None, _stream_of(stream, dev)
-    if isinstance(kv, PagedKV4):
+    if kv.four:
         if scores is not None:
             raise ValueError("a cache held in 4 bits keeps no scores")
         call("b2_paged_kv4_decode_gqa", q.data_ptr(), ldq, kv.ref, lst, n, out.data_ptr(), B, nq, kv.nkv, D,
@@ -534,15 +540,28 @@ class Rope:
         self.ref = C.addressof(self.inv_freq)
 
 
-def _rows(t, name, B, S, D, dtype, dev):
-    """View of [B, S, heads, D] rows."""
-    if t.dim() != 4 or t.shape[0] != B or t.shape[1] != S or t.shape[3] != D or t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype} [{B}, {S}, heads, {D}], got {t.dtype} {tuple(t.shape)}")
-    if t.get_device() != dev:
-        raise ValueError(f"{name} is on {t.device}, the cache on cuda:{dev}")
+_PACK2, _PACK4 = struct.Struct("10q").pack_into, struct.Struct("20q").pack_into
+_LOCAL = threading.local()
+
+
+def _views():
+    """Room for four KVViews and its address, one per thread: the library reads them before a call returns, and
+    filling them costs a tenth of what making KVViews does (2 us a call)."""
+    try:
+        return _LOCAL.views
+    except AttributeError:
+        buf = (i64 * 20)()
+        _LOCAL.views = buf, C.addressof(buf)
+        return _LOCAL.views
+
+
+def _rows(t, name, shape, dtype, dev):
+    """A KVView's numbers for [B, S, heads, D] rows."""
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must be {dtype} {shape} on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     b, s, h, d = t.stride()
     # the stride of a dimension of one may be anything and is never used
-    return KVView(t.data_ptr(), b if B > 1 else 0, h if t.shape[2] > 1 else 0, s if S > 1 else 0, d if D > 1 else 1)
+    return t.data_ptr(), b if shape[0] > 1 else 0, h if shape[2] > 1 else 0, s if shape[1] > 1 else 0, d
 
 
 def paged_kv_append(kv, k, v, q=None, q_out=None, rope: Rope | None = None, counts=None, positions=None, stream=None):
@@ -557,32 +576,41 @@ def paged_kv_append(kv, k, v, q=None, q_out=None, rope: Rope | None = None, coun
     dev = _device_of(k, "k")
     if kv.device != dev:
         raise ValueError(f"k is on {k.device}, the cache on cuda:{kv.device}")
-    if k.dim() != 4 or k.shape[2] != kv.nkv or v.shape != k.shape:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not fit a cache of {kv.nkv} heads of {kv.head_dim}")
-    B, S, D = kv.batch, k.shape[1], kv.head_dim
-    kview, vview = _rows(k, "k", B, S, D, kv.dtype, dev), _rows(v, "v", B, S, D, kv.dtype, dev)
-    qr = qor = None
+    B, D, dtype = kv.batch, kv.head_dim, kv.dtype
+    if k.dim() != 4:
+        raise ValueError(f"k must be [{B}, S, {kv.nkv}, {D}], got {tuple(k.shape)}")
+    S = k.shape[1]
+    shape = (B, S, kv.nkv, D)
+    kn, vn = _rows(k, "k", shape, dtype, dev), _rows(v, "v", shape, dtype, dev)
     nq = 0
     if q is not None:
-        if q_out is None:
-            q_out = q
-        if q_out.shape != q.shape:
-            raise ValueError(f"q_out {tuple(q_out.shape)} must have q's shape {tuple(q.shape)}")
-        qview, qoview = _rows(q, "q", B, S, D, kv.dtype, dev), _rows(q_out, "q_out", B, S, D, kv.dtype, dev)
-        nq, qr, qor = q.shape[2], C.addressof(qview), C.addressof(qoview)
+        if q.dim() != 4:
+            raise ValueError(f"q must be [{B}, {S}, heads, {D}], got {tuple(q.shape)}")
+        nq = q.shape[2]
+        shape = (B, S, nq, D)
+        qn = _rows(q, "q", shape, dtype, dev)
+        views, at = _views()
+        _PACK4(views, 0, *kn, *vn, *qn, *(qn if q_out is None else _rows(q_out, "q_out", shape, dtype, dev)))
+        qr, qor = at + 80, at + 120
     elif q_out is not None:
         raise ValueError("q_out without q")
-    cp = pp = None
+    else:
+        views, at = _views()
+        _PACK2(views, 0, *kn, *vn)
+        qr = qor = None
+    cp = pp = rp = None
+    rot = 0
+    if rope is not None:
+        rp, rot = rope.ref, rope.rotary_dim
     if counts is not None:
-        _need(counts, "counts", _torch().int32, (B,), dev)
+        _need(counts, "counts", _TORCH.int32, (B,), dev)
         cp = counts.data_ptr()
     if positions is not None:
-        _need(positions, "positions", _torch().int32, (B,), dev)
+        _need(positions, "positions", _TORCH.int32, (B,), dev)
         pp = positions.data_ptr()
-    call("b2_paged_kv4_append" if isinstance(kv, PagedKV4) else "b2_paged_kv_append", kv.ref, kview, vview, qr, qor,
-         rope.ref if rope is not None else None, rope.rotary_dim if rope is not None else 0, cp, pp, B, S, nq, kv.nkv, D,
-         _stream_of(stream, dev))
-    return q_out
+    call("b2_paged_kv4_append" if kv.four else "b2_paged_kv_append", kv.ref, at, at + 40, qr, qor, rp, rot, cp, pp, B, S, nq,
+         kv.nkv, D, _stream_of(stream, dev))
+    return q if q_out is None else q_out
 
 
 def paged_kv_read(kv: PagedKV4, k_out, v_out, counts=None, stream=None):
@@ -590,21 +618,23 @@ def paged_kv_read(kv: PagedKV4, k_out, v_out, counts=None, stream=None):
     min(counts, T, length) positions, in order, into k_out and v_out [B, T, nkv, D]
     (any strides with contiguous 16-byte-aligned rows; other rows are left as they
     were)."""
-    if not isinstance(kv, PagedKV4):
+    if not kv.four:
         raise ValueError("only a cache held in 4 bits is read back: a PagedKV's rows are its tensors")
     dev = _device_of(k_out, "k_out")
     if kv.device != dev:
         raise ValueError(f"k_out is on {k_out.device}, the cache on cuda:{kv.device}")
-    if k_out.dim() != 4 or k_out.shape[2] != kv.nkv or v_out.shape != k_out.shape:
-        raise ValueError(f"k_out {tuple(k_out.shape)} and v_out {tuple(v_out.shape)} do not fit a cache of {kv.nkv} heads "
-                         f"of {kv.head_dim}")
-    B, T, D = kv.batch, k_out.shape[1], kv.head_dim
-    kview, vview = _rows(k_out, "k_out", B, T, D, kv.dtype, dev), _rows(v_out, "v_out", B, T, D, kv.dtype, dev)
+    B, D = kv.batch, kv.head_dim
+    if k_out.dim() != 4:
+        raise ValueError(f"k_out must be [{B}, T, {kv.nkv}, {D}], got {tuple(k_out.shape)}")
+    T = k_out.shape[1]
+    shape = (B, T, kv.nkv, D)
+    views, at = _views()
+    _PACK2(views, 0, *_rows(k_out, "k_out", shape, kv.dtype, dev), *_rows(v_out, "v_out", shape, kv.dtype, dev))
     cp = None
     if counts is not None:
-        _need(counts, "counts", _torch().int32, (B,), dev)
+        _need(counts, "counts", _TORCH.int32, (B,), dev)
         cp = counts.data_ptr()
-    call("b2_paged_kv4_read", kv.ref, kview, vview, cp, B, T, kv.nkv, D, _stream_of(stream, dev))
+    call("b2_paged_kv4_read", kv.ref, at, at + 40, cp, B, T, kv.nkv, D, _stream_of(stream, dev))
 
 
 class BlockBounds:
@@ -642,7 +672,7 @@ def paged_block_bounds(kv, bounds: BlockBounds, newest=None, stream=None):
     if newest is not None:
         _need(newest, "newest", _torch().int32, (kv.batch,), dev)
         np_ = newest.data_ptr()
-    call("b2_paged_kv4_block_bounds" if isinstance(kv, PagedKV4) else "b2_paged_block_bounds", kv.ref, np_,
+    call("b2_paged_kv4_block_bounds" if kv.four else "b2_paged_block_bounds", kv.ref, np_,
          bounds.codes.data_ptr(), bounds.scale.data_ptr(), kv.batch, kv.nkv, kv.head_dim, _stream_of(stream, dev))
 
 

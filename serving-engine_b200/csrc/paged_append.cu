@@ -9,7 +9,7 @@
 //   / 15), u = (x - m) / s rounded to even and clamped to 0 .. 15
 //
 // One read of q, k and v and one write of q and the rows: HBM bounds long
-// prompts, latency single tokens.  A CTA takes up to 16 consecutive tokens of a
+// prompts, latency single tokens.  A CTA takes up to 8 consecutive tokens of a
 // sequence (all heads, or a share of them where there are few tokens), so the
 // angles are worked out once per token and not per head.  The angle is kept as
 // turns: position times f / 2 pi in 64 bits, its whole part dropped, so that far
@@ -33,7 +33,7 @@ namespace b2 {
 using namespace packed;
 
 constexpr int kApThreads = 256;
-constexpr int kApTokens = 16;
+constexpr int kApTokens = 8;
 constexpr int64_t kNoRow = INT64_MIN;  // a token whose rows have no place
 
 struct AppendArgs {
@@ -513,17 +513,17 @@ static bool rows_fit(const b2_kv_view& v) {
 }
 
 // What both kinds of cache share: arguments checked and filled in but for the cache.
-static int append_args(AppendArgs& a, const b2_kv_view* q, const b2_kv_view* q_out, b2_kv_view k, b2_kv_view v,
+static int append_args(AppendArgs& a, const b2_kv_view* q, const b2_kv_view* q_out, const b2_kv_view* k, const b2_kv_view* v,
                        const double* inv_freq, int rot, const int* counts, const int* positions, int batch, int64_t S,
                        int nq, int nkv, int D) {
-    B2_REQUIRE(k.data && v.data && nkv > 0 && D > 0 && rot >= 0 && (rot == 0 || inv_freq) && !q == !q_out);
+    B2_REQUIRE(k && v && k->data && v->data && nkv > 0 && D > 0 && rot >= 0 && (rot == 0 || inv_freq) && !q == !q_out);
     B2_REQUIRE(!q || (q->data && q_out->data && nq > 0));
-    if (rot > D || (rot & 7) || S > (1 << 30) || batch > 65535 || !rows_fit(k) || !rows_fit(v) ||
+    if (rot > D || (rot & 7) || S > (1 << 30) || batch > 65535 || !rows_fit(*k) || !rows_fit(*v) ||
         (q && (!rows_fit(*q) || !rows_fit(*q_out))))
         return B2_ERR_UNSUPPORTED;
     if (q) a.q = *q, a.q_out = *q_out;
-    a.k = k;
-    a.v = v;
+    a.k = *k;
+    a.v = *v;
     a.counts = counts;
     a.positions = positions;
     a.S = (int)S;
@@ -565,7 +565,7 @@ static cudaError_t read_launch(const ReadArgs& a, dim3 grid, cudaStream_t s) {
 
 }  // namespace b2
 
-extern "C" int b2_paged_kv_append(const b2_paged_kv* kv, b2_kv_view k, b2_kv_view v, const b2_kv_view* q,
+extern "C" int b2_paged_kv_append(const b2_paged_kv* kv, const b2_kv_view* k, const b2_kv_view* v, const b2_kv_view* q,
                                   const b2_kv_view* q_out, const double* inv_freq, int rotary_dim, const int* counts,
                                   const int* positions, int batch, int64_t S, int nq, int nkv, int D, void* stream) {
     using namespace b2;
@@ -585,7 +585,7 @@ extern "C" int b2_paged_kv_append(const b2_paged_kv* kv, b2_kv_view k, b2_kv_vie
     return append_launch<false>(a, batch, as_stream(stream));
 }
 
-extern "C" int b2_paged_kv4_append(const b2_paged_kv4* kv, b2_kv_view k, b2_kv_view v, const b2_kv_view* q,
+extern "C" int b2_paged_kv4_append(const b2_paged_kv4* kv, const b2_kv_view* k, const b2_kv_view* v, const b2_kv_view* q,
                                    const b2_kv_view* q_out, const double* inv_freq, int rotary_dim, const int* counts,
                                    const int* positions, int batch, int64_t S, int nq, int nkv, int D, void* stream) {
     using namespace b2;
@@ -607,17 +607,17 @@ extern "C" int b2_paged_kv4_append(const b2_paged_kv4* kv, b2_kv_view k, b2_kv_v
     return append_launch<true>(a, batch, as_stream(stream));
 }
 
-extern "C" int b2_paged_kv4_read(const b2_paged_kv4* kv, b2_kv_view k_out, b2_kv_view v_out, const int* counts,
+extern "C" int b2_paged_kv4_read(const b2_paged_kv4* kv, const b2_kv_view* k_out, const b2_kv_view* v_out, const int* counts,
                                  int batch, int64_t T, int nkv, int D, void* stream) {
     using namespace b2;
     if (batch <= 0 || T <= 0) return B2_OK;
-    B2_REQUIRE(k_out.data && v_out.data);
+    B2_REQUIRE(k_out && v_out && k_out->data && v_out->data);
     const int rc = check_paged4(kv, nkv, D);
     if (rc != B2_OK) return rc;
-    if (!rows_fit(k_out) || !rows_fit(v_out) || batch > 65535 || nkv > 65535 || T > (1 << 30)) return B2_ERR_UNSUPPORTED;
+    if (!rows_fit(*k_out) || !rows_fit(*v_out) || batch > 65535 || nkv > 65535 || T > (1 << 30)) return B2_ERR_UNSUPPORTED;
     ReadArgs a = {};
-    a.k = k_out;
-    a.v = v_out;
+    a.k = *k_out;
+    a.v = *v_out;
     a.pool = static_cast<const uint8_t*>(kv->pool);
     a.pool_block = kv->stride_block;
     a.head_bytes = (int64_t)(kv->block_size / 16) * kv4_tile(kv4_dp(D));

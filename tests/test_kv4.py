@@ -50,12 +50,12 @@ FREQ = (C.c_double * 32)(*([1.0] * 32))
 
 def append(kv, k=None, v=None, q=None, q_out=None, freq=FREQ, rot=64, batch=1, S=1, nq=4, nkv=2, D=64):
     fn = b2.lib().b2_paged_kv4_append if isinstance(kv, b2.PagedKV4Struct) else b2.lib().b2_paged_kv_append
-    return fn(ref(kv), k or view(), v or view(), ref(q), ref(q_out), C.addressof(freq) if freq else None, rot, None,
+    return fn(ref(kv), ref(k or view()), ref(v or view()), ref(q), ref(q_out), C.addressof(freq) if freq else None, rot, None,
               None, batch, S, nq, nkv, D, None)
 
 
 def read(kv, k=None, v=None, batch=1, T=1, nkv=2, D=64):
-    return b2.lib().b2_paged_kv4_read(ref(kv), k or view(), v or view(), None, batch, T, nkv, D, None)
+    return b2.lib().b2_paged_kv4_read(ref(kv), ref(k or view()), ref(v or view()), None, batch, T, nkv, D, None)
 
 
 def bounds(kv, codes=FAKE, scale=FAKE, batch=1, nkv=2, D=64):
