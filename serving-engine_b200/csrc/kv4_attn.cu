@@ -44,6 +44,7 @@
 // Split: paged_split.cuh.  Each of 4 warps streams tiles of 16 positions (kv4.cuh)
 // through its own ring of shared-memory stages (cp.async).
 #include <cmath>
+#include <type_traits>
 
 #include "kv4.cuh"
 #include "paged_split.cuh"
@@ -68,14 +69,16 @@ struct Kv4Cfg {
     static constexpr int NG = kv4_groups(DP);
     static constexpr int W = DP / 32;                  // K words of a lane and row, V pieces of a lane
     static constexpr int TILE = kv4_tile(DP);
-    static constexpr int T = DP <= 128 ? 2 : 1;        // tiles per warp and unit
+    // tiles per warp and unit: as many as there are registers for (128 channels, 4 heads: 187 us for 32 x 32768 with 4,
+    // 210 with 2 and three CTAs per SM, 250 with 1 and four)
+    static constexpr int T = DP <= 128 && H <= 8 ? 4 : 2;
     static constexpr int U = kPgWarps * T * 16;        // positions per unit
-    static constexpr int STAGES = DP <= 128 ? 3 : 2;
+    static constexpr int STAGES = DP <= 96 || T == 2 && DP == 128 ? 3 : 2;
     static constexpr int STAGE = T * TILE;
     static constexpr int LDO = DP + 4;
     static constexpr int OFF_O = kPgWarps * STAGES * STAGE;
     static constexpr int BYTES = OFF_O + 2 * H * LDO * 4;
-    static constexpr int CTAS = DP <= 128 ? (H <= 8 ? 3 : 2) : (H <= 8 ? 3 : 2);  // per SM
+    static constexpr int CTAS = 2;                     // per SM
 };
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
@@ -128,7 +131,11 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
     constexpr int NT = H == 16 ? 2 : 1;  // products side by side, 8 heads each
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ SplitShared s_split;
-    __shared__ __align__(4) uint16_t s_vis[kPgWarps][C::STAGES][T];  // visible rows of a tile, first | end << 8; 0: none
+    // what is looked at once a segment or once a batch of units lies here and not in registers: the CTA's place and share,
+    // each warp's place of its next batch
+    __shared__ Place<U, LIST> s_at, s_next[kPgWarps];
+    __shared__ Share s_share;
+    __shared__ __align__(8) uint16_t s_vis[kPgWarps][C::STAGES][T];  // visible rows of a tile, first | end << 8; 0: none
     __shared__ float s_m[kPgWarps][16], s_l[kPgWarps][16];
     __shared__ float2 s_ml[16];
     float* s_o = reinterpret_cast<float*>(smem + C::OFF_O);
@@ -138,16 +145,22 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
     griddep_wait();
     griddep_launch_dependents();
 
-    Share w;
-    Place<U, LIST> at;
-    if (!split_units(a, s_split, w, at)) return;
-    const int r0 = w.r0, r1 = w.r1;
+    int r0, r1, seg0, seg_n;  // this CTA's units; the current segment's first one and how many it has
+    {
+        Share w;
+        Place<U, LIST> at;
+        if (!split_units(a, s_split, w, at)) return;
+        r0 = w.r0, r1 = w.r1;
+        seg0 = r0 - at.u, seg_n = at.s.n;
+        if (lane == 0) s_next[warp] = at;
+        if (tid == 0) s_at = at, s_share = w;
+        __syncthreads();
+    }
 
     // ---- producer: tiles of the next unit into a stage.  Where they are is looked up for up to 32 tiles of the warp at a
     // time, one per lane, a batch before it is needed (looked up unit by unit, that alone was 100 of 380 instructions a
     // tile)
     constexpr int BATCH = 32 / T;            // units of a batch, all of one segment
-    Place<U, LIST> pp = at;
     int pr = r0, pf = r0;                    // units requested, units looked up
     int used = 0, count = 0, next = 0;       // units of the current batch: requested, all; units of the next batch
     int pid = -1, vis2 = 0, vis = 0;         // table entry and visible rows (first | end << 8) of the next batch; current
@@ -155,8 +168,10 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
     auto lookup = [&]() {
         pid = -1;
         vis2 = 0;
+        next = 0;
+        if (pf >= r1) return;
+        Place<U, LIST> pp = s_next[warp];
         next = min(BATCH, min(pp.s.n - pp.u, r1 - pf));
-        if (next <= 0) return;
         const int u = pp.u + lane / T;
         if (lane < next * T) {
             const int pos = pp.s.base(u) + (warp * T + lane % T) * 16;
@@ -182,6 +197,9 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
         pf += next;
         pp.u += next - 1;
         pp.next(a);
+        __syncwarp();
+        if (lane == 0) s_next[warp] = pp;
+        __syncwarp();
     };
     const uint64_t policy = read_once();
     uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
@@ -199,16 +217,23 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
             }
             const int v = __shfl_sync(~0u, vis, used * T + lane % T);
             if (lane < T) s_vis[warp][stage][lane] = (uint16_t)v;
+            int64_t f[T];
+            bool all = true;
 #pragma unroll
-            for (int t = 0; t < T; ++t) {
-                const int64_t f = __shfl_sync(~0u, from, used * T + t);
-                if (f >= 0) {
-                    const uint32_t dst = ring_at + stage * C::STAGE + t * C::TILE;
+            for (int t = 0; t < T; ++t) f[t] = __shfl_sync(~0u, from, used * T + t), all = all && f[t] >= 0;
+            auto copy = [&](int t) {
+                const uint32_t dst = ring_at + stage * C::STAGE + t * C::TILE;
 #pragma unroll
-                    for (int i = 0; i < (C::TILE + 511) / 512; ++i)
-                        if (i < C::TILE / 512 || lane * 16 < C::TILE % 512)
-                            cp16(dst + i * 512, pool + f + i * 512, true, policy);
-                }
+                for (int i = 0; i < (C::TILE + 511) / 512; ++i)
+                    if (i < C::TILE / 512 || lane * 16 < C::TILE % 512) cp16(dst + i * 512, pool + f[t] + i * 512, true, policy);
+            };
+            if (all) {
+#pragma unroll
+                for (int t = 0; t < T; ++t) copy(t);
+            } else {
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+                    if (f[t] >= 0) copy(t);
             }
             ++used;
             ++pr;
@@ -226,6 +251,7 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
     float o[W][2][NT][4], m[NT][2], l[NT][2], am[NT][2][NG];
     int E;                                       // scales of V below 2^E so far: weights are 2^(14 - E) times theirs
     auto start = [&]() {  // a new segment (or the rest of one): its queries, nothing summed yet
+        const Place<U, LIST>& at = s_at;
         const int h0 = at.head0(a), nh = at.heads(a);
         const uint16_t* q = static_cast<const uint16_t*>(a.q) + at.b * a.ldq + (int64_t)h0 * a.D;
 #pragma unroll
@@ -307,13 +333,11 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
     for (int r = r0; r < r1; ++r) {
         cp_wait<C::STAGES - 1>();
         __syncwarp();
-        uint32_t seen;
-        if constexpr (T == 2)
-            seen = *reinterpret_cast<const uint32_t*>(s_vis[warp][stage]);
-        else
-            seen = s_vis[warp][stage][0];
+        using Seen16 = std::conditional_t<T == 4, uint64_t, std::conditional_t<T == 2, uint32_t, uint16_t>>;
+        const Seen16 seen = *reinterpret_cast<const Seen16*>(s_vis[warp][stage]);  // 16 bits a tile
+        constexpr Seen16 kFull = (Seen16)0x1000100010001000ull;
         const uint8_t* const unit = ring + stage * C::STAGE;
-        if (__any_sync(~0u, seen != 0u)) {
+        if (__any_sync(~0u, seen != 0)) {
             constexpr float zero[4] = {0.f, 0.f, 0.f, 0.f};
             float x[T][NT][4];        // scores of (lr, 2 lc), (lr, 2 lc + 1), (lr + 8, ..)
             uint32_t vm[T][2][NG];    // scale words of V at positions lr and lr + 8
@@ -367,10 +391,10 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[t][n][i] = fmaf(x[t][n][i], 1048576.f, y[n][i]);
             }
-            if (seen != (T == 2 ? 0x10001000u : 0x1000u)) {  // rows that are not visible hold anything
+            if (seen != kFull) {  // rows that are not visible hold anything
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
-                    const int v0 = seen >> (16 * t) & 255, v1 = seen >> (16 * t + 8) & 255;
+                    const int v0 = (int)(seen >> (16 * t)) & 255, v1 = (int)(seen >> (16 * t + 8)) & 255;
 #pragma unroll
                     for (int pp = 0; pp < 2; ++pp) {
                         const bool there = lr + 8 * pp >= v0 && lr + 8 * pp < v1;
@@ -517,8 +541,7 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
         issue(stage);
         stage = stage + 1 == C::STAGES ? 0 : stage + 1;
 
-        const bool done = at.u == at.s.n - 1;
-        if (done || r == r1 - 1) {
+        if (r - seg0 == seg_n - 1 || r == r1 - 1) {
             // ---- the warps meet: max and sum of each head, then the outputs, in warp order
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -593,15 +616,21 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                 const float4 y = *reinterpret_cast<const float4*>(s_o + (H + row) * C::LDO + d);
                 return make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
             };
+            Place<U, LIST> at = s_at;
+            Share w = s_share;
+            at.u = r - seg0;
             finish_piece(a, s_split, w, at, r, piece0, s_ml, sum, [&](int64_t i, float4 v, float scale) {
                 store4<BF16>(a.out, i, v, scale);
             });
             __syncthreads();
-            at.next(a);
-            piece0 = r + 1;
-            if (r + 1 < r1) start();
-        } else {
-            at.next(a);
+            if (r + 1 < r1) {
+                at.next(a);
+                seg0 = piece0 = r + 1;
+                seg_n = at.s.n;
+                if (tid == 0) s_at = at;
+                __syncthreads();
+                start();
+            }
         }
     }
 }
@@ -611,30 +640,19 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
 // ---------------------------------------------------------------------------
 
 struct Kv4Sizes {
-    int gs, hg, h, ctas, grid, unit;
+    int gs, hg, h, grid;
     size_t parts, pml;  // bytes
 };
 
-template <int DP>
-static void kv4_shape(Kv4Sizes& z) {
-    z.ctas = z.h == 16 ? Kv4Cfg<DP, 16>::CTAS : z.h == 8 ? Kv4Cfg<DP, 8>::CTAS : Kv4Cfg<DP, 4>::CTAS;
-    z.unit = Kv4Cfg<DP, 4>::U;
-}
-// Segments take up to 16 heads; a larger group is cut evenly.
+// Segments take up to 16 heads, 8 above 128 channels (the outputs of 16 would not fit the registers); a larger group is
+// cut evenly.
 static Kv4Sizes kv4_sizes(int nq, int nkv, int D) {
     Kv4Sizes z = {};
-    const int group = nq / nkv;
-    z.hg = (group + 15) / 16;
+    const int group = nq / nkv, most = D <= 128 ? 16 : 8;
+    z.hg = (group + most - 1) / most;
     z.gs = (group + z.hg - 1) / z.hg;
     z.h = z.gs <= 4 ? 4 : z.gs <= 8 ? 8 : 16;
-    switch (kv4_dp(D)) {
-        case 64: kv4_shape<64>(z); break;
-        case 96: kv4_shape<96>(z); break;
-        case 128: kv4_shape<128>(z); break;
-        case 192: kv4_shape<192>(z); break;
-        default: kv4_shape<256>(z); break;
-    }
-    z.grid = sm_count() * z.ctas;
+    z.grid = sm_count() * Kv4Cfg<128, 4>::CTAS;
     z.parts = (size_t)2 * z.grid * z.gs * D * sizeof(float);
     z.pml = (size_t)2 * z.grid * z.gs * sizeof(float2);
     return z;
@@ -654,8 +672,9 @@ static int kv4_dispatch(const Kv4Args& a, const Kv4Sizes& z, cudaStream_t s) {
 }
 template <int DP, bool LIST>
 static int kv4_dispatch(const Kv4Args& a, const Kv4Sizes& z, cudaStream_t s) {
-    return z.h == 16 ? kv4_dispatch<DP, 16, LIST>(a, z, s)
-                     : z.h == 8 ? kv4_dispatch<DP, 8, LIST>(a, z, s) : kv4_dispatch<DP, 4, LIST>(a, z, s);
+    if constexpr (DP <= 128)
+        if (z.h == 16) return kv4_dispatch<DP, 16, LIST>(a, z, s);
+    return z.h == 8 ? kv4_dispatch<DP, 8, LIST>(a, z, s) : kv4_dispatch<DP, 4, LIST>(a, z, s);
 }
 template <bool LIST>
 static int kv4_dispatch(const Kv4Args& a, const Kv4Sizes& z, cudaStream_t s) {
@@ -693,7 +712,7 @@ extern "C" int b2_paged_kv4_decode_gqa(const void* q, int64_t ldq, const b2_page
     const Kv4Sizes z = kv4_sizes(nq, nkv, D);
     const int64_t span = (int64_t)(blocks ? listed : kv->max_blocks) * kv->block_size;
     // positions and units are counted in 32 bits
-    if (span > (1 << 30) || (int64_t)batch * nkv * z.hg * (span / z.unit + 4) > (1ll << 31) - 1)
+    if (span > (1 << 30) || (int64_t)batch * nkv * z.hg * (span / Kv4Cfg<256, 4>::U + 4) > (1ll << 31) - 1)
         return B2_ERR_UNSUPPORTED;
     Kv4Args a = {};
     a.q = q;
