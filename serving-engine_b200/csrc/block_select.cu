@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(kBdThreads, 7) bounds_kernel(const BoundsArgs 
 static int bounds_launch(const BoundsArgs& a, bool kv4, cudaStream_t s) {
     // the blocks of a head are dealt out in turn to as many CTAs as fill the GPU once
     const int64_t most = (int64_t)a.batch * a.max_blocks;
-    int64_t grid = (8 * sm_count() + a.nkv - 1) / a.nkv;
-    if (grid > most) grid = most;
+    int64_t grid = 7 * sm_count() / a.nkv;
+    grid = grid < 1 ? 1 : grid > most ? most : grid;
     const dim3 g((unsigned)grid, (unsigned)a.nkv);
     if (kv4)
         B2_TRY(launch(bounds_kernel<true, false>, g, dim3(kBdThreads), 0, s, true, a));

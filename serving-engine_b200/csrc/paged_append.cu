@@ -146,7 +146,8 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
         const bool both = c1 < a.D;
         const int tp = min(nt, fit), groups = fit / tp, mine = lead % tp, group = lead / tp;  // tokens, and threads for each
         // rows of `heads` heads from h0 on; TURN: rotated.  Into the cache where `to` is null
-        auto all_of = [&](auto turn, const b2_kv_view& view, int h0, int heads, uint16_t* to, int64_t to_s, int64_t to_h) {
+        auto all_of = [&](auto turn, const b2_kv_view& view, int h0, int heads, uint16_t* to, int64_t to_s, int64_t to_h,
+                          int group, int groups) {
             constexpr bool TURN = decltype(turn)::value;
             constexpr int ON = 4;  // rows of a thread on their way
             for (int tok = mine; tok < nt && group < groups; tok += tp) {
@@ -197,15 +198,23 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
                 }
             }
         };
-        if (q1 > q0)
-            all_of(std::true_type{}, a.q, q0, q1 - q0,
-                   static_cast<uint16_t*>(const_cast<void*>(a.q_out.data)) + b * a.q_out.stride_b + t0 * a.q_out.stride_s +
-                       q0 * a.q_out.stride_h,
-                   a.q_out.stride_s, a.q_out.stride_h);
-        if (!KV4 && k1 > k0) {
-            // (heads are counted from k0 in the cache too)
-            all_of(std::true_type{}, a.k, k0, k1 - k0, nullptr, 0, a.kv.stride_head);
-            all_of(std::false_type{}, a.v, k0, k1 - k0, nullptr, 0, a.kv.stride_head);
+        uint16_t* const qo = static_cast<uint16_t*>(const_cast<void*>(a.q_out.data)) + b * a.q_out.stride_b +
+                             t0 * a.q_out.stride_s + q0 * a.q_out.stride_h;
+        const int nqh = q1 - q0, nkh = KV4 ? 0 : k1 - k0;  // (heads are counted from k0 in the cache too)
+        if (groups < 3 || nqh == 0 || nkh == 0) {
+            if (nqh) all_of(std::true_type{}, a.q, q0, nqh, qo, a.q_out.stride_s, a.q_out.stride_h, group, groups);
+            if (nkh) {
+                all_of(std::true_type{}, a.k, k0, nkh, nullptr, 0, a.kv.stride_head, group, groups);
+                all_of(std::false_type{}, a.v, k0, nkh, nullptr, 0, a.kv.stride_head, group, groups);
+            }
+        } else {  // each thread has queries, keys or values, in the proportion of their heads
+            const int gk = max(1, groups * nkh / (nqh + 2 * nkh)), gq = groups - 2 * gk;
+            if (group < gq)
+                all_of(std::true_type{}, a.q, q0, nqh, qo, a.q_out.stride_s, a.q_out.stride_h, group, gq);
+            else if (group < gq + gk)
+                all_of(std::true_type{}, a.k, k0, nkh, nullptr, 0, a.kv.stride_head, group - gq, gk);
+            else
+                all_of(std::false_type{}, a.v, k0, nkh, nullptr, 0, a.kv.stride_head, group - gq - gk, gk);
         }
     }
     if (!rows4) return;
@@ -214,7 +223,6 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
     const int DP = kv4_dp(a.D), NG = kv4_groups(DP), kvh = k1 - k0;
     const int wide = DP == 64 ? 3 : DP <= 128 ? 4 : 5, at_once = 32 >> wide;
     const int sub = lane >> wide, c = (lane & ((1 << wide) - 1)) * 8;
-    const int nr = nt * kvh;  // rows of K, and of V
     const bool in = c < a.D, turned = c < a.rot;
     const bool empty = (c & ~63) >= a.D;  // a group of padding alone
     // K is rotated with the sign of the sine taken to the partner: whole chunks of 4 channels have one sign
@@ -224,24 +232,33 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
     constexpr int STEP = kApThreads / 32;
     // this lane's places in a K row, among a position's V units, among its scales
     const int in_k = (((c >> 3) & 3) * (DP / 32) + (c >> 5)) * 4, in_v = ((c >> 5) * 8 + ((c & 31) >> 2)) * 32, in_s = (c >> 6) * 4;
-    auto rows_of = [&](auto is_key) {
+    // a warp has a token (several warps where there are fewer tokens than warps): its angles and places stay in registers
+    // while the warp goes through heads, K's from the first warp on, V's from the last one
+    const int team = max(1, STEP / nt), member = warp % team;
+    auto rows_of = [&](auto is_key, int tok, int first_h) {
     constexpr bool key = decltype(is_key)::value;
     const b2_kv_view& view = key ? a.k : a.v;
-    const uint16_t* const base = static_cast<const uint16_t*>(view.data) + b * view.stride_b + t0 * view.stride_s + k0 * view.stride_h;
+    const int64_t at = s_row[tok];
+    const int by = team * at_once;  // heads from a row to the lane's next one
+    int h = first_h + sub;
+    const uint16_t* src = static_cast<const uint16_t*>(view.data) + b * view.stride_b + (int64_t)(t0 + tok) * view.stride_s +
+                          (k0 + h) * view.stride_h + c;
+    uint8_t* tile = a.pool + at + (k0 + h) * a.head_bytes;
+    const int64_t step = by * view.stride_h, tile_step = by * a.head_bytes;
+    const int place = s_in[tok][key ? 0 : 1] + (key ? in_k : in_v), scales = s_in[tok][2] + (key ? 0 : 64 * NG) + in_s;
+    float4 cs[4];
+    if (key && turned) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) cs[i / 2] = s_cs[tok][(VEC == 8 || i < 4 ? e0 + i : e1 + i - 4) >> 1];
+    }
     // a row and the partners of its channels: the next row's are on their way while one is worked on
     struct Row {
         uint4 own;
         uint2 other[2];
     };
-    const int dt = STEP * at_once / kvh, dh = STEP * at_once - dt * kvh;  // from a row to the lane's next one
-    int tok = (warp * at_once + sub) / kvh, h = warp * at_once + sub - tok * kvh;
-    const uint16_t* src = base + (int64_t)tok * view.stride_s + h * view.stride_h + c;
-    const int64_t step = dt * view.stride_s + dh * view.stride_h, wrap = view.stride_s - kvh * view.stride_h;
-    uint8_t* pool = a.pool + (k0 + h) * a.head_bytes;  // of the lane's head
-    const int64_t pool_step = dh * a.head_bytes, pool_wrap = kvh * a.head_bytes;
-    auto fetch = [&](int r, const uint16_t* p) {
+    auto fetch = [&](int hh, const uint16_t* p) {
         Row w;
-        const bool there = in && r < nr;
+        const bool there = in && hh < kvh;
         w.own = there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
         w.other[0] = w.other[1] = make_uint2(0, 0);
         if (key && turned && there) {
@@ -255,20 +272,17 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
         }
         return w;
     };
-    Row ahead = fetch(warp * at_once + sub, src);
-    for (int r0 = warp * at_once; r0 < nr; r0 += STEP * at_once) {
+    Row ahead = fetch(h, src);
+    for (int hb = first_h; hb < kvh; hb += by) {
         const Row row = ahead;
-        const int row_tok = min(tok, nt - 1);
-        uint8_t* const head = pool;
+        const bool mine = h < kvh && c < DP;
+        uint8_t* const to = tile;
         src += step;
-        h += dh;
-        tok += dt;
-        pool += pool_step;
-        if (h >= kvh) h -= kvh, ++tok, src += wrap, pool -= pool_wrap;
-        ahead = fetch(r0 + sub + STEP * at_once, src);
+        h += by;
+        tile += tile_step;
+        ahead = fetch(h, src);
         const uint4 own = row.own;
         const uint2 other[2] = {row.other[0], row.other[1]};
-        const int64_t at = s_row[row_tok];
         float f[8];
         auto unpack = [&](uint2 x, float* v) {
             const float2 p0 = unpack2<BF16>(x.x), p1 = unpack2<BF16>(x.y);
@@ -283,7 +297,7 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
             unpack(make_uint2(other[1].x ^ n1, other[1].y ^ n1), g + 4);
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                const float4 t = s_cs[row_tok][(VEC == 8 || i < 4 ? e0 + i : e1 + i - 4) >> 1];
+                const float4 t = cs[i / 2];
                 const float2 y = two(fma2(pair(make_float2(f[i], f[i + 1])), pair(make_float2(t.x, t.y)),
                                           mul2(pair(make_float2(g[i], g[i + 1])), pair(make_float2(t.z, t.w)))));
                 f[i] = y.x, f[i + 1] = y.y;
@@ -366,7 +380,7 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
                 float u[4], g[4];
                 unpack(own4, u);
                 unpack(oth, g);
-                const int64_t pos = first + row_tok;
+                const int64_t pos = first + tok;
 #pragma unroll 1
                 for (int i = 0; i < 4; ++i) {
                     y[i] = u[i];
@@ -396,27 +410,26 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
                 codes |= (uint32_t)(t < 0.0 ? 0.0 : t > 15.0 ? 15.0 : t) << (4 * i);
             }
         }
-        if (at == kNoRow || r0 + sub >= nr || c >= DP) continue;
+        if (!mine) continue;
         if (!in || !fine) codes = 0;
-        uint8_t* tile = head + at;
         if (key) {
-            *reinterpret_cast<uint32_t*>(tile + s_in[row_tok][0] + in_k) = codes;
+            *reinterpret_cast<uint32_t*>(to + place) = codes;
         } else {
-            uint8_t* to = tile + s_in[row_tok][1] + in_v;
-            *reinterpret_cast<uint16_t*>(to) = (uint16_t)codes;
-            *reinterpret_cast<uint16_t*>(to + 32) = (uint16_t)(codes >> 16);
+            *reinterpret_cast<uint16_t*>(to + place) = (uint16_t)codes;
+            *reinterpret_cast<uint16_t*>(to + place + 32) = (uint16_t)(codes >> 16);
         }
         if ((c & 63) == 0) {
             __half2 sm = __floats2half2_rn(s, m);
             if (!fine) sm = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff));
             if (empty) sm = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-            *reinterpret_cast<__half2*>(tile + s_in[row_tok][2] + (key ? 0 : 64 * NG) + in_s) = sm;
+            *reinterpret_cast<__half2*>(to + scales) = sm;
         }
     }
     };
-    if (nr > 0) {
-        rows_of(std::true_type{});
-        rows_of(std::false_type{});
+    for (int tok = warp / team; tok < nt && warp < nt * team; tok += STEP / team) {
+        if (s_row[tok] == kNoRow) continue;
+        rows_of(std::true_type{}, tok, member * at_once);
+        rows_of(std::false_type{}, tok, (team - 1 - member) * at_once);
     }
 }
 
