@@ -92,8 +92,9 @@ __global__ void __launch_bounds__(kBdThreads, 7) bounds_kernel(const BoundsArgs 
     griddep_launch_dependents();
     // a lane has 8 channels, 8, 16 or 32 lanes a row
     const int DP = kv4_dp(a.D), NG = kv4_groups(DP), wide = DP == 64 ? 3 : DP <= 128 ? 4 : 5;
-    const int sub = lane >> wide, c = (lane & ((1 << wide) - 1)) * 8;
-    const bool in = c < a.D;
+    const int sub = lane >> wide, own_c = (lane & ((1 << wide) - 1)) * 8;
+    const bool in = own_c < a.D;
+    const int c = in ? own_c : 0;  // (lanes past the row read its first channels and keep them to themselves)
     int base = 0;  // blocks of the sequences before b0
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
         // every warp by itself: lane b for the blocks that sequence b0 + b's newest positions lie in
@@ -128,48 +129,43 @@ __global__ void __launch_bounds__(kBdThreads, 7) bounds_kernel(const BoundsArgs 
                 for (int e = 0; e < 8; ++e) lo[e] = INFINITY, hi[e] = -INFINITY;
                 const uint8_t* at = a.pool + (int64_t)id * a.stride_block + h * a.stride_head;
                 const int j = c >> 3, word = ((j & 3) * (DP / 32) + (j >> 2)) * 4, meta = 16 * DP + (c >> 6) * 4;
-                for (int r = r0; r < rows; r += ON * step) {
+                for (int r = 0; r < rows; r += ON * step) {
                     uint32_t w[ON], m[ON];
 #pragma unroll
                     for (int k = 0; k < ON; ++k) {
-                        const int rr = r + k * step;
-                        if (in && rr < rows) {
-                            const uint8_t* tile = at + (rr >> 4) * kv4_tile(DP);
-                            w[k] = *reinterpret_cast<const uint32_t*>(tile + (rr & 15) * (DP / 2) + word);
-                            m[k] = *reinterpret_cast<const uint32_t*>(tile + meta + kv4_slot(rr & 15) * NG * 4);
-                        }
+                        const int rr = min(r + r0 + k * step, rows - 1);  // (the last row once more changes nothing)
+                        const uint8_t* tile = at + (rr >> 4) * kv4_tile(DP);
+                        w[k] = *reinterpret_cast<const uint32_t*>(tile + (rr & 15) * (DP / 2) + word);
+                        m[k] = *reinterpret_cast<const uint32_t*>(tile + meta + kv4_slot(rr & 15) * NG * 4);
                     }
 #pragma unroll
-                    for (int k = 0; k < ON; ++k)
-                        if (in && r + k * step < rows) {
-                            const float2 sm = h2_to_f2(m[k]);
+                    for (int k = 0; k < ON; ++k) {
+                        const float2 sm = h2_to_f2(m[k]);
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float f = fmaf((float)((w[k] >> (4 * e)) & 15), sm.x, sm.y);
-                                lo[e] = min_nan(lo[e], f);
-                                hi[e] = max_nan(hi[e], f);
-                            }
+                        for (int e = 0; e < 8; ++e) {
+                            const float f = fmaf((float)((w[k] >> (4 * e)) & 15), sm.x, sm.y);
+                            lo[e] = min_nan(lo[e], f);
+                            hi[e] = max_nan(hi[e], f);
                         }
+                    }
                 }
             } else {
                 // (of 16-bit numbers the least and the largest are such numbers: two at a time, a NaN staying one)
                 uint32_t l[4], u[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) l[e] = BF16 ? 0x7f807f80u : 0x7c007c00u, u[e] = l[e] | 0x80008000u;
-                const int64_t inc = step * a.stride_slot;
-                const uint16_t* p = a.k + (int64_t)id * a.stride_block + (int64_t)h * a.stride_head + c + r0 * a.stride_slot;
-                for (int r = r0; r < rows; r += ON * step) {
+                const uint16_t* const at = a.k + (int64_t)id * a.stride_block + (int64_t)h * a.stride_head + c;
+                for (int r = 0; r < rows; r += ON * step) {
                     uint4 w[ON];
 #pragma unroll
-                    for (int k = 0; k < ON; ++k, p += inc)
-                        if (in && r + k * step < rows) w[k] = *reinterpret_cast<const uint4*>(p);
+                    for (int k = 0; k < ON; ++k)  // (the last row once more changes nothing)
+                        w[k] = *reinterpret_cast<const uint4*>(at + min(r + r0 + k * step, rows - 1) * a.stride_slot);
 #pragma unroll
-                    for (int k = 0; k < ON; ++k)
-                        if (in && r + k * step < rows) {
-                            const uint32_t x[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+                    for (int k = 0; k < ON; ++k) {
+                        const uint32_t x[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) l[e] = least2<BF16>(l[e], x[e]), u[e] = most2<BF16>(u[e], x[e]);
-                        }
+                        for (int e = 0; e < 4; ++e) l[e] = least2<BF16>(l[e], x[e]), u[e] = most2<BF16>(u[e], x[e]);
+                    }
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
