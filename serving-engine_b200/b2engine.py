@@ -510,6 +510,8 @@ def paged_kv_evict(kv: PagedKV, scores, budget, kept, new_lens, sinks=0, recent=
     max_dst_blocks]).  kept int32 [B, nkv, budget] (-1 past a sequence's new
     length), new_lens int32 [B] (may be kv.seq_lens)."""
     torch = _torch()
+    if kv.four:
+        raise ValueError("a cache held in 4 bits keeps no scores to evict by")
     dev = _device_of(kv.k, "the cache")
     _need(scores, "scores", torch.float32, kv.scores_shape, dev)
     _need(kept, "kept", torch.int32, (kv.batch, kv.nkv, budget), dev)
@@ -644,6 +646,8 @@ class BlockBounds:
 
     def __init__(self, num_blocks=None, nkv=None, head_dim=None, codes=None, scale=None):
         torch = _torch()
+        if (codes is None) != (scale is None):
+            raise ValueError("codes and scale go together")
         if codes is None:
             codes = torch.zeros(num_blocks, nkv, 2, head_dim, dtype=torch.int8, device="cuda")
             scale = torch.ones(num_blocks, nkv, dtype=torch.float32, device="cuda")
@@ -700,7 +704,8 @@ def paged_block_select(q, kv, bounds: BlockBounds, blocks, first=1, last=1, ws: 
     _need(blocks, "blocks", _torch().int32, (B, kv.nkv, n), dev)
     call("b2_paged_block_select", q.data_ptr(), ldq, _is_bf16(q), kv.block_tables.data_ptr(), kv.seq_lens.data_ptr(),
          kv.num_blocks, kv.block_size, kv.block_tables.shape[1], bounds.codes.data_ptr(), bounds.scale.data_ptr(),
-         blocks.data_ptr(), n, first, last, B, nq, kv.nkv, D, ws.h if ws is not None else None, _stream_of(stream, dev))
+         blocks.data_ptr(), n, _clamp(first, _MOST32), _clamp(last, _MOST32), B, nq, kv.nkv, D,
+         ws.h if ws is not None else None, _stream_of(stream, dev))
     return blocks
 
 

@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kBdThreads, 7) bounds_kernel(const BoundsArgs 
 #pragma unroll
                     for (int k = 0; k < ON; ++k) {
                         const int rr = min(r + r0 + k * step, rows - 1);  // (the last row once more changes nothing)
-                        const uint8_t* tile = at + (rr >> 4) * kv4_tile(DP);
+                        const uint8_t* tile = at + (int64_t)(rr >> 4) * kv4_tile(DP);
                         w[k] = *reinterpret_cast<const uint32_t*>(tile + (rr & 15) * (DP / 2) + word);
                         m[k] = *reinterpret_cast<const uint32_t*>(tile + meta + kv4_slot(rr & 15) * NG * 4);
                     }
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kScThreads, 2) score_kernel(const SelectArgs a
     bool there[ON], next[ON];
     auto look = [&](int j0) {
 #pragma unroll
-        for (int n = 0; n < ON; ++n) id[n] = j0 + n * step < c1 ? __ldg(bt + j0 + n * step) : -1;
+        for (int n = 0; n < ON; ++n) id[n] = j0 + n * step < c1 ? bt[j0 + n * step] : -1;
     };
     auto fetch = [&]() {
 #pragma unroll
@@ -322,8 +322,8 @@ __global__ void __launch_bounds__(kScThreads, 2) score_kernel(const SelectArgs a
             const int64_t row = (next[n] ? id[n] : 0) * (int64_t)a.nkv;
             const uint4* src = codes + row * pieces;
 #pragma unroll
-            for (int p = 0; p < P; ++p) w[n][p] = __ldg(src + shift[p]);
-            sc[n] = __ldg(scales + row);
+            for (int p = 0; p < P; ++p) w[n][p] = src[shift[p]];
+            sc[n] = scales[row];
         }
     };
     look(first);

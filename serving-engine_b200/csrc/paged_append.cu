@@ -72,12 +72,6 @@ __device__ __forceinline__ float fmax_nan(float a, float b) {
 
 __device__ __forceinline__ uint64_t pair(float2 x) { return pair(x.x, x.y); }
 
-// How many new rows sequence b has, and where the first one goes.
-__device__ __forceinline__ int2 new_rows(const int* seq_lens, const int* counts, int b, int S) {
-    const int n = counts ? max(0, min(S, counts[b])) : S;
-    return make_int2(n, seq_lens[b] - n);
-}
-
 // KV4: rows of 4 bits.  VEC: channels per load, 8, or 4 where half the rotated
 // channels are no multiple of 8.
 template <bool KV4, int VEC, bool BF16>
@@ -92,11 +86,12 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
     const int b = blockIdx.z, share = blockIdx.y - (rows4 ? a.q_shares : 0), t0 = blockIdx.x * a.tokens;
     griddep_wait();
     griddep_launch_dependents();
-    const int2 rows = new_rows(a.seq_lens, a.counts, b, a.S);
-    const int nt = min(a.tokens, rows.x - t0);
+    const int news = a.counts ? max(0, min(a.S, a.counts[b])) : a.S;
+    const int64_t place = (int64_t)a.seq_lens[b] - news + t0;  // of this CTA's first token
+    const int nt = min(a.tokens, news - t0);
     if (nt <= 0) return;
     if (tid < nt) {
-        const int64_t pos = (int64_t)rows.y + t0 + tid;
+        const int64_t pos = place + tid;
         int64_t at = kNoRow;
         if (pos >= 0 && pos < (int64_t)a.max_blocks * a.block_size) {
             const int blk = (int)pos / a.block_size, slot = (int)pos - blk * a.block_size;
@@ -116,7 +111,7 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
         s_row[tid] = at;
     }
     const int half = a.rot / 2;
-    const int64_t first = a.positions ? (int64_t)a.positions[b] + t0 : (int64_t)rows.y + t0;
+    const int64_t first = a.positions ? (int64_t)a.positions[b] + t0 : place;
     for (int i = tid; i < nt * half; i += kApThreads) {
         const int t = i / half, e = i - t * half;
         double turn = (double)(first + t) * a.turns[e];
@@ -231,200 +226,201 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
     const int g0 = low0 ? c + half : c - half, g1 = low1 ? c + 4 + half : c + 4 - half;  // and their partners
     constexpr int STEP = kApThreads / 32;
     // this lane's places in a K row, among a position's V units, among its scales
-    const int in_k = (((c >> 3) & 3) * (DP / 32) + (c >> 5)) * 4, in_v = ((c >> 5) * 8 + ((c & 31) >> 2)) * 32, in_s = (c >> 6) * 4;
+    const int in_k = (((c >> 3) & 3) * (DP / 32) + (c >> 5)) * 4, in_v = ((c >> 5) * 8 + ((c & 31) >> 2)) * 32;
+    const int in_s = (c >> 6) * 4;
     // a warp has a token (several warps where there are fewer tokens than warps): its angles and places stay in registers
     // while the warp goes through heads, K's from the first warp on, V's from the last one
     const int team = max(1, STEP / nt), member = warp % team;
     auto rows_of = [&](auto is_key, int tok, int first_h) {
-    constexpr bool key = decltype(is_key)::value;
-    const b2_kv_view& view = key ? a.k : a.v;
-    const int64_t at = s_row[tok];
-    const int by = team * at_once;  // heads from a row to the lane's next one
-    int h = first_h + sub;
-    const uint16_t* src = static_cast<const uint16_t*>(view.data) + b * view.stride_b + (int64_t)(t0 + tok) * view.stride_s +
-                          (k0 + h) * view.stride_h + c;
-    uint8_t* tile = a.pool + at + (k0 + h) * a.head_bytes;
-    const int64_t step = by * view.stride_h, tile_step = by * a.head_bytes;
-    const int place = s_in[tok][key ? 0 : 1] + (key ? in_k : in_v), scales = s_in[tok][2] + (key ? 0 : 64 * NG) + in_s;
-    float4 cs[4];
-    if (key && turned) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) cs[i / 2] = s_cs[tok][(VEC == 8 || i < 4 ? e0 + i : e1 + i - 4) >> 1];
-    }
-    // a row and the partners of its channels: the next row's are on their way while one is worked on
-    struct Row {
-        uint4 own;
-        uint2 other[2];
-    };
-    auto fetch = [&](int hh, const uint16_t* p) {
-        Row w;
-        const bool there = in && hh < kvh;
-        w.own = there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
-        w.other[0] = w.other[1] = make_uint2(0, 0);
-        if (key && turned && there) {
-            if (VEC == 8) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p + (g0 - c));
-                w.other[0] = make_uint2(x.x, x.y), w.other[1] = make_uint2(x.z, x.w);
-            } else {
-                w.other[0] = *reinterpret_cast<const uint2*>(p + (g0 - c));
-                w.other[1] = *reinterpret_cast<const uint2*>(p + (g1 - c));
-            }
-        }
-        return w;
-    };
-    Row ahead = fetch(h, src);
-    for (int hb = first_h; hb < kvh; hb += by) {
-        const Row row = ahead;
-        const bool mine = h < kvh && c < DP;
-        uint8_t* const to = tile;
-        src += step;
-        h += by;
-        tile += tile_step;
-        ahead = fetch(h, src);
-        const uint4 own = row.own;
-        const uint2 other[2] = {row.other[0], row.other[1]};
-        float f[8];
-        auto unpack = [&](uint2 x, float* v) {
-            const float2 p0 = unpack2<BF16>(x.x), p1 = unpack2<BF16>(x.y);
-            v[0] = p0.x, v[1] = p0.y, v[2] = p1.x, v[3] = p1.y;
-        };
-        unpack(make_uint2(own.x, own.y), f);
-        unpack(make_uint2(own.z, own.w), f + 4);
+        constexpr bool key = decltype(is_key)::value;
+        const b2_kv_view& view = key ? a.k : a.v;
+        const int64_t at = s_row[tok];
+        const int by = team * at_once;  // heads from a row to the lane's next one
+        int h = first_h + sub;
+        const uint16_t* src = static_cast<const uint16_t*>(view.data) + b * view.stride_b + (int64_t)(t0 + tok) * view.stride_s +
+                              (k0 + h) * view.stride_h + c;
+        uint8_t* tile = a.pool + at + (k0 + h) * a.head_bytes;
+        const int64_t step = by * view.stride_h, tile_step = by * a.head_bytes;
+        const int place = s_in[tok][key ? 0 : 1] + (key ? in_k : in_v), scales = s_in[tok][2] + (key ? 0 : 64 * NG) + in_s;
+        float4 cs[4];
         if (key && turned) {
-            const uint32_t n0 = low0 ? 0x80008000u : 0u, n1 = (VEC == 8 ? low0 : low1) ? 0x80008000u : 0u;
-            float g[8];
-            unpack(make_uint2(other[0].x ^ n0, other[0].y ^ n0), g);
-            unpack(make_uint2(other[1].x ^ n1, other[1].y ^ n1), g + 4);
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float4 t = cs[i / 2];
-                const float2 y = two(fma2(pair(make_float2(f[i], f[i + 1])), pair(make_float2(t.x, t.y)),
-                                          mul2(pair(make_float2(g[i], g[i + 1])), pair(make_float2(t.z, t.w)))));
-                f[i] = y.x, f[i + 1] = y.y;
-            }
+    #pragma unroll
+            for (int i = 0; i < 8; i += 2) cs[i / 2] = s_cs[tok][(VEC == 8 || i < 4 ? e0 + i : e1 + i - 4) >> 1];
         }
-        float lo = f[0], hi = f[0], most = fabsf(f[0]);
-#pragma unroll
-        for (int i = 1; i < 8; ++i) {
-            lo = fminf(lo, f[i]);
-            hi = fmaxf(hi, f[i]);
-            most = fmax_nan(most, fabsf(f[i]));
-        }
-        if (!in) lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
-            most = fmax_nan(most, __shfl_xor_sync(~0u, most, o));
-        }
-        const bool fine = most < INFINITY;
-        // what f is off by, at most: sine and cosine 2^-25 each, a product 2^-24 |x2|, the sum 2^-24 of itself.  Turning
-        // keeps x1^2 + x2^2, so with M the larger of what the two become |x1| + |x2| <= 2 M and |x2| <= 1.42 M: 2^-22 M
-        float off = 0.f;
-        if (key && a.rot) {
-            off = most;
-            for (int o = 8; o < (1 << wide); o <<= 1) off = fmax_nan(off, __shfl_xor_sync(~0u, off, o));
-            off *= 0x1p-22f;
-        }
-        auto to_half = [](float x) { return __half2float(__float2half_rn(x)); };
-        auto finite_half = [&](float x) { return to_half(fminf(fmaxf(x, -65504.f), 65504.f)); };
-        float m = finite_half(lo);
-        // the span is off by off + 2^-24 (hi - m), as a 15th of it by two roundings more
-        const float span = fmaxf((hi - m) * (1.f / 15.f), 0.f), wrong = fmaf(off, 1.f / 15.f, span * 0x1p-22f);
-        float s = to_half(fminf(span, 65504.f));
-        bool sure = to_half(span - wrong) == to_half(span + wrong);
-        if (key) sure = sure && to_half(lo - off) == to_half(lo + off);
-        sure = sure && most < 65000.f;
-        // u as the nearest whole number to t = (f - m) / s, cut to 0 .. 15: a 15th of it is cut to 0 .. 1 by its
-        // multiply-add; adding 1.5 * 2^23 then leaves the whole number in the low bits
-        constexpr float MAGIC = 12582912.f;
-        const float rs = s > 0.f ? __frcp_rn(s) : 0.f, r15 = rs * (1.f / 15.f), m15 = -m * r15;
-        uint32_t codes = 0;
-        float worst = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float t = __saturatef(fmaf(f[i], r15, m15)), v = fmaf(t, 15.f, MAGIC);
-            worst = fmaxf(worst, fabsf(fmaf(t, 15.f, MAGIC - v)));
-            codes += __float_as_uint(v) << (4 * i);
-        }
-        codes -= 0x4b400000u * 0x11111111u;
-        // t is off by (off + 2^-21 most) / s and 2^-18: nearer to a half than that, it may round otherwise
-        if (!in) worst = 0.f;
-        bool near = !(worst < 0.5f - (fmaf(most, 0x1p-21f, off) * rs + 0x1p-18f));
-        if (__any_sync(~0u, near && fine && off == 0.f)) {
-            // numbers of 8 or 11 bits often lie half way exactly (1 group in 30 of bf16): what is left of f - m is exact in
-            // 32 bits then, where f - m is
-            bool exact = true;
-            uint32_t fixed = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = f[i] - m, back = d - f[i];
-                exact = exact && (f[i] - (d - back)) == (m + back);
-                float u = fminf(fmaxf(rintf(d * rs), 0.f), 15.f);
-                const float left = fmaf(-u, s, d);
-                const bool odd = (int)u & 1;
-                if (left > 0.5f * s || (left == 0.5f * s && odd)) u += 1.f;
-                if (left < -0.5f * s || (left == -0.5f * s && odd)) u -= 1.f;
-                fixed |= (uint32_t)fminf(fmaxf(u, 0.f), 15.f) << (4 * i);
-            }
-            if (off == 0.f) {
-                codes = s > 0.f ? fixed : 0u;
-                near = near && !exact;
-            }
-        }
-        sure = sure && !near;
-        if (__any_sync(~0u, !(sure || !fine || empty))) {
-            // in 64 bits
-            double x[8];
-            auto four = [&](uint2 own4, uint2 oth, bool low, int e, double* y) {
-                float u[4], g[4];
-                unpack(own4, u);
-                unpack(oth, g);
-                const int64_t pos = first + tok;
-#pragma unroll 1
-                for (int i = 0; i < 4; ++i) {
-                    y[i] = u[i];
-                    if (key && turned) {
-                        double turn = (double)pos * a.turns[e + i], sn, cn;
-                        turn -= rint(turn);
-                        sincospi(2.0 * turn, &sn, &cn);
-                        y[i] = fma((double)u[i], cn, (low ? -(double)g[i] : (double)g[i]) * sn);
-                    }
+        // a row and the partners of its channels: the next row's are on their way while one is worked on
+        struct Row {
+            uint4 own;
+            uint2 other[2];
+        };
+        auto fetch = [&](int hh, const uint16_t* p) {
+            Row w;
+            const bool there = in && hh < kvh;
+            w.own = there ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+            w.other[0] = w.other[1] = make_uint2(0, 0);
+            if (key && turned && there) {
+                if (VEC == 8) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(p + (g0 - c));
+                    w.other[0] = make_uint2(x.x, x.y), w.other[1] = make_uint2(x.z, x.w);
+                } else {
+                    w.other[0] = *reinterpret_cast<const uint2*>(p + (g0 - c));
+                    w.other[1] = *reinterpret_cast<const uint2*>(p + (g1 - c));
                 }
+            }
+            return w;
+        };
+        Row ahead = fetch(h, src);
+        for (int hb = first_h; hb < kvh; hb += by) {
+            const Row row = ahead;
+            const bool mine = h < kvh && c < DP;
+            uint8_t* const to = tile;
+            src += step;
+            h += by;
+            tile += tile_step;
+            ahead = fetch(h, src);
+            const uint4 own = row.own;
+            const uint2 other[2] = {row.other[0], row.other[1]};
+            float f[8];
+            auto unpack = [&](uint2 x, float* v) {
+                const float2 p0 = unpack2<BF16>(x.x), p1 = unpack2<BF16>(x.y);
+                v[0] = p0.x, v[1] = p0.y, v[2] = p1.x, v[3] = p1.y;
             };
-            four(make_uint2(own.x, own.y), other[0], low0, e0, x);
-            four(make_uint2(own.z, own.w), other[1], VEC == 8 ? low0 : low1, VEC == 8 ? e0 + 4 : e1, x + 4);
-            double l = in ? x[0] : INFINITY, u = in ? x[0] : -INFINITY;
-            for (int i = 1; i < 8; ++i)
-                if (in) l = x[i] < l ? x[i] : l, u = x[i] > u ? x[i] : u;
+            unpack(make_uint2(own.x, own.y), f);
+            unpack(make_uint2(own.z, own.w), f + 4);
+            if (key && turned) {
+                const uint32_t n0 = low0 ? 0x80008000u : 0u, n1 = (VEC == 8 ? low0 : low1) ? 0x80008000u : 0u;
+                float g[8];
+                unpack(make_uint2(other[0].x ^ n0, other[0].y ^ n0), g);
+                unpack(make_uint2(other[1].x ^ n1, other[1].y ^ n1), g + 4);
+    #pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float4 t = cs[i / 2];
+                    const float2 y = two(fma2(pair(make_float2(f[i], f[i + 1])), pair(make_float2(t.x, t.y)),
+                                              mul2(pair(make_float2(g[i], g[i + 1])), pair(make_float2(t.z, t.w)))));
+                    f[i] = y.x, f[i + 1] = y.y;
+                }
+            }
+            float lo = f[0], hi = f[0], most = fabsf(f[0]);
+    #pragma unroll
+            for (int i = 1; i < 8; ++i) {
+                lo = fminf(lo, f[i]);
+                hi = fmaxf(hi, f[i]);
+                most = fmax_nan(most, fabsf(f[i]));
+            }
+            if (!in) lo = INFINITY, hi = -INFINITY;
+    #pragma unroll
             for (int o = 1; o < 8; o <<= 1) {
-                const double y = __shfl_xor_sync(~0u, l, o), z = __shfl_xor_sync(~0u, u, o);
-                l = y < l ? y : l;
-                u = z > u ? z : u;
+                lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
+                hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
+                most = fmax_nan(most, __shfl_xor_sync(~0u, most, o));
             }
-            m = finite_half((float)l);
-            s = finite_half(fmaxf((float)((u - (double)m) / 15.0), 0.f));
-            codes = 0;
+            const bool fine = most < INFINITY;
+            // what f is off by, at most: sine and cosine 2^-25 each, a product 2^-24 |x2|, the sum 2^-24 of itself.  Turning
+            // keeps x1^2 + x2^2, so with M the larger of what the two become |x1| + |x2| <= 2 M and |x2| <= 1.42 M: 2^-22 M
+            float off = 0.f;
+            if (key && a.rot) {
+                off = most;
+                for (int o = 8; o < (1 << wide); o <<= 1) off = fmax_nan(off, __shfl_xor_sync(~0u, off, o));
+                off *= 0x1p-22f;
+            }
+            auto to_half = [](float x) { return __half2float(__float2half_rn(x)); };
+            auto finite_half = [&](float x) { return to_half(fminf(fmaxf(x, -65504.f), 65504.f)); };
+            float m = finite_half(lo);
+            // the span is off by off + 2^-24 (hi - m), as a 15th of it by two roundings more
+            const float span = fmaxf((hi - m) * (1.f / 15.f), 0.f), wrong = fmaf(off, 1.f / 15.f, span * 0x1p-22f);
+            float s = to_half(fminf(span, 65504.f));
+            bool sure = to_half(span - wrong) == to_half(span + wrong);
+            if (key) sure = sure && to_half(lo - off) == to_half(lo + off);
+            sure = sure && most < 65000.f;
+            // u as the nearest whole number to t = (f - m) / s, cut to 0 .. 15: a 15th of it is cut to 0 .. 1 by its
+            // multiply-add; adding 1.5 * 2^23 then leaves the whole number in the low bits
+            constexpr float MAGIC = 12582912.f;
+            const float rs = s > 0.f ? __frcp_rn(s) : 0.f, r15 = rs * (1.f / 15.f), m15 = -m * r15;
+            uint32_t codes = 0;
+            float worst = 0.f;
+    #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const double t = s > 0.f ? rint((x[i] - (double)m) / (double)s) : 0.0;
-                codes |= (uint32_t)(t < 0.0 ? 0.0 : t > 15.0 ? 15.0 : t) << (4 * i);
+                const float t = __saturatef(fmaf(f[i], r15, m15)), v = fmaf(t, 15.f, MAGIC);
+                worst = fmaxf(worst, fabsf(fmaf(t, 15.f, MAGIC - v)));
+                codes += __float_as_uint(v) << (4 * i);
+            }
+            codes -= 0x4b400000u * 0x11111111u;
+            // t is off by (off + 2^-21 most) / s and 2^-18: nearer to a half than that, it may round otherwise
+            if (!in) worst = 0.f;
+            bool near = !(worst < 0.5f - (fmaf(most, 0x1p-21f, off) * rs + 0x1p-18f));
+            if (__any_sync(~0u, near && fine && off == 0.f)) {
+                // numbers of 8 or 11 bits often lie half way exactly (1 group in 30 of bf16): what is left of f - m is exact in
+                // 32 bits then, where f - m is
+                bool exact = true;
+                uint32_t fixed = 0;
+    #pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float d = f[i] - m, back = d - f[i];
+                    exact = exact && (f[i] - (d - back)) == (m + back);
+                    float u = fminf(fmaxf(rintf(d * rs), 0.f), 15.f);
+                    const float left = fmaf(-u, s, d);
+                    const bool odd = (int)u & 1;
+                    if (left > 0.5f * s || (left == 0.5f * s && odd)) u += 1.f;
+                    if (left < -0.5f * s || (left == -0.5f * s && odd)) u -= 1.f;
+                    fixed |= (uint32_t)fminf(fmaxf(u, 0.f), 15.f) << (4 * i);
+                }
+                if (off == 0.f) {
+                    codes = s > 0.f ? fixed : 0u;
+                    near = near && !exact;
+                }
+            }
+            sure = sure && !near;
+            if (__any_sync(~0u, !(sure || !fine || empty))) {
+                // in 64 bits
+                double x[8];
+                auto four = [&](uint2 own4, uint2 oth, bool low, int e, double* y) {
+                    float u[4], g[4];
+                    unpack(own4, u);
+                    unpack(oth, g);
+                    const int64_t pos = first + tok;
+    #pragma unroll 1
+                    for (int i = 0; i < 4; ++i) {
+                        y[i] = u[i];
+                        if (key && turned) {
+                            double turn = (double)pos * a.turns[e + i], sn, cn;
+                            turn -= rint(turn);
+                            sincospi(2.0 * turn, &sn, &cn);
+                            y[i] = fma((double)u[i], cn, (low ? -(double)g[i] : (double)g[i]) * sn);
+                        }
+                    }
+                };
+                four(make_uint2(own.x, own.y), other[0], low0, e0, x);
+                four(make_uint2(own.z, own.w), other[1], VEC == 8 ? low0 : low1, VEC == 8 ? e0 + 4 : e1, x + 4);
+                double l = in ? x[0] : INFINITY, u = in ? x[0] : -INFINITY;
+                for (int i = 1; i < 8; ++i)
+                    if (in) l = x[i] < l ? x[i] : l, u = x[i] > u ? x[i] : u;
+                for (int o = 1; o < 8; o <<= 1) {
+                    const double y = __shfl_xor_sync(~0u, l, o), z = __shfl_xor_sync(~0u, u, o);
+                    l = y < l ? y : l;
+                    u = z > u ? z : u;
+                }
+                m = finite_half((float)l);
+                s = finite_half(fmaxf((float)((u - (double)m) / 15.0), 0.f));
+                codes = 0;
+                for (int i = 0; i < 8; ++i) {
+                    const double t = s > 0.f ? rint((x[i] - (double)m) / (double)s) : 0.0;
+                    codes |= (uint32_t)(t < 0.0 ? 0.0 : t > 15.0 ? 15.0 : t) << (4 * i);
+                }
+            }
+            if (!mine) continue;
+            if (!in || !fine) codes = 0;
+            if (key) {
+                *reinterpret_cast<uint32_t*>(to + place) = codes;
+            } else {
+                *reinterpret_cast<uint16_t*>(to + place) = (uint16_t)codes;
+                *reinterpret_cast<uint16_t*>(to + place + 32) = (uint16_t)(codes >> 16);
+            }
+            if ((c & 63) == 0) {
+                __half2 sm = __floats2half2_rn(s, m);
+                if (!fine) sm = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff));
+                if (empty) sm = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+                *reinterpret_cast<__half2*>(to + scales) = sm;
             }
         }
-        if (!mine) continue;
-        if (!in || !fine) codes = 0;
-        if (key) {
-            *reinterpret_cast<uint32_t*>(to + place) = codes;
-        } else {
-            *reinterpret_cast<uint16_t*>(to + place) = (uint16_t)codes;
-            *reinterpret_cast<uint16_t*>(to + place + 32) = (uint16_t)(codes >> 16);
-        }
-        if ((c & 63) == 0) {
-            __half2 sm = __floats2half2_rn(s, m);
-            if (!fine) sm = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff));
-            if (empty) sm = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-            *reinterpret_cast<__half2*>(to + scales) = sm;
-        }
-    }
     };
     for (int tok = warp / team; tok < nt && warp < nt * team; tok += STEP / team) {
         if (s_row[tok] == kNoRow) continue;
@@ -525,6 +521,11 @@ static bool rows_fit(const b2_kv_view& v) {
     return aligned16(v.data) && v.stride_d == 1 && !((v.stride_b | v.stride_h | v.stride_s) & 7);
 }
 
+// Rows that are written have places of their own: no stride of 0.
+static bool rows_apart(const b2_kv_view& v, int batch, int64_t S, int heads) {
+    return (batch == 1 || v.stride_b) && (S == 1 || v.stride_s) && (heads == 1 || v.stride_h);
+}
+
 // What both kinds of cache share: arguments checked and filled in but for the cache.
 static int append_args(AppendArgs& a, const b2_kv_view* q, const b2_kv_view* q_out, const b2_kv_view* k, const b2_kv_view* v,
                        const double* inv_freq, int rot, const int* counts, const int* positions, int batch, int64_t S,
@@ -534,6 +535,7 @@ static int append_args(AppendArgs& a, const b2_kv_view* q, const b2_kv_view* q_o
     if (rot > D || (rot & 7) || S > (1 << 30) || batch > 65535 || !rows_fit(*k) || !rows_fit(*v) ||
         (q && (!rows_fit(*q) || !rows_fit(*q_out))))
         return B2_ERR_UNSUPPORTED;
+    B2_REQUIRE(!q || rows_apart(*q_out, batch, S, nq));
     if (q) a.q = *q, a.q_out = *q_out;
     a.k = *k;
     a.v = *v;
@@ -560,7 +562,8 @@ template <bool KV4>
 static int append_launch(AppendArgs& a, int batch, cudaStream_t s) {
     const int vec = (a.rot / 2) % 8 == 0 ? 8 : 4;
     a.per = a.rot / (2 * vec) + (a.D - a.rot + 2 * vec - 1) / (2 * vec);
-    const dim3 grid((unsigned)((a.S + a.tokens - 1) / a.tokens), (unsigned)(KV4 ? a.q_shares + a.shares : a.shares), (unsigned)batch);
+    const dim3 grid((unsigned)((a.S + a.tokens - 1) / a.tokens), (unsigned)(KV4 ? a.q_shares + a.shares : a.shares),
+                    (unsigned)batch);
     if (a.bf16)
         B2_TRY(vec == 8 ? launch(append_kernel<KV4, 8, true>, grid, dim3(kApThreads), 0, s, true, a)
                         : launch(append_kernel<KV4, 4, true>, grid, dim3(kApThreads), 0, s, true, a));
@@ -628,6 +631,7 @@ extern "C" int b2_paged_kv4_read(const b2_paged_kv4* kv, const b2_kv_view* k_out
     const int rc = check_paged4(kv, nkv, D);
     if (rc != B2_OK) return rc;
     if (!rows_fit(*k_out) || !rows_fit(*v_out) || batch > 65535 || nkv > 65535 || T > (1 << 30)) return B2_ERR_UNSUPPORTED;
+    B2_REQUIRE(rows_apart(*k_out, batch, T, nkv) && rows_apart(*v_out, batch, T, nkv));
     ReadArgs a = {};
     a.k = *k_out;
     a.v = *v_out;

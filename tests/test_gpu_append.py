@@ -274,6 +274,13 @@ def test_binding_refuses(cuda):
         with pytest.raises(b2.B2Error) as e:
             b2.paged_kv_append(kv, **{**dict(k=x, v=x), **more})
         assert e.value.status == -2
+    wide = q[:, :, :1].expand(-1, -1, 4, -1)  # four heads in one place: may be read, not written
+    for call in (lambda: b2.paged_kv_append(kv, x, x, q=wide), lambda: b2.paged_kv_append(kv, x, x, q=q, q_out=wide),
+                 lambda: b2.paged_kv_read(kv, x[:, :, :1].expand(-1, -1, 2, -1), x)):
+        with pytest.raises(b2.B2Error) as e:
+            call()
+        assert e.value.status == -1
+    b2.paged_kv_append(kv, x, x, q=wide, q_out=q)
     for more in (dict(k_out=x[:1]), dict(v_out=x[:, :2]), dict(k_out=x.float()), dict(counts=n.long())):
         with pytest.raises(ValueError):
             b2.paged_kv_read(kv, **{**dict(k_out=x, v_out=x), **more})

@@ -184,6 +184,10 @@ def test_refusals(cuda):
         with pytest.raises(b2.B2Error) as e:
             b2.paged_block_select(q, kv, bd, out, **more)
         assert e.value.status == status
+    for more in (dict(first=2 ** 32), dict(last=2 ** 32 + 1), dict(first=-2 ** 32), dict(last=-1)):  # no bits are dropped
+        with pytest.raises(b2.B2Error) as e:
+            b2.paged_block_select(q, kv, bd, out, ws=ws, **more)
+        assert e.value.status == -1
     with pytest.raises(ValueError):
         b2.paged_block_bounds(kv, other)
     with pytest.raises(ValueError):

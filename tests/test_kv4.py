@@ -110,6 +110,7 @@ def test_append_refuses(make):
     assert append(make(), k=view(data=FAKE + 8)) == -2 and append(make(), v=view(stride=60)) == -2
     assert append(make(), k=view(d=2)) == -2
     assert append(make(), q=view(data=FAKE + 4), q_out=view()) == -2
+    assert append(make(), q=view(), q_out=view(stride=0)) == -1  # heads written to one place
     assert append(make(), D=60) == -2 and append(make(), S=2 ** 31) == -2 and append(make(), batch=65536) == -2
 
 
@@ -117,6 +118,7 @@ def test_read_refuses():
     assert read(cache4(), T=0) == 0 and read(None, batch=0) == 0
     assert read(None) == -1 and read(cache4(), k=view(data=None)) == -1
     assert read(cache4(), k=view(d=2)) == -2 and read(cache4(), v=view(stride=4)) == -2
+    assert read(cache4(), k=view(stride=0)) == -1 and read(cache4(), v=view(stride=0)) == -1  # heads to one place
     assert read(cache4(), T=2 ** 31) == -2 and read(cache4(), batch=65536) == -2
 
 
@@ -187,6 +189,15 @@ def test_binding_refuses():
         b2.BlockBounds(codes=torch.zeros(8, 2, 2, 64, dtype=torch.int8), scale=torch.ones(8, 3))
     with pytest.raises(ValueError):
         b2.BlockBounds(codes=torch.zeros(8, 2, 3, 64, dtype=torch.int8), scale=torch.ones(8, 2))
+
+
+def test_binding_refuses_what_does_not_go_together():
+    kv = cpu_cache4()
+    with pytest.raises(ValueError, match="4 bits"):
+        b2.paged_kv_evict(kv, torch.zeros(8, 2, 16), 4, torch.zeros(1, 2, 4, dtype=torch.int32), kv.seq_lens)
+    for alone in (dict(codes=torch.zeros(8, 2, 2, 64, dtype=torch.int8)), dict(scale=torch.ones(8, 2))):
+        with pytest.raises(ValueError, match="together"):
+            b2.BlockBounds(**alone)
 
 
 def test_rope_frequencies():
