@@ -10,8 +10,8 @@ reaches its capacity the cache is cut back to its budget: sinks, the most
 recent rows, and the rows with the most weight.  Rows keep the position
 encoding they were written with, so q and k come in already rotated.  A decode
 window counts the rows held: once something above `recent` has been evicted it
-reaches further back in tokens than its number says.  Rows are written by plain
-indexing, one sequence at a time; a server would append them in one kernel."""
+reaches further back in tokens than its number says.  Rows are appended in one
+launch for all sequences."""
 from __future__ import annotations
 
 import os
@@ -35,7 +35,7 @@ class BoundedLayer:
                              f"rows, got {budget}, {sinks} and {recent}")
         blocks = -(-capacity // block_size)
         self.capacity, self.budget, self.sinks, self.recent, self.window = capacity, budget, sinks, recent, window
-        self.block_size, self.nq = block_size, nq
+        self.nq = nq
         k = torch.zeros(batch * blocks, block_size, nkv, head_dim, dtype=dtype, device="cuda")
         tables = torch.randperm(batch * blocks, device="cuda").to(torch.int32).view(batch, blocks)
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device="cuda")
@@ -45,12 +45,6 @@ class BoundedLayer:
         self.ws = b2.Workspace(b2.paged_decode_workspace_bytes(batch, nq, nkv, head_dim, blocks * block_size,
                                                                scored=True))
         self.rows = [0] * batch  # the lengths as the host knows them
-
-    def _write(self, b, start, k, v):
-        pos = torch.arange(start, start + k.shape[0], device="cuda")
-        blk = self.kv.block_tables[b].long()[pos // self.block_size]
-        self.kv.k[blk, pos % self.block_size] = k
-        self.kv.v[blk, pos % self.block_size] = v
 
     def prefill(self, q, k, v, chunk=512, observe=16):
         """Prompts [B, S, heads, head_dim] of one length S <= capacity;
@@ -64,9 +58,9 @@ class BoundedLayer:
             part = torch.empty(B, end - at, *q.shape[2:], dtype=q.dtype, device="cuda")
             b2.window_prefill_gqa(q[:, at:end], k[:, :end], v[:, :end], part, window=self.window, sinks=self.sinks)
             out[:, at:end] = part
-        for b in range(B):
-            self._write(b, 0, k[b], v[b])
-            self.rows[b] = S
+        self.seq_lens.fill_(S)
+        b2.paged_kv_append(self.kv, k, v)
+        self.rows = [S] * B
         self.scores.zero_()
         # what the last prompt queries look at ranks the rows of the prompt
         probe = torch.empty(B, self.nq, q.shape[3], dtype=q.dtype, device="cuda")
@@ -81,10 +75,9 @@ class BoundedLayer:
         head_dim].  Returns the attention outputs [B, nq, head_dim]."""
         if max(self.rows) == self.capacity:
             self.evict()
-        for b in range(len(self.rows)):
-            self._write(b, self.rows[b], k[b:b + 1], v[b:b + 1])
-            self.rows[b] += 1
+        self.rows = [n + 1 for n in self.rows]
         self.seq_lens += 1
+        b2.paged_kv_append(self.kv, k[:, None], v[:, None])
         out = torch.empty(q.shape, dtype=q.dtype, device="cuda")
         return b2.paged_decode_gqa(q, self.kv, out, window=self.window, sinks=self.sinks, scores=self.scores,
                                    ws=self.ws)
