@@ -43,8 +43,9 @@ struct AppendArgs {
     int64_t pool_block, head_bytes;
     const int *block_tables, *seq_lens, *counts, *positions;
     int num_blocks, block_size, max_blocks;
-    int S, nq, nkv, D, rot, tokens, shares, q_shares, bf16;
-    int per;              // items of a row
+    int S, nq, nkv, D, rot, tokens, shares, q_shares, q_heads, k_heads, bf16;  // heads of a share
+    int vec, per, fit, groups;  // threads that a row takes; rows side by side, and for each token where a CTA has all of its
+    uint32_t per_inv, tokens_inv, half_inv;  // 2^20 / d + 1 of them
     double turns[128];    // f_i / 2 pi
 };
 
@@ -70,20 +71,24 @@ __device__ __forceinline__ float fmax_nan(float a, float b) {
     return r;
 }
 
+// floor(i / d) by inv = 2^20 / d + 1, for i d < 2^20
+__device__ __forceinline__ int over(int i, uint32_t inv) { return (int)(((uint32_t)i * inv) >> 20); }
 __device__ __forceinline__ uint64_t pair(float2 x) { return pair(x.x, x.y); }
 
-// KV4: rows of 4 bits.  VEC: channels per load, 8, or 4 where half the rotated
+// WIDE: rows of 4 bits, 1 << WIDE lanes for each; 0: rows of 16 bits.  VEC: channels per load, 8, or 4 where half the rotated
 // channels are no multiple of 8.
-template <bool KV4, int VEC, bool BF16>
+template <int WIDE, int VEC, bool BF16>
 __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_constant__ AppendArgs a) {
     using Vec = typename Chunk<VEC>::T;
+    constexpr bool KV4 = WIDE > 0;
     __shared__ float4 s_cs[kApTokens][64];  // of two pairs of channels: cosines, sines
     __shared__ int64_t s_row[kApTokens];  // where a token's rows go: element offset of its first head, or byte offset of its tile
     __shared__ int s_in[KV4 ? kApTokens : 1][3];  // in the tile: K row, V units, scales
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // rows of 4 bits have CTAs of their own, behind those of the queries
-    const bool rows4 = KV4 && (int)blockIdx.y >= a.q_shares;
-    const int b = blockIdx.z, share = blockIdx.y - (rows4 ? a.q_shares : 0), t0 = blockIdx.x * a.tokens;
+    // rows of 4 bits have CTAs of their own, in turn with those of the queries
+    const int kinds = KV4 ? a.q_shares + a.shares : a.shares, kind = blockIdx.x % kinds;
+    const bool rows4 = KV4 && kind >= a.q_shares;
+    const int b = blockIdx.y, share = kind - (rows4 ? a.q_shares : 0), t0 = blockIdx.x / kinds * a.tokens;
     griddep_wait();
     griddep_launch_dependents();
     const int news = a.counts ? max(0, min(a.S, a.counts[b])) : a.S;
@@ -105,7 +110,7 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
                     s_in[tid][2] = 16 * DP + kv4_slot(p) * kv4_groups(DP) * 4;
                 } else
                     at = (int64_t)id * a.kv.stride_block + (int64_t)slot * a.kv.stride_slot +
-                         (a.nkv * share / a.shares) * a.kv.stride_head;
+                         share * a.k_heads * a.kv.stride_head;
             }
         }
         s_row[tid] = at;
@@ -113,7 +118,7 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
     const int half = a.rot / 2;
     const int64_t first = a.positions ? (int64_t)a.positions[b] + t0 : place;
     for (int i = tid; i < nt * half; i += kApThreads) {
-        const int t = i / half, e = i - t * half;
+        const int t = over(i, a.half_inv), e = i - t * half;
         double turn = (double)(first + t) * a.turns[e];
         turn -= rint(turn);
         float sn, cn;
@@ -130,16 +135,19 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
     }
     __syncthreads();
 
-    const int q0 = a.nq * share / a.shares, q1 = a.nq * (share + 1) / a.shares;
-    const int k0 = a.nkv * share / a.shares, k1 = a.nkv * (share + 1) / a.shares;
+    const int q0 = min(a.nq, share * a.q_heads), q1 = min(a.nq, q0 + a.q_heads);
+    const int k0 = min(a.nkv, share * a.k_heads), k1 = min(a.nkv, k0 + a.k_heads);
     // ---- rows of 16 bits: a thread has two chunks of VEC channels that are rotated together, or two to be copied, of one
     // token (its angles stay in registers) and goes through heads
     if (!rows4) {
-        const int pairs = a.rot / (2 * VEC), e = tid % a.per, lead = tid / a.per, fit = kApThreads / a.per;
+        const int pairs = a.rot / (2 * VEC), lead = over(tid, a.per_inv), e = tid - lead * a.per;
         const bool turns = e < pairs;
         const int c0 = turns ? e * VEC : a.rot + (e - pairs) * 2 * VEC, c1 = turns ? half + c0 : c0 + VEC;
         const bool both = c1 < a.D;
-        const int tp = min(nt, fit), groups = fit / tp, mine = lead % tp, group = lead / tp;  // tokens, and threads for each
+        // tokens side by side, and threads for each; this thread's
+        const bool all = nt == a.tokens;
+        const int tp = min(nt, a.fit), groups = all ? a.groups : a.fit / tp, group = all ? over(lead, a.tokens_inv) : lead / tp;
+        const int mine = lead - group * tp;
         // rows of `heads` heads from h0 on; TURN: rotated.  Into the cache where `to` is null
         auto all_of = [&](auto turn, const b2_kv_view& view, int h0, int heads, uint16_t* to, int64_t to_s, int64_t to_h,
                           int group, int groups) {
@@ -216,10 +224,10 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
 
     // ---- rows of 4 bits: a lane holds 8 channels, 8 lanes a group, 8, 16 or 32 lanes a row
     const int DP = kv4_dp(a.D), NG = kv4_groups(DP), kvh = k1 - k0;
-    const int wide = DP == 64 ? 3 : DP <= 128 ? 4 : 5, at_once = 32 >> wide;
-    const int sub = lane >> wide, c = (lane & ((1 << wide) - 1)) * 8;
+    constexpr int at_once = 32 >> WIDE;
+    const int sub = lane >> WIDE, c = (lane & ((1 << WIDE) - 1)) * 8;
     const bool in = c < a.D, turned = c < a.rot;
-    const bool empty = (c & ~63) >= a.D;  // a group of padding alone
+    const bool empty = c >= DP;  // (192 channels: 8 lanes have nothing)
     // K is rotated with the sign of the sine taken to the partner: whole chunks of 4 channels have one sign
     const bool low0 = c < half, low1 = c + 4 < half;
     const int e0 = low0 ? c : c - half, e1 = low1 ? c + 4 : c + 4 - half;  // pairs of channels c and c + 4
@@ -319,7 +327,7 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
             float off = 0.f;
             if (key && a.rot) {
                 off = most;
-                for (int o = 8; o < (1 << wide); o <<= 1) off = fmax_nan(off, __shfl_xor_sync(~0u, off, o));
+                for (int o = 8; o < (1 << WIDE); o <<= 1) off = fmax_nan(off, __shfl_xor_sync(~0u, off, o));
                 off *= 0x1p-22f;
             }
             auto to_half = [](float x) { return __half2float(__float2half_rn(x)); };
@@ -417,7 +425,6 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
             if ((c & 63) == 0) {
                 __half2 sm = __floats2half2_rn(s, m);
                 if (!fine) sm = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff));
-                if (empty) sm = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
                 *reinterpret_cast<__half2*>(to + scales) = sm;
             }
         }
@@ -553,23 +560,31 @@ static int append_args(AppendArgs& a, const b2_kv_view* q, const b2_kv_view* q_o
     const int64_t ctas = (S + a.tokens - 1) / a.tokens * batch;
     a.shares = 1;
     while (a.shares < nkv && a.shares < 8 && ctas * a.shares * 2 <= sm_count()) a.shares *= 2;
-    if (a.shares > nkv) a.shares = nkv;
+    a.k_heads = (nkv + a.shares - 1) / a.shares;
+    a.q_heads = (a.nq + a.shares - 1) / a.shares;
     a.q_shares = q ? a.shares : 0;
+    auto inverse = [](int d) { return (uint32_t)((1 << 20) / d + 1); };
+    a.vec = (rot / 2) % 8 == 0 ? 8 : 4;
+    a.per = rot / (2 * a.vec) + (D - rot + 2 * a.vec - 1) / (2 * a.vec);
+    a.fit = kApThreads / a.per;
+    const int side = a.tokens < a.fit ? a.tokens : a.fit;
+    a.groups = a.fit / side;
+    a.per_inv = inverse(a.per);
+    a.tokens_inv = inverse(side);
+    a.half_inv = rot ? inverse(rot / 2) : 0;
     return B2_OK;
 }
 
-template <bool KV4>
+template <int WIDE>
 static int append_launch(AppendArgs& a, int batch, cudaStream_t s) {
-    const int vec = (a.rot / 2) % 8 == 0 ? 8 : 4;
-    a.per = a.rot / (2 * vec) + (a.D - a.rot + 2 * vec - 1) / (2 * vec);
-    const dim3 grid((unsigned)((a.S + a.tokens - 1) / a.tokens), (unsigned)(KV4 ? a.q_shares + a.shares : a.shares),
-                    (unsigned)batch);
+    // (with several shares there are few CTAs)
+    const dim3 grid((unsigned)((a.S + a.tokens - 1) / a.tokens * (WIDE ? a.q_shares + a.shares : a.shares)), (unsigned)batch);
     if (a.bf16)
-        B2_TRY(vec == 8 ? launch(append_kernel<KV4, 8, true>, grid, dim3(kApThreads), 0, s, true, a)
-                        : launch(append_kernel<KV4, 4, true>, grid, dim3(kApThreads), 0, s, true, a));
+        B2_TRY(a.vec == 8 ? launch(append_kernel<WIDE, 8, true>, grid, dim3(kApThreads), 0, s, true, a)
+                        : launch(append_kernel<WIDE, 4, true>, grid, dim3(kApThreads), 0, s, true, a));
     else
-        B2_TRY(vec == 8 ? launch(append_kernel<KV4, 8, false>, grid, dim3(kApThreads), 0, s, true, a)
-                        : launch(append_kernel<KV4, 4, false>, grid, dim3(kApThreads), 0, s, true, a));
+        B2_TRY(a.vec == 8 ? launch(append_kernel<WIDE, 8, false>, grid, dim3(kApThreads), 0, s, true, a)
+                        : launch(append_kernel<WIDE, 4, false>, grid, dim3(kApThreads), 0, s, true, a));
     return B2_OK;
 }
 
@@ -598,7 +613,7 @@ extern "C" int b2_paged_kv_append(const b2_paged_kv* kv, const b2_kv_view* k, co
     a.block_size = kv->block_size;
     a.max_blocks = kv->max_blocks;
     a.bf16 = kv->bf16;
-    return append_launch<false>(a, batch, as_stream(stream));
+    return append_launch<0>(a, batch, as_stream(stream));
 }
 
 extern "C" int b2_paged_kv4_append(const b2_paged_kv4* kv, const b2_kv_view* k, const b2_kv_view* v, const b2_kv_view* q,
@@ -620,7 +635,8 @@ extern "C" int b2_paged_kv4_append(const b2_paged_kv4* kv, const b2_kv_view* k, 
     a.block_size = kv->block_size;
     a.max_blocks = kv->max_blocks;
     a.bf16 = kv->bf16;
-    return append_launch<true>(a, batch, as_stream(stream));
+    cudaStream_t s = as_stream(stream);
+    return D <= 64 ? append_launch<3>(a, batch, s) : D <= 128 ? append_launch<4>(a, batch, s) : append_launch<5>(a, batch, s);
 }
 
 extern "C" int b2_paged_kv4_read(const b2_paged_kv4* kv, const b2_kv_view* k_out, const b2_kv_view* v_out, const int* counts,
