@@ -24,7 +24,15 @@
 // ordered key, 11 bits of the range still open at a time until 32 are left, and
 // lists what is above it and the first of those equal to it, in order.  (In one
 // launch, the last CTA of each pair choosing and every CTA working out P and N:
-// 54 us for 32 x 2048 blocks of 8 heads of 128, instead of TODO.)
+// 54 us for 32 x 2048 blocks of 8 heads of 128, instead of 27 and 7.)
+//
+// Measured, cold: bounds of 32768 tokens of 8 heads of 128 in 16 bits 15 us (4.5
+// TB/s: a block's loads leave together, then its warp works them off), of the
+// newest block of 8 sequences 6.3 us, a chain of three loads; scores of 32 x
+// 2048 blocks of 8 heads 27 us (5.2 TB/s), of 4094 blocks 10.5 us, five loads one
+// after the other; the choice among 2048 blocks 6.9 us, among 8188 9.5 us (14 us
+// with 512 threads and keys in shared memory): its barriers, six and five a
+// further 11 bits, and the keys' atomics.
 #include <cmath>
 
 #include "kv4.cuh"
@@ -253,9 +261,9 @@ static int bounds_launch(const BoundsArgs& a, bool kv4, cudaStream_t s) {
 
 constexpr int kScThreads = 256;  // of the scores
 constexpr int kScWarps = kScThreads / 32;
-constexpr int kSlThreads = 512;  // of a choice
+constexpr int kSlThreads = 1024;  // of a choice
 constexpr int kSlWarps = kSlThreads / 32;
-constexpr int kSlKeys = 8192;  // keys of a choice kept in shared memory; of longer ones they are read again
+constexpr int kSlKeys = 8;  // keys that a thread keeps
 constexpr int kSlBins = 2048;
 constexpr uint32_t kSlStays = 0xffffffffu;  // blocks that are chosen in any case
 
@@ -415,15 +423,23 @@ __global__ void __launch_bounds__(kScThreads, 2) score_kernel(const SelectArgs a
     }
 }
 
-// One CTA per (sequence, kv head).
+// One CTA per (sequence, kv head).  Keys stay in registers (up to 8 of a thread;
+// of longer sequences they are read again from the workspace).
 __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) {
-    __shared__ uint32_t s_keys[kSlKeys], s_few32[32];
+    __shared__ uint32_t s_few32[32];
     __shared__ int s_hist[kSlBins];
-    __shared__ int s_wsum[kSlWarps][2];
+    __shared__ int s_sum[kSlWarps];
+    __shared__ uint32_t s_count[kSlKeys][kSlWarps];  // keys above the border, and equal to it << 16
     __shared__ int s_bin, s_above, s_in, s_few;
     __shared__ uint32_t s_range[2][kSlWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = blockIdx.x, b = blockIdx.y;
+    constexpr int PER = kSlBins / kSlThreads;
+    auto clear = [&]() {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) s_hist[i * kSlThreads + tid] = 0;
+    };
+    clear();
     griddep_wait();
     griddep_launch_dependents();
     const int len = max(0, min(a.seq_lens[b], a.max_blocks * a.block_size));
@@ -435,14 +451,29 @@ __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) 
         return;
     }
     const uint32_t* keys = a.keys + pair * a.max_blocks;
-    const bool fits = nb <= kSlKeys;
+    constexpr int ROUND = kSlKeys * kSlThreads;  // keys at a time
+    uint32_t key[kSlKeys];
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int j = 0; j < kSlKeys; ++j) {
+            const int i = i0 + j * kSlThreads + tid;
+            key[j] = i < nb ? __ldcg(keys + i) : kSlStays;  // (what stays is left out of the ranking)
+        }
+    };
+    // f(key) for all of this thread's
+    auto each = [&](auto f) {
+        for (int i0 = 0; i0 < nb; i0 += ROUND) {
+            if (nb > ROUND) fetch(i0);
+#pragma unroll
+            for (int j = 0; j < kSlKeys; ++j)
+                if (i0 + j * kSlThreads < nb) f(key[j]);
+        }
+    };
+    if (nb <= ROUND) fetch(0);
     uint32_t lowest = ~0u, highest = 0u;
-    for (int i = tid; i < nb; i += kSlThreads) {
-        const uint32_t k = __ldcg(keys + i);
-        if (fits) s_keys[i] = k;
+    each([&](uint32_t k) {
         if (k != kSlStays) lowest = min(lowest, k), highest = max(highest, k);
-    }
-    auto key = [&](int i) -> uint32_t { return fits ? s_keys[i] : __ldcg(keys + i); };
+    });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         lowest = min(lowest, __shfl_xor_sync(~0u, lowest, o));
@@ -450,22 +481,23 @@ __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) 
     }
     if (lane == 0) s_range[0][warp] = lowest, s_range[1][warp] = highest;
     __syncthreads();
+    lowest = s_range[0][lane], highest = s_range[1][lane];
 #pragma unroll
-    for (int w = 0; w < kSlWarps; ++w) lowest = min(lowest, s_range[0][w]), highest = max(highest, s_range[1][w]);
+    for (int o = 16; o > 0; o >>= 1) {
+        lowest = min(lowest, __shfl_xor_sync(~0u, lowest, o));
+        highest = max(highest, __shfl_xor_sync(~0u, highest, o));
+    }
     // want: how many of the keys lowest .. highest are chosen; all above are
     int want = a.n - a.first - a.last;
     while (want > 0 && lowest < highest) {
         const uint32_t range = highest - lowest;
         const int shift = max(0, 21 - __clz(range));  // range >> shift below 2048
-        for (int i = tid; i < kSlBins; i += kSlThreads) s_hist[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < nb; i += kSlThreads) {
-            const uint32_t k = key(i) - lowest;
+        each([&](uint32_t k) {
+            k -= lowest;
             if (k <= range) atomicAdd(&s_hist[k >> shift], 1);
-        }
+        });
         __syncthreads();
-        // the bin of the want-th best: thread t sums the bins 8 t' .. 8 t' + 7, t' counting from the top
-        constexpr int PER = kSlBins / kSlThreads;
+        // the bin of the want-th best: thread t sums the bins PER t' .. PER t' + PER - 1, t' counting from the top
         const int top_bin = kSlBins - 1 - tid * PER;
         int mine = 0;
 #pragma unroll
@@ -476,11 +508,12 @@ __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) 
             const int v = __shfl_up_sync(~0u, incl, o);
             if (lane >= o) incl += v;
         }
-        if (lane == 31) s_wsum[warp][0] = incl;
+        if (lane == 31) s_sum[warp] = incl;
         __syncthreads();
+        int before = lane < warp ? s_sum[lane] : 0;
 #pragma unroll
-        for (int w = 0; w < kSlWarps; ++w)
-            if (w < warp) incl += s_wsum[w][0];
+        for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
+        incl += before;
         if (incl >= want && incl - mine < want) {
             int above = incl - mine, bin = top_bin;
             while (above + s_hist[bin] < want) above += s_hist[bin--];
@@ -493,20 +526,21 @@ __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) 
         want -= s_above;
         lowest += (uint32_t)s_bin << shift;
         highest = min(highest, lowest + ((1u << shift) - 1));
-        if (s_in <= 32 && lowest < highest) {  // few enough to be ranked side by side in every warp
-            for (int i = tid; i < nb; i += kSlThreads) {
-                const uint32_t k = key(i);
+        clear();
+        const int in = s_in;
+        if (in <= 32 && lowest < highest) {  // few enough to be ranked side by side in every warp
+            each([&](uint32_t k) {
                 if (k - lowest <= highest - lowest) s_few32[atomicAdd(&s_few, 1)] = k;
-            }
+            });
             __syncthreads();
-            const uint32_t k = lane < s_in ? s_few32[lane] : 0u;
+            const uint32_t k = lane < in ? s_few32[lane] : 0u;
             int more = 0, same = 0;  // candidates above this lane's, and equal to it
-            for (int i = 0; i < s_in; ++i) {
+            for (int i = 0; i < in; ++i) {
                 const uint32_t o = __shfl_sync(~0u, k, i);
                 more += o > k;
                 same += o == k;
             }
-            const int who = __ffs(__ballot_sync(~0u, lane < s_in && more < want && more + same >= want)) - 1;
+            const int who = __ffs(__ballot_sync(~0u, lane < in && more < want && more + same >= want)) - 1;
             lowest = highest = __shfl_sync(~0u, k, who);
             want -= __shfl_sync(~0u, more, who);
         }
@@ -514,27 +548,42 @@ __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) 
     }
     // ---- what is above, and the first `want` that equal it, in order (want 0: nothing below the blocks that stay)
     const uint32_t border = want > 0 ? lowest : kSlStays - 1;
-    const int per = ((nb + kSlWarps - 1) / kSlWarps + 31) & ~31, i0 = warp * per, i1 = min(nb, i0 + per);
-    int above = 0, equal = 0;
-    for (int i = i0; i < i1; i += 32) {
-        const uint32_t k = i + lane < i1 ? key(i + lane) : 0u;
-        above += __popc(__ballot_sync(~0u, k > border));
-        equal += __popc(__ballot_sync(~0u, k == border && i + lane < i1));
-    }
-    if (lane == 0) s_wsum[warp][0] = above, s_wsum[warp][1] = equal;
-    __syncthreads();
-    above = equal = 0;  // before this warp's own
+    const uint32_t below = (1u << lane) - 1;
+    int above = 0, equal = 0;  // before the keys of this round
+    for (int i0 = 0; i0 < nb; i0 += ROUND) {
+        if (nb > ROUND) {
+            fetch(i0);
+            __syncthreads();
+        }
+        const int rows = min(kSlKeys, (nb - i0 + kSlThreads - 1) / kSlThreads);
 #pragma unroll
-    for (int w = 0; w < kSlWarps; ++w)
-        if (w < warp) above += s_wsum[w][0], equal += s_wsum[w][1];
-    const uint32_t before = (1u << lane) - 1;
-    for (int i = i0; i < i1; i += 32) {
-        const uint32_t k = i + lane < i1 ? key(i + lane) : 0u;
-        const uint32_t up = __ballot_sync(~0u, k > border), eq = __ballot_sync(~0u, k == border && i + lane < i1);
-        const int e = equal + __popc(eq & before), at = above + __popc(up & before) + min(e, want);
-        if ((k > border || (k == border && i + lane < i1 && e < want)) && at < a.n) out[at] = i + lane;
-        above += __popc(up);
-        equal += __popc(eq);
+        for (int j = 0; j < kSlKeys; ++j) {
+            if (j >= rows) break;
+            const bool there = i0 + j * kSlThreads + tid < nb;
+            const uint32_t up = __ballot_sync(~0u, there && key[j] > border), eq = __ballot_sync(~0u, there && key[j] == border);
+            if (lane == 0) s_count[j][warp] = __popc(up) | __popc(eq) << 16;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kSlKeys; ++j) {
+            if (j >= rows) break;
+            const int i = i0 + j * kSlThreads + tid;
+            const bool there = i < nb, over = there && key[j] > border, same = there && key[j] == border;
+            const uint32_t up = __ballot_sync(~0u, over), eq = __ballot_sync(~0u, same);
+            uint32_t sum = s_count[j][lane];  // of warps 0 .. lane
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(~0u, sum, o);
+                if (lane >= o) sum += v;
+            }
+            const uint32_t all = __shfl_sync(~0u, sum, 31), prior = __shfl_sync(~0u, sum, warp - 1 & 31);
+            const uint32_t before = warp > 0 ? prior : 0u;
+            const int e = equal + (int)(before >> 16) + __popc(eq & below);
+            const int at = above + (int)(before & 0xffffu) + __popc(up & below) + min(e, want);
+            if ((over || (same && e < want)) && at < a.n) out[at] = i;
+            above += (int)(all & 0xffffu);
+            equal += (int)(all >> 16);
+        }
     }
 }
 
