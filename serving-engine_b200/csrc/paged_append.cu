@@ -20,8 +20,17 @@
 // otherwise fall either way by the rounding of whoever rotates it.  Rows are
 // quantised in 32 bits with a bound on what that is off by; where the minimum,
 // the scale or a code could round otherwise within it (1 row in 100 or so) the
-// warp does them again in 64 bits.  (All of it in 64 bits: 540 instructions for
-// 8 channels a lane instead of 200, 101 us for 8192 tokens instead of TODO.)
+// warp does them again in 64 bits, from sines and cosines kept as two 32-bit
+// numbers each.  (All of it in 64 bits: 540 instructions for 8 channels a lane,
+// 101 us for 8192 tokens.)
+//
+// Measured: 8192 tokens, 32 query and 8 K/V heads of 128, into a 4-bit cache 58
+// us (floor 27), 39 of them for keys and values alone: 360 instructions for 8
+// channels a lane, two thirds of the issue slots taken; the queries alone are
+// bound by HBM (21 us), and their CTAs stand between the others (one kind after
+// the other: 63 us).  16 channels a lane: fewer instructions by an eighth, but
+// too many registers (68 us).  One token of one sequence 4 us in a graph: the
+// chain length, table entry, row.
 #include <cmath>
 #include <type_traits>
 
@@ -64,6 +73,9 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
     return BF16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) : h2_to_f2(x);
 }
 
+// Where quad x of angles stands: lanes 4 or 8 quads apart read different banks.
+__device__ __forceinline__ int spread(int x) { return x + (x >> 3); }
+
 // The larger, or a NaN if one is.
 __device__ __forceinline__ float fmax_nan(float a, float b) {
     float r;
@@ -81,7 +93,8 @@ template <int WIDE, int VEC, bool BF16>
 __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_constant__ AppendArgs a) {
     using Vec = typename Chunk<VEC>::T;
     constexpr bool KV4 = WIDE > 0;
-    __shared__ float4 s_cs[kApTokens][64];  // of two pairs of channels: cosines, sines
+    // of two pairs of channels, at spread(pair / 2): cosines, sines; and what their rounding to 32 bits left
+    __shared__ float4 s_cs[kApTokens][72], s_rest[KV4 ? kApTokens : 1][72];
     __shared__ int64_t s_row[kApTokens];  // where a token's rows go: element offset of its first head, or byte offset of its tile
     __shared__ int s_in[KV4 ? kApTokens : 1][3];  // in the tile: K row, V units, scales
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -126,10 +139,13 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
             double sd, cd;
             sincospi(2.0 * turn, &sd, &cd);
             sn = (float)sd, cn = (float)cd;
+            float* rest = reinterpret_cast<float*>(&s_rest[KV4 ? t : 0][spread(e >> 1)]) + (e & 1);
+            rest[0] = (float)(cd - cn);
+            rest[2] = (float)(sd - sn);
         } else {
             sincospif((float)(2.0 * turn), &sn, &cn);
         }
-        float* cs = reinterpret_cast<float*>(&s_cs[t][e >> 1]) + (e & 1);
+        float* cs = reinterpret_cast<float*>(&s_cs[t][spread(e >> 1)]) + (e & 1);
         cs[0] = cn;
         cs[2] = sn;
     }
@@ -165,7 +181,7 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
                 if (TURN && turns) {
 #pragma unroll
                     for (int j = 0; j < VEC / 2; ++j) {
-                        const float4 t = s_cs[tok][(c0 >> 1) + j];
+                        const float4 t = s_cs[tok][spread((c0 >> 1) + j)];
                         cn[j] = pair(t.x, t.y), sn[j] = pair(t.z, t.w), ns[j] = pair(-t.z, -t.w);
                     }
                 }
@@ -253,7 +269,7 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
         float4 cs[4];
         if (key && turned) {
     #pragma unroll
-            for (int i = 0; i < 8; i += 2) cs[i / 2] = s_cs[tok][(VEC == 8 || i < 4 ? e0 + i : e1 + i - 4) >> 1];
+            for (int i = 0; i < 8; i += 2) cs[i / 2] = s_cs[tok][spread((VEC == 8 || i < 4 ? e0 + i : e1 + i - 4) >> 1)];
         }
         // a row and the partners of its channels: the next row's are on their way while one is worked on
         struct Row {
@@ -384,14 +400,13 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
                     float u[4], g[4];
                     unpack(own4, u);
                     unpack(oth, g);
-                    const int64_t pos = first + tok;
-    #pragma unroll 1
+                    const float *cs = reinterpret_cast<const float*>(s_cs[tok]), *rest = reinterpret_cast<const float*>(s_rest[tok]);
+#pragma unroll 1
                     for (int i = 0; i < 4; ++i) {
                         y[i] = u[i];
                         if (key && turned) {
-                            double turn = (double)pos * a.turns[e + i], sn, cn;
-                            turn -= rint(turn);
-                            sincospi(2.0 * turn, &sn, &cn);
+                            const int n = spread((e + i) >> 1) * 4 + (i & 1);  // (e is a multiple of 4)
+                            const double cn = (double)cs[n] + rest[n], sn = (double)cs[n + 2] + rest[n + 2];
                             y[i] = fma((double)u[i], cn, (low ? -(double)g[i] : (double)g[i]) * sn);
                         }
                     }
@@ -408,10 +423,17 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
                 }
                 m = finite_half((float)l);
                 s = finite_half(fmaxf((float)((u - (double)m) / 15.0), 0.f));
+                const double rs64 = s > 0.f ? __frcp_rn(s) : 0.f;  // (off by 2^-24: one step at most, put right by what is left)
                 codes = 0;
-                for (int i = 0; i < 8; ++i) {
-                    const double t = s > 0.f ? rint((x[i] - (double)m) / (double)s) : 0.0;
-                    codes |= (uint32_t)(t < 0.0 ? 0.0 : t > 15.0 ? 15.0 : t) << (4 * i);
+#pragma unroll 1
+                for (int i = 0; i < 8; ++i) {  // the nearest whole number to d / s, of two equally near ones the even
+                    const double d = x[i] - (double)m;
+                    int n = (int)rint(fmin(fmax(d * rs64, 0.0), 15.0));
+                    const double left = fma((double)-n, (double)s, d);
+                    const bool odd = n & 1;
+                    if (left > 0.5 * s || (left == 0.5 * s && odd)) ++n;
+                    if (left < -0.5 * s || (left == -0.5 * s && odd)) --n;
+                    if (s > 0.f) codes |= (uint32_t)max(0, min(n, 15)) << (4 * i);
                 }
             }
             if (!mine) continue;
