@@ -413,11 +413,21 @@ int b2_paged_decode_gqa_blocks(const void* q, int64_t ldq, const b2_paged_kv* kv
                                void* out, int batch, int num_q_heads, int num_kv_heads, int head_dim,
                                b2_workspace* ws, void* stream);
 
+/* What an append takes: k and v are [batch][S][num_kv_heads][head_dim] views of
+ * the cache's type (stride_b, stride_s, stride_h; rows contiguous and 16-byte
+ * aligned; the stride of a dimension of one is not looked at), q and q_out (both,
+ * or data NULL in both) the same of num_q_heads; q_out may be q. */
+typedef struct b2_append {
+    b2_kv_view k, v, q, q_out;
+    const double* inv_freq; /* host */
+    const int* counts;      /* device, or NULL */
+    const int* positions;   /* device, or NULL */
+    int64_t S;
+    int batch, num_q_heads, num_kv_heads, head_dim, rotary_dim;
+} b2_append;
+
 /* The rows of new tokens into a paged cache, with the position rotation of
- * their queries and keys on the way; one launch.  k and v are [batch][S]
- * [num_kv_heads][head_dim] views of the cache's type (stride_b, stride_s,
- * stride_h; rows contiguous and 16-byte aligned), q and q_out (both or neither)
- * the same of num_q_heads; q_out may be q.  counts (device int32 [batch], NULL:
+ * their queries and keys on the way; one launch.  counts (device int32 [batch], NULL:
  * S each) says how many of a sequence's S rows are new tokens; the others are
  * neither read nor written.  seq_lens counts them already: row i of n goes to
  * position seq_lens[b] - n + i, as long as that is at least 0, inside the
@@ -429,25 +439,23 @@ int b2_paged_decode_gqa_blocks(const void* q, int64_t ldq, const b2_paged_kv* kv
  * cache, or counts up from positions[b] (device int32 [batch]) where that is
  * given: after an eviction the two differ.  Angles are reduced in 64 bits.
  *
- * Sequences of one call must not share the blocks that they write.  Allocates
- * nothing; graph-capturable.  S at most 2^30, batch at most 65535. */
-int b2_paged_kv_append(const b2_paged_kv* kv, const b2_kv_view* k, const b2_kv_view* v, const b2_kv_view* q,
-                       const b2_kv_view* q_out, const double* inv_freq, int rotary_dim, const int* counts,
-                       const int* positions, int batch, int64_t S, int num_q_heads, int num_kv_heads, int head_dim,
-                       void* stream);
-/* The same into a cache held in 4 bits.  Keys are rotated in 64 bits and every
- * code is the one of exact arithmetic (m and s by way of 32 bits). */
-int b2_paged_kv4_append(const b2_paged_kv4* kv, const b2_kv_view* k, const b2_kv_view* v, const b2_kv_view* q,
-                        const b2_kv_view* q_out, const double* inv_freq, int rotary_dim, const int* counts,
-                        const int* positions, int batch, int64_t S, int num_q_heads, int num_kv_heads, int head_dim,
-                        void* stream);
+ * Sequences of one call must not share the blocks that they write, and what is
+ * read must not overlap what is written (q_out may be q).  Inputs may have
+ * strides of 0, q_out not.  Allocates nothing; graph-capturable.  S at most 2^30,
+ * batch at most 65535. */
+int b2_paged_kv_append(const b2_paged_kv* kv, const b2_append* rows, void* stream);
+/* The same into a cache held in 4 bits.  Codes are decided by keys rotated to
+ * 2^-47 of the row's largest, not by a 32-bit rounding of them (m and s go by
+ * way of 32 bits). */
+int b2_paged_kv4_append(const b2_paged_kv4* kv, const b2_append* rows, void* stream);
 
 /* The newest rows of each sequence out of a cache held in 4 bits, as 16-bit
  * rows (for the attention of a prompt's next chunk, say): the last n =
  * min(counts[b], T, seq_lens[b]) positions (counts NULL: T), in order, into
  * rows 0 .. n-1 of k_out and v_out, [batch][T][num_kv_heads][head_dim] views as
  * above.  Other rows, and those whose table entry is outside [0, num_blocks),
- * are left as they were. */
+ * are left as they were.  A length past the table's row counts as the row's end;
+ * strides of 0 are refused. */
 int b2_paged_kv4_read(const b2_paged_kv4* kv, const b2_kv_view* k_out, const b2_kv_view* v_out, const int* counts,
                       int batch, int64_t T, int num_kv_heads, int head_dim, void* stream);
 
@@ -458,8 +466,9 @@ int b2_paged_kv4_read(const b2_paged_kv4* kv, const b2_kv_view* k_out, const b2_
  * for the blocks that the last newest[b] positions of each sequence lie in
  * (device int32 [batch]; NULL: all its blocks), over all rows below seq_lens[b].
  * A block that holds a NaN or an infinity gets codes 0 and an infinite scale.
- * Blocks shared by sequences have to be full in all of them.  One launch;
- * allocates nothing. */
+ * Blocks shared by sequences have to be full in all of them.  Bounds go with the
+ * blocks' rows: after anything but an append (an eviction, say) they are brought
+ * up to date without newest.  One launch; allocates nothing. */
 int b2_paged_block_bounds(const b2_paged_kv* kv, const int* newest, void* codes, float* scale, int batch,
                           int num_kv_heads, int head_dim, void* stream);
 int b2_paged_kv4_block_bounds(const b2_paged_kv4* kv, const int* newest, void* codes, float* scale, int batch,

@@ -44,6 +44,12 @@ class PagedKV4Struct(C.Structure):
                 ("block_size", i32), ("max_blocks", i32), ("bf16", i32)]
 
 
+class AppendStruct(C.Structure):
+    _fields_ = [("k", KVView), ("v", KVView), ("q", KVView), ("q_out", KVView), ("inv_freq", vp), ("counts", vp),
+                ("positions", vp), ("S", i64), ("batch", i32), ("num_q_heads", i32), ("num_kv_heads", i32),
+                ("head_dim", i32), ("rotary_dim", i32)]
+
+
 class TokenizerInfo(C.Structure):
     _fields_ = [("vocab_size", i64), ("n_ids", i64), ("n_merges", i64), ("pre_tokenizer", i32), ("nfc", i32),
                 ("ignore_merges", i32), ("chat_format", i32), ("bos_id", i32), ("eos_id", i32), ("n_stop", i32),
@@ -91,8 +97,8 @@ _SIGS = {
     "b2_kv4_tile_bytes": (C.c_size_t, [i32]),
     "b2_paged_kv4_decode_gqa": (i32, [vp, i64, vp, vp, i32, vp, i32, i32, i32, i32, i32, i32, vp, vp]),
     "b2_paged_kv4_decode_workspace_bytes": (C.c_size_t, [i32, i32, i32]),
-    "b2_paged_kv_append": (i32, [vp, vp, vp, vp, vp, vp, i32, vp, vp, i32, i64, i32, i32, i32, vp]),
-    "b2_paged_kv4_append": (i32, [vp, vp, vp, vp, vp, vp, i32, vp, vp, i32, i64, i32, i32, i32, vp]),
+    "b2_paged_kv_append": (i32, [vp, vp, vp]),
+    "b2_paged_kv4_append": (i32, [vp, vp, vp]),
     "b2_paged_kv4_read": (i32, [vp, vp, vp, vp, i32, i64, i32, i32, vp]),
     "b2_paged_block_bounds": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
     "b2_paged_kv4_block_bounds": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
@@ -542,17 +548,18 @@ class Rope:
         self.ref = C.addressof(self.inv_freq)
 
 
-_PACK2, _PACK4 = struct.Struct("10q").pack_into, struct.Struct("20q").pack_into
+_PACK_VIEWS, _PACK_APPEND = struct.Struct("10q").pack_into, struct.Struct("24q5i").pack_into
+_NO_VIEW = 0, 0, 0, 0, 0
 _LOCAL = threading.local()
 
 
 def _views():
-    """Room for four KVViews and its address, one per thread: the library reads them before a call returns, and
-    filling them costs a tenth of what making KVViews does (2 us a call)."""
+    """Room for an AppendStruct or two KVViews and its address, one per thread: the library reads them before a call
+    returns, and filling them costs a tenth of what making KVViews does (2 us a call)."""
     try:
         return _LOCAL.views
     except AttributeError:
-        buf = (i64 * 20)()
+        buf = AppendStruct()
         _LOCAL.views = buf, C.addressof(buf)
         return _LOCAL.views
 
@@ -562,8 +569,7 @@ def _rows(t, name, shape, dtype, dev):
     if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
         raise ValueError(f"{name} must be {dtype} {shape} on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     b, s, h, d = t.stride()
-    # the stride of a dimension of one may be anything and is never used
-    return t.data_ptr(), b if shape[0] > 1 else 0, h if shape[2] > 1 else 0, s if shape[1] > 1 else 0, d
+    return t.data_ptr(), b, h, s, d
 
 
 def paged_kv_append(kv, k, v, q=None, q_out=None, rope: Rope | None = None, counts=None, positions=None, stream=None):
@@ -584,24 +590,17 @@ def paged_kv_append(kv, k, v, q=None, q_out=None, rope: Rope | None = None, coun
     S = k.shape[1]
     shape = (B, S, kv.nkv, D)
     kn, vn = _rows(k, "k", shape, dtype, dev), _rows(v, "v", shape, dtype, dev)
-    nq = 0
+    nq, qn, qo = 0, _NO_VIEW, _NO_VIEW
     if q is not None:
         if q.dim() != 4:
             raise ValueError(f"q must be [{B}, {S}, heads, {D}], got {tuple(q.shape)}")
         nq = q.shape[2]
         shape = (B, S, nq, D)
         qn = _rows(q, "q", shape, dtype, dev)
-        views, at = _views()
-        _PACK4(views, 0, *kn, *vn, *qn, *(qn if q_out is None else _rows(q_out, "q_out", shape, dtype, dev)))
-        qr, qor = at + 80, at + 120
+        qo = qn if q_out is None else _rows(q_out, "q_out", shape, dtype, dev)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    else:
-        views, at = _views()
-        _PACK2(views, 0, *kn, *vn)
-        qr = qor = None
-    cp = pp = rp = None
-    rot = 0
+    cp = pp = rp = rot = 0
     if rope is not None:
         rp, rot = rope.ref, rope.rotary_dim
     if counts is not None:
@@ -610,8 +609,9 @@ def paged_kv_append(kv, k, v, q=None, q_out=None, rope: Rope | None = None, coun
     if positions is not None:
         _need(positions, "positions", _TORCH.int32, (B,), dev)
         pp = positions.data_ptr()
-    call("b2_paged_kv4_append" if kv.four else "b2_paged_kv_append", kv.ref, at, at + 40, qr, qor, rp, rot, cp, pp, B, S, nq,
-         kv.nkv, D, _stream_of(stream, dev))
+    views, at = _views()
+    _PACK_APPEND(views, 0, *kn, *vn, *qn, *qo, rp, cp, pp, S, B, nq, kv.nkv, D, rot)
+    call("b2_paged_kv4_append" if kv.four else "b2_paged_kv_append", kv.ref, at, _stream_of(stream, dev))
     return q if q_out is None else q_out
 
 
@@ -631,7 +631,7 @@ def paged_kv_read(kv: PagedKV4, k_out, v_out, counts=None, stream=None):
     T = k_out.shape[1]
     shape = (B, T, kv.nkv, D)
     views, at = _views()
-    _PACK2(views, 0, *_rows(k_out, "k_out", shape, kv.dtype, dev), *_rows(v_out, "v_out", shape, kv.dtype, dev))
+    _PACK_VIEWS(views, 0, *_rows(k_out, "k_out", shape, kv.dtype, dev), *_rows(v_out, "v_out", shape, kv.dtype, dev))
     cp = None
     if counts is not None:
         _need(counts, "counts", _TORCH.int32, (B,), dev)

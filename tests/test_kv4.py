@@ -50,8 +50,10 @@ FREQ = (C.c_double * 32)(*([1.0] * 32))
 
 def append(kv, k=None, v=None, q=None, q_out=None, freq=FREQ, rot=64, batch=1, S=1, nq=4, nkv=2, D=64):
     fn = b2.lib().b2_paged_kv4_append if isinstance(kv, b2.PagedKV4Struct) else b2.lib().b2_paged_kv_append
-    return fn(ref(kv), ref(k or view()), ref(v or view()), ref(q), ref(q_out), C.addressof(freq) if freq else None, rot, None,
-              None, batch, S, nq, nkv, D, None)
+    none = view(data=None)
+    rows = b2.AppendStruct(k or view(), v or view(), q or none, q_out or none, C.addressof(freq) if freq else None, None, None,
+                           S, batch, nq, nkv, D, rot)
+    return fn(ref(kv), ref(rows), None)
 
 
 def read(kv, k=None, v=None, batch=1, T=1, nkv=2, D=64):
@@ -98,7 +100,8 @@ def test_listed_decode_refuses():
 
 @pytest.mark.parametrize("make", [cache16, cache4])
 def test_append_refuses(make):
-    assert append(None, batch=0) == 0 if make is cache16 else True
+    fn = b2.lib().b2_paged_kv_append if make is cache16 else b2.lib().b2_paged_kv4_append
+    assert fn(ref(make()), None, None) == -1 and fn(None, ref(b2.AppendStruct(batch=0, S=1)), None) == 0
     assert append(make(), S=0) == 0 and append(make(), batch=0) == 0
     assert append(make(block_tables=None)) == -1 and append(make(num_blocks=0)) == -1
     assert append(make(), k=view(data=None)) == -1 and append(make(), v=view(data=None)) == -1
