@@ -30,7 +30,7 @@
 // TB/s: a block's loads leave together, then its warp works them off), of the
 // newest block of 8 sequences 6.3 us, a chain of three loads; scores of 32 x
 // 2048 blocks of 8 heads 27 us (5.2 TB/s), of 4094 blocks 10.5 us, five loads one
-// after the other; the choice among 2048 blocks 6.9 us, among 8188 9.5 us (14 us
+// after the other; the choice among 2048 blocks 6.6 us, among 8188 9.5 us (14 us
 // with 512 threads and keys in shared memory): its barriers, six and five a
 // further 11 bits, and the keys' atomics.
 #include <cmath>
@@ -261,8 +261,6 @@ static int bounds_launch(const BoundsArgs& a, bool kv4, cudaStream_t s) {
 
 constexpr int kScThreads = 256;  // of the scores
 constexpr int kScWarps = kScThreads / 32;
-constexpr int kSlThreads = 1024;  // of a choice
-constexpr int kSlWarps = kSlThreads / 32;
 constexpr int kSlKeys = 8;  // keys that a thread keeps
 constexpr int kSlBins = 2048;
 constexpr uint32_t kSlStays = 0xffffffffu;  // blocks that are chosen in any case
@@ -425,19 +423,21 @@ __global__ void __launch_bounds__(kScThreads, 2) score_kernel(const SelectArgs a
 
 // One CTA per (sequence, kv head).  Keys stay in registers (up to 8 of a thread;
 // of longer sequences they are read again from the workspace).
-__global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) choose_kernel(const SelectArgs a) {
+    constexpr int WARPS = THREADS / 32;
     __shared__ uint32_t s_few32[32];
     __shared__ int s_hist[kSlBins];
-    __shared__ int s_sum[kSlWarps];
-    __shared__ uint32_t s_count[kSlKeys][kSlWarps];  // keys above the border, and equal to it << 16
+    __shared__ int s_sum[WARPS];
+    __shared__ uint32_t s_count[kSlKeys][WARPS];  // keys above the border, and equal to it << 16
     __shared__ int s_bin, s_above, s_in, s_few;
-    __shared__ uint32_t s_range[2][kSlWarps];
+    __shared__ uint32_t s_range[2][WARPS];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = blockIdx.x, b = blockIdx.y;
-    constexpr int PER = kSlBins / kSlThreads;
+    constexpr int PER = kSlBins / THREADS;
     auto clear = [&]() {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) s_hist[i * kSlThreads + tid] = 0;
+        for (int i = 0; i < PER; ++i) s_hist[i * THREADS + tid] = 0;
     };
     clear();
     griddep_wait();
@@ -447,16 +447,16 @@ __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) 
     const int64_t pair = (int64_t)b * a.nkv + h;
     int* out = a.out + pair * a.n;
     if (nb <= a.n) {  // every block
-        for (int i = tid; i < a.n; i += kSlThreads) out[i] = i < nb ? i : -1;
+        for (int i = tid; i < a.n; i += THREADS) out[i] = i < nb ? i : -1;
         return;
     }
     const uint32_t* keys = a.keys + pair * a.max_blocks;
-    constexpr int ROUND = kSlKeys * kSlThreads;  // keys at a time
+    constexpr int ROUND = kSlKeys * THREADS;  // keys at a time
     uint32_t key[kSlKeys];
     auto fetch = [&](int i0) {
 #pragma unroll
         for (int j = 0; j < kSlKeys; ++j) {
-            const int i = i0 + j * kSlThreads + tid;
+            const int i = i0 + j * THREADS + tid;
             key[j] = i < nb ? __ldcg(keys + i) : kSlStays;  // (what stays is left out of the ranking)
         }
     };
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) 
             if (nb > ROUND) fetch(i0);
 #pragma unroll
             for (int j = 0; j < kSlKeys; ++j)
-                if (i0 + j * kSlThreads < nb) f(key[j]);
+                if (i0 + j * THREADS < nb) f(key[j]);
         }
     };
     if (nb <= ROUND) fetch(0);
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) 
     }
     if (lane == 0) s_range[0][warp] = lowest, s_range[1][warp] = highest;
     __syncthreads();
-    lowest = s_range[0][lane], highest = s_range[1][lane];
+    lowest = s_range[0][lane % WARPS], highest = s_range[1][lane % WARPS];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         lowest = min(lowest, __shfl_xor_sync(~0u, lowest, o));
@@ -555,11 +555,11 @@ __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) 
             fetch(i0);
             __syncthreads();
         }
-        const int rows = min(kSlKeys, (nb - i0 + kSlThreads - 1) / kSlThreads);
+        const int rows = min(kSlKeys, (nb - i0 + THREADS - 1) / THREADS);
 #pragma unroll
         for (int j = 0; j < kSlKeys; ++j) {
             if (j >= rows) break;
-            const bool there = i0 + j * kSlThreads + tid < nb;
+            const bool there = i0 + j * THREADS + tid < nb;
             const uint32_t up = __ballot_sync(~0u, there && key[j] > border), eq = __ballot_sync(~0u, there && key[j] == border);
             if (lane == 0) s_count[j][warp] = __popc(up) | __popc(eq) << 16;
         }
@@ -567,10 +567,10 @@ __global__ void __launch_bounds__(kSlThreads) choose_kernel(const SelectArgs a) 
 #pragma unroll
         for (int j = 0; j < kSlKeys; ++j) {
             if (j >= rows) break;
-            const int i = i0 + j * kSlThreads + tid;
+            const int i = i0 + j * THREADS + tid;
             const bool there = i < nb, over = there && key[j] > border, same = there && key[j] == border;
             const uint32_t up = __ballot_sync(~0u, over), eq = __ballot_sync(~0u, same);
-            uint32_t sum = s_count[j][lane];  // of warps 0 .. lane
+            uint32_t sum = lane < WARPS ? s_count[j][lane] : 0u;  // of warps 0 .. lane
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint32_t v = __shfl_up_sync(~0u, sum, o);
@@ -591,7 +591,13 @@ template <int P>
 static int select_launch(const SelectArgs& a, int batch, cudaStream_t s) {
     const dim3 grid((unsigned)((a.max_blocks + a.chunk - 1) / a.chunk), (unsigned)((a.nkv + a.heads - 1) / a.heads), (unsigned)batch);
     B2_TRY(launch(score_kernel<P>, grid, dim3(kScThreads), 0, s, true, a));
-    B2_TRY(launch(choose_kernel, dim3((unsigned)a.nkv, (unsigned)batch), dim3(kSlThreads), 0, s, true, a));
+    // as many threads as keep all keys in registers (2048 blocks of 256 pairs: 8.5 us with 512, 11 with 1024, 8.9 with 256;
+    // 4094 blocks of 8 pairs: 7.4 with 512, 7.5 with 1024)
+    const dim3 pairs((unsigned)a.nkv, (unsigned)batch);
+    if (a.max_blocks <= 512 * kSlKeys)
+        B2_TRY(launch(choose_kernel<512>, pairs, dim3(512), 0, s, true, a));
+    else
+        B2_TRY(launch(choose_kernel<1024>, pairs, dim3(1024), 0, s, true, a));
     return B2_OK;
 }
 
