@@ -111,6 +111,12 @@ CASES = [
     (2, 30, [30, 30], None, 4, 2, 128, 16, 32, "bf16"),
     (1, 300, [300], None, 2, 2, 64, 16, 64, "fp16"),
     (1, 1, [100], None, 40, 5, 64, 128, 64, "fp16"),
+    # several tokens in one place: 2, 4 and 8 at a time, the last ones of a sequence fewer
+    (3, 301, [301, 400, 301], [301, 150, 1], 3, 2, 64, 16, 64, "bf16"),
+    (3, 611, [611, 611, 700], [3, 611, 610], 2, 1, 72, 16, 72, "fp16"),
+    (60, 61, [61 + i for i in range(60)], [61 - i for i in range(60)], 5, 2, 128, 16, 128, "bf16"),
+    (60, 61, [61 + i for i in range(60)], [i + 1 for i in range(60)], 2, 3, 96, 32, 64, "fp16"),
+    (1, 4003, [4003], None, 2, 1, 256, 64, 256, "bf16"),
 ]
 
 

@@ -128,11 +128,27 @@ def bare(seed, lens, nkv, D, bs, dt, group, blocks=None):
     ([600, 90], 2, 256, 8, "fp16", 11, 1, 1),
     ([20000, 7777, 30], 2, 64, 4, "fp16", 64, 1, 2),
     ([140000], 1, 64, 2, "bf16", 300, 4, 4),
+    ([131072], 2, 64, 2, "fp16", 40, 1, 2),
+    ([100000, 70000], 1, 8, 1, "bf16", 64, 0, 0),
     ([33] * 600, 8, 64, 1, "fp16", 2, 0, 1),
 ])
 def test_choice(cuda, lens, nkv, D, group, dt, n, first, last):
     q, kv, bd = bare(3, lens, nkv, D, 16, dt, group, blocks=min(4000, sum(-(-x // 16) for x in lens) + 5))
     assert torch.equal(chosen(q, kv, bd, n, first, last), want_blocks(q, kv, bd, lens, n, first, last))
+
+
+@pytest.mark.parametrize("L", [65536, 131072, 300000])
+def test_ties_of_long_sequences(cuda, L):
+    """Scores of three values: the best of the best one's blocks, then the first of the next one's."""
+    q, kv, bd = bare(5, [L], 1, 64, 16, "fp16", 2)
+    nb = L // 16
+    kv.block_tables.copy_(torch.arange(nb, device="cuda")[None])
+    bd.scale.fill_(1.0)
+    bd.codes.fill_(3)
+    bd.codes[::10, :, 1], bd.codes[5::1000, :, 1] = 20, 90
+    q.fill_(1.0)
+    n = nb // 1000 + 1 + nb // 20
+    assert torch.equal(chosen(q, kv, bd, n, 1, 1), want_blocks(q, kv, bd, [L], n, 1, 1))
 
 
 @pytest.mark.parametrize("what", ["ties", "zero query", "nan query", "infinite query", "infinite scale", "no block",
