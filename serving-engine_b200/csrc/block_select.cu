@@ -440,6 +440,7 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(const SelectArgs a) {
         for (int i = 0; i < PER; ++i) s_hist[i * THREADS + tid] = 0;
     };
     clear();
+    if (tid == 0) s_bin = s_above = s_in = s_few = 0;
     griddep_wait();
     griddep_launch_dependents();
     const int len = max(0, min(a.seq_lens[b], a.max_blocks * a.block_size));
@@ -530,7 +531,10 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(const SelectArgs a) {
         const int in = s_in;
         if (in <= 32 && lowest < highest) {  // few enough to be ranked side by side in every warp
             each([&](uint32_t k) {
-                if (k - lowest <= highest - lowest) s_few32[atomicAdd(&s_few, 1)] = k;
+                if (k - lowest <= highest - lowest) {
+                    const int at = atomicAdd(&s_few, 1);
+                    if (at < 32) s_few32[at] = k;  // (more only if the keys change under way: a workspace used twice at once)
+                }
             });
             __syncthreads();
             const uint32_t k = lane < in ? s_few32[lane] : 0u;
