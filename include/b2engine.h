@@ -406,9 +406,10 @@ size_t b2_paged_kv4_decode_workspace_bytes(int num_q_heads, int num_kv_heads, in
 /* b2_paged_decode_gqa in which each (sequence, kv head) sees the positions of
  * the listed blocks of its sequence alone, below seq_lens[b]: blocks is device
  * int32 [batch][num_kv_heads][listed], indexes into the sequence's row of the
- * block tables.  Entries outside [0, max_blocks) or past the sequence's end
- * add nothing (pad with -1); a block listed twice counts twice.  Same
- * workspace. */
+ * block tables.  Of a sequence of nb blocks the first min(listed, nb) entries
+ * are looked at, so padding stands behind what is listed.  Of those, entries
+ * outside [0, max_blocks) or past the sequence's end add nothing; a block listed
+ * twice counts twice.  Same workspace. */
 int b2_paged_decode_gqa_blocks(const void* q, int64_t ldq, const b2_paged_kv* kv, const int* blocks, int listed,
                                void* out, int batch, int num_q_heads, int num_kv_heads, int head_dim,
                                b2_workspace* ws, void* stream);

@@ -467,7 +467,8 @@ def paged_decode_gqa(q, kv, out, window=0, sinks=0, scores=None, ws: Workspace |
     optional, PagedKV only) accumulates every visible position's weight and
     needs a workspace.  blocks (int32 [B, nkv, n], optional, without window and
     scores): the blocks of its sequence that each K/V head sees, as
-    paged_block_select gives them; -1 is none."""
+    paged_block_select gives them; -1 is none, and a sequence of fewer than n
+    blocks is shown as many entries as it has blocks."""
     shape = q.shape
     B, nq, D = shape
     ldq, sh, sd = q.stride()

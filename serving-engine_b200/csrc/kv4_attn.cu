@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
             int blk = a.div.block(pos), v0 = 0, v1 = 0;
             const int slot = a.div.slot(pos, blk);
             if constexpr (LIST) {  // blk counts entries of the list
-                if (blk < a.listed) {
+                if (blk < pp.s.s0) {
                     blk = a.blocks[((int64_t)pp.b * a.nkv + pp.kvh) * a.listed + blk];
                     if ((unsigned)blk < (unsigned)a.max_blocks) v1 = min(16, pp.s.L - blk * a.block_size - slot);
                 }

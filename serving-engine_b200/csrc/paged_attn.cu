@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn
             bool sees = pp.s.sees(pp.u, pos);
             if constexpr (LIST) {  // blk counts entries of the list
                 sees = false;
-                if (blk < a.listed) {
+                if (blk < pp.s.s0) {
                     blk = a.blocks[((int64_t)pp.b * a.nkv + pp.kvh) * a.listed + blk];
                     sees = (unsigned)blk < (unsigned)a.max_blocks && slot < pp.s.L - blk * a.block_size;
                 }

@@ -195,7 +195,7 @@ def decode(q, k, v, tables, lens, window=0, sinks=0, blocks=None):
             if blocks is None:
                 pos = [t for t in range(n) if window == 0 or t < sinks or n - t <= window]
             else:
-                pos = [j * bs + i for j in blocks[b, h].tolist() if 0 <= j < tables.shape[1] for i in range(bs)
+                pos = [j * bs + i for j in blocks[b, h].tolist()[:-(-n // bs)] if 0 <= j < tables.shape[1] for i in range(bs)
                        if j * bs + i < n]
             at = [(int(tables[b, t // bs]), t % bs) for t in pos]
             at = [(x, y) for x, y in at if 0 <= x < nb]

@@ -307,6 +307,21 @@ def test_listed_blocks_of_any_size(cuda, bs):
 
 
 @pytest.mark.parametrize("bits", [4, 16])
+def test_lists_longer_than_the_sequences(cuda, bits):
+    """As many entries as a sequence has blocks are looked at: what stands behind them is padding, whatever it says."""
+    lens = [1, 16, 17, 0, 400]
+    q, kv, k, v = (make if bits == 4 else make16)(13, lens, 8, 2, 64, 16, "bf16")
+    blocks = torch.arange(60, dtype=torch.int32).expand(5, 2, 60).contiguous() % 25
+    outs = []
+    for x in (blocks, torch.where(torch.arange(60) < torch.tensor([1, 1, 2, 0, 25])[:, None, None], blocks, -1)):
+        outs.append(torch.empty_like(q))
+        b2.paged_decode_gqa(q, kv, outs[-1], blocks=x.cuda(), ws=ws_for(kv, 8))
+    want, mag = R.decode(q, k, v, kv.block_tables, lens)
+    close(outs[0], want, mag, q, k, v, 400)
+    assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("bits", [4, 16])
 def test_all_blocks_listed_is_the_whole_cache(cuda, bits):
     q, kv, k, v = (make if bits == 4 else make16)(12, [333, 60], 8, 2, 128, 16, "bf16")
     mb = kv.block_tables.shape[1]
