@@ -475,12 +475,24 @@ int b2_paged_block_bounds(const b2_paged_kv* kv, const int* newest, void* codes,
 int b2_paged_kv4_block_bounds(const b2_paged_kv4* kv, const int* newest, void* codes, float* scale, int batch,
                               int num_kv_heads, int head_dim, void* stream);
 
+/* What a choice of blocks takes (device pointers). */
+typedef struct b2_block_select {
+    const void* q; /* [batch][num_q_heads][head_dim], ldq elements from row to row; no alignment needed */
+    int64_t ldq;
+    const int *block_tables, *seq_lens; /* as in b2_paged_kv */
+    const void* codes;                  /* as in b2_paged_block_bounds */
+    const float* scale;
+    int* blocks; /* out: [batch][num_kv_heads][n] */
+    int bf16;    /* type of q */
+    int num_blocks, block_size, max_blocks, n, first, last, batch, num_q_heads, num_kv_heads, head_dim;
+} b2_block_select;
+
 /* The n blocks of each sequence that a new token looks at, per kv head: the
  * first `first`, the last `last` (first + last <= n) and, of those between, the
  * ones with the largest score (equal scores: the lowest block).  blocks (int32
  * [batch][num_kv_heads][n]) receives indexes into the sequence's row of the
  * block tables, ascending, -1 past the last; all blocks when there are at most
- * n.  q as in b2_paged_decode_gqa (no alignment needed), bf16 its type.
+ * n.
  *
  * score = float(sum_d hi_d P_d + lo_d N_d) * scale over the bounds' codes,
  * where P_d and N_d are the sums of the positive and of the negative q_hd over
@@ -493,10 +505,7 @@ int b2_paged_kv4_block_bounds(const b2_paged_kv4* kv, const int* newest, void* c
  *
  * ws needs b2_paged_block_select_workspace_bytes(...) bytes.  Two launches;
  * allocates nothing.  batch and num_kv_heads at most 65535. */
-int b2_paged_block_select(const void* q, int64_t ldq, int bf16, const int* block_tables, const int* seq_lens,
-                          int num_blocks, int block_size, int max_blocks, const void* codes, const float* scale,
-                          int* blocks, int n, int first, int last, int batch, int num_q_heads, int num_kv_heads,
-                          int head_dim, b2_workspace* ws, void* stream);
+int b2_paged_block_select(const b2_block_select* s, b2_workspace* ws, void* stream);
 size_t b2_paged_block_select_workspace_bytes(int batch, int num_kv_heads, int max_blocks);
 
 /* ---------------------------------------------------------------------------

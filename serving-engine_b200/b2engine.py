@@ -50,6 +50,12 @@ class AppendStruct(C.Structure):
                 ("head_dim", i32), ("rotary_dim", i32)]
 
 
+class BlockSelectStruct(C.Structure):
+    _fields_ = [("q", vp), ("ldq", i64), ("block_tables", vp), ("seq_lens", vp), ("codes", vp), ("scale", vp),
+                ("blocks", vp)] + [(n, i32) for n in ("bf16", "num_blocks", "block_size", "max_blocks", "n", "first", "last",
+                                                      "batch", "num_q_heads", "num_kv_heads", "head_dim")]
+
+
 class TokenizerInfo(C.Structure):
     _fields_ = [("vocab_size", i64), ("n_ids", i64), ("n_merges", i64), ("pre_tokenizer", i32), ("nfc", i32),
                 ("ignore_merges", i32), ("chat_format", i32), ("bos_id", i32), ("eos_id", i32), ("n_stop", i32),
@@ -102,8 +108,7 @@ _SIGS = {
     "b2_paged_kv4_read": (i32, [vp, vp, vp, vp, i32, i64, i32, i32, vp]),
     "b2_paged_block_bounds": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
     "b2_paged_kv4_block_bounds": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
-    "b2_paged_block_select": (i32, [vp, i64, i32, vp, vp, i32, i32, i32, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
-                                    vp, vp]),
+    "b2_paged_block_select": (i32, [vp, vp, vp]),
     "b2_paged_block_select_workspace_bytes": (C.c_size_t, [i32, i32, i32]),
     "b2_paged_kv_evict": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, vp]),
     "b2_swiglu": (i32, [vp, vp, vp, i64, vp]),
@@ -550,13 +555,14 @@ class Rope:
 
 
 _PACK_VIEWS, _PACK_APPEND = struct.Struct("10q").pack_into, struct.Struct("24q5i").pack_into
+_PACK_SELECT = struct.Struct("7q11i").pack_into
 _NO_VIEW = 0, 0, 0, 0, 0
 _LOCAL = threading.local()
 
 
 def _views():
-    """Room for an AppendStruct or two KVViews and its address, one per thread: the library reads them before a call
-    returns, and filling them costs a tenth of what making KVViews does (2 us a call)."""
+    """Room for an AppendStruct, a BlockSelectStruct or two KVViews and its address, one per thread: the library reads
+    them before a call returns, and filling them costs a tenth of what making KVViews does (2 us a call)."""
     try:
         return _LOCAL.views
     except AttributeError:
@@ -702,11 +708,12 @@ def paged_block_select(q, kv, bounds: BlockBounds, blocks, first=1, last=1, ws: 
     if ws is not None and ws.device != dev:
         raise ValueError(f"q is on {q.device}, the workspace on cuda:{ws.device}")
     n = blocks.shape[-1]
-    _need(blocks, "blocks", _torch().int32, (B, kv.nkv, n), dev)
-    call("b2_paged_block_select", q.data_ptr(), ldq, _is_bf16(q), kv.block_tables.data_ptr(), kv.seq_lens.data_ptr(),
-         kv.num_blocks, kv.block_size, kv.block_tables.shape[1], bounds.codes.data_ptr(), bounds.scale.data_ptr(),
-         blocks.data_ptr(), n, _clamp(first, _MOST32), _clamp(last, _MOST32), B, nq, kv.nkv, D,
-         ws.h if ws is not None else None, _stream_of(stream, dev))
+    _need(blocks, "blocks", _TORCH.int32, (B, kv.nkv, n), dev)
+    views, at = _views()
+    _PACK_SELECT(views, 0, q.data_ptr(), ldq, kv.block_tables.data_ptr(), kv.seq_lens.data_ptr(), bounds.codes.data_ptr(),
+                 bounds.scale.data_ptr(), blocks.data_ptr(), _is_bf16(q), kv.num_blocks, kv.block_size,
+                 kv.block_tables.shape[1], n, _clamp(first, _MOST32), _clamp(last, _MOST32), B, nq, kv.nkv, D)
+    call("b2_paged_block_select", at, ws.h if ws is not None else None, _stream_of(stream, dev))
     return blocks
 
 

@@ -672,38 +672,38 @@ extern "C" size_t b2_paged_block_select_workspace_bytes(int batch, int nkv, int 
     return (size_t)batch * nkv * max_blocks * sizeof(uint32_t);
 }
 
-extern "C" int b2_paged_block_select(const void* q, int64_t ldq, int bf16, const int* block_tables, const int* seq_lens,
-                                     int num_blocks, int block_size, int max_blocks, const void* codes,
-                                     const float* scale, int* blocks, int n, int first, int last, int batch, int nq,
-                                     int nkv, int D, b2_workspace* ws, void* stream) {
+extern "C" int b2_paged_block_select(const b2_block_select* r, b2_workspace* ws, void* stream) {
     using namespace b2;
+    B2_REQUIRE(r);
+    const int batch = r->batch, nq = r->num_q_heads, nkv = r->num_kv_heads, D = r->head_dim, max_blocks = r->max_blocks;
     if (batch <= 0) return B2_OK;
-    B2_REQUIRE(q && block_tables && seq_lens && blocks && num_blocks > 0 && block_size > 0 && max_blocks > 0 && n > 0 &&
-               first >= 0 && last >= 0 && (int64_t)first + last <= n && nq > 0 && nkv > 0 && nq % nkv == 0 && D > 0);
-    const int rc = bounds_check(codes, scale, batch, nkv, max_blocks);
+    B2_REQUIRE(r->q && r->block_tables && r->seq_lens && r->blocks && r->num_blocks > 0 && r->block_size > 0 && max_blocks > 0 &&
+               r->n > 0 && r->first >= 0 && r->last >= 0 && (int64_t)r->first + r->last <= r->n && nq > 0 && nkv > 0 &&
+               nq % nkv == 0 && D > 0);
+    const int rc = bounds_check(r->codes, r->scale, batch, nkv, max_blocks);
     if (rc != B2_OK) return rc;
-    if (D > 256 || (D & 7) || (int64_t)max_blocks * block_size > (1 << 30) || batch > 65535 || nkv > 65535)
+    if (D > 256 || (D & 7) || (int64_t)max_blocks * r->block_size > (1 << 30) || batch > 65535 || nkv > 65535)
         return B2_ERR_UNSUPPORTED;
     if (!ws || ws->bytes < b2_paged_block_select_workspace_bytes(batch, nkv, max_blocks)) return B2_ERR_WORKSPACE;
     SelectArgs a = {};
-    a.q = q;
-    a.ldq = ldq;
-    a.block_tables = block_tables;
-    a.seq_lens = seq_lens;
-    a.num_blocks = num_blocks;
-    a.block_size = block_size;
+    a.q = r->q;
+    a.ldq = r->ldq;
+    a.block_tables = r->block_tables;
+    a.seq_lens = r->seq_lens;
+    a.num_blocks = r->num_blocks;
+    a.block_size = r->block_size;
     a.max_blocks = max_blocks;
-    a.codes = static_cast<const int8_t*>(codes);
-    a.scale = scale;
-    a.out = blocks;
+    a.codes = static_cast<const int8_t*>(r->codes);
+    a.scale = r->scale;
+    a.out = r->blocks;
     a.nq = nq;
     a.nkv = nkv;
     a.D = D;
     a.group = nq / nkv;
-    a.bf16 = bf16;
-    a.n = n;
-    a.first = first;
-    a.last = last;
+    a.bf16 = r->bf16;
+    a.n = r->n;
+    a.first = r->first;
+    a.last = r->last;
     a.keys = static_cast<uint32_t*>(ws->ptr);
     // up to 8 heads per CTA, and as many CTAs as an SM holds together where that leaves each a few steps
     a.heads = nkv < kScWarps ? nkv : kScWarps;

@@ -67,8 +67,9 @@ def bounds(kv, codes=FAKE, scale=FAKE, batch=1, nkv=2, D=64):
 
 def select(q=FAKE, ldq=256, tables=FAKE, lens=FAKE, num_blocks=8, bs=16, mb=4, codes=FAKE, scale=FAKE, blocks=FAKE, n=2,
            first=1, last=1, batch=1, nq=4, nkv=2, D=64, ws=None):
-    return b2.lib().b2_paged_block_select(q, ldq, 0, tables, lens, num_blocks, bs, mb, codes, scale, blocks, n, first,
-                                          last, batch, nq, nkv, D, ws, None)
+    what = b2.BlockSelectStruct(q, ldq, tables, lens, codes, scale, blocks, 0, num_blocks, bs, mb, n, first, last, batch, nq,
+                                nkv, D)
+    return b2.lib().b2_paged_block_select(ref(what), ws, None)
 
 
 def test_decode_refuses():
@@ -134,7 +135,7 @@ def test_bounds_refuse(make):
 
 
 def test_select_refuses():
-    assert select(batch=0) == 0
+    assert select(batch=0) == 0 and b2.lib().b2_paged_block_select(None, None, None) == -1
     for name in ("q", "tables", "lens", "codes", "scale", "blocks"):
         assert select(**{name: None}) == -1, name
     assert select(n=0, first=0, last=0) == -1 and select(first=2, last=1) == -1 and select(first=-1) == -1
