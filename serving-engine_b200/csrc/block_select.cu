@@ -28,11 +28,11 @@
 //
 // Measured, cold: bounds of 32768 tokens of 8 heads of 128 in 16 bits 15 us (4.5
 // TB/s: a block's loads leave together, then its warp works them off), of the
-// newest block of 8 sequences 6.3 us, a chain of three loads; scores of 32 x
-// 2048 blocks of 8 heads 27 us (5.2 TB/s), of 4094 blocks 10.5 us, five loads one
-// after the other; the choice among 2048 blocks 6.6 us, among 8188 9.5 us (14 us
-// with 512 threads and keys in shared memory): its barriers, six and five a
-// further 11 bits, and the keys' atomics.
+// newest block of 8 sequences 6.3 us, a chain of three loads; scores of 32 x up to
+// 2048 blocks of 8 heads 28 us (117 MB, 4.3 TB/s with its start), of 4094 blocks
+// 11 us, five loads one after the other; the choice among 2048 blocks 6.6 us (8.5
+// of 256 pairs), among 8188 9.5 us (14 us with 512 threads and keys in shared
+// memory): its barriers, six and five a further 11 bits, and the keys' atomics.
 #include <cmath>
 
 #include "kv4.cuh"
