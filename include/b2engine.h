@@ -397,7 +397,7 @@ size_t b2_kv4_tile_bytes(int head_dim);
  * b2_paged_decode_gqa_blocks (window 0 then).  ws as there, of
  * b2_paged_kv4_decode_workspace_bytes(...) bytes, or NULL.  Sums, softmax
  * statistics and outputs in progress are 32-bit; codes enter the products
- * exactly. */
+ * exactly, weights with 22 bits. */
 int b2_paged_kv4_decode_gqa(const void* q, int64_t ldq, const b2_paged_kv4* kv, const int* blocks, int listed,
                             void* out, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window,
                             int sinks, b2_workspace* ws, void* stream);

@@ -21,36 +21,36 @@
 //            terms are a product too, of the scale words as they are stored with
 //            the sums of q as half and remainder.
 //   outputs  o_d = sum_i (p_i s_ig) (u_id - 8) + sum_i p_i (m_ig + 8 s_ig): the
-//            weights times the scale are the operand, rounded to halves; for
-//            outputs in half with what the rounding left as a half beside it, so
-//            that they cost no accuracy beside the output's own rounding (bf16
-//            rounds 8 times coarser than the weights are, and goes without: 1 %
-//            on the error of an exact result).  The second sum is kept in 32 bits
-//            per group.  Less 8, because sums of codes of one sign would be far
-//            larger than the output that is left of them (at 131001 tokens the
-//            rounding of the sums would show in the output: 5e-4 instead of
-//            1.7e-4 of it): a product with a constant -8 is where each unit's
-//            sums start.
+//            weights times the scale are the operand, as a half and what its
+//            rounding left as a half beside it: 22 bits of each.  (A bare half is
+//            off by up to 2^-11 of p s |u - 8|, while the m + u s that the two
+//            sums come to may vanish.)  The second sum is kept in 32 bits per
+//            group.  Less 8, because sums of codes of one sign would be far larger
+//            than the output that is left of them: a product with a constant -8
+//            is where each unit's sums start.  What shows at long contexts is the
+//            truncation of the matrix instruction's own sums: 131001 tokens in
+//            half are off by 2.24e-4 of the result, 2.08e-4 being the output's
+//            rounding (sums that start at -8 with every second tile: 2.16e-4 and 3 %
+//            slower, with every tile: 2.10e-4 and 7 %); in bf16 it does not.
 // Queries are scaled by a power of two into the middle of the halves' range
 // (bf16 ones are then exact in half), the weights by one that follows the
 // largest scale seen so far, like the running max of the softmax.
 //
 // Layout of the products: positions, then channels, are the 16 rows and the
-// heads the 8 columns.  Up to 4 heads (H = 4) stand twice in the columns: with
-// remainders the second copy becomes those, in the same product.  (Heads as the rows
+// heads the 8 columns.  Up to 4 heads (H = 4) stand twice in the columns: for the
+// outputs the second copy holds the remainders, in the same product.  (Heads as the rows
 // of S take twice the products and, since half of each operand's registers are
 // then zeros that have to be put there, 456 instructions a tile instead of 340.)
 //
 // Split: paged_split.cuh.  Each of 4 warps streams tiles of 16 positions (kv4.cuh)
 // through its own ring of shared-memory stages (cp.async).
 //
-// Measured: 32 sequences of up to 32768 tokens, 32/8 heads of 128: 187 us (5.5 TB/s,
-// 84 % of a copy; floor 158), 208 us under the power limit of a long run: 236
-// instructions a tile, half of the issue slots, 8 warps per SM that wait for one
-// another's pipes.  131001 tokens, 64/8 heads: 48 us (floor 23): eight columns of
-// heads, the remainders in products of their own, 37 pieces joined per segment.  8
-// sequences of up to 4096: 16 us, 301 tokens of 14/2 heads of 64: 7 us: the chain
-// length, table, rows, merge, join.
+// Measured: 32 sequences of up to 32768 tokens, 32/8 heads of 128, bf16: 227 us in a
+// long run (4.6 TB/s, 70 % of a copy; floor 158; without remainders 218): half of
+// the issue slots, 8 warps per SM that wait for one another's pipes.  131001 tokens,
+// 64/8 heads: 48 us (floor 23): eight columns of heads, the remainders in products of
+// their own, 37 pieces joined per segment.  8 sequences of up to 4096: 17 us, 301
+// tokens of 14/2 heads of 64: 7 us: the chain length, table, rows, merge, join.
 #include <cmath>
 #include <type_traits>
 
@@ -130,12 +130,12 @@ __device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// BF16: type of q and out; without it weights are split.
+// BF16: type of q and out.
 template <int DP, int H, bool BF16, bool LIST>
 __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kernel(const Kv4Args a) {
     using C = Kv4Cfg<DP, H>;
     constexpr int U = C::U, T = C::T, W = C::W, NG = C::NG;
-    constexpr bool SPLIT = !BF16, TWO = SPLIT && H > 4;  // remainders of the weights; in products of their own
+    constexpr bool TWO = H > 4;          // remainders of the weights in products of their own
     constexpr int NT = H == 16 ? 2 : 1;  // products side by side, 8 heads each
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ SplitShared s_split;
@@ -496,13 +496,10 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                             am[n][1][g] = fmaf(p1, mid, am[n][1][g]);
                             const float w0 = p0 * sm.x, w1 = p1 * sm.x;
                             const uint32_t u = f2_to_h2(w0, w1);
-                            if constexpr (SPLIT) {  // (in one multiply-add of halves and a 32-bit number each)
-                                const uint32_t r = f2_to_h2(fma_f16_f32<0>(u, 0xbc00bc00u, w0), fma_f16_f32<1>(u, 0xbc00bc00u, w1));
-                                hi[t][n][pp] = transpose8x8(TWO || lc < 2 ? u : r);
-                                if constexpr (TWO) lo[t][n][pp] = transpose8x8(r);
-                            } else {
-                                hi[t][n][pp] = transpose8x8(u);
-                            }
+                            // (in one multiply-add of halves and a 32-bit number each)
+                            const uint32_t r = f2_to_h2(fma_f16_f32<0>(u, 0xbc00bc00u, w0), fma_f16_f32<1>(u, 0xbc00bc00u, w1));
+                            hi[t][n][pp] = transpose8x8(TWO || lc < 2 ? u : r);
+                            if constexpr (TWO) lo[t][n][pp] = transpose8x8(r);
                         }
                     }
                     // -8 units in the rows of either nibble: what the products of the codes start from
@@ -590,7 +587,7 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                 }
             // rows of codes in the low nibble of a byte hold sums 16 times smaller
             constexpr float k0 = 16777216.f, k1 = 1048576.f;
-            if (H == 4 && SPLIT) {
+            if (H == 4) {
 #pragma unroll
                 for (int x = 0; x < W; ++x)
 #pragma unroll
