@@ -500,8 +500,9 @@ typedef struct b2_block_select {
  * two that 32767 multiples of cover the largest of them: whole numbers, so the
  * choice does not depend on the order of any sum.  Up to that rounding and a
  * positive factor it is an upper bound of the sum of the group's logits.  q with
- * a NaN or an infinity scores 0 everywhere; blocks of infinite scale rank first;
- * those whose table entry is outside [0, num_blocks) rank last.
+ * a NaN or an infinity scores 0 everywhere; blocks of infinite scale rank first,
+ * behind those of a scale that is NaN (never written, say); those whose table
+ * entry is outside [0, num_blocks) rank last.
  *
  * ws needs b2_paged_block_select_workspace_bytes(...) bytes.  Two launches;
  * allocates nothing.  batch and num_kv_heads at most 65535. */

@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(THREADS) choose_kernel(const SelectArgs a) {
         __syncthreads();
         want -= s_above;
         lowest += (uint32_t)s_bin << shift;
-        highest = min(highest, lowest + ((1u << shift) - 1));
+        highest = lowest + min(highest - lowest, (1u << shift) - 1);  // (the end of a bin near the top is past 32 bits)
         clear();
         const int in = s_in;
         if (in <= 32 && lowest < highest) {  // few enough to be ranked side by side in every warp
