@@ -492,7 +492,9 @@ def paged_decode_gqa(q, kv, out, window=0, sinks=0, scores=None, ws: Workspace |
     if blocks is not None:
         if window or sinks or scores is not None:
             raise ValueError("a list of blocks goes without window, sinks and scores")
-        n = blocks.shape[-1]
+        n = blocks.shape[-1] if blocks.dim() else 0
+        if n == 0:  # (and without elements it would have no address, as no list has none)
+            raise ValueError(f"blocks must be int32 [{B}, {kv.nkv}, n] with n of at least 1, got {tuple(blocks.shape)}")
         _need(blocks, "blocks", _torch().int32, (B, kv.nkv, n), dev)
         lst = blocks.data_ptr()
     wsh, st = ws.h if ws is not None else None, _stream_of(stream, dev)
