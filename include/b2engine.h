@@ -438,7 +438,8 @@ typedef struct b2_append {
  * (i, i + rotary_dim/2) by position * inv_freq[i]; inv_freq is read on the host
  * during the call (rotary_dim/2 numbers).  The position is the row's in the
  * cache, or counts up from positions[b] (device int32 [batch]) where that is
- * given: after an eviction the two differ.  Angles are reduced in 64 bits.
+ * given: after an eviction the two differ.  Angles lose nothing far out: whole
+ * turns are dropped before anything is rounded.
  *
  * Sequences of one call must not share the blocks that they write, and what is
  * read must not overlap what is written (q_out may be q).  Inputs may have
