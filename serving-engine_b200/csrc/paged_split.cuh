@@ -170,9 +170,10 @@ __device__ __forceinline__ bool split_units(const SplitArgs& a, SplitShared& sh,
         } else if (can_piece) {
             int pick = -1;
 #pragma unroll
-            for (int k = 7; k >= 0; --k)
-                if (near(k) && (int)__reduce_add_sync(~0u, (unsigned)(s.n + size_of(k) - 1) / (unsigned)size_of(k)) * heads <= grid)
-                    pick = k;
+            for (int k = 7; k >= 0; --k) {  // (the sum over the warp whatever near() says)
+                const int all = (int)__reduce_add_sync(~0u, (unsigned)(s.n + size_of(k) - 1) / (unsigned)size_of(k)) * heads;
+                if (all <= grid && near(k)) pick = k;
+            }
             if (pick >= 0) {
                 pieced = true;
                 upc = size_of(pick);
