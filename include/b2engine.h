@@ -443,7 +443,7 @@ typedef struct b2_append {
  *
  * Sequences of one call must not share the blocks that they write, and what is
  * read must not overlap what is written (q_out may be q).  Inputs may have
- * strides of 0, q_out not.  Allocates nothing; graph-capturable.  S at most 2^30,
+ * strides of 0, q_out and the cache not.  Allocates nothing; graph-capturable.  S at most 2^30,
  * batch at most 65535. */
 int b2_paged_kv_append(const b2_paged_kv* kv, const b2_append* rows, void* stream);
 /* The same into a cache held in 4 bits.  Codes are decided by keys rotated to

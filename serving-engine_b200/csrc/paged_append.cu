@@ -642,6 +642,8 @@ extern "C" int b2_paged_kv_append(const b2_paged_kv* kv, const b2_append* rows, 
     AppendArgs a = {};
     rc = append_args(a, *rows);
     if (rc != B2_OK) return rc;
+    B2_REQUIRE((kv->num_blocks == 1 || kv->stride_block) && (kv->block_size == 1 || kv->stride_slot) &&
+               (rows->num_kv_heads == 1 || kv->stride_head));
     a.kv = *kv;
     a.block_tables = kv->block_tables;
     a.seq_lens = kv->seq_lens;
