@@ -23,6 +23,13 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import b2engine as b2  # noqa: E402
 
 
+def whole_rows(t):
+    """t with its rows as an append takes them, contiguous and 16-byte aligned: t itself, or a copy."""
+    fits = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
+        all(n == 1 or step % 8 == 0 for n, step in zip(t.shape[:-1], t.stride()[:-1]))
+    return t if fits else t.clone(memory_format=torch.contiguous_format)
+
+
 class BoundedLayer:
     """K/V pool, block tables, lengths and scores of `batch` sequences of one
     layer.  A sequence holds at most `capacity` rows; eviction leaves
@@ -46,6 +53,14 @@ class BoundedLayer:
                                                                scored=True))
         self.rows = [0] * batch  # the lengths as the host knows them
 
+    def _append(self, k, v):
+        """Rows of new tokens, which seq_lens counts already; rows that are refused leave the layer as it was."""
+        try:
+            b2.paged_kv_append(self.kv, whole_rows(k), whole_rows(v))
+        except Exception:
+            self.seq_lens.copy_(torch.tensor(self.rows, dtype=torch.int32))
+            raise
+
     def prefill(self, q, k, v, chunk=512, observe=16):
         """Prompts [B, S, heads, head_dim] of one length S <= capacity;
         returns the attention outputs [B, S, nq, head_dim]."""
@@ -59,7 +74,7 @@ class BoundedLayer:
             b2.window_prefill_gqa(q[:, at:end], k[:, :end], v[:, :end], part, window=self.window, sinks=self.sinks)
             out[:, at:end] = part
         self.seq_lens.fill_(S)
-        b2.paged_kv_append(self.kv, k, v)
+        self._append(k, v)
         self.rows = [S] * B
         self.scores.zero_()
         # what the last prompt queries look at ranks the rows of the prompt
@@ -75,9 +90,9 @@ class BoundedLayer:
         head_dim].  Returns the attention outputs [B, nq, head_dim]."""
         if max(self.rows) == self.capacity:
             self.evict()
-        self.rows = [n + 1 for n in self.rows]
         self.seq_lens += 1
-        b2.paged_kv_append(self.kv, k[:, None], v[:, None])
+        self._append(k[:, None], v[:, None])
+        self.rows = [n + 1 for n in self.rows]
         out = torch.empty(q.shape, dtype=q.dtype, device="cuda")
         return b2.paged_decode_gqa(q, self.kv, out, window=self.window, sinks=self.sinks, scores=self.scores,
                                    ws=self.ws)
