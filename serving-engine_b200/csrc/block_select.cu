@@ -58,21 +58,13 @@ struct BoundsArgs {
     float* scale;
 };
 
-// 2^e as a float, e from -126 to 127
-__device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }
-
-// The smaller and the larger of two numbers, or a NaN if one is.
+// The smaller, or a NaN if one is.
 __device__ __forceinline__ float min_nan(float a, float b) {
     float r;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-// The same of two 16-bit numbers each.
+// The same, and the larger, of two 16-bit numbers each.
 template <bool BF16>
 __device__ __forceinline__ uint32_t least2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -219,7 +211,7 @@ __global__ void __launch_bounds__(kBdThreads, 7) bounds_kernel(const BoundsArgs 
             const uint32_t bits = __float_as_uint(top);
             const int e = top == 0.f ? 0 : max(-126, (int)(bits >> 23) - 127 - ((bits & 0x7fffffu) > 0x7e0000u ? 5 : 6));
             if (sub == 0 && in) {
-                const float back = fine ? power(-e) : 0.f;
+                const float back = fine ? pow2(-e) : 0.f;
                 // (a product that vanishes still is on its side of zero)
                 uint32_t d[2] = {0, 0}, u[2] = {0, 0};
 #pragma unroll
@@ -233,7 +225,7 @@ __global__ void __launch_bounds__(kBdThreads, 7) bounds_kernel(const BoundsArgs 
                 int8_t* out = a.codes + ((int64_t)id * a.nkv + h) * 2 * a.D + c;
                 *reinterpret_cast<uint2*>(out) = make_uint2(d[0], d[1]);
                 *reinterpret_cast<uint2*>(out + a.D) = make_uint2(u[0], u[1]);
-                if (lane == 0) a.scale[(int64_t)id * a.nkv + h] = fine ? power(e) : INFINITY;
+                if (lane == 0) a.scale[(int64_t)id * a.nkv + h] = fine ? pow2(e) : INFINITY;
             }
         }
         base += all;

@@ -89,8 +89,6 @@ struct Kv4Cfg {
     static constexpr int CTAS = 2;                     // per SM
 };
 
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
-
 // N consecutive 32-bit words of shared memory at an address aligned to the largest of 16, 8 and 4 bytes that divides 4 N
 template <int N>
 __device__ __forceinline__ void lds(uint32_t (&w)[N], const uint8_t* p) {

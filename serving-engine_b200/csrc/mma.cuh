@@ -65,6 +65,15 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// 2^e, e from -126 to 127
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+// The larger, or a NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 namespace packed {
 
 // two 32-bit numbers in a register pair: one instruction for both

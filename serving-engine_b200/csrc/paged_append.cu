@@ -79,13 +79,6 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
 // Where quad x of angles stands: lanes 4 or 8 quads apart read different banks.
 __device__ __forceinline__ int spread(int x) { return x + (x >> 3); }
 
-// The larger, or a NaN if one is.
-__device__ __forceinline__ float fmax_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
 // floor(i / d) by inv = 2^20 / d + 1, for i d < 2^20
 __device__ __forceinline__ int over(int i, uint32_t inv) { return (int)(((uint32_t)i * inv) >> 20); }
 __device__ __forceinline__ uint64_t pair(float2 x) { return pair(x.x, x.y); }
@@ -333,14 +326,14 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
             for (int i = 1; i < 8; ++i) {
                 lo = fminf(lo, f[i]);
                 hi = fmaxf(hi, f[i]);
-                most = fmax_nan(most, fabsf(f[i]));
+                most = max_nan(most, fabsf(f[i]));
             }
             if (!in) lo = INFINITY, hi = -INFINITY;
     #pragma unroll
             for (int o = 1; o < 8; o <<= 1) {
                 lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
                 hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
-                most = fmax_nan(most, __shfl_xor_sync(~0u, most, o));
+                most = max_nan(most, __shfl_xor_sync(~0u, most, o));
             }
             const bool fine = most < INFINITY;
             // what f is off by, at most: sine and cosine 2^-25 each, a product 2^-24 |x2|, the sum 2^-24 of itself.  Turning
@@ -348,7 +341,7 @@ __global__ void __launch_bounds__(kApThreads, 3) append_kernel(const __grid_cons
             float off = 0.f;
             if (key && a.rot) {
                 off = most;
-                for (int o = 8; o < (1 << WIDE); o <<= 1) off = fmax_nan(off, __shfl_xor_sync(~0u, off, o));
+                for (int o = 8; o < (1 << WIDE); o <<= 1) off = max_nan(off, __shfl_xor_sync(~0u, off, o));
                 off *= 0x1p-22f;
             }
             auto to_half = [](float x) { return __half2float(__float2half_rn(x)); };

@@ -76,6 +76,20 @@ struct PagedCfg {
     static constexpr int CTAS = DP == 256 ? 1 : 2;    // per SM
 };
 
+// (a, b) as 16-bit values and what the rounding left, again in 16 bits
+template <bool BF16>
+__device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack16<BF16>(a, b);
+    float2 f;
+    if constexpr (BF16) {
+        f.x = __uint_as_float(hi << 16);
+        f.y = __uint_as_float(hi & 0xffff0000u);
+    } else {
+        f = h2_to_f2(hi);
+    }
+    lo = pack16<BF16>(a - f.x, b - f.y);
+}
+
 template <int DP, bool GH, bool BF16, bool LIST>
 __global__ void __launch_bounds__(kPgThreads, PagedCfg<DP, GH>::CTAS) paged_attn_kernel(const PagedArgs a) {
     using C = PagedCfg<DP, GH>;

@@ -60,19 +60,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// (a, b) as 16-bit values and what the rounding left, again in 16 bits
-template <bool BF16>
-__device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
-    hi = pack16<BF16>(a, b);
-    float2 f;
-    if constexpr (BF16) {
-        f.x = __uint_as_float(hi << 16);
-        f.y = __uint_as_float(hi & 0xffff0000u);
-    } else {
-        f = h2_to_f2(hi);
-    }
-    lo = pack16<BF16>(a - f.x, b - f.y);
-}
 template <bool BF16>
 __device__ __forceinline__ void store4(void* p, int64_t i, float4 v, float scale) {
     const uint2 x = make_uint2(pack16<BF16>(v.x * scale, v.y * scale), pack16<BF16>(v.z * scale, v.w * scale));

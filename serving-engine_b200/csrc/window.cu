@@ -280,11 +280,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // added to the exponent.  Below -126 x counts as -126.  NaN (which fmaxf would
 // take for -126 too) gives the largest float: infinity as a 16-bit weight, so
 // that it shows in the output.
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
 __device__ __forceinline__ float2 ex2_fma(float2 x) {
     const uint64_t y = two(max_nan(x.x, -126.f), max_nan(x.y, -126.f));
     const uint64_t t = add2(y, two(12582912.f, 12582912.f));
