@@ -20,18 +20,18 @@
 //            per group into its own sums, then one multiply-add each; the second
 //            terms are a product too, of the scale words as they are stored with
 //            the sums of q as half and remainder.
-//   outputs  o_d = sum_i (p_i s_ig) (u_id - 8) + sum_i p_i (m_ig + 8 s_ig): the
+//   outputs  o_d = sum_i (p_i s_ig) (u_id - 4) + sum_i p_i (m_ig + 4 s_ig): the
 //            weights times the scale are the operand, as a half and what its
-//            rounding left as a half beside it: 22 bits of each.  (A bare half is
-//            off by up to 2^-11 of p s |u - 8|, while the m + u s that the two
-//            sums come to may vanish.)  The second sum is kept in 32 bits per
-//            group.  Less 8, because sums of codes of one sign would be far larger
-//            than the output that is left of them: a product with a constant -8
-//            is where each unit's sums start.  What shows at long contexts is the
-//            truncation of the matrix instruction's own sums: 131001 tokens in
-//            half are off by 2.24e-4 of the result, 2.08e-4 being the output's
-//            rounding (sums that start at -8 with every second tile: 2.16e-4 and 3 %
-//            slower, with every tile: 2.10e-4 and 7 %); in bf16 it does not.
+//            rounding left as a half beside it: 22 bits of each, or 2^-39 of the
+//            largest.  (A bare half is off by up to 2^-11 of p s |u - 4|, while
+//            the m + u s that the two sums come to may vanish.)  The second sum is
+//            kept in 32 bits per group.  Less 4, because the matrix instruction
+//            truncates what it adds to the size of its sum: a product with a
+//            constant -4 is where each unit's sums start, and with codes of 7.5
+//            on average they go through zero on their way (131001 tokens, 8 heads,
+//            in half: the arithmetic is off by a quarter of what the output's
+//            rounding is; less 8 by up to 0.4 of it; less 5, whose own products
+//            are truncated, by more than it).
 // Queries are scaled by a power of two into the middle of the halves' range
 // (bf16 ones are then exact in half), the weights by one that follows the
 // largest scale seen so far, like the running max of the softmax.
@@ -48,7 +48,7 @@
 // Measured: 32 sequences of up to 32768 tokens, 32/8 heads of 128, bf16: 227 us in a
 // long run (4.6 TB/s, 70 % of a copy; floor 158; without remainders 218): half of
 // the issue slots, 8 warps per SM that wait for one another's pipes.  131001 tokens,
-// 64/8 heads: 48 us (floor 23): eight columns of heads, the remainders in products of
+// 64/8 heads, half: 49 us (floor 23): eight columns of heads, the remainders in products of
 // their own, 37 pieces joined per segment.  8 sequences of up to 4096: 17 us, 301
 // tokens of 14/2 heads of 64: 7 us: the chain length, table, rows, merge, join.
 #include <cmath>
@@ -133,7 +133,11 @@ template <int DP, int H, bool BF16, bool LIST>
 __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kernel(const Kv4Args a) {
     using C = Kv4Cfg<DP, H>;
     constexpr int U = C::U, T = C::T, W = C::W, NG = C::NG;
-    constexpr bool TWO = H > 4;          // remainders of the weights in products of their own
+    constexpr bool TWO = H > 4;  // remainders of the weights in products of their own
+    // and in sums of their own: added to the weights' they are truncated to the size of those (131001 tokens, 8 heads,
+    // standard normal rows, in half: 8 % above the error that the output's rounding leaves, 2.5 % so, for 2 % of the time; in
+    // bf16 neither shows)
+    constexpr bool APART = TWO && !BF16;
     constexpr int NT = H == 16 ? 2 : 1;  // products side by side, 8 heads each
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ SplitShared s_split;
@@ -475,18 +479,18 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                             l[n][h] += p;
                         }
                 }
-            // O += V^T (P s), group by group, with codes less 8; the weights as half and remainder, turned from
+            // O += V^T (P s), group by group, with codes less 4; the weights as half and remainder, turned from
             // (position, head) to (head, position) pairs
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 uint32_t hi[T][NT][2], lo[T][NT][2];
-                float less[NT][4];
+                float less[APART ? 2 * NT : NT][4];  // (the remainders' behind)
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
 #pragma unroll
                     for (int pp = 0; pp < 2; ++pp) {
                         const float2 sm = h2_to_f2(vm[t][pp][g]);
-                        const float mid = fmaf(8.f, sm.x, sm.y);
+                        const float mid = fmaf(4.f, sm.x, sm.y);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             const float p0 = x[t][n][2 * pp], p1 = x[t][n][2 * pp + 1];
@@ -500,14 +504,16 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                             if constexpr (TWO) lo[t][n][pp] = transpose8x8(r);
                         }
                     }
-                    // -8 units in the rows of either nibble: what the products of the codes start from
+                    // -4 units in the rows of either nibble: what the products of the codes start from
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        mma_f16(less[n], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, hi[t][n][0], hi[t][n][1],
+                        mma_f16(less[n], 0x80048004u, 0x80408040u, 0x80048004u, 0x80408040u, hi[t][n][0], hi[t][n][1],
                                 t ? less[n] : zero);
-                        if (TWO)
-                            mma_f16(less[n], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, lo[t][n][0], lo[t][n][1],
-                                    less[n]);
+                        if constexpr (TWO) {
+                            float(&d)[4] = less[APART ? NT + n : n];
+                            mma_f16(d, 0x80048004u, 0x80408040u, 0x80048004u, 0x80408040u, lo[t][n][0], lo[t][n][1],
+                                    APART && t == 0 ? zero : d);
+                        }
                     }
                 }
 #pragma unroll
@@ -517,7 +523,7 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
                     for (int t = 0; t < T; ++t) lds(vw[t], unit + t * C::TILE + 8 * DP + (v * 32 + lane) * 8);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        float c[NT][4];
+                        float c[APART ? 2 * NT : NT][4];
 #pragma unroll
                         for (int t = 0; t < T; ++t) {
                             const uint32_t u0 = vw[t][0] >> (8 * k), u1 = vw[t][1] >> (8 * k);
@@ -526,12 +532,21 @@ __global__ void __launch_bounds__(kPgThreads, Kv4Cfg<DP, H>::CTAS) kv4_attn_kern
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
                                 mma_f16(c[n], b0, b1, b2, b3, hi[t][n][0], hi[t][n][1], t ? c[n] : less[n]);
-                                if (TWO) mma_f16(c[n], b0, b1, b2, b3, lo[t][n][0], lo[t][n][1], c[n]);
+                                if constexpr (TWO) {
+                                    constexpr int r = APART ? NT : 0;
+                                    mma_f16(c[r + n], b0, b1, b2, b3, lo[t][n][0], lo[t][n][1],
+                                            APART && t == 0 ? less[r + n] : c[r + n]);
+                                }
                             }
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             float(&d)[4] = o[v][k][n];
+                            if constexpr (APART) {
+                                const float2 z0 = two(add2(pair(c[n][0], c[n][1]), pair(c[NT + n][0], c[NT + n][1])));
+                                const float2 z1 = two(add2(pair(c[n][2], c[n][3]), pair(c[NT + n][2], c[NT + n][3])));
+                                c[n][0] = z0.x, c[n][1] = z0.y, c[n][2] = z1.x, c[n][3] = z1.y;
+                            }
                             const float2 y0 = two(add2(pair(d[0], d[1]), pair(c[n][0], c[n][1])));
                             const float2 y1 = two(add2(pair(d[2], d[3]), pair(c[n][2], c[n][3])));
                             d[0] = y0.x, d[1] = y0.y, d[2] = y1.x, d[3] = y1.y;

@@ -7,8 +7,8 @@ whose number is c modulo the channels, else 0, so an output is the share of the
 weight that its tiles have, and a tile that is left out or taken twice moves it by a
 large part of itself.  Bound: half a step of the type, 2^-17 M of every weight as in
 test_gpu_kv4.py (M = sum |q| 3 max|k| / sqrt(D)) and 2^-18 for the exponential and
-the split of the weights, of the output.  Beside those, as codes' sums start at -8 of
-all weights, with a scale of 1 / 15: a unit's 16 products off by 2^-22 of 31 / 15
+the split of the weights, of the output.  Beside those, as codes' sums start at up to
+-8 of all weights, with a scale of 1 / 15: a unit's 16 products off by 2^-22 of 31 / 15
 of its weight; and of all weights so far, times 16 / 15, 2^-24 in each of 9
 additions a unit (one of the outputs, 8 of what is added back) for the n units that
 a CTA adds up."""
