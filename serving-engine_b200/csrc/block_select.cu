@@ -27,8 +27,8 @@
 // 54 us for 32 x 2048 blocks of 8 heads of 128, instead of 27 and 7.)
 //
 // Measured, cold: bounds of 32768 tokens of 8 heads of 128 in 16 bits 15 us (4.5
-// TB/s: a block's loads leave together, then its warp works them off), of the
-// newest block of 8 sequences 6.3 us, a chain of three loads; scores of 32 x up to
+// TB/s: a block's loads leave together, 112 KB per SM, then its warp works them off
+// before it looks up the next one), of the newest block of 8 sequences 6.3 us, a chain of three loads; scores of 32 x up to
 // 2048 blocks of 8 heads 28 us (117 MB, 4.3 TB/s with its start), of 4094 blocks
 // 11 us, five loads one after the other; the choice among 2048 blocks 6.6 us (8.5
 // of 256 pairs), among 8188 9.5 us (14 us with 512 threads and keys in shared

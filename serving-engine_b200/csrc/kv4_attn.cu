@@ -46,11 +46,13 @@
 // through its own ring of shared-memory stages (cp.async).
 //
 // Measured: 32 sequences of up to 32768 tokens, 32/8 heads of 128, bf16: 227 us in a
-// long run (4.6 TB/s, 70 % of a copy; floor 158; without remainders 218): half of
-// the issue slots, 8 warps per SM that wait for one another's pipes.  131001 tokens,
-// 64/8 heads, half: 49 us (floor 23): eight columns of heads, the remainders in products of
-// their own, 37 pieces joined per segment.  8 sequences of up to 4096: 17 us, 301
-// tokens of 14/2 heads of 64: 7 us: the chain length, table, rows, merge, join.
+// long run (4.5 TB/s, 69 % of a copy; floor 158; without remainders 218), 210 for one
+// launch: 252 instructions a tile, 0.54 of the issue slots with 8 warps per SM, whose
+// stalls are mostly the fixed wait for the instruction before.  131001 tokens,
+// 64/8 heads, half: 49 us (floor 23): eight columns of heads, the remainders in
+// products of their own, 295 instructions a tile, 37 pieces joined per segment.  8
+// sequences of up to 4096: 17 us, 301 tokens of 14/2 heads of 64: 7 us: the chain
+// length, table, rows, merge, join.
 #include <cmath>
 #include <type_traits>
 
@@ -77,8 +79,8 @@ struct Kv4Cfg {
     static constexpr int NG = kv4_groups(DP);
     static constexpr int W = DP / 32;                  // K words of a lane and row, V pieces of a lane
     static constexpr int TILE = kv4_tile(DP);
-    // tiles per warp and unit: as many as there are registers for (128 channels, 4 heads: 187 us for 32 x 32768 with 4,
-    // 210 with 2 and three CTAs per SM, 250 with 1 and four)
+    // tiles per warp and unit: as many as there are registers for (128 channels, 4 heads, without remainders, one launch:
+    // 187 us for 32 x 32768 with 4, 210 with 2 and three CTAs per SM, 250 with 1 and four)
     static constexpr int T = DP <= 128 && H <= 8 ? 4 : 2;
     static constexpr int U = kPgWarps * T * 16;        // positions per unit
     static constexpr int STAGES = DP <= 96 || T == 2 && DP == 128 ? 3 : 2;

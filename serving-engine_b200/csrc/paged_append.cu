@@ -27,11 +27,12 @@
 // 101 us for 8192 tokens.)
 //
 // Measured: 8192 tokens, 32 query and 8 K/V heads of 128, into a 4-bit cache 58
-// us (floor 27), 39 of them for keys and values alone: 360 instructions for 8
-// channels a lane, two thirds of the issue slots taken; the queries alone are
-// bound by HBM (21 us), and their CTAs stand between the others (one kind after
-// the other: 63 us).  16 channels a lane: fewer instructions by an eighth, but
-// too many registers (68 us).  One token of one sequence 4 us in a graph: the
+// us (floor 27): keys and values alone 39, 365 instructions for 8 channels a lane,
+// 0.59 of the issue slots with the 20 warps per SM that 80 registers leave (56 bytes
+// spilled, 88 at 64 channels, 24 for rows of 16 bits); queries alone 21, bound by
+// HBM.  Their CTAs stand between the others, which overlaps little (one kind after
+// the other: 63 us).  16 channels a lane: fewer instructions by an eighth, but more
+// spills (68 us).  One token of one sequence 4 us in a graph: the
 // chain length, table entry, row.
 #include <cmath>
 #include <type_traits>
